@@ -30,6 +30,10 @@ extern "C" {
 #define SB_DTYPE_F16 1
 #define SB_DTYPE_F32 2
 
+/* Activations of the gated experts. */
+#define SB_ACT_SILU 0
+#define SB_ACT_GELU 1
+
 /* Message of the last failed call on this thread ("" if none). */
 const char* sb_last_error(void);
 
@@ -274,6 +278,88 @@ int sb_layer_assigned(const void* x, const void* token_of_copy, int32_t token_is
 int sb_layer_rounded(const void* x, const float* scores, const void* w1, const void* w2, void* out, void* workspace,
                      int64_t workspace_bytes, int64_t num_tokens, int32_t num_experts, int32_t k, int32_t tile,
                      int64_t d_model, int64_t ffn_dim, void* stream);
+
+/* ---- The layer with gated experts, forward and backward --------------- */
+
+/* No counterpart in the reference: the MoE layer with gated experts,
+ *   G | U = x[t] W1[e],  H = a(G) U,  out[t] = sum_j gates[t, j] H W2[e],
+ * x [T, D], w1 [E, D, 2F] (the gate's F columns, then the up projection's F),
+ * w2 [E, F, D], all bf16; act is an SB_ACT_* code; expert_idx, gates and
+ * valid_tokens as in sb_layer (a copy with an expert id out of range adds
+ * nothing). D and F are multiples of 128, and D F 4 bytes stay under 2 GiB.
+ *
+ * sb_gated_layer runs the forward pass. sb_gated_train runs the same (the
+ * same bits) and leaves in `saved` what sb_gated_backward reads: the layout,
+ * G | U and H W2 in bf16. sb_gated_backward takes the gradient of out and
+ * writes, all of them whole and with no atomics:
+ *   grad_x [T, D] bf16, grad_gates [T, k] in the gates' dtype (0 for a copy
+ *   that was not routed), grad_w1 and grad_w2 in bf16 (0 for experts without
+ *   tokens); rows t >= *valid_tokens of grad_x and grad_gates are not written.
+ * Its other operands are the forward pass's, unchanged since. `saved` is only
+ * read: the call may be repeated.
+ *
+ * sb_gated_sizes: bytes of sb_gated_layer's workspace, of `saved`, and of
+ * sb_gated_train's and sb_gated_backward's workspaces (each pointer may be
+ * NULL); all 256-byte aligned, free once the stream has passed the call. */
+int sb_gated_sizes(int64_t num_tokens, int32_t k, int32_t num_experts, int64_t d_model, int64_t ffn_dim,
+                   int64_t* layer_bytes, int64_t* saved_bytes, int64_t* train_bytes, int64_t* backward_bytes);
+int sb_gated_layer(const void* x, const void* expert_idx, int32_t idx_is_i64, const void* gates, int32_t gate_dtype,
+                   const void* w1, const void* w2, void* out, int32_t act, void* workspace, int64_t workspace_bytes,
+                   int64_t num_tokens, int32_t k, int32_t num_experts, int64_t d_model, int64_t ffn_dim,
+                   const int32_t* valid_tokens, void* stream);
+int sb_gated_train(const void* x, const void* expert_idx, int32_t idx_is_i64, const void* gates, int32_t gate_dtype,
+                   const void* w1, const void* w2, void* out, int32_t act, void* saved, int64_t saved_bytes,
+                   void* workspace, int64_t workspace_bytes, int64_t num_tokens, int32_t k, int32_t num_experts,
+                   int64_t d_model, int64_t ffn_dim, const int32_t* valid_tokens, void* stream);
+int sb_gated_backward(const void* grad_out, const void* x, const void* gates, int32_t gate_dtype, const void* w1,
+                      const void* w2, const void* saved, int64_t saved_bytes, void* grad_x, void* grad_gates,
+                      void* grad_w1, void* grad_w2, int32_t act, void* workspace, int64_t workspace_bytes,
+                      int64_t num_tokens, int32_t k, int32_t num_experts, int64_t d_model, int64_t ffn_dim,
+                      const int32_t* valid_tokens, void* stream);
+
+/* ---- The AdamW step ---------------------------------------------------- */
+
+/* One tensor of sb_adamw: contiguous arrays of numel values. param and grad
+ * are of their SB_DTYPE_* codes; master is NULL, or fp32 weights that are
+ * updated in the parameter's place and rounded into it. State bits 32:
+ * exp_avg and exp_avg_sq are fp32 (the scales unused); 8: exp_avg is int8 and
+ * exp_avg_sq uint8, in blocks of 256 values with a scale each (ceil(numel /
+ * 256) of them): the first moment is c |c| scale, the second (c^2 scale)^2. */
+typedef struct {
+  void* param;
+  const void* grad;
+  float* master;
+  void* exp_avg;
+  void* exp_avg_sq;
+  float* exp_avg_scale;
+  float* exp_avg_sq_scale;
+  int64_t numel;
+  int32_t param_dtype;
+  int32_t grad_dtype;
+} SbAdamwTensor;
+
+/* No counterpart in the reference: one AdamW step of `count` tensors, in place.
+ *   m = b1 m + (1 - b1) g,  v = b2 v + (1 - b2) g^2,  g = grad * *grad_scale
+ *   w = w (1 - lr weight_decay) - lr / (1 - b1^s) m / (sqrt(v / (1 - b2^s)) + eps)
+ * step [2] int32 on the device: step[0] = steps done (s is one more; the call
+ * advances it), step[1] = 0; calls that share it must be ordered. lr_ptr and
+ * grad_scale: NULL, or one fp32 on the device. seed: of the 8-bit states'
+ * stochastic rounding, with the step, the tensor's place in the list and the
+ * value's in the tensor. `tensors` is read before the call returns. */
+int sb_adamw(const SbAdamwTensor* tensors, int64_t count, int32_t state_bits, int32_t* step, float lr,
+             const float* lr_ptr, double beta1, double beta2, float eps, float weight_decay, const float* grad_scale,
+             uint32_t seed, void* stream);
+
+/* out[i] = the values that 8-bit states stand for, in out_dtype: c |c| scale
+ * of int8 codes (is_signed), c^2 scale of uint8 codes (the second moment's root). */
+typedef struct {
+  const void* codes;
+  const float* scales;
+  void* out;
+  int64_t numel;
+  int64_t is_signed;
+} SbQuantized;
+int sb_dequantize(const SbQuantized* tensors, int64_t count, int32_t out_dtype, void* stream);
 
 #ifdef __cplusplus
 }

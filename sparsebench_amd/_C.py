@@ -14,6 +14,8 @@ kernel.
 
 from __future__ import annotations
 
+import array
+import contextlib
 import ctypes
 import functools
 
@@ -654,4 +656,232 @@ def layer_rounded_cuda(x: torch.Tensor, scores: torch.Tensor, k: int, w1: torch.
         x.data_ptr(), scores.data_ptr(), w1.data_ptr(), w2.data_ptr(), out.data_ptr(), workspace.data_ptr(), size,
         num_tokens, num_experts, k, tile, d_model, ffn_dim, stream_of(dev),
     ))
+    return out
+
+
+# ---- the layer with gated experts, forward and backward (this build's C ABI) ----
+
+_ACTIVATIONS = {"silu": 0, "gelu": 1}
+
+
+def _device_of(t: torch.Tensor) -> contextlib.AbstractContextManager:
+    """Makes t's device current for a launch, where it is not."""
+    if t.device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(t.device)
+
+
+@functools.lru_cache(maxsize=256)
+def gated_bytes(num_tokens: int, k: int, num_experts: int, d_model: int, ffn_dim: int) -> tuple[int, int, int, int]:
+    """Bytes of gated_layer_cuda's workspace, of what gated_train_cuda keeps, and of
+    its and gated_backward_cuda's workspaces."""
+    sizes = [ctypes.c_int64() for _ in range(4)]
+    check(lib().sb_gated_sizes(num_tokens, k, num_experts, d_model, ffn_dim, *(ctypes.byref(s) for s in sizes)))
+    return tuple(s.value for s in sizes)
+
+
+def _check_gated(x: torch.Tensor, expert_idx: torch.Tensor | None, gates: torch.Tensor, w1: torch.Tensor,
+                 w2: torch.Tensor, activation: str, valid_tokens: torch.Tensor | None) -> tuple[int, ...]:
+    """(T, k, E, D, F) of operands that the gated layer's calls take as they are."""
+    if not (x.is_cuda and w1.device == x.device and w2.device == x.device and gates.device == x.device
+            and (expert_idx is None or expert_idx.device == x.device)):
+        _fail("all inputs must be on the same GPU")
+    if x.dtype != torch.bfloat16 or w1.dtype != torch.bfloat16 or w2.dtype != torch.bfloat16:
+        _fail("x, w1 and w2 must be bfloat16")
+    if not (x.dim() == 2 and w1.dim() == 3 and w2.dim() == 3):
+        _fail(f"x must be [T, D], w1 [E, D, 2F] and w2 [E, F, D], got {_shape(x)}, {_shape(w1)} and {_shape(w2)}")
+    num_experts, ffn_dim, d_model = w2.shape
+    if x.shape[1] != d_model or w1.shape != (num_experts, d_model, 2 * ffn_dim):
+        _fail(f"x must be [T, D], w1 [E, D, 2F] and w2 [E, F, D], got {_shape(x)}, {_shape(w1)} and {_shape(w2)}")
+    if not (x.is_contiguous() and w1.is_contiguous() and w2.is_contiguous()):
+        _fail("x, w1 and w2 must be contiguous")
+    if (x.data_ptr() | w1.data_ptr() | w2.data_ptr()) % 16:
+        _fail("x, w1 and w2 must be 16-byte aligned")
+    if gates.dim() != 2 or gates.shape[0] != x.shape[0] or gates.shape[1] == 0:
+        _fail(f"expert_weight must be [T, k] with k > 0, got {_shape(gates)}")
+    if gates.dtype not in _GATE_DTYPES:
+        _fail(f"expert_weight must be bfloat16, float16 or float32, got {gates.dtype}")
+    if expert_idx is not None:
+        if expert_idx.shape != gates.shape:
+            _fail(f"expert_idx must be [T, k] as expert_weight, got {_shape(expert_idx)}")
+        if expert_idx.dtype not in _INDEX_DTYPES:
+            _fail(f"expert_idx must be int32 or int64, got {expert_idx.dtype}")
+    if not 0 < num_experts <= _MAX_EXPERTS:
+        _fail(f"num_experts must be in [1, {_MAX_EXPERTS}], got {num_experts}")
+    if activation not in _ACTIVATIONS:
+        _fail(f"activation must be one of {sorted(_ACTIVATIONS)}, got {activation!r}")
+    if valid_tokens is not None and not (valid_tokens.device == x.device and _valid_tokens_ok(valid_tokens)):
+        _fail("valid_tokens must be a one-element int32 CUDA tensor")
+    return x.shape[0], gates.shape[1], num_experts, d_model, ffn_dim
+
+
+def gated_layer_cuda(x: torch.Tensor, expert_idx: torch.Tensor, expert_weight: torch.Tensor, w1: torch.Tensor,
+                     w2: torch.Tensor, activation: str, valid_tokens: torch.Tensor | None = None) -> torch.Tensor:
+    """The layer with gated experts: out [T, D] bf16. Rows t >= valid_tokens (if given) are left unwritten."""
+    t, k, e, d, f = _check_gated(x, expert_idx, expert_weight, w1, w2, activation, valid_tokens)
+    out = torch.empty_like(x)
+    if t == 0:
+        return out
+    expert_idx, gates = expert_idx.contiguous(), expert_weight.contiguous()
+    size = gated_bytes(t, k, e, d, f)[0]
+    workspace = torch.empty(size, dtype=torch.uint8, device=x.device)
+    with _device_of(x):
+        check(lib().sb_gated_layer(
+            x.data_ptr(), expert_idx.data_ptr(), _INDEX_DTYPES[expert_idx.dtype], gates.data_ptr(),
+            _GATE_DTYPES[gates.dtype], w1.data_ptr(), w2.data_ptr(), out.data_ptr(), _ACTIVATIONS[activation],
+            workspace.data_ptr(), size, t, k, e, d, f, _ptr(valid_tokens), stream_of(x.device),
+        ))
+    return out
+
+
+def gated_train_cuda(x: torch.Tensor, expert_idx: torch.Tensor, expert_weight: torch.Tensor, w1: torch.Tensor,
+                     w2: torch.Tensor, activation: str, valid_tokens: torch.Tensor | None = None
+                     ) -> tuple[torch.Tensor, torch.Tensor]:
+    """(out, saved): gated_layer_cuda's output, and the bytes that gated_backward_cuda reads."""
+    t, k, e, d, f = _check_gated(x, expert_idx, expert_weight, w1, w2, activation, valid_tokens)
+    out = torch.empty_like(x)
+    if t == 0:
+        return out, torch.empty(0, dtype=torch.uint8, device=x.device)
+    expert_idx, gates = expert_idx.contiguous(), expert_weight.contiguous()
+    _, saved_size, size, _ = gated_bytes(t, k, e, d, f)
+    saved = torch.empty(saved_size, dtype=torch.uint8, device=x.device)
+    workspace = torch.empty(size, dtype=torch.uint8, device=x.device)
+    with _device_of(x):
+        check(lib().sb_gated_train(
+            x.data_ptr(), expert_idx.data_ptr(), _INDEX_DTYPES[expert_idx.dtype], gates.data_ptr(),
+            _GATE_DTYPES[gates.dtype], w1.data_ptr(), w2.data_ptr(), out.data_ptr(), _ACTIVATIONS[activation],
+            saved.data_ptr(), saved_size, workspace.data_ptr(), size, t, k, e, d, f, _ptr(valid_tokens),
+            stream_of(x.device),
+        ))
+    return out, saved
+
+
+def gated_backward_cuda(grad_out: torch.Tensor, x: torch.Tensor, expert_weight: torch.Tensor, w1: torch.Tensor,
+                        w2: torch.Tensor, saved: torch.Tensor, activation: str,
+                        valid_tokens: torch.Tensor | None = None
+                        ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """The gradients (x, expert_weight, w1, w2) of gated_train_cuda's output, each of its operand's shape and dtype.
+    saved: what that call kept. Rows t >= valid_tokens (if given) of the first two are left unwritten."""
+    t, k, e, d, f = _check_gated(x, None, expert_weight, w1, w2, activation, valid_tokens)
+    if grad_out.device != x.device or grad_out.dtype != torch.bfloat16 or grad_out.shape != x.shape:
+        _fail(f"grad_out must be a {_shape(x)} bfloat16 tensor on the same GPU, got {_shape(grad_out)} {grad_out.dtype}")
+    if t == 0:
+        return torch.empty_like(x), torch.empty_like(expert_weight), torch.zeros_like(w1), torch.zeros_like(w2)
+    _, saved_size, _, size = gated_bytes(t, k, e, d, f)
+    if not (saved.device == x.device and saved.dtype == torch.uint8 and saved.numel() == saved_size
+            and saved.is_contiguous()):
+        _fail("saved is not what gated_train_cuda kept for these operands")
+    grad_out, gates = grad_out.contiguous(), expert_weight.contiguous()
+    if grad_out.data_ptr() % 16:
+        grad_out = grad_out.clone()
+    grads = torch.empty_like(x), torch.empty_like(gates), torch.empty_like(w1), torch.empty_like(w2)
+    workspace = torch.empty(size, dtype=torch.uint8, device=x.device)
+    with _device_of(x):
+        check(lib().sb_gated_backward(
+            grad_out.data_ptr(), x.data_ptr(), gates.data_ptr(), _GATE_DTYPES[gates.dtype], w1.data_ptr(),
+            w2.data_ptr(), saved.data_ptr(), saved_size, *(g.data_ptr() for g in grads), _ACTIVATIONS[activation],
+            workspace.data_ptr(), size, t, k, e, d, f, _ptr(valid_tokens), stream_of(x.device),
+        ))
+    return grads
+
+
+# ---- the AdamW step (this build's C ABI) ----
+
+QUANT_BLOCK = 256
+
+
+def _check_state(p: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype, name: str) -> None:
+    if codes.dtype != dtype or codes.numel() != p.numel() or not codes.is_contiguous() or codes.device != p.device:
+        _fail(f"{name} codes must be contiguous {dtype} of the parameter's length, on its GPU")
+    if (scales.dtype != torch.float32 or scales.numel() != -(-p.numel() // QUANT_BLOCK)
+            or not scales.is_contiguous() or scales.device != p.device):
+        _fail(f"{name} scales must be contiguous float32, one for each {QUANT_BLOCK} values, on the parameter's GPU")
+
+
+def _device_scalar(t, name: str, device: torch.device) -> int | None:
+    if not isinstance(t, torch.Tensor):
+        return None
+    if t.device != device or t.dtype != torch.float32 or t.numel() != 1:
+        _fail(f"{name} must be a number or a one-element float32 tensor on the parameters' GPU")
+    return t.data_ptr()
+
+
+def adamw_cuda(params, grads, masters, exp_avgs, exp_avg_sqs, step: torch.Tensor, lr, beta1: float, beta2: float,
+               eps: float, weight_decay: float, grad_scale, seed: int) -> None:
+    """One AdamW step of a list of tensors, in place (include/sparsebench_hip.h: sb_adamw).
+
+    exp_avgs / exp_avg_sqs: fp32 tensors, or (codes, scales) pairs of 8-bit
+    states; masters: None or a list of fp32 tensors; step [2] int32."""
+    n = len(params)
+    if not (len(grads) == len(exp_avgs) == len(exp_avg_sqs) == n) or (masters is not None and len(masters) != n):
+        _fail("params, grads, masters and states must be lists of one length")
+    if not (step.is_cuda and step.dtype == torch.int32 and step.numel() == 2 and step.is_contiguous()):
+        _fail("step must be a contiguous int32 CUDA tensor of two elements")
+    dev = step.device
+    eight = n > 0 and not isinstance(exp_avgs[0], torch.Tensor)
+    words = array.array("q")
+    for i in range(n):
+        p, g, m, v = params[i], grads[i], exp_avgs[i], exp_avg_sqs[i]
+        count = p.numel()
+        p_code, g_code = _GATE_DTYPES.get(p.dtype), _GATE_DTYPES.get(g.dtype)
+        if p_code is None or g_code is None:
+            _fail(f"parameters and gradients must be bfloat16, float16 or float32, got {p.dtype} and {g.dtype}")
+        if p.device != dev or g.device != dev or g.shape != p.shape:
+            _fail("each gradient must have its parameter's shape, all on the step's GPU")
+        if not (p.is_contiguous() and g.is_contiguous()):
+            _fail("parameters and gradients must be contiguous")
+        w = 0
+        if masters is not None:
+            t = masters[i]
+            if t.dtype != torch.float32 or t.shape != p.shape or t.device != dev or not t.is_contiguous():
+                _fail("each master must be contiguous float32 of its parameter's shape, on its GPU")
+            w = t.data_ptr()
+        if isinstance(m, torch.Tensor) == eight or isinstance(v, torch.Tensor) == eight:
+            _fail("all states must be of one kind: float32 tensors, or 8-bit codes and scales")
+        if eight:
+            _check_state(p, *m, torch.int8, "exp_avg")
+            _check_state(p, *v, torch.uint8, "exp_avg_sq")
+            state = m[0].data_ptr(), v[0].data_ptr(), m[1].data_ptr(), v[1].data_ptr()
+        else:
+            for t in (m, v):
+                if t.dtype != torch.float32 or t.shape != p.shape or t.device != dev or not t.is_contiguous():
+                    _fail("each float32 state must be contiguous, of its parameter's shape, on its GPU")
+            state = m.data_ptr(), v.data_ptr(), 0, 0
+        words.extend((p.data_ptr(), g.data_ptr(), w, *state, count, p_code | g_code << 32))
+    lr_ptr, scale_ptr = _device_scalar(lr, "lr", dev), _device_scalar(grad_scale, "grad_scale", dev)
+    with _device_of(step):
+        if scale_ptr is None and grad_scale is not None:  # a number: as a device scalar
+            scale = torch.full((1,), float(grad_scale), dtype=torch.float32, device=dev)
+            scale_ptr = scale.data_ptr()
+        check(lib().sb_adamw(words.buffer_info()[0], n, 8 if eight else 32, step.data_ptr(),
+                             0.0 if lr_ptr else float(lr), lr_ptr, beta1, beta2, eps, weight_decay, scale_ptr,
+                             seed & 0xFFFFFFFF, stream_of(dev)))
+
+
+def dequantize_cuda(pairs, dtype: torch.dtype) -> list[torch.Tensor]:
+    """The values of 8-bit states, (codes, scales) each, in `dtype` (include/sparsebench_hip.h: sb_dequantize)."""
+    if dtype not in _GATE_DTYPES:
+        _fail(f"values must be bfloat16, float16 or float32, got {dtype}")
+    if not pairs:
+        return []
+    dev = pairs[0][0].device
+    if dev.type != "cuda":
+        _fail("codes must be CUDA tensors")
+    # Each value list starts at a multiple of 16 bytes of one buffer.
+    step = 16 // dtype.itemsize
+    starts, total = [], 0
+    for codes, scales in pairs:
+        if codes.dtype not in (torch.int8, torch.uint8) or codes.device != dev:
+            _fail("codes must be int8 or uint8 tensors on one GPU")
+        _check_state(codes, codes, scales, codes.dtype, "state")
+        starts.append(total)
+        total += -(-codes.numel() // step) * step
+    flat = torch.empty(total, dtype=dtype, device=dev)
+    out = [flat[a:a + codes.numel()].view(codes.shape) for a, (codes, _) in zip(starts, pairs)]
+    words = array.array("q")
+    for (codes, scales), o in zip(pairs, out):
+        words.extend((codes.data_ptr(), scales.data_ptr(), o.data_ptr(), codes.numel(),
+                      1 if codes.dtype == torch.int8 else 0))
+    with _device_of(flat):
+        check(lib().sb_dequantize(words.buffer_info()[0], len(pairs), _GATE_DTYPES[dtype], stream_of(dev)))
     return out

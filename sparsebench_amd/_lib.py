@@ -18,6 +18,9 @@ LIB_PATH = pathlib.Path(__file__).resolve().parent / "libsparsebench_hip.so"
 _c_int = ctypes.c_int
 _i32 = ctypes.c_int32
 _i64 = ctypes.c_int64
+_u32 = ctypes.c_uint32
+_f32 = ctypes.c_float
+_f64 = ctypes.c_double
 _ptr = ctypes.c_void_p
 
 # name -> (restype, argtypes); mirrors include/sparsebench_hip.h
@@ -80,6 +83,28 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "sb_layer_rounded": (
         _c_int, [_ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _i64, _i64, _i32, _i32, _i32, _i64, _i64, _ptr]
     ),
+    "sb_gated_sizes": (
+        _c_int, [_i64, _i32, _i32, _i64, _i64, *[ctypes.POINTER(_i64)] * 4]
+    ),
+    "sb_gated_layer": (
+        _c_int,
+        [_ptr, _ptr, _i32, _ptr, _i32, _ptr, _ptr, _ptr, _i32, _ptr, _i64, _i64, _i32, _i32, _i64, _i64, _ptr, _ptr],
+    ),
+    "sb_gated_train": (
+        _c_int,
+        [_ptr, _ptr, _i32, _ptr, _i32, _ptr, _ptr, _ptr, _i32, _ptr, _i64, _ptr, _i64, _i64, _i32, _i32, _i64, _i64,
+         _ptr, _ptr],
+    ),
+    "sb_gated_backward": (
+        _c_int,
+        [_ptr, _ptr, _ptr, _i32, _ptr, _ptr, _ptr, _i64, _ptr, _ptr, _ptr, _ptr, _i32, _ptr, _i64, _i64, _i32, _i32,
+         _i64, _i64, _ptr, _ptr],
+    ),
+    "sb_adamw": (
+        _c_int,
+        [_ptr, _i64, _i32, _ptr, _f32, _ptr, _f64, _f64, _f32, _f32, _ptr, _u32, _ptr],
+    ),
+    "sb_dequantize": (_c_int, [_ptr, _i64, _i32, _ptr]),
 }
 
 SB_OK = 0

@@ -8,11 +8,10 @@
 // token row, gathers the k rows with 16-byte loads and writes 16 bytes.
 
 #include "common.hpp"
+#include "gated.hpp"
 
 namespace sb {
 namespace {
-
-typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 
 template <typename G>
 __device__ __forceinline__ float gate_f32(const G* g, int64_t i);
@@ -27,6 +26,13 @@ __device__ __forceinline__ float gate_f32<_Float16>(const _Float16* g, int64_t i
 template <>
 __device__ __forceinline__ float gate_f32<float>(const float* g, int64_t i) {
   return g[i];
+}
+
+// No gates: each copy counts as it is.
+struct NoGate {};
+template <>
+__device__ __forceinline__ float gate_f32<NoGate>(const NoGate*, int64_t) {
+  return 1.0f;
 }
 
 // KMAX > 0: k == KMAX, known at compile time, so the k row indices, then
@@ -110,6 +116,12 @@ int launch_combine(const void* y, const int32_t* copy_row, const void* gates, vo
 }
 
 }  // namespace
+
+int launch_sum_copies(const void* y, const int32_t* copy_row, void* out, int64_t num_tokens, int32_t k,
+                      int64_t d_model, int64_t y_rows, const int32_t* valid_tokens, hipStream_t stream) {
+  return launch_combine<NoGate>(y, copy_row, nullptr, out, num_tokens, k, d_model, y_rows, valid_tokens, stream);
+}
+
 }  // namespace sb
 
 using namespace sb;

@@ -37,6 +37,7 @@ namespace sb {
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef short i16x4_t __attribute__((ext_vector_type(4)));
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) void lds_void_t;
@@ -96,8 +97,16 @@ __device__ __forceinline__ void wait_vmcnt() {
 // XW: waves of the workgroup past the WM x WN that compute (PIPE 5,
 // unpaired): they issue their share of the loads and keep the barriers, for
 // tiles narrower than their kernel's workgroup.
+// AT: A is stored with its rows along K (row k holds BM consecutive m), and
+// sits in LDS as B does; its fragments are read transposed. BT: B is stored
+// with its columns as rows (row n holds consecutive k), and sits in LDS as A
+// does, one 16-byte read a fragment. GATED: the tile's columns are BN / 2 of
+// one matrix, then as many of another; a wave's 32-column blocks alternate
+// between the two, so that acc[2j] and acc[2j + 1] hold the same columns of
+// the first and the second.
 template <int BM_, int BN_, int BK_, int STAGES_, int WM_ = 2, int WN_ = 2, int CPA_ = 0, int CPB_ = 0, int PIPE_ = 0,
-          int EPI_PARTS_ = 1, int APAIR_ = 0, int BSTAGES_ = 0, int XW_ = 0>
+          int EPI_PARTS_ = 1, int APAIR_ = 0, int BSTAGES_ = 0, int XW_ = 0, int AT_ = 0, int BT_ = 0,
+          int GATED_ = 0>
 struct DmaCfg {
   static constexpr int BM = BM_, BN = BN_, BK = BK_, STAGES = STAGES_;
   static constexpr int BSTAGES = BSTAGES_ > 0 ? BSTAGES_ : STAGES_;
@@ -106,6 +115,7 @@ struct DmaCfg {
   static constexpr int PIPE = PIPE_;
   static constexpr int EPI_PARTS = EPI_PARTS_;
   static constexpr bool APAIR = APAIR_ != 0;
+  static constexpr bool AT = AT_ != 0, BT = BT_ != 0, GATED = GATED_ != 0;
   static constexpr int WM = WM_, WN = WN_;
   static constexpr int kComputeWaves = WM * WN;
   static constexpr int kWaves = kComputeWaves + XW_;
@@ -113,16 +123,20 @@ struct DmaCfg {
   static constexpr int WTM = BM / WM, WTN = BN / WN;
   static constexpr int TM = WTM / 32, TN = WTN / 32;
   static constexpr int kABK = APAIR ? 2 * BK : BK;  // K width of one A slot
-  static constexpr int kARowBytes = kABK * 2;
-  static constexpr int kAChunksPerRow = kABK / 8;
+  static constexpr int kARowBytes = AT ? BM * 2 : kABK * 2;
+  static constexpr int kAChunksPerRow = kARowBytes / 16;
+  static constexpr int kARows = AT ? BK : BM;
   // DMA instructions per wave for one A slot, and its area. When BM rows do
   // not split into whole 1 KB rows per wave, the area is rounded up: the
   // DMA rows past BM are loaded out of range (zeros, no memory read) and
   // never read back.
-  static constexpr int kAInstr = (BM * kARowBytes + 1024 * kWaves - 1) / (1024 * kWaves);
+  static constexpr int kAInstr = (kARows * kARowBytes + 1024 * kWaves - 1) / (1024 * kWaves);
   static constexpr int kABytes = kAInstr * kWaves * 1024;
-  static constexpr int kBRowBytes = BN * 2;
-  static constexpr int kBBytes = BK * kBRowBytes;
+  static constexpr int kBRowBytes = BT ? BK * 2 : BN * 2;
+  static constexpr int kBRows = BT ? BN : BK;
+  static constexpr int kBBytes = kBRows * kBRowBytes;
+  // LDS reads of a 16-deep sub-step's fragments, per lane.
+  static constexpr int kFragReads = (AT ? 2 : 1) * TM + (BT ? 1 : 2) * TN;
   static constexpr int kStageBytes = kABytes + kBBytes;
   static constexpr int kLdsBytes =
       APAIR ? 2 * kABytes + STAGES * kBBytes : (SPLIT ? STAGES * kABytes + BSTAGES * kBBytes : STAGES * kStageBytes);
@@ -142,12 +156,16 @@ struct DmaCfg {
   static constexpr int kARowsPerInstr = 1024 / kARowBytes;
   static constexpr int kBRowsPerInstr = kBRowBytes >= 1024 ? 1 : 1024 / kBRowBytes;
   static_assert(kBRowBytes <= 1024, "one DMA row per instruction at most");
-  static constexpr int kBChunksPerRow = BN / 8;
+  static constexpr int kBChunksPerRow = kBRowBytes / 16;
+  static_assert(!AT || (!APAIR && kARowBytes <= 1024 && kAInstr * kWaves * 1024 == kARows * kARowBytes &&
+                        (BM == 64 || BM == 128 || BM == 256 || BM == 512)),
+                "A along K splits into whole 1 KB DMA rows");
+  static_assert(!GATED || (TN % 2 == 0 && BN >= 128 && !BT), "gated tiles: pairs of column blocks");
   static_assert(BK == 32 || BK == 64, "BK");
   static_assert(XW_ == 0 || (PIPE == 5 && !APAIR && !SPLIT), "load-only waves: run_xs");
   static_assert(BN == 64 || BN == 128 || BN == 256 || BN == 512, "BN");
   static_assert(WTM % 32 == 0 && WTN % 32 == 0, "waves own whole 32 x 32 blocks");
-  static_assert(kAInstr >= 1 && kABytes >= BM * kARowBytes, "the A area holds BM rows");
+  static_assert(kAInstr >= 1 && kABytes >= kARows * kARowBytes, "the A area holds its rows");
   static_assert(kBInstr >= 1 && kBInstr * kWaves * 1024 == kBBytes, "B step splits into whole 1 KB DMA rows");
   static_assert(STAGES >= 2 && STAGES <= 8, "STAGES");
   static_assert(kLdsAlloc <= 160 * 1024, "LDS");
@@ -217,6 +235,38 @@ struct BDmaPos {
       row[q] = Cfg::kBRowsPerInstr * (Cfg::kBInstr * wave + q) + lane / Cfg::kBChunksPerRow;
       const int p = lane % Cfg::kBChunksPerRow;
       col[q] = 8 * (p ^ (4 * swz_b<Cfg::BN>(row[q])));
+    }
+  }
+};
+
+// The same for A stored along K: lane rows are k, columns 8 consecutive m.
+template <class Cfg>
+struct AtDmaPos {
+  int row[Cfg::kAInstr];
+  int col[Cfg::kAInstr];
+  __device__ __forceinline__ AtDmaPos() {
+    static_assert(Cfg::AT, "A along K");
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int q = 0; q < Cfg::kAInstr; ++q) {
+      row[q] = Cfg::kARowsPerInstr * (Cfg::kAInstr * wave + q) + lane / Cfg::kAChunksPerRow;
+      col[q] = 8 * ((lane % Cfg::kAChunksPerRow) ^ (4 * swz_b<Cfg::BM>(row[q])));
+    }
+  }
+};
+
+// And for B stored with its columns as rows: lane rows are n, chunks 8 consecutive k.
+template <class Cfg>
+struct BtDmaPos {
+  int row[Cfg::kBInstr];
+  int chunk[Cfg::kBInstr];
+  __device__ __forceinline__ BtDmaPos() {
+    static_assert(Cfg::BT, "B's columns as rows");
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int q = 0; q < Cfg::kBInstr; ++q) {
+      row[q] = Cfg::kBRowsPerInstr * (Cfg::kBInstr * wave + q) + lane / Cfg::kBChunksPerRow;
+      chunk[q] = (lane % Cfg::kBChunksPerRow) ^ swz_a<Cfg::BK>(row[q]);
     }
   }
 };
@@ -398,7 +448,11 @@ struct DmaMainloop {
   //   W side (MFMA src A): lane j of its 16-group reads row (k0 + j/4),
   //   columns n0 + 16 (group % 2) + 4 (j % 4); chunk block (4 chunks =
   //   64 B) of n block jn is XORed with (k & 3) = j / 4.
-  struct Frags {
+  struct BtSwizzles {
+    int b_swz[Cfg::TN];
+  };
+  struct NoBtSwizzles {};
+  struct Frags : std::conditional_t<Cfg::BT, BtSwizzles, NoBtSwizzles> {
     int a_row_off[Cfg::TM], a_swz[Cfg::TM], b_off[Cfg::TN];
     int h;
     __device__ __forceinline__ Frags() {
@@ -407,23 +461,46 @@ struct DmaMainloop {
       h = lane >> 5;
 #pragma unroll
       for (int i = 0; i < Cfg::TM; ++i) {
-        const int r = wm * Cfg::WTM + 32 * i + (lane & 31);
-        a_row_off[i] = r * Cfg::kARowBytes;
-        a_swz[i] = swz_a<Cfg::kABK>(r);
+        if constexpr (Cfg::AT) {
+          const int blk = (wm * Cfg::WTM) / 32 + i;  // 32-row block index
+          const int ag = lane >> 4, aj = lane & 15;
+          const int arow = 8 * (ag >> 1) + (aj >> 2);
+          const int chunk = 4 * (blk ^ swz_b<Cfg::BM>(arow)) + 2 * (ag & 1) + ((aj & 3) >> 1);
+          a_row_off[i] = arow * Cfg::kARowBytes + chunk * 16 + (aj & 1) * 8;
+        } else {
+          const int r = wm * Cfg::WTM + 32 * i + (lane & 31);
+          a_row_off[i] = r * Cfg::kARowBytes;
+          a_swz[i] = swz_a<Cfg::kABK>(r);
+        }
       }
       const int g = lane >> 4, jj = lane & 15;
       const int krow = 8 * (g >> 1) + (jj >> 2);
 #pragma unroll
       for (int jn = 0; jn < Cfg::TN; ++jn) {
-        const int blk = (wn * Cfg::WTN) / 32 + jn;  // 32-column block index
-        const int chunk = 4 * (blk ^ swz_b<Cfg::BN>(krow)) + 2 * (g & 1) + ((jj & 3) >> 1);
-        b_off[jn] = krow * Cfg::kBRowBytes + chunk * 16 + (jj & 1) * 8;
+        if constexpr (Cfg::BT) {
+          const int r = wn * Cfg::WTN + 32 * jn + (lane & 31);
+          b_off[jn] = r * Cfg::kBRowBytes;
+          this->b_swz[jn] = swz_a<Cfg::BK>(r);
+        } else {
+          // 32-column block index
+          const int blk = Cfg::GATED ? (jn & 1) * (Cfg::BN / 64) + wn * (Cfg::TN / 2) + jn / 2
+                                     : (wn * Cfg::WTN) / 32 + jn;
+          const int chunk = 4 * (blk ^ swz_b<Cfg::BN>(krow)) + 2 * (g & 1) + ((jj & 3) >> 1);
+          b_off[jn] = krow * Cfg::kBRowBytes + chunk * 16 + (jj & 1) * 8;
+        }
       }
     }
     // Sub-step s's A fragment of row group i (K half `khalf` of a paired slot).
     __device__ __forceinline__ bf16x8_t read_a1(const uint8_t* __restrict__ as, int khalf, int s, int i) const {
-      const int kc = 4 * khalf + h;
-      return *reinterpret_cast<const bf16x8_t*>(as + a_row_off[i] + (((2 * s + kc) ^ a_swz[i]) << 4));
+      if constexpr (Cfg::AT) {
+        const uint8_t* p = as + a_row_off[i] + 16 * s * Cfg::kARowBytes;
+        const i16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t*)(p));
+        const i16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t*)(p + 4 * Cfg::kARowBytes));
+        return __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+      } else {
+        const int kc = 4 * khalf + h;
+        return *reinterpret_cast<const bf16x8_t*>(as + a_row_off[i] + (((2 * s + kc) ^ a_swz[i]) << 4));
+      }
     }
     __device__ __forceinline__ void read_a(const uint8_t* __restrict__ as, int khalf, int s,
                                            bf16x8_t (&a)[Cfg::TM]) const {
@@ -433,10 +510,14 @@ struct DmaMainloop {
     __device__ __forceinline__ void read_b(const uint8_t* __restrict__ bs, int s, bf16x8_t (&b)[Cfg::TN]) const {
 #pragma unroll
       for (int jn = 0; jn < Cfg::TN; ++jn) {
-        const uint8_t* p = bs + b_off[jn] + 16 * s * Cfg::kBRowBytes;
-        const i16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t*)(p));
-        const i16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t*)(p + 4 * Cfg::kBRowBytes));
-        b[jn] = __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+        if constexpr (Cfg::BT) {
+          b[jn] = *reinterpret_cast<const bf16x8_t*>(bs + b_off[jn] + (((2 * s + h) ^ this->b_swz[jn]) << 4));
+        } else {
+          const uint8_t* p = bs + b_off[jn] + 16 * s * Cfg::kBRowBytes;
+          const i16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t*)(p));
+          const i16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t*)(p + 4 * Cfg::kBRowBytes));
+          b[jn] = __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+        }
       }
     }
   };
@@ -489,7 +570,7 @@ struct DmaMainloop {
     }
     if constexpr (Cfg::PIPE == 3) {
       constexpr int kMfma = Cfg::TM * Cfg::TN;
-      constexpr int kReads = Cfg::TM + 2 * Cfg::TN;
+      constexpr int kReads = Cfg::kFragReads;
       constexpr int kPer = (kReads + kMfma - 1) / kMfma;
       constexpr int kDma = Dma::kCount;
       bf16x8_t a[2][Cfg::TM], b[2][Cfg::TN];
@@ -538,7 +619,7 @@ struct DmaMainloop {
         // Interleave: the first sub-step's reads, then per later sub-step
         // its MFMAs alternating with the next sub-step's reads.
         constexpr int kMfma = Cfg::TM * Cfg::TN;
-        constexpr int kReads = Cfg::TM + 2 * Cfg::TN;
+        constexpr int kReads = Cfg::kFragReads;
         constexpr int kPer = (kReads + kMfma - 1) / kMfma;
         __builtin_amdgcn_sched_group_barrier(0x100, kReads, 0);  // DS reads of sub-step 0
 #pragma unroll
@@ -569,7 +650,7 @@ struct DmaMainloop {
     constexpr int kSub = Cfg::BK / 16;
     static_assert(kSub % 2 == 0, "the last sub-step uses the second register set");
     constexpr int kMfma = Cfg::TM * Cfg::TN;
-    constexpr int kReads = Cfg::TM + 2 * Cfg::TN;
+    constexpr int kReads = Cfg::kFragReads;
     constexpr int kPer = (kReads + kMfma - 1) / kMfma;
     constexpr int kDma = Dma::kCount;
     auto mfmas = [&](const bf16x8_t (&fa)[Cfg::TM], const bf16x8_t (&fb)[Cfg::TN]) { DmaMainloop::mfmas(acc, fa, fb); };

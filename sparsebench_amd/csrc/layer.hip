@@ -8,24 +8,12 @@
 // stages' entry points, so results and checks are theirs.
 
 #include "common.hpp"
+#include "workspace.hpp"
 
 namespace sb {
 namespace {
 
 constexpr int64_t kBlock = 128;
-constexpr int64_t kI32Limit = int64_t{1} << 31;
-
-// Hands out 256-byte aligned pieces of a workspace; with no base it only adds up.
-struct Carver {
-  uint8_t* base;
-  int64_t used = 0;
-  template <class T>
-  T* take(int64_t count) {
-    T* p = base ? reinterpret_cast<T*>(base + used) : nullptr;
-    used += (count * static_cast<int64_t>(sizeof(T)) + 255) / 256 * 256;
-    return p;
-  }
-};
 
 // A routing layout (sb_routing's outputs) and the blocks of H and rows of y on it.
 struct LayerBuffers {
@@ -99,15 +87,6 @@ int carve_rounded(Carver& ws, int64_t num_tokens, int32_t num_experts, int32_t k
   b->weight_of_copy = ws.take<float>(b->capacity);
   b->num_assignments = ws.take<int32_t>(1);
   b->token_offsets = ws.take<int32_t>(num_tokens + 1);
-  return SB_OK;
-}
-
-int check_workspace(const void* workspace, int64_t workspace_bytes, int64_t needed) {
-  if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255u) != 0)
-    return fail(SB_ERR_INVALID, "layer: the workspace must be 256-byte aligned");
-  if (workspace_bytes < needed)
-    return fail(SB_ERR_INVALID, "layer: workspace of %lld bytes, %lld needed", static_cast<long long>(workspace_bytes),
-                static_cast<long long>(needed));
   return SB_OK;
 }
 

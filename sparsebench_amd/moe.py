@@ -11,6 +11,8 @@ real size from padded_offsets / row_offsets on the GPU.
 from __future__ import annotations
 
 from collections.abc import Callable
+from dataclasses import dataclass
+from typing import NamedTuple
 
 import torch
 
@@ -208,3 +210,85 @@ def moe_forward_rounded(
             return out
     routing = route_rounded(scores, k, ffn_dim, BLOCK_SIZE, tile)
     return _assigned_layer(x, routing, routing.weight_of_copy, w1, w2, mark, None)
+
+
+# ---- gated experts: forward, and forward and backward for training ----
+
+
+def moe_forward_gated(
+    x: torch.Tensor,
+    expert_idx: torch.Tensor,
+    expert_weight: torch.Tensor,
+    w1: torch.Tensor,
+    w2: torch.Tensor,
+    activation: str = "silu",
+    valid_tokens: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """moe_forward with gated experts: H = a(x @ gate) * (x @ up), out = sum_j w_j (H @ w2).
+
+    x [T, D], expert_idx / expert_weight [T, k], w1 [E, D, 2F] (each expert's
+    gate columns, then its up columns), w2 [E, F, D] -> [T, D], all bf16 but
+    the ids (int32 / int64) and the weights (bf16 / fp16 / fp32). activation:
+    "silu" or "gelu" (the erf form). D and F are multiples of 128. Like
+    moe_forward, an id outside [0, E) adds nothing, valid_tokens restricts
+    the layer to the first T' tokens, and nothing syncs: the call can be
+    captured in a graph.
+    """
+    from sparsebench_amd import _C
+
+    return _C.gated_layer_cuda(x, expert_idx, expert_weight, w1, w2, activation, valid_tokens)
+
+
+@dataclass(frozen=True)
+class GatedSaved:
+    """What moe_gated_backward needs of a moe_gated_train call: its operands,
+    which must not change in between, and what the forward pass kept of the
+    routing and of its intermediates (`kept`, in the library's own layout)."""
+
+    x: torch.Tensor
+    expert_weight: torch.Tensor
+    w1: torch.Tensor
+    w2: torch.Tensor
+    activation: str
+    valid_tokens: torch.Tensor | None
+    kept: torch.Tensor
+
+
+class GatedGrads(NamedTuple):
+    """Gradients of moe_gated_train's operands, each of its operand's shape and dtype."""
+
+    x: torch.Tensor
+    expert_weight: torch.Tensor
+    w1: torch.Tensor
+    w2: torch.Tensor
+
+
+def moe_gated_train(
+    x: torch.Tensor,
+    expert_idx: torch.Tensor,
+    expert_weight: torch.Tensor,
+    w1: torch.Tensor,
+    w2: torch.Tensor,
+    activation: str = "silu",
+    valid_tokens: torch.Tensor | None = None,
+) -> tuple[torch.Tensor, GatedSaved]:
+    """moe_forward_gated for training: (its output, what moe_gated_backward
+    takes). It keeps G = x @ gate and U = x @ up and each copy's expert output
+    in bf16, 2 (2 F + D) bytes a routed copy. No autograd graph is built."""
+    from sparsebench_amd import _C
+
+    out, kept = _C.gated_train_cuda(x, expert_idx, expert_weight, w1, w2, activation, valid_tokens)
+    return out, GatedSaved(x, expert_weight, w1, w2, activation, valid_tokens, kept)
+
+
+def moe_gated_backward(saved: GatedSaved, grad_out: torch.Tensor) -> GatedGrads:
+    """The gradients of a moe_gated_train call's operands, from the gradient
+    [T, D] bf16 of its output. Nothing syncs, no sum's order changes from call
+    to call, and `saved` may be used again. Copies that were not routed (an id
+    out of range) have gradient 0, as have the weights of experts without
+    tokens; rows t >= valid_tokens of the gradients of x and expert_weight are
+    left unwritten."""
+    from sparsebench_amd import _C
+
+    return GatedGrads(*_C.gated_backward_cuda(grad_out, saved.x, saved.expert_weight, saved.w1, saved.w2, saved.kept,
+                                              saved.activation, saved.valid_tokens))
