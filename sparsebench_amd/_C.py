@@ -18,6 +18,8 @@ import array
 import contextlib
 import ctypes
 import functools
+import itertools
+import operator
 
 import torch
 
@@ -790,12 +792,36 @@ def gated_backward_cuda(grad_out: torch.Tensor, x: torch.Tensor, expert_weight: 
 QUANT_BLOCK = 256
 
 
-def _check_state(p: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype, name: str) -> None:
-    if codes.dtype != dtype or codes.numel() != p.numel() or not codes.is_contiguous() or codes.device != p.device:
-        _fail(f"{name} codes must be contiguous {dtype} of the parameter's length, on its GPU")
-    if (scales.dtype != torch.float32 or scales.numel() != -(-p.numel() // QUANT_BLOCK)
-            or not scales.is_contiguous() or scales.device != p.device):
-        _fail(f"{name} scales must be contiguous float32, one for each {QUANT_BLOCK} values, on the parameter's GPU")
+_dtype_of, _shape_of = operator.attrgetter("dtype"), operator.attrgetter("shape")
+_addresses = functools.partial(map, torch.Tensor.data_ptr)
+_lengths = functools.partial(map, torch.Tensor.numel)
+
+
+def _check_list(tensors, device: int, what: str, dtype: torch.dtype | None = None, lengths=None) -> None:
+    """All contiguous, on GPU `device`, of one dtype and of these lengths, if given. (Whole
+    lists at a time: a step of many small tensors is bound by these checks.)"""
+    if not set(map(torch.Tensor.get_device, tensors)) <= {device}:
+        _fail(f"{what} must be on the step's GPU")
+    if not all(map(torch.Tensor.is_contiguous, tensors)):
+        _fail(f"{what} must be contiguous")
+    if dtype is not None and not set(map(_dtype_of, tensors)) <= {dtype}:
+        _fail(f"{what} must be {dtype}")
+    if lengths is not None and list(_lengths(tensors)) != lengths:
+        _fail(f"{what} must have the parameters' lengths")
+
+
+def _state_lists(states, eight: bool, signed: bool, name: str, device: int, lengths: list[int]):
+    """(values or codes, scales or None) of a list of states, checked."""
+    if any(isinstance(s, torch.Tensor) == eight for s in states):
+        _fail("all states must be of one kind: float32 tensors, or 8-bit codes and scales")
+    if not eight:
+        _check_list(states, device, f"float32 states ({name})", torch.float32, lengths)
+        return states, None
+    codes, scales = [s[0] for s in states], [s[1] for s in states]
+    _check_list(codes, device, f"{name} codes", torch.int8 if signed else torch.uint8, lengths)
+    _check_list(scales, device, f"{name} scales (one for each {QUANT_BLOCK} values)", torch.float32,
+                [-(-n // QUANT_BLOCK) for n in lengths])
+    return codes, scales
 
 
 def _device_scalar(t, name: str, device: torch.device) -> int | None:
@@ -817,37 +843,27 @@ def adamw_cuda(params, grads, masters, exp_avgs, exp_avg_sqs, step: torch.Tensor
         _fail("params, grads, masters and states must be lists of one length")
     if not (step.is_cuda and step.dtype == torch.int32 and step.numel() == 2 and step.is_contiguous()):
         _fail("step must be a contiguous int32 CUDA tensor of two elements")
-    dev = step.device
+    dev, index = step.device, step.get_device()
     eight = n > 0 and not isinstance(exp_avgs[0], torch.Tensor)
-    words = array.array("q")
-    for i in range(n):
-        p, g, m, v = params[i], grads[i], exp_avgs[i], exp_avg_sqs[i]
-        count = p.numel()
-        p_code, g_code = _GATE_DTYPES.get(p.dtype), _GATE_DTYPES.get(g.dtype)
-        if p_code is None or g_code is None:
-            _fail(f"parameters and gradients must be bfloat16, float16 or float32, got {p.dtype} and {g.dtype}")
-        if p.device != dev or g.device != dev or g.shape != p.shape:
-            _fail("each gradient must have its parameter's shape, all on the step's GPU")
-        if not (p.is_contiguous() and g.is_contiguous()):
-            _fail("parameters and gradients must be contiguous")
-        w = 0
-        if masters is not None:
-            t = masters[i]
-            if t.dtype != torch.float32 or t.shape != p.shape or t.device != dev or not t.is_contiguous():
-                _fail("each master must be contiguous float32 of its parameter's shape, on its GPU")
-            w = t.data_ptr()
-        if isinstance(m, torch.Tensor) == eight or isinstance(v, torch.Tensor) == eight:
-            _fail("all states must be of one kind: float32 tensors, or 8-bit codes and scales")
-        if eight:
-            _check_state(p, *m, torch.int8, "exp_avg")
-            _check_state(p, *v, torch.uint8, "exp_avg_sq")
-            state = m[0].data_ptr(), v[0].data_ptr(), m[1].data_ptr(), v[1].data_ptr()
-        else:
-            for t in (m, v):
-                if t.dtype != torch.float32 or t.shape != p.shape or t.device != dev or not t.is_contiguous():
-                    _fail("each float32 state must be contiguous, of its parameter's shape, on its GPU")
-            state = m.data_ptr(), v.data_ptr(), 0, 0
-        words.extend((p.data_ptr(), g.data_ptr(), w, *state, count, p_code | g_code << 32))
+    _check_list(params, index, "parameters")
+    _check_list(grads, index, "gradients")
+    if list(map(_shape_of, params)) != list(map(_shape_of, grads)):
+        _fail("each gradient must have its parameter's shape")
+    lengths = list(_lengths(params))
+    if masters is not None:
+        _check_list(masters, index, "masters", torch.float32, lengths)
+    m, m_scales = _state_lists(exp_avgs, eight, True, "exp_avg", index, lengths)
+    v, v_scales = _state_lists(exp_avg_sqs, eight, False, "exp_avg_sq", index, lengths)
+    try:
+        codes = [_GATE_DTYPES[p] | _GATE_DTYPES[g] << 32
+                 for p, g in zip(map(_dtype_of, params), map(_dtype_of, grads))]
+    except KeyError as e:
+        _fail(f"parameters and gradients must be bfloat16, float16 or float32, got {e.args[0]}")
+    none = itertools.repeat(0)
+    words = array.array("q", itertools.chain.from_iterable(zip(
+        _addresses(params), _addresses(grads), none if masters is None else _addresses(masters), _addresses(m),
+        _addresses(v), _addresses(m_scales) if eight else none, _addresses(v_scales) if eight else none, lengths,
+        codes)))
     lr_ptr, scale_ptr = _device_scalar(lr, "lr", dev), _device_scalar(grad_scale, "grad_scale", dev)
     with _device_of(step):
         if scale_ptr is None and grad_scale is not None:  # a number: as a device scalar
@@ -867,17 +883,20 @@ def dequantize_cuda(pairs, dtype: torch.dtype) -> list[torch.Tensor]:
     dev = pairs[0][0].device
     if dev.type != "cuda":
         _fail("codes must be CUDA tensors")
+    lengths = [codes.numel() for codes, _ in pairs]
+    _check_list([codes for codes, _ in pairs], dev.index, "codes")
+    _check_list([scales for _, scales in pairs], dev.index, f"scales (one for each {QUANT_BLOCK} values)", torch.float32,
+                [-(-n // QUANT_BLOCK) for n in lengths])
     # Each value list starts at a multiple of 16 bytes of one buffer.
     step = 16 // dtype.itemsize
     starts, total = [], 0
-    for codes, scales in pairs:
-        if codes.dtype not in (torch.int8, torch.uint8) or codes.device != dev:
-            _fail("codes must be int8 or uint8 tensors on one GPU")
-        _check_state(codes, codes, scales, codes.dtype, "state")
+    for (codes, _), n in zip(pairs, lengths):
+        if codes.dtype not in (torch.int8, torch.uint8):
+            _fail(f"codes must be int8 or uint8, got {codes.dtype}")
         starts.append(total)
-        total += -(-codes.numel() // step) * step
+        total += -(-n // step) * step
     flat = torch.empty(total, dtype=dtype, device=dev)
-    out = [flat[a:a + codes.numel()].view(codes.shape) for a, (codes, _) in zip(starts, pairs)]
+    out = [flat[a:a + n].view(codes.shape) for a, n, (codes, _) in zip(starts, lengths, pairs)]
     words = array.array("q")
     for (codes, scales), o in zip(pairs, out):
         words.extend((codes.data_ptr(), scales.data_ptr(), o.data_ptr(), codes.numel(),

@@ -171,7 +171,7 @@ def test_adamw_operands_are_refused() -> None:
         (([p], [p, p], [m], [v], step, 0.1), "one length"),
         (([p], [p.double()], [m], [v], step, 0.1), "bfloat16"),
         (([p[::2]], [p[::2]], [m[:256]], [v[:256]], step, 0.1), "contiguous"),
-        (([p], [p], [m.bfloat16()], [v], step, 0.1), "float32 state"),
+        (([p], [p], [m.bfloat16()], [v], step, 0.1), "float32 states"),
         (([p], [p], [m], [v8], step, 0.1), "one kind"),
         (([p], [p], [v8], [m8], step, 0.1), "codes"),
         (([p], [p], [optim.Quantized(m8.codes, m8.scales[:1])], [v8], step, 0.1), "scales"),
