@@ -19,47 +19,47 @@
 namespace sb {
 namespace {
 
-template <class Cfg, bool kWideX, bool kKeep, int ACT>
-__global__ void __launch_bounds__(Cfg::kThreads)
-    gated_up_kernel(const uint16_t* __restrict__ x, const uint16_t* __restrict__ w1, GatedLayout layout,
-                    uint16_t* __restrict__ h, uint16_t* __restrict__ gu, int32_t num_tokens, int32_t d_model,
-                    int32_t ffn_dim) {
-  using ML = DmaMainloop<Cfg>;
-  constexpr int kHalf = Cfg::BN / 2;  // columns of F
-  static_assert(Cfg::BM == kBS && Cfg::GATED && Cfg::EPI_PARTS == 1, "one row block per tile");
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[Cfg::kLdsAlloc];
-  const int slices = ffn_dim / kHalf;
-  RowBlock b;
-  int slice;
-  if (!row_block_tile(static_cast<int>(blockIdx.x), slices, layout, kTileGroup, &b, &slice)) return;
-  const int n0 = slice * kHalf;
+struct UpArgs {
+  const uint16_t *x, *w1;
+  GatedLayout layout;
+  uint16_t *h, *gu;
+  int32_t num_tokens, d_model, ffn_dim;
+};
 
+// Rows ch of H and (kKeep) G | U, their columns n0 .. n0 + BN / 2 of F.
+template <class Cfg, bool kWideX, bool kKeep, int ACT>
+__device__ __forceinline__ void gated_up_tile(uint8_t* __restrict__ lds, const UpArgs& a, const Chunk& ch, int n0) {
+  using ML = DmaMainloop<Cfg>;
+  constexpr int kHalf = Cfg::BN / 2;
+  static_assert(Cfg::GATED && Cfg::EPI_PARTS == 1, "gated tiles");
   SddDmaSrc<Cfg, kWideX> src;
-  src.x_rsrc = make_rsrc(x, kWideX ? 0u : static_cast<uint32_t>(num_tokens) * static_cast<uint32_t>(d_model) * 2u);
-  src.w_rsrc = make_rsrc(w1 + static_cast<int64_t>(b.expert) * d_model * (2 * static_cast<int64_t>(ffn_dim)),
-                         static_cast<uint32_t>(d_model) * static_cast<uint32_t>(ffn_dim) * 4u);
-  src.b_step_bytes = static_cast<uint32_t>(Cfg::BK) * static_cast<uint32_t>(ffn_dim) * 4u;
+  src.x_rsrc =
+      make_rsrc(a.x, kWideX ? 0u : static_cast<uint32_t>(a.num_tokens) * static_cast<uint32_t>(a.d_model) * 2u);
+  src.w_rsrc = make_rsrc(a.w1 + static_cast<int64_t>(ch.expert) * a.d_model * (2 * static_cast<int64_t>(a.ffn_dim)),
+                         static_cast<uint32_t>(a.d_model) * static_cast<uint32_t>(a.ffn_dim) * 4u);
+  src.b_step_bytes = static_cast<uint32_t>(Cfg::BK) * static_cast<uint32_t>(a.ffn_dim) * 4u;
   const ADmaPos<Cfg> ap;
 #pragma unroll
   for (int q = 0; q < Cfg::kAInstr; ++q) {
-    const int32_t tok = ap.row[q] < b.rows ? layout.row_token[b.row0 + ap.row[q]] : -1;
-    src.set_row(q, tok < num_tokens ? tok : -1, ap.chunk[q], x, d_model);
+    const int32_t tok = ap.row[q] < ch.rows ? a.layout.row_token[ch.row0 + ap.row[q]] : -1;
+    src.set_row(q, tok < a.num_tokens ? tok : -1, ap.chunk[q], a.x, a.d_model);
   }
   const BDmaPos<Cfg> bp;
 #pragma unroll
   for (int q = 0; q < Cfg::kBInstr; ++q) {
-    const int col = bp.col[q] < kHalf ? n0 + bp.col[q] : ffn_dim + n0 + bp.col[q] - kHalf;
-    src.b_off[q] = (static_cast<uint32_t>(bp.row[q]) * (2 * ffn_dim) + col) * 2u;
+    const int col = bp.col[q] < kHalf ? n0 + bp.col[q] : a.ffn_dim + n0 + bp.col[q] - kHalf;
+    src.b_off[q] = (static_cast<uint32_t>(bp.row[q]) * (2 * a.ffn_dim) + col) * 2u;
   }
 
   typename ML::Acc acc;
-  ML::run(lds, src, d_model / Cfg::BK, acc);
+  ML::run(lds, src, a.d_model / Cfg::BK, acc);
 
   // Staged as bf16 rows of kHalf columns: G, then U below it, then (over
   // both) H; each written row by row in 16-byte chunks.
   const int lane = threadIdx.x & 63, wn = (threadIdx.x >> 6) % Cfg::WN;
   constexpr int kRowBytes = kHalf * 2;
   auto stage = [&](int base, auto value) {
+    if (!ML::computes()) return;
 #pragma unroll
     for (int j = 0; j < Cfg::TN / 2; ++j)
 #pragma unroll
@@ -78,7 +78,7 @@ __global__ void __launch_bounds__(Cfg::kThreads)
   };
   constexpr int kChunksPerRow = kHalf / 8;
   auto write = [&](int base, auto to) {
-    for (int q = threadIdx.x; q < b.rows * kChunksPerRow; q += Cfg::kThreads) {
+    for (int q = threadIdx.x; q < ch.rows * kChunksPerRow; q += Cfg::kThreads) {
       const int r = q / kChunksPerRow, c = q % kChunksPerRow;
       *reinterpret_cast<u32x4_t*>(to(r, c * 8)) =
           *reinterpret_cast<const u32x4_t*>(lds + base + staged_at<kRowBytes>(r, c));
@@ -86,77 +86,85 @@ __global__ void __launch_bounds__(Cfg::kThreads)
   };
   __syncthreads();  // every wave is done reading the ring
   if constexpr (kKeep) {
-    constexpr int kUp = kBS * kRowBytes;
+    constexpr int kUp = Cfg::BM * kRowBytes;
     stage(0, [](float g, float) { return g; });
     stage(kUp, [](float, float u) { return u; });
     __syncthreads();
-    uint16_t* rows = gu + static_cast<int64_t>(b.row0) * 2 * ffn_dim + n0;
-    write(0, [&](int r, int col) { return rows + static_cast<int64_t>(r) * 2 * ffn_dim + col; });
-    write(kUp, [&](int r, int col) { return rows + static_cast<int64_t>(r) * 2 * ffn_dim + ffn_dim + col; });
+    uint16_t* rows = a.gu + static_cast<int64_t>(ch.row0) * 2 * a.ffn_dim + n0;
+    write(0, [&](int r, int col) { return rows + static_cast<int64_t>(r) * 2 * a.ffn_dim + col; });
+    write(kUp, [&](int r, int col) { return rows + static_cast<int64_t>(r) * 2 * a.ffn_dim + a.ffn_dim + col; });
     __syncthreads();
   }
   stage(0, [](float g, float u) { return gated_act<ACT>(g) * u; });
   __syncthreads();
-  uint16_t* blocks = h + static_cast<int64_t>(b.row0) * ffn_dim;  // the row block's first BSR block
+  uint16_t* blocks = a.h + static_cast<int64_t>(ch.row0) * a.ffn_dim;  // the first row block's first BSR block
   write(0, [&](int r, int col) {
     const int f = n0 + col;
-    return blocks + static_cast<int64_t>(f / kBS) * kBS * kBS + r * kBS + f % kBS;
+    return blocks + static_cast<int64_t>(r / kBS) * kBS * a.ffn_dim + static_cast<int64_t>(f / kBS) * kBS * kBS +
+           (r % kBS) * kBS + f % kBS;
   });
 }
 
-// The per-row-block SDD's tile shapes, gated: 512 columns (256 of F), and 256
-// and 128 where F or the number of tiles asks for narrower ones.
-using GatedWide = DmaCfg<128, 512, 32, 3, 2, 4, 0, 2, 3, 1, 1, 0, 0, 0, 0, 1>;
-using GatedMid = DmaCfg<128, 256, 64, 3, 2, 4, 0, 2, 3, 1, 0, 0, 0, 0, 0, 1>;
-using GatedNarrow = DmaCfg<128, 128, 64, 3, 2, 2, 0, 2, 5, 1, 0, 0, 0, 0, 0, 1>;
+template <class Cfg, bool kWideX, bool kKeep, int ACT>
+__global__ void __launch_bounds__(Cfg::kThreads) gated_up_kernel(UpArgs a) {
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[Cfg::kLdsAlloc];
+  Chunk ch;
+  int slice;
+  if (!row_block_tile(static_cast<int>(blockIdx.x), a.ffn_dim / (Cfg::BN / 2), a.layout, &ch, &slice)) return;
+  gated_up_tile<Cfg, kWideX, kKeep, ACT>(lds, a, ch, slice * (Cfg::BN / 2));
+}
 
-struct UpArgs {
-  const void *x, *w1;
-  GatedLayout layout;
-  void *h, *gu;
-  int64_t num_tokens, d_model, ffn_dim;
-  hipStream_t stream;
-};
+template <bool kKeep, int ACT>
+__global__ void __launch_bounds__(512) gated_up_chunk_kernel(UpArgs a) {
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[GatedUpCfg<kGatedRmax>::kLdsAlloc];
+  Chunk ch{-1, 0, 0, 0};
+  int slice = 0;
+  if (!gated_chunk_tile(static_cast<int>(blockIdx.x), a.ffn_dim / (kGatedBN / 2), a.layout, &ch, &slice)) return;
+  with_chunk_groups(ch.groups, [&](auto rc) {
+    using Cfg = GatedUpCfg<decltype(rc)::value>;
+    static_assert(Cfg::kLdsAlloc <= sizeof(lds) && Cfg::kThreads == 512, "one workgroup for all heights");
+    gated_up_tile<Cfg, false, kKeep, ACT>(lds, a, ch, slice * (kGatedBN / 2));
+  });
+}
+
+// Row-block tiles: 128 columns (64 of F), and 256 for x of 2 GiB or more,
+// which the chunk form's 32-bit offsets do not reach.
+using GatedNarrow = DmaCfg<128, 128, 64, 3, 2, 2, 0, 2, 5, 1, 0, 0, 0, 0, 0, 1>;
+using GatedMid = DmaCfg<128, 256, 64, 3, 2, 4, 0, 2, 3, 1, 0, 0, 0, 0, 0, 1>;
 
 template <class Cfg, bool kWideX, bool kKeep, int ACT>
-int launch_up(const UpArgs& a) {
-  if (!reduction_fits<Cfg>(a.d_model)) return fail(SB_ERR_INVALID, "gated experts: D is not whole K steps");
-  const int64_t tiles = a.layout.max_row_blocks * (a.ffn_dim / (Cfg::BN / 2));
-  if (tiles > 2147483647LL) return fail(SB_ERR_INVALID, "gated experts: too many tiles");
-  gated_up_kernel<Cfg, kWideX, kKeep, ACT><<<static_cast<uint32_t>(tiles), Cfg::kThreads, 0, a.stream>>>(
-      static_cast<const uint16_t*>(a.x), static_cast<const uint16_t*>(a.w1), a.layout, static_cast<uint16_t*>(a.h),
-      static_cast<uint16_t*>(a.gu), static_cast<int32_t>(a.num_tokens), static_cast<int32_t>(a.d_model),
-      static_cast<int32_t>(a.ffn_dim));
+int launch_up(const UpArgs& a, hipStream_t stream) {
+  const int64_t tiles = int64_t{a.layout.max_row_blocks} * (a.ffn_dim / (Cfg::BN / 2));
+  if (!reduction_fits<Cfg>(a.d_model) || tiles > 2147483647LL) return fail(SB_ERR_INVALID, "problem too large");
+  gated_up_kernel<Cfg, kWideX, kKeep, ACT><<<static_cast<uint32_t>(tiles), Cfg::kThreads, 0, stream>>>(a);
   return check_launch("gated experts");
 }
 
-template <bool kWideX, bool kKeep, int ACT>
-int launch_up_width(const UpArgs& a, int width) {
-  switch (width) {
-    case 512: return launch_up<GatedWide, kWideX, kKeep, ACT>(a);
-    case 256: return launch_up<GatedMid, kWideX, kKeep, ACT>(a);
-    default: return launch_up<GatedNarrow, kWideX, kKeep, ACT>(a);
-  }
-}
-
-template <bool kWideX, bool kKeep>
-int launch_up_act(const UpArgs& a, int width, int32_t act) {
-  return act == SB_ACT_SILU ? launch_up_width<kWideX, kKeep, SB_ACT_SILU>(a, width)
-                            : launch_up_width<kWideX, kKeep, SB_ACT_GELU>(a, width);
+template <bool kKeep, int ACT>
+int launch_up_form(const UpArgs& a, int64_t num_copies, bool chunks, hipStream_t stream) {
+  if (sdd_wide_x(a.num_tokens, a.d_model)) return launch_up<GatedMid, true, kKeep, ACT>(a, stream);
+  if (!chunks) return launch_up<GatedNarrow, false, kKeep, ACT>(a, stream);
+  const int64_t grid = gated_chunk_grid(a.layout, num_copies, a.ffn_dim / (kGatedBN / 2));
+  if (!reduction_fits<GatedUpCfg<kGatedRmax>>(a.d_model) || grid > 2147483647LL)
+    return fail(SB_ERR_INVALID, "problem too large");
+  gated_up_chunk_kernel<kKeep, ACT><<<static_cast<uint32_t>(grid), 512, 0, stream>>>(a);
+  return check_launch("gated experts");
 }
 
 }  // namespace
 
 int launch_gated_up(const void* x, const void* w1, const GatedLayout& layout, void* h, void* gu, int64_t num_tokens,
                     int64_t num_copies, int64_t d_model, int64_t ffn_dim, int32_t act, hipStream_t stream) {
-  int cus = 0;
-  if (const int rc = device_cus(&cus)) return rc;
-  const UpArgs a{x, w1, layout, h, gu, num_tokens, d_model, ffn_dim, stream};
-  // Each live row block holds a copy at least.
-  const int width = fit_width(std::min<int64_t>(layout.max_row_blocks, num_copies), 2 * ffn_dim, cus);
-  if (sdd_wide_x(num_tokens, d_model))
-    return gu ? launch_up_act<true, true>(a, width, act) : launch_up_act<true, false>(a, width, act);
-  return gu ? launch_up_act<false, true>(a, width, act) : launch_up_act<false, false>(a, width, act);
+  const UpArgs a{static_cast<const uint16_t*>(x), static_cast<const uint16_t*>(w1), layout,
+                 static_cast<uint16_t*>(h), static_cast<uint16_t*>(gu), static_cast<int32_t>(num_tokens),
+                 static_cast<int32_t>(d_model), static_cast<int32_t>(ffn_dim)};
+  bool chunks = false;
+  if (const int rc = gated_chunks(layout, num_copies, 2 * ffn_dim, &chunks)) return rc;
+  if (gu)
+    return act == SB_ACT_SILU ? launch_up_form<true, SB_ACT_SILU>(a, num_copies, chunks, stream)
+                              : launch_up_form<true, SB_ACT_GELU>(a, num_copies, chunks, stream);
+  return act == SB_ACT_SILU ? launch_up_form<false, SB_ACT_SILU>(a, num_copies, chunks, stream)
+                            : launch_up_form<false, SB_ACT_GELU>(a, num_copies, chunks, stream);
 }
 
 }  // namespace sb

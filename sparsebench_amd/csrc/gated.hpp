@@ -53,29 +53,129 @@ int launch_sum_copies(const void* y, const int32_t* copy_row, void* out, int64_t
 
 // ------------------------------------------------------------- in tiles ---
 
-// The row block of a tile: its expert, first padded row and real rows (1 .. 128).
-struct RowBlock {
-  int32_t expert, row0, rows;
-};
+// A tile's rows are a Chunk (expert_chunks.hpp): real rows of one expert from
+// a padded row that is a multiple of 128.
+//
+// Two forms, with the same results: row blocks (up to 128 rows, narrow tiles,
+// for grids that leave CUs idle) and chunks of up to 256 rows, 256 columns wide.
 
 // Tile `bid` of max_row_blocks * slices -> (row block, column slice); false
 // past the live row blocks. Live tiles are spread over the XCDs in contiguous
 // ranges, row blocks in groups (tile_coords).
-__device__ __forceinline__ bool row_block_tile(int bid, int slices, const GatedLayout& l, int group, RowBlock* b,
-                                               int* slice) {
+__device__ __forceinline__ bool row_block_tile(int bid, int slices, const GatedLayout& l, Chunk* ch, int* slice) {
   const int live_rb = __builtin_amdgcn_readfirstlane(l.padded_offsets[l.num_experts]) / kBS;
   if (live_rb > l.max_row_blocks || bid >= live_rb * slices) return false;
   int rb;
-  tile_coords(xcd_remap(bid, live_rb * slices), live_rb, slices, group, &rb, slice);
+  tile_coords(xcd_remap(bid, live_rb * slices), live_rb, slices, kTileGroup, &rb, slice);
   const int32_t e = __builtin_amdgcn_readfirstlane(l.row_block_expert[rb]);
   if (e < 0 || e >= l.num_experts) return false;
   const int32_t n = __builtin_amdgcn_readfirstlane(l.tokens_per_expert[e]);
   const int32_t first = rb * kBS - __builtin_amdgcn_readfirstlane(l.padded_offsets[e]);
   if (first < 0 || first >= n) return false;  // not a routing layout
-  b->expert = e;
-  b->row0 = rb * kBS;
-  b->rows = min(n - first, kBS);
+  *ch = Chunk{e, rb * kBS, min(n - first, kBS), 4};
   return true;
+}
+
+// The chunk form's tiles: chunks of 256 rows, the last of up to 320, x slices of 256 columns, 8
+// waves in two rows of 4 (128 x 64 a wave at 256 rows). Each tile is cut to its
+// chunk's rows in steps of R = 2 row groups of 32 (one row of 8 waves would
+// take odd R too, but reads more LDS fragments per MFMA than R + 1 groups in
+// two rows). An expert's weights are streamed once per 256 rows, and padding
+// rows past a chunk's last 64 are neither computed nor read.
+//   gated (W1, its rows along K): K steps of 32 through a 4-stage ring, A two
+//     steps at a time (APAIR).
+//   BT (rows of W1 or W2 as columns): K steps of 64, since a row's piece of 32
+//     is half a cache line (D = 4096, F = 14336, 512 rows an expert: 1592 us
+//     with steps of 32); 160 KB hold 2 stages of A and 3 of B at R = 8.
+constexpr int kGatedRmax = 10, kGatedBN = 256;
+template <int R>
+using GatedUpCfg = DmaCfg<32 * R, kGatedBN, 32, 4, 2, 4, 0, 2, 5, 1, 1, 0, 0, 0, 0, 1>;
+template <int R>
+using BtChunkCfg = std::conditional_t<
+    (R >= 6), DmaCfg<32 * R, kGatedBN, 64, 2, 2, 4, 0, 0, 5, 1, 0, (R <= 8 ? 3 : 0), 0, 0, 1>,
+    DmaCfg<32 * R, kGatedBN, 64, (R == 4 ? 3 : 4), 2, 4, 0, 0, 5, 1, 0, 0, 0, 0, 1>>;
+
+// f(integral_constant<int, R>) for a chunk of `groups` row groups.
+template <class F>
+__device__ __forceinline__ void with_chunk_groups(int groups, F&& f) {
+  static_for<1, kGatedRmax / 2 + 1>([&](auto rc) {
+    constexpr int R = 2 * decltype(rc)::value;
+    if (groups == R - 1 || groups == R) f(std::integral_constant<int, R>{});
+  });
+}
+
+// Tile `bid` of the chunk form; false past its tiles. Experts of several chunks
+// come first, in order, then the others, largest first, so that the last tiles
+// to start are short. Workgroups go to the XCDs one by one, so whatever the
+// routing every XCD gets a like share of full tiles and small ones (with a
+// contiguous range of tiles an XCD, two chunks leave six XCDs idle: D = 4096,
+// F = 14336, one token, 222 against 71 us). An expert of c chunks runs in bands of
+// 8 slices, chunk by chunk: a slice's chunks follow each other on one XCD, if
+// the slices are a multiple of 8, and meet its weights in that L2.
+__device__ __forceinline__ bool gated_chunk_tile(int bid, int slices, const GatedLayout& l, Chunk* ch, int* slice) {
+  const int32_t first = expert_counts(l.tokens_per_expert, l.num_experts, 0);
+  auto counts = [&](int base) { return base == 0 ? first : expert_counts(l.tokens_per_expert, l.num_experts, base); };
+  auto chunks_of = [](int32_t n) { return n > 32 * kGatedRmax ? Chunking<kGatedRmax>::count(n) : 0; };  // several
+  int several = 0;
+#pragma unroll 1
+  for (int base = 0; base < l.num_experts; base += 64) several += wave_inclusive_scan_total(chunks_of(counts(base)));
+  const int c = uniform(bid / slices);
+  if (c >= several) {
+    int32_t hist[kGatedRmax + 1];
+    single_chunk_hist<kGatedRmax>(l.tokens_per_expert, l.num_experts, first, hist);
+    *ch = find_single_chunk_by_size<kGatedRmax>(l.tokens_per_expert, l.num_experts, c - several, first, hist);
+    *slice = uniform(bid - c * slices);
+  } else {
+    int before = 0, rows_before = 0;
+#pragma unroll 1
+    for (int base = 0; base < l.num_experts; base += 64) {
+      const int32_t n = counts(base);
+      const int mine = chunks_of(n);
+      const int incl = wave_inclusive_scan(mine), padded = wave_inclusive_scan(padded_rows(n));
+      const uint64_t reach = __ballot(before + incl > c);
+      if (reach != 0) {
+        const int e = __builtin_ctzll(reach);
+        const int count = lane_value(mine, e);
+        const int t = bid - (before + lane_value(incl, e) - count) * slices;  // among the expert's tiles
+        const int band = uniform(t / (kNumXcd * count));
+        const int width = min(kNumXcd, slices - band * kNumXcd);
+        const int in = t - band * kNumXcd * count;
+        const int i = uniform(in / width);
+        *slice = uniform(band * kNumXcd + in - i * width);
+        const int start = i * Chunking<kGatedRmax>::kRows;
+        ch->expert = uniform(base + e);
+        ch->row0 = uniform(rows_before + lane_value(padded - padded_rows(n), e) + start);
+        ch->rows = uniform(i + 1 < count ? Chunking<kGatedRmax>::kRows : lane_value(n, e) - start);
+        ch->groups = (ch->rows + 31) / 32;
+        break;
+      }
+      before += lane_value(incl, 63);
+      rows_before += lane_value(padded, 63);
+    }
+  }
+  // None, or not a routing layout (the chunk would leave the buffers): skip it.
+  return ch->expert >= 0 && ch->row0 >= 0 && ch->rows >= 1 && ch->groups <= kGatedRmax &&
+         ch->row0 + ch->rows <= l.max_row_blocks * kBS;
+}
+
+// Workgroups of the chunk form: an expert of n rows has ceil(n / 256) chunks,
+// (one less if the
+// last piece joins the one before), so N copies at most N / 256 + min(E, N).
+inline int64_t gated_chunk_grid(const GatedLayout& l, int64_t num_copies, int64_t slices) {
+  return std::min<int64_t>(l.max_row_blocks,
+                           num_copies / Chunking<kGatedRmax>::kRows + std::min<int64_t>(l.num_experts, num_copies)) *
+         slices;
+}
+
+// Whether `columns` columns run in the chunk form: when 128-wide tiles of the
+// row blocks have no CU each, and 256 divide them. (Each live row block holds
+// a copy at least.)
+inline int gated_chunks(const GatedLayout& l, int64_t num_copies, int64_t columns, bool* chunks) {
+  int cus = 0;
+  if (const int rc = device_cus(&cus)) return rc;
+  *chunks = columns % kGatedBN == 0 &&
+            fit_width(std::min<int64_t>(l.max_row_blocks, num_copies), columns, cus) > 128;
+  return SB_OK;
 }
 
 // LDS offset of 16-byte chunk `chunk` of row r in a staged tile of ROW_BYTES

@@ -123,15 +123,15 @@ struct RowsBtSrc {
     *r = rb;
     *s = static_cast<uint32_t>(t) * (Cfg::BK * 2);
   }
-  __device__ __forceinline__ RowsBtSrc(const uint16_t* a, const uint16_t* b, const RowBlock& block, int32_t n0,
-                                       int32_t n, int32_t k) {
-    ra = make_rsrc(a + static_cast<int64_t>(block.row0) * k, static_cast<uint32_t>(block.rows) * k * 2u);
-    rb = make_rsrc(b + static_cast<int64_t>(block.expert) * n * k,
+  __device__ __forceinline__ RowsBtSrc(const uint16_t* a, const uint16_t* b, const Chunk& ch, int32_t n0, int32_t n,
+                                       int32_t k) {
+    ra = make_rsrc(a + static_cast<int64_t>(ch.row0) * k, static_cast<uint32_t>(ch.rows) * k * 2u);
+    rb = make_rsrc(b + static_cast<int64_t>(ch.expert) * n * k,
                    static_cast<uint32_t>(n) * static_cast<uint32_t>(k) * 2u);
     const ADmaPos<Cfg> ap;
 #pragma unroll
     for (int q = 0; q < Cfg::kAInstr; ++q)
-      a_off[q] = ap.row[q] < block.rows ? (static_cast<uint32_t>(ap.row[q]) * k + ap.chunk[q] * 8) * 2u : kOutOfRange;
+      a_off[q] = ap.row[q] < ch.rows ? (static_cast<uint32_t>(ap.row[q]) * k + ap.chunk[q] * 8) * 2u : kOutOfRange;
     const BtDmaPos<Cfg> bp;
 #pragma unroll
     for (int q = 0; q < Cfg::kBInstr; ++q)
@@ -139,92 +139,149 @@ struct RowsBtSrc {
   }
 };
 
+struct RowsBtArgs {
+  const uint16_t *a, *b;
+  GatedLayout layout;
+  uint16_t* out;
+  int32_t n, k;
+};
+
 template <class Cfg>
-__global__ void __launch_bounds__(Cfg::kThreads)
-    rows_bt_kernel(const uint16_t* __restrict__ a, const uint16_t* __restrict__ b, GatedLayout layout,
-                   uint16_t* __restrict__ out, int32_t n, int32_t k) {
+__device__ __forceinline__ void rows_bt_tile(uint8_t* __restrict__ lds, const RowsBtArgs& p, const Chunk& ch, int n0) {
   using ML = DmaMainloop<Cfg>;
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[Cfg::kLdsAlloc];
-  RowBlock block;
-  int slice;
-  if (!row_block_tile(static_cast<int>(blockIdx.x), n / Cfg::BN, layout, kTileGroup, &block, &slice)) return;
-  const int n0 = slice * Cfg::BN;
-  const RowsBtSrc<Cfg> src(a, b, block, n0, n, k);
+  const RowsBtSrc<Cfg> src(p.a, p.b, ch, n0, p.n, p.k);
   typename ML::Acc acc;
-  ML::run(lds, src, k / Cfg::BK, acc);
+  ML::run(lds, src, p.k / Cfg::BK, acc);
   ML::stage_tile(lds, acc, [](float v) { return v; });
-  uint16_t* rows = out + static_cast<int64_t>(block.row0) * n + n0;
+  uint16_t* rows = p.out + static_cast<int64_t>(ch.row0) * p.n + n0;
   ML::for_each_staged_chunk(lds, [&](int r, int col, u32x4_t v) {
-    if (r < block.rows) *reinterpret_cast<u32x4_t*>(rows + static_cast<int64_t>(r) * n + col) = v;
+    if (r < ch.rows) *reinterpret_cast<u32x4_t*>(rows + static_cast<int64_t>(r) * p.n + col) = v;
   });
 }
 
-// The epilogue stages the tile as fp32 (a lane's results are 4 columns of 32
-// rows), then each lane takes 8 columns of a row: 16-byte loads of G and U,
-// 16-byte stores of dG, dU and wh.
+struct SlopeArgs {
+  const uint16_t *gog, *w2, *gu;
+  const float* row_gate;
+  GatedLayout layout;
+  uint16_t *grad_gu, *wh;
+  int32_t d_model, ffn_dim;
+};
+
+// The epilogue stages the tile as fp32, up to 128 rows at a time (a lane's
+// results are 4 columns of 32 rows), then each lane takes 8 columns of a row:
+// 16-byte loads of G and U, 16-byte stores of dG, dU and wh.
 template <class Cfg, int ACT>
-__global__ void __launch_bounds__(Cfg::kThreads)
-    gated_slope_kernel(const uint16_t* __restrict__ gog, const uint16_t* __restrict__ w2,
-                       const uint16_t* __restrict__ gu, const float* __restrict__ row_gate, GatedLayout layout,
-                       uint16_t* __restrict__ grad_gu, uint16_t* __restrict__ wh, int32_t d_model, int32_t ffn_dim) {
+__device__ __forceinline__ void gated_slope_tile(uint8_t* __restrict__ lds, const SlopeArgs& p, const Chunk& ch,
+                                                 int n0) {
   using ML = DmaMainloop<Cfg>;
   constexpr int BN = Cfg::BN, kRowBytes = BN * 4;
-  constexpr int kLds = Cfg::kLdsAlloc > kBS * kRowBytes ? Cfg::kLdsAlloc : kBS * kRowBytes;
-  static_assert(Cfg::BM == kBS && kLds <= 160 * 1024, "the fp32 tile fits LDS");
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[kLds];
-  RowBlock block;
-  int slice;
-  if (!row_block_tile(static_cast<int>(blockIdx.x), ffn_dim / BN, layout, kTileGroup, &block, &slice)) return;
-  const int n0 = slice * BN;
-  const RowsBtSrc<Cfg> src(gog, w2, block, n0, ffn_dim, d_model);
+  // Row groups of a wave in one part, and the part's rows: Cfg::WM runs of them.
+  constexpr int kGroups = 4 / Cfg::WM < Cfg::TM ? 4 / Cfg::WM : Cfg::TM;
+  constexpr int kParts = (Cfg::TM + kGroups - 1) / kGroups;
+  const RowsBtSrc<Cfg> src(p.gog, p.w2, ch, n0, p.ffn_dim, p.d_model);
   typename ML::Acc acc;
-  ML::run(lds, src, d_model / Cfg::BK, acc);
+  ML::run(lds, src, p.d_model / Cfg::BK, acc);
 
-  __syncthreads();  // every wave is done reading the ring
+  const int lane = threadIdx.x & 63, wm = (threadIdx.x >> 6) / Cfg::WN;
+  static_for<0, kParts>([&](auto pc) {
+    constexpr int i0 = decltype(pc)::value * kGroups;
+    constexpr int kRun = 32 * (Cfg::TM - i0 < kGroups ? Cfg::TM - i0 : kGroups);  // rows of each wave row in this part
+    __syncthreads();  // every wave is done reading the ring, or the part before
 #pragma unroll
-  for (int jn = 0; jn < Cfg::TN; ++jn)
+    for (int jn = 0; jn < Cfg::TN; ++jn)
 #pragma unroll
-    for (int i = 0; i < Cfg::TM; ++i) {
-      const int m = ML::out_row(i);
+      for (int i = i0; i < i0 + kRun / 32; ++i) {
+        const int m = wm * kRun + 32 * (i - i0) + (lane & 31);
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const f32x4_t v = {acc[jn][i][4 * g], acc[jn][i][4 * g + 1], acc[jn][i][4 * g + 2], acc[jn][i][4 * g + 3]};
-        *reinterpret_cast<f32x4_t*>(lds + staged_at<kRowBytes>(m, ML::out_col(jn, g) >> 2)) = v;
+        for (int g = 0; g < 4; ++g) {
+          const f32x4_t v = {acc[jn][i][4 * g], acc[jn][i][4 * g + 1], acc[jn][i][4 * g + 2], acc[jn][i][4 * g + 3]};
+          *reinterpret_cast<f32x4_t*>(lds + staged_at<kRowBytes>(m, ML::out_col(jn, g) >> 2)) = v;
+        }
       }
-    }
-  __syncthreads();
-  constexpr int kChunksPerRow = BN / 8;
-  for (int q = threadIdx.x; q < block.rows * kChunksPerRow; q += Cfg::kThreads) {
-    const int r = q / kChunksPerRow, c = q % kChunksPerRow;
-    const int64_t row = block.row0 + r;
-    const int64_t at = row * 2 * ffn_dim + n0 + c * 8;
-    const u32x4_t gv = *reinterpret_cast<const u32x4_t*>(gu + at);
-    const u32x4_t uv = *reinterpret_cast<const u32x4_t*>(gu + at + ffn_dim);
-    const float w = row_gate[row];
-    const f32x4_t lo = *reinterpret_cast<const f32x4_t*>(lds + staged_at<kRowBytes>(r, 2 * c));
-    const f32x4_t hi = *reinterpret_cast<const f32x4_t*>(lds + staged_at<kRowBytes>(r, 2 * c + 1));
-    u32x4_t dg, du, hw;
+    __syncthreads();
+    constexpr int kChunksPerRow = BN / 8;
+    for (int q = threadIdx.x; q < Cfg::WM * kRun * kChunksPerRow; q += Cfg::kThreads) {
+      const int m = q / kChunksPerRow, c = q % kChunksPerRow;
+      const int r = m / kRun * Cfg::WTM + 32 * i0 + m % kRun;  // of the chunk
+      if (r >= ch.rows) continue;
+      const int64_t row = ch.row0 + r;
+      const int64_t at = row * 2 * p.ffn_dim + n0 + c * 8;
+      const u32x4_t gv = *reinterpret_cast<const u32x4_t*>(p.gu + at);
+      const u32x4_t uv = *reinterpret_cast<const u32x4_t*>(p.gu + at + p.ffn_dim);
+      const float w = p.row_gate[row];
+      const f32x4_t lo = *reinterpret_cast<const f32x4_t*>(lds + staged_at<kRowBytes>(m, 2 * c));
+      const f32x4_t hi = *reinterpret_cast<const f32x4_t*>(lds + staged_at<kRowBytes>(m, 2 * c + 1));
+      u32x4_t dg, du, hw;
 #pragma unroll
-    for (int p = 0; p < 4; ++p) {
-      float og[2], ou[2], oh[2];
+      for (int h = 0; h < 4; ++h) {
+        float og[2], ou[2], oh[2];
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const float g = __uint_as_float(e ? gv[p] & 0xffff0000u : gv[p] << 16);
-        const float u = __uint_as_float(e ? uv[p] & 0xffff0000u : uv[p] << 16);
-        const float dh = w * (p < 2 ? lo[2 * p + e] : hi[2 * p - 4 + e]);
-        const ActSlope a = gated_act_slope<ACT>(g);
-        og[e] = dh * u * a.slope;
-        ou[e] = dh * a.value;
-        oh[e] = w * (a.value * u);
+        for (int e = 0; e < 2; ++e) {
+          const float g = __uint_as_float(e ? gv[h] & 0xffff0000u : gv[h] << 16);
+          const float u = __uint_as_float(e ? uv[h] & 0xffff0000u : uv[h] << 16);
+          const float dh = w * (h < 2 ? lo[2 * h + e] : hi[2 * h - 4 + e]);
+          const ActSlope a = gated_act_slope<ACT>(g);
+          og[e] = dh * u * a.slope;
+          ou[e] = dh * a.value;
+          oh[e] = w * (a.value * u);
+        }
+        dg[h] = pack_bf16x2(og[0], og[1]);
+        du[h] = pack_bf16x2(ou[0], ou[1]);
+        hw[h] = pack_bf16x2(oh[0], oh[1]);
       }
-      dg[p] = pack_bf16x2(og[0], og[1]);
-      du[p] = pack_bf16x2(ou[0], ou[1]);
-      hw[p] = pack_bf16x2(oh[0], oh[1]);
+      *reinterpret_cast<u32x4_t*>(p.grad_gu + at) = dg;
+      *reinterpret_cast<u32x4_t*>(p.grad_gu + at + p.ffn_dim) = du;
+      *reinterpret_cast<u32x4_t*>(p.wh + row * p.ffn_dim + n0 + c * 8) = hw;
     }
-    *reinterpret_cast<u32x4_t*>(grad_gu + at) = dg;
-    *reinterpret_cast<u32x4_t*>(grad_gu + at + ffn_dim) = du;
-    *reinterpret_cast<u32x4_t*>(wh + row * ffn_dim + n0 + c * 8) = hw;
-  }
+  });
+}
+
+// Both products' row-block form: 128 x 128 tiles.
+using BtNarrow = DmaCfg<128, 128, 64, 3, 2, 2, 0, 0, 5, 1, 0, 0, 0, 0, 1>;
+
+template <int BN>
+constexpr int slope_lds(int ring) { return ring > kBS * BN * 4 ? ring : kBS * BN * 4; }
+
+__global__ void __launch_bounds__(BtNarrow::kThreads) rows_bt_kernel(RowsBtArgs p) {
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[BtNarrow::kLdsAlloc];
+  Chunk ch;
+  int slice;
+  if (!row_block_tile(static_cast<int>(blockIdx.x), p.n / BtNarrow::BN, p.layout, &ch, &slice)) return;
+  rows_bt_tile<BtNarrow>(lds, p, ch, slice * BtNarrow::BN);
+}
+
+__global__ void __launch_bounds__(512) rows_bt_chunk_kernel(RowsBtArgs p) {
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[160 * 1024];
+  Chunk ch{-1, 0, 0, 0};
+  int slice = 0;
+  if (!gated_chunk_tile(static_cast<int>(blockIdx.x), p.n / kGatedBN, p.layout, &ch, &slice)) return;
+  with_chunk_groups(ch.groups, [&](auto rc) {
+    using Cfg = BtChunkCfg<decltype(rc)::value>;
+    static_assert(Cfg::kLdsAlloc <= sizeof(lds) && Cfg::kThreads == 512, "one workgroup for all heights");
+    rows_bt_tile<Cfg>(lds, p, ch, slice * kGatedBN);
+  });
+}
+
+template <int ACT>
+__global__ void __launch_bounds__(BtNarrow::kThreads) gated_slope_kernel(SlopeArgs p) {
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[slope_lds<BtNarrow::BN>(BtNarrow::kLdsAlloc)];
+  Chunk ch;
+  int slice;
+  if (!row_block_tile(static_cast<int>(blockIdx.x), p.ffn_dim / BtNarrow::BN, p.layout, &ch, &slice)) return;
+  gated_slope_tile<BtNarrow, ACT>(lds, p, ch, slice * BtNarrow::BN);
+}
+
+template <int ACT>
+__global__ void __launch_bounds__(512) gated_slope_chunk_kernel(SlopeArgs p) {
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[160 * 1024];
+  Chunk ch{-1, 0, 0, 0};
+  int slice = 0;
+  if (!gated_chunk_tile(static_cast<int>(blockIdx.x), p.ffn_dim / kGatedBN, p.layout, &ch, &slice)) return;
+  with_chunk_groups(ch.groups, [&](auto rc) {
+    using Cfg = BtChunkCfg<decltype(rc)::value>;
+    static_assert(Cfg::kLdsAlloc <= sizeof(lds) && Cfg::kThreads == 512, "one workgroup for all heights");
+    gated_slope_tile<Cfg, ACT>(lds, p, ch, slice * kGatedBN);
+  });
 }
 
 // ------------------------------------------------- weight gradients ---
@@ -254,21 +311,30 @@ struct OuterSrc {
   }
 };
 
+// Each expert's tiles over all XCDs, a contiguous part of them each: whatever
+// the routing, every XCD gets an eighth of each expert's K steps.
+constexpr int64_t outer_tiles(int64_t m, int64_t n) { return (m * n + kNumXcd - 1) / kNumXcd * kNumXcd; }
+
+// Two workgroups a CU (at most 128 registers a lane, 72 KB of LDS): one's
+// output and first loads overlap the other's products, which are few where an
+// expert has few rows.
 template <class Cfg>
-__global__ void __launch_bounds__(Cfg::kThreads)
+__global__ void __launch_bounds__(Cfg::kThreads) __attribute__((amdgpu_waves_per_eu(Cfg::kWaves / 2)))
     expert_outer_kernel(const uint16_t* __restrict__ a, const uint16_t* __restrict__ b, GatedLayout layout,
                         uint16_t* __restrict__ out, int32_t m, int32_t n) {
   using ML = DmaMainloop<Cfg>;
   __shared__ __attribute__((aligned(1024))) uint8_t lds[Cfg::kLdsAlloc];
   const int slices = n / Cfg::BN, row_tiles = m / Cfg::BM;
-  const int per_expert = slices * row_tiles;
-  const int tile = xcd_remap(static_cast<int>(blockIdx.x), layout.num_experts * per_expert);
-  const int e = uniform(tile / per_expert);
+  const int tiles = static_cast<int>(outer_tiles(row_tiles, slices));
+  const int e = uniform(static_cast<int>(blockIdx.x) / tiles);
+  const int tile = xcd_remap(static_cast<int>(blockIdx.x) - e * tiles, tiles);
+  if (tile >= row_tiles * slices) return;
   int mt, nt;
-  tile_coords(tile - e * per_expert, row_tiles, slices, kTileGroup, &mt, &nt);
+  tile_coords(tile, row_tiles, slices, kTileGroup, &mt, &nt);
   const int m0 = mt * Cfg::BM, n0 = nt * Cfg::BN;
   const int32_t rows = uniform(layout.tokens_per_expert[e]);
   const int32_t row0 = uniform(layout.padded_offsets[e]);
+  if (row0 < 0 || row0 + rows > layout.max_row_blocks * kBS) return;  // not a routing layout
   uint16_t* tile_out = out + (static_cast<int64_t>(e) * m + m0) * n + n0;
 
   OuterSrc<Cfg> src;
@@ -292,49 +358,34 @@ __global__ void __launch_bounds__(Cfg::kThreads)
   });
 }
 
-using BtWide = DmaCfg<128, 256, 64, 3, 2, 4, 0, 0, 3, 1, 0, 0, 0, 0, 1>;
-using BtNarrow = DmaCfg<128, 128, 64, 3, 2, 2, 0, 0, 5, 1, 0, 0, 0, 0, 1>;
 using OuterWide = DmaCfg<128, 256, 32, 3, 2, 4, 0, 0, 5, 1, 0, 0, 0, 1>;
 using OuterNarrow = DmaCfg<128, 128, 32, 3, 2, 2, 0, 0, 5, 1, 0, 0, 0, 1>;
 
-template <class Cfg, int ACT>
-int run_slope(const void* gog, const void* w2, const void* gu, const float* row_gate, const GatedLayout& layout,
-              void* grad_gu, void* wh, int64_t d_model, int64_t ffn_dim, hipStream_t stream) {
-  const int64_t tiles = layout.max_row_blocks * (ffn_dim / Cfg::BN);
-  gated_slope_kernel<Cfg, ACT><<<static_cast<uint32_t>(tiles), Cfg::kThreads, 0, stream>>>(
-      static_cast<const uint16_t*>(gog), static_cast<const uint16_t*>(w2), static_cast<const uint16_t*>(gu), row_gate,
-      layout, static_cast<uint16_t*>(grad_gu), static_cast<uint16_t*>(wh), static_cast<int32_t>(d_model),
-      static_cast<int32_t>(ffn_dim));
-  return check_launch("gated backward: slope");
-}
-
-template <class Cfg>
-int run_rows_bt(const void* a, const void* b, const GatedLayout& layout, void* out, int64_t n, int64_t k,
-                hipStream_t stream) {
-  const int64_t tiles = layout.max_row_blocks * (n / Cfg::BN);
-  rows_bt_kernel<Cfg><<<static_cast<uint32_t>(tiles), Cfg::kThreads, 0, stream>>>(
-      static_cast<const uint16_t*>(a), static_cast<const uint16_t*>(b), layout, static_cast<uint16_t*>(out),
-      static_cast<int32_t>(n), static_cast<int32_t>(k));
-  return check_launch("gated backward: rows @ w^T");
+// A product's launch in the form that its columns take.
+template <class Args>
+int launch_bt(void (*row_blocks)(Args), void (*chunk_form)(Args), const Args& args, const GatedLayout& layout,
+              int64_t num_copies, int64_t columns, int64_t k, hipStream_t stream) {
+  if (!reduction_fits<BtNarrow>(k) || !reduction_fits<BtChunkCfg<kGatedRmax>>(k))
+    return fail(SB_ERR_INVALID, "gated backward: not whole K steps");
+  bool chunks = false;
+  if (const int rc = gated_chunks(layout, num_copies, columns, &chunks)) return rc;
+  const int64_t grid = chunks ? gated_chunk_grid(layout, num_copies, columns / kGatedBN)
+                              : layout.max_row_blocks * (columns / BtNarrow::BN);
+  if (grid > 2147483647LL) return fail(SB_ERR_INVALID, "problem too large");
+  if (chunks) chunk_form<<<static_cast<uint32_t>(grid), 512, 0, stream>>>(args);
+  else row_blocks<<<static_cast<uint32_t>(grid), BtNarrow::kThreads, 0, stream>>>(args);
+  return check_launch("gated backward");
 }
 
 template <class Cfg>
 int run_outer(const void* a, const void* b, const GatedLayout& layout, void* out, int64_t m, int64_t n,
               hipStream_t stream) {
-  const int64_t tiles = layout.num_experts * (m / Cfg::BM) * (n / Cfg::BN);
-  if (tiles > 2147483647LL) return fail(SB_ERR_INVALID, "gated backward: too many tiles");
-  expert_outer_kernel<Cfg><<<static_cast<uint32_t>(tiles), Cfg::kThreads, 0, stream>>>(
+  const int64_t grid = layout.num_experts * outer_tiles(m / Cfg::BM, n / Cfg::BN);
+  if (grid > 2147483647LL) return fail(SB_ERR_INVALID, "problem too large");
+  expert_outer_kernel<Cfg><<<static_cast<uint32_t>(grid), Cfg::kThreads, 0, stream>>>(
       static_cast<const uint16_t*>(a), static_cast<const uint16_t*>(b), layout, static_cast<uint16_t*>(out),
       static_cast<int32_t>(m), static_cast<int32_t>(n));
   return check_launch("gated backward: weight gradient");
-}
-
-// 256 columns, or 128 when 256 do not divide them or leave CUs without a tile.
-int bt_width(const GatedLayout& layout, int64_t num_copies, int64_t n, int* width) {
-  int cus = 0;
-  if (const int rc = device_cus(&cus)) return rc;
-  *width = std::min(256, fit_width(std::min<int64_t>(layout.max_row_blocks, num_copies), n, cus));
-  return SB_OK;
 }
 
 }  // namespace
@@ -357,21 +408,20 @@ int launch_grad_rows(const void* x, const void* grad_out, const void* y, const G
 int launch_gated_slope(const void* gog, const void* w2, const void* gu, const float* row_gate,
                        const GatedLayout& layout, void* grad_gu, void* wh, int64_t num_copies, int64_t d_model,
                        int64_t ffn_dim, int32_t act, hipStream_t stream) {
-  int width = 0;
-  if (const int rc = bt_width(layout, num_copies, ffn_dim, &width)) return rc;
-  auto run = [&](auto launch) {
-    return launch(gog, w2, gu, row_gate, layout, grad_gu, wh, d_model, ffn_dim, stream);
-  };
-  if (width == 256) return run(act == SB_ACT_SILU ? run_slope<BtWide, SB_ACT_SILU> : run_slope<BtWide, SB_ACT_GELU>);
-  return run(act == SB_ACT_SILU ? run_slope<BtNarrow, SB_ACT_SILU> : run_slope<BtNarrow, SB_ACT_GELU>);
+  const SlopeArgs args{static_cast<const uint16_t*>(gog), static_cast<const uint16_t*>(w2),
+                       static_cast<const uint16_t*>(gu), row_gate, layout, static_cast<uint16_t*>(grad_gu),
+                       static_cast<uint16_t*>(wh), static_cast<int32_t>(d_model), static_cast<int32_t>(ffn_dim)};
+  return act == SB_ACT_SILU ? launch_bt(gated_slope_kernel<SB_ACT_SILU>, gated_slope_chunk_kernel<SB_ACT_SILU>, args,
+                                        layout, num_copies, ffn_dim, d_model, stream)
+                            : launch_bt(gated_slope_kernel<SB_ACT_GELU>, gated_slope_chunk_kernel<SB_ACT_GELU>, args,
+                                        layout, num_copies, ffn_dim, d_model, stream);
 }
 
 int launch_rows_bt(const void* a, const void* b, const GatedLayout& layout, void* out, int64_t num_copies, int64_t n,
                    int64_t k, hipStream_t stream) {
-  int width = 0;
-  if (const int rc = bt_width(layout, num_copies, n, &width)) return rc;
-  return width == 256 ? run_rows_bt<BtWide>(a, b, layout, out, n, k, stream)
-                      : run_rows_bt<BtNarrow>(a, b, layout, out, n, k, stream);
+  const RowsBtArgs args{static_cast<const uint16_t*>(a), static_cast<const uint16_t*>(b), layout,
+                        static_cast<uint16_t*>(out), static_cast<int32_t>(n), static_cast<int32_t>(k)};
+  return launch_bt(rows_bt_kernel, rows_bt_chunk_kernel, args, layout, num_copies, n, k, stream);
 }
 
 int launch_expert_outer(const void* a, const void* b, const GatedLayout& layout, void* out, int64_t m, int64_t n,
