@@ -47,11 +47,25 @@ int launch_rows_bt(const void* a, const void* b, const GatedLayout& layout, void
 int launch_expert_outer(const void* a, const void* b, const GatedLayout& layout, void* out, int64_t m, int64_t n,
                         hipStream_t stream);
 
+// Both products of the weight gradients in one launch, for m % 256 == 0 and
+// n % 256 == 0 (outer_stream_fits; gated_outer.hip).
+bool outer_stream_fits(int64_t m, int64_t n);
+int launch_expert_outers(const void* a1, const void* b1, void* out1, int64_t m1, int64_t n1, const void* a2,
+                         const void* b2, void* out2, int64_t m2, int64_t n2, const GatedLayout& layout,
+                         hipStream_t stream);
+
 // out[t] = sum_j y[copy_row[t k + j]], fp32 sums (combine.hip).
 int launch_sum_copies(const void* y, const int32_t* copy_row, void* out, int64_t num_tokens, int32_t k,
                       int64_t d_model, int64_t y_rows, const int32_t* valid_tokens, hipStream_t stream);
 
 // ------------------------------------------------------------- in tiles ---
+
+// *p for a uniform p that this kernel does not write: a scalar load. (Of a
+// pointer inside a struct the compiler cannot tell, and takes a vector load,
+// whose wait is then one for every load before it.)
+__device__ __forceinline__ int32_t scalar_load(const int32_t* p) {
+  return *(const __attribute__((address_space(4))) int32_t*)(reinterpret_cast<uintptr_t>(p));
+}
 
 // A tile's rows are a Chunk (expert_chunks.hpp): real rows of one expert from
 // a padded row that is a multiple of 128.
@@ -63,14 +77,14 @@ int launch_sum_copies(const void* y, const int32_t* copy_row, void* out, int64_t
 // past the live row blocks. Live tiles are spread over the XCDs in contiguous
 // ranges, row blocks in groups (tile_coords).
 __device__ __forceinline__ bool row_block_tile(int bid, int slices, const GatedLayout& l, Chunk* ch, int* slice) {
-  const int live_rb = __builtin_amdgcn_readfirstlane(l.padded_offsets[l.num_experts]) / kBS;
+  const int live_rb = scalar_load(l.padded_offsets + l.num_experts) / kBS;
   if (live_rb > l.max_row_blocks || bid >= live_rb * slices) return false;
   int rb;
   tile_coords(xcd_remap(bid, live_rb * slices), live_rb, slices, kTileGroup, &rb, slice);
-  const int32_t e = __builtin_amdgcn_readfirstlane(l.row_block_expert[rb]);
+  const int32_t e = scalar_load(l.row_block_expert + rb);
   if (e < 0 || e >= l.num_experts) return false;
-  const int32_t n = __builtin_amdgcn_readfirstlane(l.tokens_per_expert[e]);
-  const int32_t first = rb * kBS - __builtin_amdgcn_readfirstlane(l.padded_offsets[e]);
+  const int32_t n = scalar_load(l.tokens_per_expert + e);
+  const int32_t first = rb * kBS - scalar_load(l.padded_offsets + e);
   if (first < 0 || first >= n) return false;  // not a routing layout
   *ch = Chunk{e, rb * kBS, min(n - first, kBS), 4};
   return true;

@@ -332,8 +332,8 @@ __global__ void __launch_bounds__(Cfg::kThreads) __attribute__((amdgpu_waves_per
   int mt, nt;
   tile_coords(tile, row_tiles, slices, kTileGroup, &mt, &nt);
   const int m0 = mt * Cfg::BM, n0 = nt * Cfg::BN;
-  const int32_t rows = uniform(layout.tokens_per_expert[e]);
-  const int32_t row0 = uniform(layout.padded_offsets[e]);
+  const int32_t rows = scalar_load(layout.tokens_per_expert + e);
+  const int32_t row0 = scalar_load(layout.padded_offsets + e);
   if (row0 < 0 || row0 + rows > layout.max_row_blocks * kBS) return;  // not a routing layout
   uint16_t* tile_out = out + (static_cast<int64_t>(e) * m + m0) * n + n0;
 

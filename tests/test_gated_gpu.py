@@ -51,7 +51,7 @@ def check_all(args, act="silu", valid=None):
 
 
 SHAPES = [(1, 1, 1, 128, 128), (1, 2, 8, 256, 512), (7, 3, 5, 128, 384), (250, 2, 8, 256, 512), (130, 1, 2, 384, 128),
-          (300, 8, 16, 256, 256), (513, 2, 3, 640, 256), (129, 4, 130, 128, 128), (1100, 2, 2, 256, 640)]
+          (300, 8, 16, 256, 256), (520, 3, 4, 512, 768), (513, 2, 3, 640, 256), (129, 4, 130, 128, 128), (1100, 2, 2, 256, 640)]
 
 
 @pytest.mark.parametrize("act", ["silu", "gelu"])
