@@ -666,11 +666,12 @@ def layer_rounded_cuda(x: torch.Tensor, scores: torch.Tensor, k: int, w1: torch.
 _ACTIVATIONS = {"silu": 0, "gelu": 1}
 
 
+_HERE = contextlib.nullcontext()
+
+
 def _device_of(t: torch.Tensor) -> contextlib.AbstractContextManager:
     """Makes t's device current for a launch, where it is not."""
-    if t.device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(t.device)
+    return _HERE if t.get_device() == torch.cuda.current_device() else torch.cuda.device(t.device)
 
 
 @functools.lru_cache(maxsize=256)
@@ -685,21 +686,24 @@ def gated_bytes(num_tokens: int, k: int, num_experts: int, d_model: int, ffn_dim
 def _check_gated(x: torch.Tensor, expert_idx: torch.Tensor | None, gates: torch.Tensor, w1: torch.Tensor,
                  w2: torch.Tensor, activation: str, valid_tokens: torch.Tensor | None) -> tuple[int, ...]:
     """(T, k, E, D, F) of operands that the gated layer's calls take as they are."""
-    if not (x.is_cuda and w1.device == x.device and w2.device == x.device and gates.device == x.device
-            and (expert_idx is None or expert_idx.device == x.device)):
+    try:
+        (num_tokens, d_model), (rows, k), (num_experts, ffn_dim, columns) = x.shape, gates.shape, w2.shape
+    except ValueError:
+        _fail(f"x must be [T, D], expert_weight [T, k], w1 [E, D, 2F] and w2 [E, F, D], got {_shape(x)}, {_shape(gates)}, "
+              f"{_shape(w1)} and {_shape(w2)}")
+    device = x.get_device()
+    if (device < 0 or w1.get_device() != device or w2.get_device() != device or gates.get_device() != device
+            or (expert_idx is not None and expert_idx.get_device() != device)):
         _fail("all inputs must be on the same GPU")
-    if x.dtype != torch.bfloat16 or w1.dtype != torch.bfloat16 or w2.dtype != torch.bfloat16:
+    if not (x.dtype is w1.dtype is w2.dtype is torch.bfloat16):
         _fail("x, w1 and w2 must be bfloat16")
-    if not (x.dim() == 2 and w1.dim() == 3 and w2.dim() == 3):
-        _fail(f"x must be [T, D], w1 [E, D, 2F] and w2 [E, F, D], got {_shape(x)}, {_shape(w1)} and {_shape(w2)}")
-    num_experts, ffn_dim, d_model = w2.shape
-    if x.shape[1] != d_model or w1.shape != (num_experts, d_model, 2 * ffn_dim):
+    if columns != d_model or w1.shape != (num_experts, d_model, 2 * ffn_dim):
         _fail(f"x must be [T, D], w1 [E, D, 2F] and w2 [E, F, D], got {_shape(x)}, {_shape(w1)} and {_shape(w2)}")
     if not (x.is_contiguous() and w1.is_contiguous() and w2.is_contiguous()):
         _fail("x, w1 and w2 must be contiguous")
     if (x.data_ptr() | w1.data_ptr() | w2.data_ptr()) % 16:
         _fail("x, w1 and w2 must be 16-byte aligned")
-    if gates.dim() != 2 or gates.shape[0] != x.shape[0] or gates.shape[1] == 0:
+    if rows != num_tokens or k == 0:
         _fail(f"expert_weight must be [T, k] with k > 0, got {_shape(gates)}")
     if gates.dtype not in _GATE_DTYPES:
         _fail(f"expert_weight must be bfloat16, float16 or float32, got {gates.dtype}")
@@ -712,9 +716,9 @@ def _check_gated(x: torch.Tensor, expert_idx: torch.Tensor | None, gates: torch.
         _fail(f"num_experts must be in [1, {_MAX_EXPERTS}], got {num_experts}")
     if activation not in _ACTIVATIONS:
         _fail(f"activation must be one of {sorted(_ACTIVATIONS)}, got {activation!r}")
-    if valid_tokens is not None and not (valid_tokens.device == x.device and _valid_tokens_ok(valid_tokens)):
+    if valid_tokens is not None and not (valid_tokens.get_device() == device and _valid_tokens_ok(valid_tokens)):
         _fail("valid_tokens must be a one-element int32 CUDA tensor")
-    return x.shape[0], gates.shape[1], num_experts, d_model, ffn_dim
+    return num_tokens, k, num_experts, d_model, ffn_dim
 
 
 def gated_layer_cuda(x: torch.Tensor, expert_idx: torch.Tensor, expert_weight: torch.Tensor, w1: torch.Tensor,

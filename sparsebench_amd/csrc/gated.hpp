@@ -27,6 +27,15 @@ struct GatedLayout {
 int launch_gated_up(const void* x, const void* w1, const GatedLayout& layout, void* h, void* gu, int64_t num_tokens,
                     int64_t num_copies, int64_t d_model, int64_t ffn_dim, int32_t act, hipStream_t stream);
 
+// The whole forward pass for one or two tokens (few_copies; gated_few.hip),
+// without a routing layout. workspace: few_workspace_floats of it.
+bool few_copies(int64_t num_tokens, int32_t k);
+int64_t few_workspace_floats(int64_t num_copies, int64_t d_model, int64_t ffn_dim);
+int launch_few(const void* x, const void* expert_idx, int32_t idx_is_i64, const void* gates, int32_t gate_dtype,
+               const void* w1, const void* w2, void* out, float* workspace, int64_t num_tokens, int32_t k,
+               int64_t num_experts, int64_t d_model, int64_t ffn_dim, int32_t act, const int32_t* valid_tokens,
+               hipStream_t stream);
+
 // Per copy c = t k + j in row r: grad_gates[c] = <grad_out[t], y[r]>; per row:
 // row_gate[r] = gates[c], xg[r] = x[t], gog[r] = grad_out[t].
 int launch_grad_rows(const void* x, const void* grad_out, const void* y, const GatedLayout& layout,

@@ -172,6 +172,7 @@ extern "C" int sb_gated_sizes(int64_t num_tokens, int32_t k, int32_t num_experts
     if (to) *to = ws.used;
   };
   size(carve_layer, layer_bytes);
+  if (layer_bytes && few_copies(num_tokens, k)) *layer_bytes = few_workspace_floats(p.num_copies, d_model, ffn_dim) * 4;
   size(carve_saved, saved_bytes);
   size(carve_train, train_bytes);
   size(carve_backward, backward_bytes);
@@ -186,6 +187,13 @@ extern "C" int sb_gated_layer(const void* x, const void* expert_idx, int32_t idx
   Problem p;
   if (int rc = check_problem(num_tokens, k, num_experts, d_model, ffn_dim, &p)) return rc;
   if (int rc = check_operands({x, w1, w2, out}, {expert_idx, gates}, gate_dtype, act)) return rc;
+  if (few_copies(num_tokens, k)) {
+    if (int rc = check_workspace(workspace, workspace_bytes, few_workspace_floats(p.num_copies, d_model, ffn_dim) * 4))
+      return rc;
+    const int rc = launch_few(x, expert_idx, idx_is_i64, gates, gate_dtype, w1, w2, out, static_cast<float*>(workspace),
+                              num_tokens, k, num_experts, d_model, ffn_dim, act, valid_tokens, as_stream(stream));
+    return rc ? rc : clear_ok();
+  }
   Carver ws{static_cast<uint8_t*>(workspace)};
   const LayerBuffers b = carve_layer(ws, p);
   if (int rc = check_workspace(workspace, workspace_bytes, ws.used)) return rc;
