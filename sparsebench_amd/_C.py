@@ -884,27 +884,27 @@ def dequantize_cuda(pairs, dtype: torch.dtype) -> list[torch.Tensor]:
         _fail(f"values must be bfloat16, float16 or float32, got {dtype}")
     if not pairs:
         return []
-    dev = pairs[0][0].device
+    all_codes, all_scales = [p[0] for p in pairs], [p[1] for p in pairs]
+    dev = all_codes[0].device
     if dev.type != "cuda":
         _fail("codes must be CUDA tensors")
-    lengths = [codes.numel() for codes, _ in pairs]
-    _check_list([codes for codes, _ in pairs], dev.index, "codes")
-    _check_list([scales for _, scales in pairs], dev.index, f"scales (one for each {QUANT_BLOCK} values)", torch.float32,
+    lengths = list(_lengths(all_codes))
+    _check_list(all_codes, dev.index, "codes")
+    _check_list(all_scales, dev.index, f"scales (one for each {QUANT_BLOCK} values)", torch.float32,
                 [-(-n // QUANT_BLOCK) for n in lengths])
-    # Each value list starts at a multiple of 16 bytes of one buffer.
+    dtypes = list(map(_dtype_of, all_codes))
+    if not set(dtypes) <= {torch.int8, torch.uint8}:
+        _fail(f"codes must be int8 or uint8, got {set(dtypes)}")
+    # Each value list starts at a multiple of 16 bytes of one buffer, which is
+    # cut into value lists and the gaps after them by one call.
     step = 16 // dtype.itemsize
-    starts, total = [], 0
-    for (codes, _), n in zip(pairs, lengths):
-        if codes.dtype not in (torch.int8, torch.uint8):
-            _fail(f"codes must be int8 or uint8, got {codes.dtype}")
-        starts.append(total)
-        total += -(-n // step) * step
-    flat = torch.empty(total, dtype=dtype, device=dev)
-    out = [flat[a:a + n].view(codes.shape) for a, n, (codes, _) in zip(starts, lengths, pairs)]
-    words = array.array("q")
-    for (codes, scales), o in zip(pairs, out):
-        words.extend((codes.data_ptr(), scales.data_ptr(), o.data_ptr(), codes.numel(),
-                      1 if codes.dtype == torch.int8 else 0))
+    gaps = [-n % step for n in lengths]
+    flat = torch.empty(sum(lengths) + sum(gaps), dtype=dtype, device=dev)
+    pieces = flat.split_with_sizes(list(itertools.chain.from_iterable(zip(lengths, gaps))))[::2]
+    out = [o if codes.dim() == 1 else o.view(codes.shape) for o, codes in zip(pieces, all_codes)]
+    words = array.array("q", itertools.chain.from_iterable(zip(
+        _addresses(all_codes), _addresses(all_scales), _addresses(out), lengths,
+        [1 if d == torch.int8 else 0 for d in dtypes])))
     with _device_of(flat):
         check(lib().sb_dequantize(words.buffer_info()[0], len(pairs), _GATE_DTYPES[dtype], stream_of(dev)))
     return out

@@ -52,13 +52,8 @@ int launch_gated_slope(const void* gog, const void* w2, const void* gu, const fl
 int launch_rows_bt(const void* a, const void* b, const GatedLayout& layout, void* out, int64_t num_copies, int64_t n,
                    int64_t k, hipStream_t stream);
 
-// out[e] [M, N] = sum over e's rows of a[r]^T b[r], a [P, M], b [P, N]; zeros for an expert with no rows.
-int launch_expert_outer(const void* a, const void* b, const GatedLayout& layout, void* out, int64_t m, int64_t n,
-                        hipStream_t stream);
-
-// Both products of the weight gradients in one launch, for m % 256 == 0 and
-// n % 256 == 0 (outer_stream_fits; gated_outer.hip).
-bool outer_stream_fits(int64_t m, int64_t n);
+// out1[e] [M, N] = sum over e's rows of a1[r]^T b1[r], a1 [P, M], b1 [P, N],
+// and out2 likewise, in one launch; zeros for an expert with no rows.
 int launch_expert_outers(const void* a1, const void* b1, void* out1, int64_t m1, int64_t n1, const void* a2,
                          const void* b2, void* out2, int64_t m2, int64_t n2, const GatedLayout& layout,
                          hipStream_t stream);
@@ -109,14 +104,21 @@ __device__ __forceinline__ bool row_block_tile(int bid, int slices, const GatedL
 //     steps at a time (APAIR).
 //   BT (rows of W1 or W2 as columns): K steps of 64, since a row's piece of 32
 //     is half a cache line (D = 4096, F = 14336, 512 rows an expert: 1592 us
-//     with steps of 32); 160 KB hold 2 stages of A and 3 of B at R = 8.
+//     with steps of 32); 160 KB hold 2 stages of A and 3 of B at R = 8. Weights
+//     past the caches up to R = 4, where an expert has no other chunk to share
+//     them with (slope of 128 rows an expert 207 -> 198 us; taller ones 990 -> 1067).
 constexpr int kGatedRmax = 10, kGatedBN = 256;
 template <int R>
 using GatedUpCfg = DmaCfg<32 * R, kGatedBN, 32, 4, 2, 4, 0, 2, 5, 1, 1, 0, 0, 0, 0, 1>;
 template <int R>
 using BtChunkCfg = std::conditional_t<
     (R >= 6), DmaCfg<32 * R, kGatedBN, 64, 2, 2, 4, 0, 0, 5, 1, 0, (R <= 8 ? 3 : 0), 0, 0, 1>,
-    DmaCfg<32 * R, kGatedBN, 64, (R == 4 ? 3 : 4), 2, 4, 0, 0, 5, 1, 0, 0, 0, 0, 1>>;
+    DmaCfg<32 * R, kGatedBN, 64, (R == 4 ? 3 : 4), 2, 4, 0, 2, 5, 1, 0, 0, 0, 0, 1>>;
+
+// The last slice may be half a slice (columns are multiples of 128).
+__host__ __device__ __forceinline__ int gated_slices(int64_t columns) {
+  return static_cast<int>((columns + kGatedBN - 1) / kGatedBN);
+}
 
 // f(integral_constant<int, R>) for a chunk of `groups` row groups.
 template <class F>
@@ -191,13 +193,11 @@ inline int64_t gated_chunk_grid(const GatedLayout& l, int64_t num_copies, int64_
 }
 
 // Whether `columns` columns run in the chunk form: when 128-wide tiles of the
-// row blocks have no CU each, and 256 divide them. (Each live row block holds
-// a copy at least.)
+// row blocks have no CU each. (Each live row block holds a copy at least.)
 inline int gated_chunks(const GatedLayout& l, int64_t num_copies, int64_t columns, bool* chunks) {
   int cus = 0;
   if (const int rc = device_cus(&cus)) return rc;
-  *chunks = columns % kGatedBN == 0 &&
-            fit_width(std::min<int64_t>(l.max_row_blocks, num_copies), columns, cus) > 128;
+  *chunks = std::min<int64_t>(l.max_row_blocks, num_copies) * (columns / 128) > cus;
   return SB_OK;
 }
 

@@ -5,16 +5,16 @@
 //   gated_slope   dH = w[r] gog W2[e]^T;  dG = dH U a'(G), dU = dH a(G)
 //                 (grad_gu [P, 2F]), and wh = w[r] a(G) U (bf16, one rounding)
 //   rows_bt       dXr = [dG | dU] W1[e]^T
-//   expert_outer  dW1[e] = xg^T [dG | dU],  dW2[e] = wh^T gog over e's rows
+//   outers        dW1[e] = xg^T [dG | dU],  dW2[e] = wh^T gog over e's rows
 //
 // and dx[t] = sum over t's rows of dXr (combine.hip). The products run on the
 // LDS-DMA main loop: rows_bt and gated_slope with B's columns as rows (BT:
-// W1 and W2 are read as they are stored), expert_outer with both operands
-// along K (AT). Rows past an expert's real rows are read as zeros (past the
+// W1 and W2 are read as they are stored), the outer products (gated_outer.hip)
+// with both operands along K (AT). Rows past an expert's real rows are read as zeros (past the
 // buffer's end) and not written.
 //
 // Gathering x and grad_out once (2 P D values, a few percent of the weights'
-// bytes) lets expert_outer's loads be plain: its K runs over rows, so a
+// bytes) lets the outer products' loads be plain: its K runs over rows, so a
 // gather inside would need other addresses at every K step.
 
 #include "gated.hpp"
@@ -108,7 +108,7 @@ int run_grad_rows(const void* x, const void* grad_out, const void* y, const Gate
 // ------------------------------------------------- products with W^T ---
 
 // A: rows row0 .. of a [P, K] (rows past `rows` read as zeros); B: rows n0 ..
-// of b[e] [N, K]. Both advance BK * 2 bytes a K step.
+// of b[e] [N, K] (past N: zeros). Both advance BK * 2 bytes a K step.
 template <class Cfg>
 struct RowsBtSrc {
   __amdgpu_buffer_rsrc_t ra, rb;
@@ -155,7 +155,7 @@ __device__ __forceinline__ void rows_bt_tile(uint8_t* __restrict__ lds, const Ro
   ML::stage_tile(lds, acc, [](float v) { return v; });
   uint16_t* rows = p.out + static_cast<int64_t>(ch.row0) * p.n + n0;
   ML::for_each_staged_chunk(lds, [&](int r, int col, u32x4_t v) {
-    if (r < ch.rows) *reinterpret_cast<u32x4_t*>(rows + static_cast<int64_t>(r) * p.n + col) = v;
+    if (r < ch.rows && n0 + col < p.n) *reinterpret_cast<u32x4_t*>(rows + static_cast<int64_t>(r) * p.n + col) = v;
   });
 }
 
@@ -203,7 +203,7 @@ __device__ __forceinline__ void gated_slope_tile(uint8_t* __restrict__ lds, cons
     for (int q = threadIdx.x; q < Cfg::WM * kRun * kChunksPerRow; q += Cfg::kThreads) {
       const int m = q / kChunksPerRow, c = q % kChunksPerRow;
       const int r = m / kRun * Cfg::WTM + 32 * i0 + m % kRun;  // of the chunk
-      if (r >= ch.rows) continue;
+      if (r >= ch.rows || n0 + c * 8 >= p.ffn_dim) continue;
       const int64_t row = ch.row0 + r;
       const int64_t at = row * 2 * p.ffn_dim + n0 + c * 8;
       const u32x4_t gv = *reinterpret_cast<const u32x4_t*>(p.gu + at);
@@ -254,7 +254,7 @@ __global__ void __launch_bounds__(512) rows_bt_chunk_kernel(RowsBtArgs p) {
   __shared__ __attribute__((aligned(1024))) uint8_t lds[160 * 1024];
   Chunk ch{-1, 0, 0, 0};
   int slice = 0;
-  if (!gated_chunk_tile(static_cast<int>(blockIdx.x), p.n / kGatedBN, p.layout, &ch, &slice)) return;
+  if (!gated_chunk_tile(static_cast<int>(blockIdx.x), gated_slices(p.n), p.layout, &ch, &slice)) return;
   with_chunk_groups(ch.groups, [&](auto rc) {
     using Cfg = BtChunkCfg<decltype(rc)::value>;
     static_assert(Cfg::kLdsAlloc <= sizeof(lds) && Cfg::kThreads == 512, "one workgroup for all heights");
@@ -276,90 +276,13 @@ __global__ void __launch_bounds__(512) gated_slope_chunk_kernel(SlopeArgs p) {
   __shared__ __attribute__((aligned(1024))) uint8_t lds[160 * 1024];
   Chunk ch{-1, 0, 0, 0};
   int slice = 0;
-  if (!gated_chunk_tile(static_cast<int>(blockIdx.x), p.ffn_dim / kGatedBN, p.layout, &ch, &slice)) return;
+  if (!gated_chunk_tile(static_cast<int>(blockIdx.x), gated_slices(p.ffn_dim), p.layout, &ch, &slice)) return;
   with_chunk_groups(ch.groups, [&](auto rc) {
     using Cfg = BtChunkCfg<decltype(rc)::value>;
     static_assert(Cfg::kLdsAlloc <= sizeof(lds) && Cfg::kThreads == 512, "one workgroup for all heights");
     gated_slope_tile<Cfg, ACT>(lds, p, ch, slice * kGatedBN);
   });
 }
-
-// ------------------------------------------------- weight gradients ---
-
-// K step t: rows t BK .. of the expert's `rows` rows of a [P, M] and b [P, N].
-// Each step's buffers start at its first row and end at the expert's last
-// one, so rows past it read as zeros.
-template <class Cfg>
-struct OuterSrc {
-  const uint16_t *a, *b;  // the expert's first row, at the tile's first column
-  int32_t rows, m, n;
-  uint32_t a_off[Cfg::kAInstr], b_off[Cfg::kBInstr];
-  __device__ __forceinline__ uint32_t a_voff(int q) const { return a_off[q]; }
-  __device__ __forceinline__ uint32_t b_voff(int q) const { return b_off[q]; }
-  // The bytes from a tile's first column in a step's first row to its last
-  // column in the last row that is there.
-  __device__ __forceinline__ static uint32_t bytes(int32_t left, int32_t stride, int32_t width) {
-    return static_cast<uint32_t>((min(left, static_cast<int32_t>(Cfg::BK)) - 1) * stride + width) * 2u;
-  }
-  __device__ __forceinline__ void a_src(int t, __amdgpu_buffer_rsrc_t* r, uint32_t* s) const {
-    *r = make_rsrc(a + static_cast<int64_t>(t) * Cfg::BK * m, bytes(rows - t * Cfg::BK, m, Cfg::BM));
-    *s = 0;
-  }
-  __device__ __forceinline__ void b_src(int t, __amdgpu_buffer_rsrc_t* r, uint32_t* s) const {
-    *r = make_rsrc(b + static_cast<int64_t>(t) * Cfg::BK * n, bytes(rows - t * Cfg::BK, n, Cfg::BN));
-    *s = 0;
-  }
-};
-
-// Each expert's tiles over all XCDs, a contiguous part of them each: whatever
-// the routing, every XCD gets an eighth of each expert's K steps.
-constexpr int64_t outer_tiles(int64_t m, int64_t n) { return (m * n + kNumXcd - 1) / kNumXcd * kNumXcd; }
-
-// Two workgroups a CU (at most 128 registers a lane, 72 KB of LDS): one's
-// output and first loads overlap the other's products, which are few where an
-// expert has few rows.
-template <class Cfg>
-__global__ void __launch_bounds__(Cfg::kThreads) __attribute__((amdgpu_waves_per_eu(Cfg::kWaves / 2)))
-    expert_outer_kernel(const uint16_t* __restrict__ a, const uint16_t* __restrict__ b, GatedLayout layout,
-                        uint16_t* __restrict__ out, int32_t m, int32_t n) {
-  using ML = DmaMainloop<Cfg>;
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[Cfg::kLdsAlloc];
-  const int slices = n / Cfg::BN, row_tiles = m / Cfg::BM;
-  const int tiles = static_cast<int>(outer_tiles(row_tiles, slices));
-  const int e = uniform(static_cast<int>(blockIdx.x) / tiles);
-  const int tile = xcd_remap(static_cast<int>(blockIdx.x) - e * tiles, tiles);
-  if (tile >= row_tiles * slices) return;
-  int mt, nt;
-  tile_coords(tile, row_tiles, slices, kTileGroup, &mt, &nt);
-  const int m0 = mt * Cfg::BM, n0 = nt * Cfg::BN;
-  const int32_t rows = scalar_load(layout.tokens_per_expert + e);
-  const int32_t row0 = scalar_load(layout.padded_offsets + e);
-  if (row0 < 0 || row0 + rows > layout.max_row_blocks * kBS) return;  // not a routing layout
-  uint16_t* tile_out = out + (static_cast<int64_t>(e) * m + m0) * n + n0;
-
-  OuterSrc<Cfg> src;
-  src.a = a + static_cast<int64_t>(row0) * m + m0;
-  src.b = b + static_cast<int64_t>(row0) * n + n0;
-  src.rows = rows;
-  src.m = m;
-  src.n = n;
-  const AtDmaPos<Cfg> ap;
-#pragma unroll
-  for (int q = 0; q < Cfg::kAInstr; ++q) src.a_off[q] = (static_cast<uint32_t>(ap.row[q]) * m + ap.col[q]) * 2u;
-  const BDmaPos<Cfg> bp;
-#pragma unroll
-  for (int q = 0; q < Cfg::kBInstr; ++q) src.b_off[q] = (static_cast<uint32_t>(bp.row[q]) * n + bp.col[q]) * 2u;
-
-  typename ML::Acc acc;
-  ML::run(lds, src, (rows + Cfg::BK - 1) / Cfg::BK, acc);  // no rows: zeros
-  ML::stage_tile(lds, acc, [](float v) { return v; });
-  ML::for_each_staged_chunk(lds, [&](int r, int col, u32x4_t v) {
-    *reinterpret_cast<u32x4_t*>(tile_out + static_cast<int64_t>(r) * n + col) = v;
-  });
-}
-
-using OuterWide = DmaCfg<128, 256, 32, 3, 2, 4, 0, 0, 5, 1, 0, 0, 0, 1>;
-using OuterNarrow = DmaCfg<128, 128, 32, 3, 2, 2, 0, 0, 5, 1, 0, 0, 0, 1>;
 
 // A product's launch in the form that its columns take.
 template <class Args>
@@ -369,23 +292,12 @@ int launch_bt(void (*row_blocks)(Args), void (*chunk_form)(Args), const Args& ar
     return fail(SB_ERR_INVALID, "gated backward: not whole K steps");
   bool chunks = false;
   if (const int rc = gated_chunks(layout, num_copies, columns, &chunks)) return rc;
-  const int64_t grid = chunks ? gated_chunk_grid(layout, num_copies, columns / kGatedBN)
+  const int64_t grid = chunks ? gated_chunk_grid(layout, num_copies, gated_slices(columns))
                               : layout.max_row_blocks * (columns / BtNarrow::BN);
   if (grid > 2147483647LL) return fail(SB_ERR_INVALID, "problem too large");
   if (chunks) chunk_form<<<static_cast<uint32_t>(grid), 512, 0, stream>>>(args);
   else row_blocks<<<static_cast<uint32_t>(grid), BtNarrow::kThreads, 0, stream>>>(args);
   return check_launch("gated backward");
-}
-
-template <class Cfg>
-int run_outer(const void* a, const void* b, const GatedLayout& layout, void* out, int64_t m, int64_t n,
-              hipStream_t stream) {
-  const int64_t grid = layout.num_experts * outer_tiles(m / Cfg::BM, n / Cfg::BN);
-  if (grid > 2147483647LL) return fail(SB_ERR_INVALID, "problem too large");
-  expert_outer_kernel<Cfg><<<static_cast<uint32_t>(grid), Cfg::kThreads, 0, stream>>>(
-      static_cast<const uint16_t*>(a), static_cast<const uint16_t*>(b), layout, static_cast<uint16_t*>(out),
-      static_cast<int32_t>(m), static_cast<int32_t>(n));
-  return check_launch("gated backward: weight gradient");
 }
 
 }  // namespace
@@ -422,12 +334,6 @@ int launch_rows_bt(const void* a, const void* b, const GatedLayout& layout, void
   const RowsBtArgs args{static_cast<const uint16_t*>(a), static_cast<const uint16_t*>(b), layout,
                         static_cast<uint16_t*>(out), static_cast<int32_t>(n), static_cast<int32_t>(k)};
   return launch_bt(rows_bt_kernel, rows_bt_chunk_kernel, args, layout, num_copies, n, k, stream);
-}
-
-int launch_expert_outer(const void* a, const void* b, const GatedLayout& layout, void* out, int64_t m, int64_t n,
-                        hipStream_t stream) {
-  return n % 256 == 0 ? run_outer<OuterWide>(a, b, layout, out, m, n, stream)
-                      : run_outer<OuterNarrow>(a, b, layout, out, m, n, stream);
 }
 
 }  // namespace sb

@@ -244,12 +244,8 @@ extern "C" int sb_gated_backward(const void* grad_out, const void* x, const void
   if (int rc = launch_sum_copies(b.dxr, s.routing.copy_row, grad_x, p.num_tokens, k, d_model, p.max_rows, valid_tokens,
                                  st))
     return rc;
-  if (outer_stream_fits(d_model, 2 * ffn_dim) && outer_stream_fits(ffn_dim, d_model)) {
-    const int rc = launch_expert_outers(b.xg, b.grad_gu, grad_w1, d_model, 2 * ffn_dim, b.wh, b.gog, grad_w2, ffn_dim,
-                                        d_model, l, st);
-    return rc ? rc : clear_ok();
-  }
-  if (int rc = launch_expert_outer(b.xg, b.grad_gu, l, grad_w1, d_model, 2 * ffn_dim, st)) return rc;
-  if (int rc = launch_expert_outer(b.wh, b.gog, l, grad_w2, ffn_dim, d_model, st)) return rc;
+  if (int rc = launch_expert_outers(b.xg, b.grad_gu, grad_w1, d_model, 2 * ffn_dim, b.wh, b.gog, grad_w2, ffn_dim,
+                                    d_model, l, st))
+    return rc;
   return clear_ok();
 }

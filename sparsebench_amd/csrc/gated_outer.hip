@@ -9,14 +9,17 @@
 // while the one before it is computed and written. The finished tile leaves
 // through LDS of its own (the ring stays in use). D = 1024, F = 4096, E = 64, 128
 // rows an expert, both products: 567 us as workgroups of their own, whatever the
-// tile (each took 11 us, most of it its start and its first loads), 473 this way;
+// tile (each took 11 us, most of it its start and its first loads), 470 this way;
 // 240 is the write alone (1.6 GB at 6.9 TB/s), 284 all but the output. D = 4096,
-// F = 14336, E = 8, 512 rows an expert 1750 us, 825 TFLOP/s: there a K step takes 1.0
+// F = 14336, E = 8, 512 rows an expert 1730 us, 835 TFLOP/s: there a K step takes 1.0
 // us, twice its MFMAs. Both operands are read transposed (ds_read_b64_tr), 98
 // KB of LDS a step, and these reads run at half the rate of the others.
 //
 // Tile 256 x 256, 8 waves (2 x 4, 128 x 64 each), K steps of 32 through a
-// 4-stage ring (128 KB), the output in four parts of 64 rows through 32 KB.
+// 4-stage ring (128 KB), the output in four parts of 64 rows through 32 KB. A
+// side that 256 do not divide ends in half a tile: what its loads find past the
+// edge are other columns' values (or zeros, past the last row), and meets only
+// results that are not written.
 // Each expert's tiles go over all XCDs, a contiguous part of them each, so
 // whatever the routing every CU gets its share of each expert's K steps.
 
@@ -25,7 +28,7 @@
 namespace sb {
 namespace {
 
-using Cfg = DmaCfg<256, 256, 32, 4, 2, 4, 0, 0, 3, 1, 0, 0, 0, 1>;
+using Cfg = DmaCfg<256, 256, 32, 4, 2, 4, 0, 0, 4, 1, 0, 0, 0, 1>;
 using ML = DmaMainloop<Cfg>;
 constexpr int kRing = Cfg::STAGES * Cfg::kStageBytes;
 constexpr int kPartRows = 64, kPartBytes = kPartRows * Cfg::BN * 2;
@@ -51,11 +54,16 @@ struct Tile {
   const uint16_t *a, *b;
   uint16_t* out;
   int32_t m, n, rows;
+  int32_t height, width;  // up to 256
 };
 
 // The K steps of a tile; one, of rows past the expert's last (zeros), for an
 // expert without rows.
 __device__ __forceinline__ int steps_of(const Tile& t) { return max(1, (t.rows + Cfg::BK - 1) / Cfg::BK); }
+
+__host__ __device__ __forceinline__ int tiles_over(int64_t length, int tile) {
+  return static_cast<int>((length + tile - 1) / tile);
+}
 
 // 64 tiles of the workgroup's list, one a lane: worked out together (the
 // divisions and the loads of an expert's rows take microseconds one by one),
@@ -77,8 +85,8 @@ struct Batch {
     const int part = per / kNumXcd, rem = per % kNumXcd, x = j % kNumXcd;
     const int tile = (x < rem ? x * (part + 1) : rem * (part + 1) + (x - rem) * part) + j / kNumXcd;
     // Groups of kTileGroup tile rows, walked down one column at a time.
-    const int row_tiles = (which ? args.p[1].m : args.p[0].m) / Cfg::BM;
-    const int slices = (which ? args.p[1].n : args.p[0].n) / Cfg::BN;
+    const int row_tiles = tiles_over(which ? args.p[1].m : args.p[0].m, Cfg::BM);
+    const int slices = tiles_over(which ? args.p[1].n : args.p[0].n, Cfg::BN);
     const int group = tile / (kTileGroup * slices);
     const int height = min(kTileGroup, row_tiles - group * kTileGroup);
     const int in = tile - group * kTileGroup * slices;
@@ -100,13 +108,15 @@ struct Batch {
     t.a = (second ? args.p[1].a : args.p[0].a) + first_row * t.m + m0;
     t.b = (second ? args.p[1].b : args.p[0].b) + first_row * t.n + n0;
     t.out = (second ? args.p[1].out : args.p[0].out) + (e * t.m + m0) * t.n + n0;
+    t.height = min(t.m - static_cast<int32_t>(m0), static_cast<int32_t>(Cfg::BM));
+    t.width = min(t.n - static_cast<int32_t>(n0), static_cast<int32_t>(Cfg::BN));
     return t;
   }
 };
 
 // This wave's loads of one step into a slot: operator()(q), q < kCount, issues
 // one (A's, then B's). The buffers start at the step's first row and end at the
-// expert's last one: rows past it read as zeros. Issued from within
+// tile's last column in the expert's last one: rows past it read as zeros. Issued from within
 // ML::compute, through a __restrict__ pointer to another slot than the one
 // that is read there: otherwise the compiler waits for them before each read.
 struct StepLoads {
@@ -123,9 +133,9 @@ struct StepLoads {
     const int left = min(t.rows - step * Cfg::BK, static_cast<int>(Cfg::BK));
     const bool some = left > 0;  // past the last tile: empty buffers, no read of memory
     ra = make_rsrc(t.a + static_cast<int64_t>(step) * Cfg::BK * m,
-                   some ? static_cast<uint32_t>((left - 1) * m + Cfg::BM) * 2u : 0u);
+                   some ? static_cast<uint32_t>((left - 1) * m + t.height) * 2u : 0u);
     rb = make_rsrc(t.b + static_cast<int64_t>(step) * Cfg::BK * n,
-                   some ? static_cast<uint32_t>((left - 1) * n + Cfg::BN) * 2u : 0u);
+                   some ? static_cast<uint32_t>((left - 1) * n + t.width) * 2u : 0u);
   }
   __device__ __forceinline__ void operator()(int q) const {
     if (q < Cfg::kAInstr)
@@ -157,15 +167,18 @@ __device__ __forceinline__ void write_part(uint8_t* __restrict__ stage, const Ti
                   pack_bf16x2(acc[jn][P][4 * g + 2], acc[jn][P][4 * g + 3])};
     }
   lds_barrier();
+  // Places past the tile's edges are out of the buffer, so every lane's stores
+  // are issued, whatever the tile: the loop's waits count them.
+  const auto out = make_rsrc(t.out, static_cast<uint32_t>((t.height - 1) * t.n + t.width) * 2u);
 #pragma unroll
   for (int s = 0; s < kStores; ++s) {
     const int q = s * Cfg::kThreads + static_cast<int>(threadIdx.x);
     const int r = q / (Cfg::BN / 8), c = q % (Cfg::BN / 8);
     const u32x4_t v = *reinterpret_cast<const u32x4_t*>(stage + staged_at<Cfg::BN * 2>(r, c));
+    const uint32_t at = static_cast<uint32_t>((r / 32 * Cfg::WTM + 32 * P + r % 32) * t.n + c * 8) * 2u;
     // Past the caches: the gradients are read next by another call, and what
     // they would displace is read by this one.
-    __builtin_nontemporal_store(
-        v, reinterpret_cast<u32x4_t*>(t.out + static_cast<int64_t>(r / 32 * Cfg::WTM + 32 * P + r % 32) * t.n + c * 8));
+    __builtin_amdgcn_raw_buffer_store_b128(v, out, c * 8 < t.width ? at : kOutOfRange, 0, 2);  // nt
   }
 }
 
@@ -239,8 +252,6 @@ __global__ void __launch_bounds__(Cfg::kThreads) expert_outer_stream_kernel(Oute
 
 }  // namespace
 
-bool outer_stream_fits(int64_t m, int64_t n) { return m % Cfg::BM == 0 && n % Cfg::BN == 0; }
-
 int launch_expert_outers(const void* a1, const void* b1, void* out1, int64_t m1, int64_t n1, const void* a2,
                          const void* b2, void* out2, int64_t m2, int64_t n2, const GatedLayout& layout,
                          hipStream_t stream) {
@@ -250,7 +261,7 @@ int launch_expert_outers(const void* a1, const void* b1, void* out1, int64_t m1,
   auto product = [&](int i, const void* a, const void* b, void* out, int64_t m, int64_t n) {
     args.p[i] = Product{static_cast<const uint16_t*>(a), static_cast<const uint16_t*>(b), static_cast<uint16_t*>(out),
                         static_cast<int32_t>(m), static_cast<int32_t>(n)};
-    const int64_t tiles = (m / Cfg::BM) * (n / Cfg::BN);
+    const int64_t tiles = static_cast<int64_t>(tiles_over(m, Cfg::BM)) * tiles_over(n, Cfg::BN);
     args.tiles[i] = static_cast<int32_t>(tiles);
     args.total[i] = static_cast<int32_t>(tiles * layout.num_experts);
     return tiles * layout.num_experts;
@@ -259,7 +270,9 @@ int launch_expert_outers(const void* a1, const void* b1, void* out1, int64_t m1,
   const int64_t total = product(0, a1, b1, out1, m1, n1) + product(1, a2, b2, out2, m2, n2);
   // Whole eighths of workgroups, so that each keeps to its XCD's tiles.
   const int64_t grid = std::max<int64_t>(kNumXcd, std::min<int64_t>(total, cus) / kNumXcd * kNumXcd);
-  if (total + 192 * grid > 2147483647LL || std::max(m1, m2) / Cfg::BM > 65535 || std::max(n1, n2) / Cfg::BN > 32767) return fail(SB_ERR_INVALID, "problem too large");
+  if (total + 192 * grid > 2147483647LL || tiles_over(std::max(m1, m2), Cfg::BM) > 65535 ||
+      tiles_over(std::max(n1, n2), Cfg::BN) > 32767)
+    return fail(SB_ERR_INVALID, "problem too large");
   expert_outer_stream_kernel<<<static_cast<uint32_t>(grid), Cfg::kThreads, 0, stream>>>(args);
   return check_launch("gated backward: weight gradients");
 }

@@ -60,6 +60,16 @@ def test_matches_64_bits(shape, act) -> None:
     check_all(make(*shape, seed=sum(shape)), act)
 
 
+# D and F that 256 do not divide, with enough row blocks for the chunk form:
+# short and tall experts (chunks of 64 to 320 rows, several an expert).
+EDGES = [(64, 2, 64, 640, 128), (40, 1, 70, 128, 896), (900, 3, 9, 384, 640), (2500, 2, 6, 896, 384)]
+
+
+@pytest.mark.parametrize("shape", EDGES)
+def test_half_slices(shape) -> None:
+    check_all(make(*shape, seed=sum(shape)))
+
+
 @pytest.mark.parametrize("gate_dtype", GATES)
 @pytest.mark.parametrize("index", [torch.int32, torch.int64])
 def test_gate_and_index_types(gate_dtype, index) -> None:
