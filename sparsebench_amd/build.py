@@ -30,7 +30,7 @@ PROBE_LIB_NAME = "libsparsebench_probe.so"
 ARCH = "gfx950"
 
 SOURCES = ["probe.hip", "routing.hip", "sdd.hip", "dsd.hip", "combine.hip", "assigned.hip", "router.hip", "experts.hip", "layer.hip",
-           "gated.hip", "gated_few.hip", "gated_grad.hip", "gated_outer.hip", "gated_layer.hip", "adamw.hip"]
+           "gated.hip", "gated_few.hip", "gated_grad.hip", "gated_outer.hip", "gated_down.hip", "gated_layer.hip", "adamw.hip"]
 PROBE_SOURCES = ["read_probe.hip", "schedule_shims.hip"]
 
 HIPCC_FLAGS = [

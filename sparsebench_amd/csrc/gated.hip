@@ -141,13 +141,12 @@ int launch_up(const UpArgs& a, hipStream_t stream) {
 }
 
 template <bool kKeep, int ACT>
-int launch_up_form(const UpArgs& a, int64_t num_copies, bool chunks, hipStream_t stream) {
+int launch_up_form(const UpArgs& a, const GatedForm& form, hipStream_t stream) {
   if (sdd_wide_x(a.num_tokens, a.d_model)) return launch_up<GatedMid, true, kKeep, ACT>(a, stream);
-  if (!chunks) return launch_up<GatedNarrow, false, kKeep, ACT>(a, stream);
-  const int64_t grid = gated_chunk_grid(a.layout, num_copies, a.ffn_dim / (kGatedBN / 2));
-  if (!reduction_fits<GatedUpCfg<kGatedRmax>>(a.d_model) || grid > 2147483647LL)
+  if (!form.chunks) return launch_up<GatedNarrow, false, kKeep, ACT>(a, stream);
+  if (!reduction_fits<GatedUpCfg<kGatedRmax>>(a.d_model) || form.grid > 2147483647LL)
     return fail(SB_ERR_INVALID, "problem too large");
-  gated_up_chunk_kernel<kKeep, ACT><<<static_cast<uint32_t>(grid), 512, 0, stream>>>(a);
+  gated_up_chunk_kernel<kKeep, ACT><<<static_cast<uint32_t>(form.grid), 512, 0, stream>>>(a);
   return check_launch("gated experts");
 }
 
@@ -158,13 +157,13 @@ int launch_gated_up(const void* x, const void* w1, const GatedLayout& layout, vo
   const UpArgs a{static_cast<const uint16_t*>(x), static_cast<const uint16_t*>(w1), layout,
                  static_cast<uint16_t*>(h), static_cast<uint16_t*>(gu), static_cast<int32_t>(num_tokens),
                  static_cast<int32_t>(d_model), static_cast<int32_t>(ffn_dim)};
-  bool chunks = false;
-  if (const int rc = gated_chunks(layout, num_copies, 2 * ffn_dim, &chunks)) return rc;
+  // H is a product of two sums: not split.
+  const GatedForm form = gated_form(layout.max_row_blocks, layout.num_experts, num_copies, 2 * ffn_dim, d_model, false);
   if (gu)
-    return act == SB_ACT_SILU ? launch_up_form<true, SB_ACT_SILU>(a, num_copies, chunks, stream)
-                              : launch_up_form<true, SB_ACT_GELU>(a, num_copies, chunks, stream);
-  return act == SB_ACT_SILU ? launch_up_form<false, SB_ACT_SILU>(a, num_copies, chunks, stream)
-                            : launch_up_form<false, SB_ACT_GELU>(a, num_copies, chunks, stream);
+    return act == SB_ACT_SILU ? launch_up_form<true, SB_ACT_SILU>(a, form, stream)
+                              : launch_up_form<true, SB_ACT_GELU>(a, form, stream);
+  return act == SB_ACT_SILU ? launch_up_form<false, SB_ACT_SILU>(a, form, stream)
+                            : launch_up_form<false, SB_ACT_GELU>(a, form, stream);
 }
 
 }  // namespace sb

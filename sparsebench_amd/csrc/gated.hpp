@@ -11,6 +11,9 @@
 // Rows past an expert's real rows are neither written nor read.
 #pragma once
 
+#include <algorithm>
+#include <limits>
+
 #include "common.hpp"
 #include "expert_chunks.hpp"
 #include "gemm_dma.hpp"
@@ -48,9 +51,17 @@ int launch_gated_slope(const void* gog, const void* w2, const void* gu, const fl
                        const GatedLayout& layout, void* grad_gu, void* wh, int64_t num_copies, int64_t d_model,
                        int64_t ffn_dim, int32_t act, hipStream_t stream);
 
-// out[P, N] = a[P, K] b[e]^T, b [E, N, K].
-int launch_rows_bt(const void* a, const void* b, const GatedLayout& layout, void* out, int64_t num_copies, int64_t n,
-                   int64_t k, hipStream_t stream);
+// y[P, D] = H W2[e] (gated_down.hip). partial: gated_form's parts (1: unused) of [P, D].
+int launch_gated_down(const void* h, const void* w2, const GatedLayout& layout, void* out, float* partial,
+                      int64_t num_copies, int64_t d_model, int64_t ffn_dim, hipStream_t stream);
+
+// out[P, N] = a[P, K] b[e]^T, b [E, N, K]. partial: gated_form's parts (1: unused) of [P, N].
+int launch_rows_bt(const void* a, const void* b, const GatedLayout& layout, void* out, float* partial,
+                   int64_t num_copies, int64_t n, int64_t k, hipStream_t stream);
+
+// out[r] = sum over parts of partial[s][r], for rows with a token.
+int launch_join_parts(const float* partial, const GatedLayout& layout, void* out, int32_t parts, int64_t columns,
+                      hipStream_t stream);
 
 // out1[e] [M, N] = sum over e's rows of a1[r]^T b1[r], a1 [P, M], b1 [P, N],
 // and out2 likewise, in one launch; zeros for an expert with no rows.
@@ -183,22 +194,90 @@ __device__ __forceinline__ bool gated_chunk_tile(int bid, int slices, const Gate
          ch->row0 + ch->rows <= l.max_row_blocks * kBS;
 }
 
-// Workgroups of the chunk form: an expert of n rows has ceil(n / 256) chunks,
-// (one less if the
-// last piece joins the one before), so N copies at most N / 256 + min(E, N).
-inline int64_t gated_chunk_grid(const GatedLayout& l, int64_t num_copies, int64_t slices) {
-  return std::min<int64_t>(l.max_row_blocks,
-                           num_copies / Chunking<kGatedRmax>::kRows + std::min<int64_t>(l.num_experts, num_copies)) *
-         slices;
+// How a product of `columns` columns and a reduction over k runs on a layout.
+struct GatedForm {
+  bool chunks;    // the chunk form, else row blocks in 128-wide tiles
+  int32_t parts;  // of the reduction, each a workgroup's
+  int64_t grid;
+};
+
+// Row blocks while their 128-wide tiles have a CU each (each live row block
+// holds a copy at least), chunks once those fill the CUs too; in between, and
+// for the parts of the reduction, whatever this estimate of the time makes
+// shortest. A round of workgroups takes 3 us and 0.65 us for 64 of the reduction
+// (128 x 128 tiles; up to 4 times that for chunks of 256 rows), and the sum of
+// the parts 6 us and its bytes at 5 TB/s. (E = 3, D = 384, F = 6400, 54 copies: y = H
+// W2 in 9 tiles 61 us, in 16 parts 9 and their sum 6.5; E = 8, D = 256, F = 6016, 16704
+// copies: dXr in 66 chunk tiles 364 us, in 3 parts 181 and 11.) The CUs are
+// counted as 256 whatever the device, so that the workspace's size and the order
+// of the sums do not depend on it.
+inline GatedForm gated_form(int64_t max_row_blocks, int64_t num_experts, int64_t num_copies, int64_t columns,
+                            int64_t k, bool splits) {
+  constexpr int64_t kCus = 256;
+  const int64_t narrow = std::min(max_row_blocks, num_copies) * (columns / 128);
+  // An expert of n rows has ceil(n / 256) chunks, or one less if the last piece
+  // joins the one before, so N copies at most N / 256 + min(E, N).
+  const int64_t chunks =
+      std::min(max_row_blocks, num_copies / Chunking<kGatedRmax>::kRows + std::min(num_experts, num_copies));
+  const int64_t wide = chunks * gated_slices(columns);
+  GatedForm best{true, 1, wide};
+  double least = std::numeric_limits<double>::infinity();
+  auto consider = [&](bool is_chunks, int64_t busy, int64_t tiles, double step_us) {
+    const int64_t most = splits ? std::min<int64_t>(16, k / 256) : 1;
+    for (int64_t parts = 1; parts <= std::max<int64_t>(1, most); ++parts) {
+      const int64_t rounds = (busy * parts + kCus - 1) / kCus, steps = (k / 64 + parts - 1) / parts;
+      const double sum_us = parts > 1 ? 6.0 + static_cast<double>(parts * num_copies) * columns * 8 / 5e6 : 0.0;
+      const double us = rounds * (3.0 + step_us * steps) + sum_us;
+      if (us < least) best = GatedForm{is_chunks, static_cast<int32_t>(parts), tiles * parts}, least = us;
+    }
+  };
+  if (narrow <= kCus || wide < kCus) consider(false, narrow, max_row_blocks * (columns / 128), 0.65);
+  if (narrow > kCus && wide < kCus)
+    consider(true, wide, wide, 0.65 * (1.0 + 3.0 * std::min(1.0, static_cast<double>(num_copies) / (256.0 * chunks))));
+  return best;
 }
 
-// Whether `columns` columns run in the chunk form: when 128-wide tiles of the
-// row blocks have no CU each. (Each live row block holds a copy at least.)
-inline int gated_chunks(const GatedLayout& l, int64_t num_copies, int64_t columns, bool* chunks) {
-  int cus = 0;
-  if (const int rc = device_cus(&cus)) return rc;
-  *chunks = std::min<int64_t>(l.max_row_blocks, num_copies) * (columns / 128) > cus;
-  return SB_OK;
+// Where a split product's parts go: [parts, P, columns] sums.
+struct SplitOut {
+  float* partial;
+  int32_t parts, tiles;  // tiles of each part
+};
+inline SplitOut split_out(const GatedForm& f, float* partial) {
+  return {partial, f.parts, static_cast<int32_t>(f.grid / f.parts)};
+}
+
+// Workgroup *tile of a split product -> its tile and part.
+__device__ __forceinline__ void split_tile(const SplitOut& s, int* tile, int* part) {
+  *part = uniform(*tile / s.tiles);
+  *tile -= *part * s.tiles;
+}
+
+// The first of `blocks` that part i of `parts` takes.
+__device__ __forceinline__ int split_start(int i, int parts, int blocks) {
+  return static_cast<int>(static_cast<int64_t>(i) * blocks / parts);
+}
+
+// A tile of part `part`, straight from the accumulators: a lane's 4 columns of
+// a row at a time (the two halves of the wave side by side).
+template <class Cfg>
+__device__ __forceinline__ void store_part(const SplitOut& s, const typename DmaMainloop<Cfg>::Acc& acc, int part,
+                                           const GatedLayout& l, const Chunk& ch, int n0, int columns) {
+  using ML = DmaMainloop<Cfg>;
+  float* out = s.partial + (static_cast<int64_t>(part) * l.max_row_blocks * kBS + ch.row0) * columns + n0;
+#pragma unroll
+  for (int i = 0; i < Cfg::TM; ++i) {
+    const int r = ML::out_row(i);
+    if (r >= ch.rows) continue;
+#pragma unroll
+    for (int jn = 0; jn < Cfg::TN; ++jn)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int col = ML::out_col(jn, g);
+        if (n0 + col < columns)
+          *reinterpret_cast<f32x4_t*>(out + static_cast<int64_t>(r) * columns + col) = f32x4_t{
+              acc[jn][i][4 * g], acc[jn][i][4 * g + 1], acc[jn][i][4 * g + 2], acc[jn][i][4 * g + 3]};
+      }
+  }
 }
 
 // LDS offset of 16-byte chunk `chunk` of row r in a staged tile of ROW_BYTES

@@ -123,11 +123,12 @@ struct RowsBtSrc {
     *r = rb;
     *s = static_cast<uint32_t>(t) * (Cfg::BK * 2);
   }
+  // The reduction starts at column k0 of the k.
   __device__ __forceinline__ RowsBtSrc(const uint16_t* a, const uint16_t* b, const Chunk& ch, int32_t n0, int32_t n,
-                                       int32_t k) {
-    ra = make_rsrc(a + static_cast<int64_t>(ch.row0) * k, static_cast<uint32_t>(ch.rows) * k * 2u);
-    rb = make_rsrc(b + static_cast<int64_t>(ch.expert) * n * k,
-                   static_cast<uint32_t>(n) * static_cast<uint32_t>(k) * 2u);
+                                       int32_t k, int32_t k0) {
+    ra = make_rsrc(a + static_cast<int64_t>(ch.row0) * k + k0, (static_cast<uint32_t>(ch.rows) * k - k0) * 2u);
+    rb = make_rsrc(b + static_cast<int64_t>(ch.expert) * n * k + k0,
+                   (static_cast<uint32_t>(n) * static_cast<uint32_t>(k) - k0) * 2u);
     const ADmaPos<Cfg> ap;
 #pragma unroll
     for (int q = 0; q < Cfg::kAInstr; ++q)
@@ -143,20 +144,28 @@ struct RowsBtArgs {
   const uint16_t *a, *b;
   GatedLayout layout;
   uint16_t* out;
+  SplitOut split;
   int32_t n, k;
 };
 
-template <class Cfg>
-__device__ __forceinline__ void rows_bt_tile(uint8_t* __restrict__ lds, const RowsBtArgs& p, const Chunk& ch, int n0) {
+template <class Cfg, bool kSplit>
+__device__ __forceinline__ void rows_bt_tile(uint8_t* __restrict__ lds, const RowsBtArgs& p, const Chunk& ch, int n0,
+                                             int part) {
   using ML = DmaMainloop<Cfg>;
-  const RowsBtSrc<Cfg> src(p.a, p.b, ch, n0, p.n, p.k);
+  const int k0 = kSplit ? split_start(part, p.split.parts, p.k / kBS) * kBS : 0;
+  const int k1 = kSplit ? split_start(part + 1, p.split.parts, p.k / kBS) * kBS : p.k;
+  const RowsBtSrc<Cfg> src(p.a, p.b, ch, n0, p.n, p.k, k0);
   typename ML::Acc acc;
-  ML::run(lds, src, p.k / Cfg::BK, acc);
-  ML::stage_tile(lds, acc, [](float v) { return v; });
-  uint16_t* rows = p.out + static_cast<int64_t>(ch.row0) * p.n + n0;
-  ML::for_each_staged_chunk(lds, [&](int r, int col, u32x4_t v) {
-    if (r < ch.rows && n0 + col < p.n) *reinterpret_cast<u32x4_t*>(rows + static_cast<int64_t>(r) * p.n + col) = v;
-  });
+  ML::run(lds, src, (k1 - k0) / Cfg::BK, acc);
+  if constexpr (kSplit) {
+    store_part<Cfg>(p.split, acc, part, p.layout, ch, n0, p.n);
+  } else {
+    ML::stage_tile(lds, acc, [](float v) { return v; });
+    uint16_t* rows = p.out + static_cast<int64_t>(ch.row0) * p.n + n0;
+    ML::for_each_staged_chunk(lds, [&](int r, int col, u32x4_t v) {
+      if (r < ch.rows && n0 + col < p.n) *reinterpret_cast<u32x4_t*>(rows + static_cast<int64_t>(r) * p.n + col) = v;
+    });
+  }
 }
 
 struct SlopeArgs {
@@ -178,7 +187,7 @@ __device__ __forceinline__ void gated_slope_tile(uint8_t* __restrict__ lds, cons
   // Row groups of a wave in one part, and the part's rows: Cfg::WM runs of them.
   constexpr int kGroups = 4 / Cfg::WM < Cfg::TM ? 4 / Cfg::WM : Cfg::TM;
   constexpr int kParts = (Cfg::TM + kGroups - 1) / kGroups;
-  const RowsBtSrc<Cfg> src(p.gog, p.w2, ch, n0, p.ffn_dim, p.d_model);
+  const RowsBtSrc<Cfg> src(p.gog, p.w2, ch, n0, p.ffn_dim, p.d_model, 0);
   typename ML::Acc acc;
   ML::run(lds, src, p.d_model / Cfg::BK, acc);
 
@@ -242,23 +251,27 @@ using BtNarrow = DmaCfg<128, 128, 64, 3, 2, 2, 0, 0, 5, 1, 0, 0, 0, 0, 1>;
 template <int BN>
 constexpr int slope_lds(int ring) { return ring > kBS * BN * 4 ? ring : kBS * BN * 4; }
 
+template <bool kSplit>
 __global__ void __launch_bounds__(BtNarrow::kThreads) rows_bt_kernel(RowsBtArgs p) {
   __shared__ __attribute__((aligned(1024))) uint8_t lds[BtNarrow::kLdsAlloc];
   Chunk ch;
-  int slice;
-  if (!row_block_tile(static_cast<int>(blockIdx.x), p.n / BtNarrow::BN, p.layout, &ch, &slice)) return;
-  rows_bt_tile<BtNarrow>(lds, p, ch, slice * BtNarrow::BN);
+  int slice, part = 0, tile = static_cast<int>(blockIdx.x);
+  if constexpr (kSplit) split_tile(p.split, &tile, &part);
+  if (!row_block_tile(tile, p.n / BtNarrow::BN, p.layout, &ch, &slice)) return;
+  rows_bt_tile<BtNarrow, kSplit>(lds, p, ch, slice * BtNarrow::BN, part);
 }
 
+template <bool kSplit>
 __global__ void __launch_bounds__(512) rows_bt_chunk_kernel(RowsBtArgs p) {
   __shared__ __attribute__((aligned(1024))) uint8_t lds[160 * 1024];
   Chunk ch{-1, 0, 0, 0};
-  int slice = 0;
-  if (!gated_chunk_tile(static_cast<int>(blockIdx.x), gated_slices(p.n), p.layout, &ch, &slice)) return;
+  int slice = 0, part = 0, tile = static_cast<int>(blockIdx.x);
+  if constexpr (kSplit) split_tile(p.split, &tile, &part);
+  if (!gated_chunk_tile(tile, gated_slices(p.n), p.layout, &ch, &slice)) return;
   with_chunk_groups(ch.groups, [&](auto rc) {
     using Cfg = BtChunkCfg<decltype(rc)::value>;
     static_assert(Cfg::kLdsAlloc <= sizeof(lds) && Cfg::kThreads == 512, "one workgroup for all heights");
-    rows_bt_tile<Cfg>(lds, p, ch, slice * kGatedBN);
+    rows_bt_tile<Cfg, kSplit>(lds, p, ch, slice * kGatedBN, part);
   });
 }
 
@@ -284,19 +297,15 @@ __global__ void __launch_bounds__(512) gated_slope_chunk_kernel(SlopeArgs p) {
   });
 }
 
-// A product's launch in the form that its columns take.
+// A product's launch in its form.
 template <class Args>
-int launch_bt(void (*row_blocks)(Args), void (*chunk_form)(Args), const Args& args, const GatedLayout& layout,
-              int64_t num_copies, int64_t columns, int64_t k, hipStream_t stream) {
+int launch_bt(void (*row_blocks)(Args), void (*chunk_form)(Args), const Args& args, const GatedForm& form, int64_t k,
+              hipStream_t stream) {
   if (!reduction_fits<BtNarrow>(k) || !reduction_fits<BtChunkCfg<kGatedRmax>>(k))
     return fail(SB_ERR_INVALID, "gated backward: not whole K steps");
-  bool chunks = false;
-  if (const int rc = gated_chunks(layout, num_copies, columns, &chunks)) return rc;
-  const int64_t grid = chunks ? gated_chunk_grid(layout, num_copies, gated_slices(columns))
-                              : layout.max_row_blocks * (columns / BtNarrow::BN);
-  if (grid > 2147483647LL) return fail(SB_ERR_INVALID, "problem too large");
-  if (chunks) chunk_form<<<static_cast<uint32_t>(grid), 512, 0, stream>>>(args);
-  else row_blocks<<<static_cast<uint32_t>(grid), BtNarrow::kThreads, 0, stream>>>(args);
+  if (form.grid > 2147483647LL) return fail(SB_ERR_INVALID, "problem too large");
+  if (form.chunks) chunk_form<<<static_cast<uint32_t>(form.grid), 512, 0, stream>>>(args);
+  else row_blocks<<<static_cast<uint32_t>(form.grid), BtNarrow::kThreads, 0, stream>>>(args);
   return check_launch("gated backward");
 }
 
@@ -323,17 +332,23 @@ int launch_gated_slope(const void* gog, const void* w2, const void* gu, const fl
   const SlopeArgs args{static_cast<const uint16_t*>(gog), static_cast<const uint16_t*>(w2),
                        static_cast<const uint16_t*>(gu), row_gate, layout, static_cast<uint16_t*>(grad_gu),
                        static_cast<uint16_t*>(wh), static_cast<int32_t>(d_model), static_cast<int32_t>(ffn_dim)};
+  // dG and dU are products with the whole sum: not split.
+  const GatedForm form = gated_form(layout.max_row_blocks, layout.num_experts, num_copies, ffn_dim, d_model, false);
   return act == SB_ACT_SILU ? launch_bt(gated_slope_kernel<SB_ACT_SILU>, gated_slope_chunk_kernel<SB_ACT_SILU>, args,
-                                        layout, num_copies, ffn_dim, d_model, stream)
+                                        form, d_model, stream)
                             : launch_bt(gated_slope_kernel<SB_ACT_GELU>, gated_slope_chunk_kernel<SB_ACT_GELU>, args,
-                                        layout, num_copies, ffn_dim, d_model, stream);
+                                        form, d_model, stream);
 }
 
-int launch_rows_bt(const void* a, const void* b, const GatedLayout& layout, void* out, int64_t num_copies, int64_t n,
-                   int64_t k, hipStream_t stream) {
+int launch_rows_bt(const void* a, const void* b, const GatedLayout& layout, void* out, float* partial,
+                   int64_t num_copies, int64_t n, int64_t k, hipStream_t stream) {
+  const GatedForm form = gated_form(layout.max_row_blocks, layout.num_experts, num_copies, n, k, true);
   const RowsBtArgs args{static_cast<const uint16_t*>(a), static_cast<const uint16_t*>(b), layout,
-                        static_cast<uint16_t*>(out), static_cast<int32_t>(n), static_cast<int32_t>(k)};
-  return launch_bt(rows_bt_kernel, rows_bt_chunk_kernel, args, layout, num_copies, n, k, stream);
+                        static_cast<uint16_t*>(out), split_out(form, partial), static_cast<int32_t>(n),
+                        static_cast<int32_t>(k)};
+  if (form.parts == 1) return launch_bt(rows_bt_kernel<false>, rows_bt_chunk_kernel<false>, args, form, k, stream);
+  if (const int rc = launch_bt(rows_bt_kernel<true>, rows_bt_chunk_kernel<true>, args, form, kBS, stream)) return rc;
+  return launch_join_parts(partial, layout, out, form.parts, n, stream);
 }
 
 }  // namespace sb

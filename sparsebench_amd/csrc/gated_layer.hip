@@ -24,7 +24,10 @@ int check_problem(int64_t num_tokens, int32_t k, int32_t num_experts, int64_t d_
       ffn_dim >= kI32Limit)
     return fail(SB_ERR_INVALID, "gated experts: D (%lld) and F (%lld) must be multiples of 128",
                 static_cast<long long>(d_model), static_cast<long long>(ffn_dim));
-  // W1[e] and W2[e] are read with 32-bit buffer offsets.
+  // A chunk's rows (320 at most) of [P, 2F] and [P, D], W1[e] and W2[e] are
+  // read with 32-bit buffer offsets.
+  if (std::max(d_model, 2 * ffn_dim) * (32 * kGatedRmax * 2) >= kI32Limit)
+    return fail(SB_ERR_INVALID, "gated experts: D or F too large for 32-bit buffer offsets");
   if (d_model * ffn_dim * 4 >= kI32Limit)
     return fail(SB_ERR_INVALID, "gated experts: one expert's weights too large for 32-bit buffer offsets");
   *p = Problem{num_tokens, num_experts, d_model, ffn_dim, k, num_tokens * k, 0, 0, 0};
@@ -73,15 +76,23 @@ SavedBuffers carve_saved(Carver& ws, const Problem& p) {
   return b;
 }
 
+// A split product's parts, if it is split.
+float* take_parts(Carver& ws, const Problem& p, int64_t columns, int64_t k) {
+  const GatedForm form = gated_form(p.max_row_blocks, p.num_experts, p.num_copies, columns, k, true);
+  return ws.take<float>(form.parts > 1 ? form.parts * p.max_rows * columns : 0);
+}
+
 struct TrainBuffers {
   int32_t* counts;
   uint16_t* h;
+  float* partial;
 };
 
 TrainBuffers carve_train(Carver& ws, const Problem& p) {
   TrainBuffers b;
   b.counts = ws.take<int32_t>(p.counts);
   b.h = ws.take<uint16_t>(p.max_rows * p.ffn_dim);
+  b.partial = take_parts(ws, p, p.d_model, p.ffn_dim);
   return b;
 }
 
@@ -100,7 +111,7 @@ LayerBuffers carve_layer(Carver& ws, const Problem& p) {
 }
 
 struct BackwardBuffers {
-  float* row_gate;
+  float *row_gate, *partial;
   uint16_t *xg, *gog, *grad_gu, *wh, *dxr;
 };
 
@@ -112,6 +123,7 @@ BackwardBuffers carve_backward(Carver& ws, const Problem& p) {
   b.grad_gu = ws.take<uint16_t>(p.max_rows * 2 * p.ffn_dim);
   b.wh = ws.take<uint16_t>(p.max_rows * p.ffn_dim);
   b.dxr = ws.take<uint16_t>(p.max_rows * p.d_model);
+  b.partial = take_parts(ws, p, p.d_model, 2 * p.ffn_dim);
   return b;
 }
 
@@ -143,14 +155,15 @@ int run_forward(const Problem& p, const RoutingBuffers& r, const TrainBuffers& t
   if (int rc = launch_gated_up(x, w1, layout_of(r, p), t.h, gu, p.num_tokens, p.num_copies, p.d_model, p.ffn_dim, act,
                                as_stream(stream)))
     return rc;
-  // The layer's DSD kernel where it takes the shape, else the per-row-block one.
-  const bool layer_dsd = p.d_model % 256 == 0 && p.max_rows * p.ffn_dim * 2 < kI32Limit;
+  // The layer's DSD kernel where it takes the shape and its tiles have the CUs.
+  const GatedForm form = gated_form(p.max_row_blocks, p.num_experts, p.num_copies, p.d_model, p.ffn_dim, true);
+  const bool layer_dsd = p.d_model % 256 == 0 && p.max_rows * p.ffn_dim * 2 < kI32Limit && form.parts == 1;
   const int rc =
       layer_dsd ? dsd_experts(t.h, w2, r.tokens_per_expert, r.padded_offsets, r.row_block_expert, r.row_offsets,
                               r.col_indices, y, p.max_row_blocks, p.num_experts, p.num_copies,
                               valid_tokens ? 0 : p.num_copies, p.ffn_dim, p.d_model, stream)
-                : sb_dsd_routed(t.h, w2, r.row_offsets, r.col_indices, y, p.max_row_blocks * (p.ffn_dim / kBlock),
-                                p.num_experts * p.ffn_dim, p.max_row_blocks, kBlock, p.d_model, 0, stream);
+                : launch_gated_down(t.h, w2, layout_of(r, p), y, t.partial, p.num_copies, p.d_model, p.ffn_dim,
+                                    as_stream(stream));
   if (rc) return rc;
   return sb_combine(y, r.copy_row, gates, gate_dtype, out, p.num_tokens, p.k, p.d_model, p.max_rows, valid_tokens,
                     stream);
@@ -240,7 +253,7 @@ extern "C" int sb_gated_backward(const void* grad_out, const void* x, const void
   if (int rc = launch_gated_slope(b.gog, w2, s.gu, b.row_gate, l, b.grad_gu, b.wh, p.num_copies, d_model, ffn_dim, act,
                                   st))
     return rc;
-  if (int rc = launch_rows_bt(b.grad_gu, w1, l, b.dxr, p.num_copies, d_model, 2 * ffn_dim, st)) return rc;
+  if (int rc = launch_rows_bt(b.grad_gu, w1, l, b.dxr, b.partial, p.num_copies, d_model, 2 * ffn_dim, st)) return rc;
   if (int rc = launch_sum_copies(b.dxr, s.routing.copy_row, grad_x, p.num_tokens, k, d_model, p.max_rows, valid_tokens,
                                  st))
     return rc;

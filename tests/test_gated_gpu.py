@@ -70,6 +70,18 @@ def test_half_slices(shape) -> None:
     check_all(make(*shape, seed=sum(shape)))
 
 
+# Few tiles and a long reduction, split over workgroups: y = H W2 alone or dX
+# too, in row blocks or chunks, D that 256 divide or not, several parts of
+# unequal lengths, rows of one expert only.
+SPLITS = [(18, 3, 3, 384, 6400, "random"), (5, 2, 4, 256, 2944, "random"), (700, 2, 3, 128, 1664, "random"),
+          (2300, 8, 8, 256, 640, "random"), (2200, 8, 9, 128, 1280, "one"), (30, 2, 2, 256, 1152, "bad")]
+
+
+@pytest.mark.parametrize("shape", SPLITS)
+def test_split_reductions(shape) -> None:
+    check_all(make(*shape[:5], seed=sum(shape[:5]), ids=shape[5]))
+
+
 @pytest.mark.parametrize("gate_dtype", GATES)
 @pytest.mark.parametrize("index", [torch.int32, torch.int64])
 def test_gate_and_index_types(gate_dtype, index) -> None:
