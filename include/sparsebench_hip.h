@@ -286,11 +286,13 @@ int sb_layer_rounded(const void* x, const float* scores, const void* w1, const v
  * x [T, D], w1 [E, D, 2F] (the gate's F columns, then the up projection's F),
  * w2 [E, F, D], all bf16; act is an SB_ACT_* code; expert_idx, gates and
  * valid_tokens as in sb_layer (a copy with an expert id out of range adds
- * nothing). D and F are multiples of 128, and D F 4 bytes stay under 2 GiB.
+ * nothing). D and F are multiples of 128; D F 4 bytes, D 640 and F 1280 stay
+ * under 2 GiB.
  *
  * sb_gated_layer runs the forward pass. sb_gated_train runs the same (the
- * same bits) and leaves in `saved` what sb_gated_backward reads: the layout,
- * G | U and H W2 in bf16. sb_gated_backward takes the gradient of out and
+ * same bits, unless T <= 2 and T k <= 64: there sb_gated_layer rounds nothing
+ * but its result) and leaves in `saved` what sb_gated_backward reads: the
+ * layout, G | U and H W2 in bf16. sb_gated_backward takes the gradient of out and
  * writes, all of them whole and with no atomics:
  *   grad_x [T, D] bf16, grad_gates [T, k] in the gates' dtype (0 for a copy
  *   that was not routed), grad_w1 and grad_w2 in bf16 (0 for experts without

@@ -94,8 +94,8 @@ def dequantize(states: Sequence[Quantized], dtype: torch.dtype = torch.float32) 
 class AdamW:
     """adamw_step with its states: step(grads) updates the parameters given here.
 
-    state_bits: 32 or 8. master_weights: fp32 masters of the parameters that
-    are not fp32 themselves (all parameters then need to be, or none)."""
+    state_bits: 32 or 8. master_weights: fp32 masters of all parameters, copied
+    from them here (self.masters); each step writes the parameters from them."""
 
     def __init__(
         self,
@@ -114,7 +114,7 @@ class AdamW:
         self.lr, self.betas, self.eps, self.weight_decay, self.seed = lr, betas, eps, weight_decay, seed
         states = [new_state(p, state_bits) for p in self.params]
         self.exp_avgs, self.exp_avg_sqs = [s[0] for s in states], [s[1] for s in states]
-        self.masters = [p.detach().float() for p in self.params] if master_weights else None
+        self.masters = [p.detach().to(torch.float32, copy=True) for p in self.params] if master_weights else None
         self.step_count = new_step(self.params[0].device)
 
     def step(self, grads: Sequence[torch.Tensor], grad_scale: float | torch.Tensor | None = None) -> None:

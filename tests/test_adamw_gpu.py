@@ -292,3 +292,46 @@ def test_a_training_step_of_a_gated_layer() -> None:
 
     for a, b in zip(run(4, False), run(4, True)):
         assert torch.equal(a, b)
+
+
+def test_masters_of_fp32_parameters_are_copies() -> None:
+    from sparsebench_amd import optim
+
+    p = tensors([600], torch.float32, 1)[0]
+    g = tensors([600], torch.float32, 2)[0]
+    q = p.clone()
+    with_masters, without = optim.AdamW([p], LR, master_weights=True), optim.AdamW([q], LR)
+    assert with_masters.masters[0].data_ptr() != p.data_ptr()
+    for _ in range(2):
+        with_masters.step([g])
+        without.step([g])
+    assert torch.equal(p, q) and torch.equal(with_masters.masters[0], p)
+
+
+def test_more_values_than_32_bits_count() -> None:
+    """Slices of a tensor of 2^31 + 4099 values against steps of copies of them:
+    the same bits with fp32 states; with 8-bit ones the same scales, and codes
+    that the random bits (of another position) put at most one apart."""
+    from sparsebench_amd import optim
+
+    n = 2**31 + 4099
+    g = torch.Generator(device="cuda").manual_seed(7)
+    grad = torch.randn(n, generator=g, device="cuda", dtype=torch.bfloat16)
+    slices = [slice(0, 4096), slice(2**31 - 2048, 2**31 + 2048), slice(2**31, n)]
+    for bits in (32, 8):
+        p = torch.ones(n, dtype=torch.bfloat16, device="cuda")
+        states, step = optim.new_state(p, bits), optim.new_step()
+        optim.adamw_step([p], [grad], [states[0]], [states[1]], step, LR, weight_decay=0.1)
+        for s in slices:
+            q = torch.ones_like(p[s])
+            small = optim.new_state(q, bits)
+            optim.adamw_step([q], [grad[s].clone()], [small[0]], [small[1]], optim.new_step(), LR, weight_decay=0.1)
+            assert torch.equal(p[s], q)
+            for big, little in zip(states, small):
+                if bits == 32:
+                    assert torch.equal(big[s], little)
+                    continue
+                blocks = slice(s.start // 256, -(-s.stop // 256))
+                assert torch.equal(big.scales[blocks], little.scales)
+                assert ((big.codes[s].int() - little.codes.int()).abs() <= 1).all()
+        del p, states

@@ -70,6 +70,16 @@ def test_half_slices(shape) -> None:
     check_all(make(*shape, seed=sum(shape)))
 
 
+def test_chunk_lengths() -> None:
+    """48 experts of up to three chunks: full, joined and short last pieces, one
+    row, none; enough of them that every product runs in chunks, with half slices."""
+    counts = torch.tensor([257, 320, 321, 64, 542, 1, 0, 255] * 6)
+    x, _, gates, w1, w2, grad = make(int(counts.sum()), 1, 48, 640, 640, seed=11)
+    idx = torch.repeat_interleave(torch.arange(48), counts)
+    idx = idx[torch.randperm(len(idx), generator=torch.Generator().manual_seed(2))][:, None]
+    check_all((x, idx, gates, w1, w2, grad), "gelu")
+
+
 # Few tiles and a long reduction, split over workgroups: y = H W2 alone or dX
 # too, in row blocks or chunks, D that 256 divide or not, several parts of
 # unequal lengths, rows of one expert only.
@@ -259,3 +269,122 @@ def test_two_streams_at_once() -> None:
     torch.cuda.synchronize()
     for w, runs in zip(want, got):
         assert all(torch.equal(a, b) for r in runs for a, b in zip(r, w))
+
+
+# ---- one or two tokens -------------------------------------------------
+
+# (T, k, E, D, F, ids): copies of one expert or spread, up to the 64 that run
+# without a routing layout and one past them; sums by the last workgroup (up to
+# 32 of them) and by a launch of their own; F in several ranges of 2048 a workgroup.
+FEW = [(1, 1, 1, 128, 128, "one"), (1, 64, 4, 128, 256, "bad"), (1, 65, 4, 128, 256, "bad"), (2, 32, 3, 128, 128, "one"),
+       (2, 33, 3, 128, 128, "bad"), (2, 17, 4, 256, 384, "bad"), (1, 2, 8, 2048, 256, "random"),
+       (2, 1, 2, 128, 4352, "random"), (1, 64, 3, 1024, 2304, "one"), (2, 16, 16, 384, 640, "random")]
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize("shape", FEW)
+def test_one_or_two_tokens(shape, act) -> None:
+    check_all(make(*shape[:5], seed=sum(shape[:5]), ids=shape[5]), act)
+
+
+@pytest.mark.parametrize("gate_dtype", GATES)
+@pytest.mark.parametrize("index", [torch.int32, torch.int64])
+def test_one_or_two_tokens_gate_and_index_types(gate_dtype, index) -> None:
+    check_all(make(2, 2, 6, 128, 256, gate_dtype=gate_dtype, index=index))
+
+
+@pytest.mark.parametrize("d", [128, 2048])
+@pytest.mark.parametrize("valid", [0, 1, 2, 3])
+def test_two_tokens_valid_ones(valid, d) -> None:
+    from sparsebench_amd import _C
+    from sparsebench_amd._lib import check, lib, stream_of
+
+    args = make(2, 3, 4, d, 256, seed=valid)
+    check_all(args, valid=min(valid, 2))
+    x, idx, gates, w1, w2, _ = (v.cuda() for v in args)
+    whole = _C.gated_layer_cuda(x, idx, gates, w1, w2, "silu")
+    vt = torch.tensor([valid], dtype=torch.int32, device="cuda")
+    out = torch.full_like(x, 7.0)
+    size = _C.gated_bytes(2, 3, 4, d, 256)[0]
+    workspace = torch.empty(size, dtype=torch.uint8, device="cuda")
+    check(lib().sb_gated_layer(x.data_ptr(), idx.data_ptr(), 1, gates.data_ptr(), 0, w1.data_ptr(), w2.data_ptr(),
+                               out.data_ptr(), 0, workspace.data_ptr(), size, 2, 3, 4, d, 256, vt.data_ptr(),
+                               stream_of(x.device)))
+    assert torch.all(out[valid:] == 7.0) and torch.equal(out[:valid], whole[:valid])
+
+
+def test_two_tokens_non_finite_values_stay_in_theirs() -> None:
+    from sparsebench_amd import moe
+
+    x, idx, gates, w1, w2, _ = (v.cuda() for v in make(2, 2, 2, 256, 128))
+    clean = moe.moe_forward_gated(x, idx, gates, w1, w2)
+    x[0, 3] = float("nan")
+    out = moe.moe_forward_gated(x, idx, gates, w1, w2)
+    assert torch.equal(out[1], clean[1]) and torch.isnan(out[0].float()).all()
+
+
+# ---- sizes past the kernels' windows ------------------------------------
+
+
+def relative(a: torch.Tensor, b: torch.Tensor) -> float:
+    return float((a.float() - b.float()).norm() / b.float().norm())
+
+
+# Two runs of the same values, each with bf16 roundings (u = 2^-8 at most) of
+# its own: of H or wH, G, U, dG | dU, y or a row of dX, and the result, fewer
+# than 6 in a chain; the 2-norm of their difference is 2 * 6 u at the very most.
+TWO_RUNS = 12 * 2.0**-8
+
+
+def test_many_experts_without_rows() -> None:
+    """1024 experts of 44 gradient tiles each, more than 128 of them a CU, 30
+    experts with rows: against the layer of those 30."""
+    from sparsebench_amd import moe
+
+    t, k, e, d, f, few = 400, 2, 1024, 896, 896, 30
+    x, idx, gates, v1, v2, grad = (v.cuda() for v in make(t, k, few, d, f, seed=4))
+    w1, w2 = torch.zeros(e, d, 2 * f, dtype=x.dtype, device="cuda"), torch.zeros(e, f, d, dtype=x.dtype, device="cuda")
+    at = torch.arange(few, device="cuda") * 35 + 1
+    w1[at], w2[at] = v1, v2
+    out, saved = moe.moe_gated_train(x, at[idx], gates, w1, w2)
+    grads = moe.moe_gated_backward(saved, grad)
+    want, want_saved = moe.moe_gated_train(x, idx, gates, v1, v2)
+    want_grads = moe.moe_gated_backward(want_saved, grad)
+    assert relative(out, want) <= TWO_RUNS and relative(grads.x, want_grads.x) <= TWO_RUNS
+    assert relative(grads.expert_weight, want_grads.expert_weight) <= TWO_RUNS
+    for got, ref in ((grads.w1, want_grads.w1), (grads.w2, want_grads.w2)):
+        for i in range(few):
+            assert relative(got[at[i]], ref[i]) <= TWO_RUNS
+        got[at] = 0
+        assert not got.any()
+
+
+def test_x_of_more_than_two_gigabytes() -> None:
+    """Each token's results against those of a layer of a few of the tokens, and
+    the weights' gradients against the sum of two halves'."""
+    from sparsebench_amd import moe
+
+    t, d, f, e = 270_000, 4096, 128, 2
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randn(t, d, generator=g, device="cuda", dtype=torch.bfloat16)
+    grad = torch.randn(t, d, generator=g, device="cuda", dtype=torch.bfloat16)
+    idx = torch.randint(0, e, (t, 1), generator=g, device="cuda")
+    gates = torch.rand(t, 1, generator=g, device="cuda") + 0.5
+    w1 = (torch.randn(e, d, 2 * f, generator=g, device="cuda") / d**0.5).bfloat16()
+    w2 = (torch.randn(e, f, d, generator=g, device="cuda") / f**0.5).bfloat16()
+    some = torch.cat([torch.arange(50), torch.arange(262_100, 262_200), torch.arange(t - 50, t)]).cuda()
+    served = moe.moe_forward_gated(x, idx, gates, w1, w2)
+    out, saved = moe.moe_gated_train(x, idx, gates, w1, w2)
+    grads = moe.moe_gated_backward(saved, grad)
+    ref = gated_reference(*(v[some].cpu() for v in (x, idx, gates)), w1.cpu(), w2.cpu(), "silu", grad[some].cpu())
+    assert_close("out", served[some], ref)
+    assert_close("out", out[some], ref)
+    assert_close("x", grads.x[some], ref)
+    assert_close("gates", grads.expert_weight[some], ref)
+    sums = [torch.zeros_like(w, dtype=torch.float32) for w in (w1, w2)]
+    for half in (slice(0, t // 2), slice(t // 2, t)):
+        _, saved = moe.moe_gated_train(x[half], idx[half], gates[half], w1, w2)
+        part = moe.moe_gated_backward(saved, grad[half])
+        for total, p in zip(sums, (part.w1, part.w2)):
+            total += p.float()
+    assert relative(grads.w1, sums[0]) <= TWO_RUNS and relative(grads.w2, sums[1]) <= TWO_RUNS

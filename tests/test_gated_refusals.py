@@ -38,6 +38,12 @@ def test_gated_sizes_refuse(lib, args, match) -> None:
     assert match in error(lib)
 
 
+@pytest.mark.parametrize(("d", "f"), [(128, 2**21), (2**22, 128)])
+def test_rows_too_long_for_32_bit_offsets(lib, d, f) -> None:
+    assert lib.sb_gated_sizes(4, 2, 4, d, f, None, None, None, None) == 1
+    assert "32-bit" in error(lib)
+
+
 def test_gated_sizes(lib) -> None:
     layer, saved, train, backward = _C.gated_bytes(100, 2, 4, 256, 384)
     rows = (200 + 4 * 127) // 128 * 128
