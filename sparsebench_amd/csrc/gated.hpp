@@ -40,10 +40,11 @@ int launch_few(const void* x, const void* expert_idx, int32_t idx_is_i64, const 
                hipStream_t stream);
 
 // Per copy c = t k + j in row r: grad_gates[c] = <grad_out[t], y[r]>; per row:
-// row_gate[r] = gates[c], xg[r] = x[t], gog[r] = grad_out[t].
+// row_gate[r] = gates[c], xg[r] = x[t], gog[r] = grad_out[t]. expert_order [E]:
+// the experts, those with most rows first.
 int launch_grad_rows(const void* x, const void* grad_out, const void* y, const GatedLayout& layout,
                      const int32_t* copy_row, const void* gates, int32_t gate_dtype, void* grad_gates, float* row_gate,
-                     void* xg, void* gog, int64_t num_tokens, int32_t k, int64_t d_model,
+                     void* xg, void* gog, int64_t num_tokens, int32_t k, int64_t d_model, int32_t* expert_order,
                      const int32_t* valid_tokens, hipStream_t stream);
 
 // dH = row_gate gog W2[e]^T; grad_gu = dH U a'(G) | dH a(G); wh [P, F] = row_gate a(G) U.
@@ -67,7 +68,7 @@ int launch_join_parts(const float* partial, const GatedLayout& layout, void* out
 // and out2 likewise, in one launch; zeros for an expert with no rows.
 int launch_expert_outers(const void* a1, const void* b1, void* out1, int64_t m1, int64_t n1, const void* a2,
                          const void* b2, void* out2, int64_t m2, int64_t n2, const GatedLayout& layout,
-                         hipStream_t stream);
+                         const int32_t* expert_order, hipStream_t stream);
 
 // out[t] = sum_j y[copy_row[t k + j]], fp32 sums (combine.hip).
 int launch_sum_copies(const void* y, const int32_t* copy_row, void* out, int64_t num_tokens, int32_t k,

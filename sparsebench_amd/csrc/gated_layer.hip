@@ -112,12 +112,14 @@ LayerBuffers carve_layer(Carver& ws, const Problem& p) {
 
 struct BackwardBuffers {
   float *row_gate, *partial;
+  int32_t* expert_order;
   uint16_t *xg, *gog, *grad_gu, *wh, *dxr;
 };
 
 BackwardBuffers carve_backward(Carver& ws, const Problem& p) {
   BackwardBuffers b;
   b.row_gate = ws.take<float>(p.max_rows);
+  b.expert_order = ws.take<int32_t>(p.num_experts);
   b.xg = ws.take<uint16_t>(p.max_rows * p.d_model);
   b.gog = ws.take<uint16_t>(p.max_rows * p.d_model);
   b.grad_gu = ws.take<uint16_t>(p.max_rows * 2 * p.ffn_dim);
@@ -248,7 +250,7 @@ extern "C" int sb_gated_backward(const void* grad_out, const void* x, const void
   const GatedLayout l = layout_of(s.routing, p);
   const hipStream_t st = as_stream(stream);
   if (int rc = launch_grad_rows(x, grad_out, s.y, l, s.routing.copy_row, gates, gate_dtype, grad_gates, b.row_gate, b.xg,
-                                b.gog, p.num_tokens, k, d_model, valid_tokens, st))
+                                b.gog, p.num_tokens, k, d_model, b.expert_order, valid_tokens, st))
     return rc;
   if (int rc = launch_gated_slope(b.gog, w2, s.gu, b.row_gate, l, b.grad_gu, b.wh, p.num_copies, d_model, ffn_dim, act,
                                   st))
@@ -258,7 +260,7 @@ extern "C" int sb_gated_backward(const void* grad_out, const void* x, const void
                                  st))
     return rc;
   if (int rc = launch_expert_outers(b.xg, b.grad_gu, grad_w1, d_model, 2 * ffn_dim, b.wh, b.gog, grad_w2, ffn_dim,
-                                    d_model, l, st))
+                                    d_model, l, b.expert_order, st))
     return rc;
   return clear_ok();
 }
