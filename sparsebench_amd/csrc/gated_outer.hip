@@ -31,7 +31,7 @@
 namespace sb {
 namespace {
 
-using Cfg = DmaCfg<256, 256, 32, 4, 2, 4, 0, 0, 4, 1, 0, 0, 0, 1>;
+using Cfg = DmaCfg<256, 256, 32, 4, 2, 4, 0, 0, 5, 1, 0, 0, 0, 1>;
 using ML = DmaMainloop<Cfg>;
 constexpr int kRing = Cfg::STAGES * Cfg::kStageBytes;
 constexpr int kPartRows = 64, kPartBytes = kPartRows * Cfg::BN * 2;
@@ -213,6 +213,14 @@ __device__ __forceinline__ void outer_stream(uint8_t* __restrict__ ring, uint8_t
 #pragma unroll
   for (int s = 0; s < S - 1; ++s) ML::issue_all(next_loads(s));
 
+  const typename ML::Frags fr;
+  typename ML::FragA fa;
+  typename ML::FragB fb;
+  wait_vmcnt<(S - 2) * kL>();
+  __builtin_amdgcn_s_barrier();
+  fr.read_a(ring, 0, 0, fa[0]);
+  fr.read_b(ring + Cfg::kABytes, 0, fb[0]);
+
   int slot = 0;
   int since = S;  // steps since the last tile was written
   for (int i = 0;; ++i) {
@@ -232,17 +240,21 @@ __device__ __forceinline__ void outer_stream(uint8_t* __restrict__ ring, uint8_t
         for (int v = 0; v < 16; ++v) acc[jn][im][v] = 0.0f;
     const int steps = steps_of(t);
     for (int k = 0; k < steps; ++k) {
-      // The step's loads have arrived once at most the operations after them
-      // are outstanding: the loads of S - 2 steps, and a tile's stores if they
-      // came in between (they were issued S - 1 steps ago).
-      if (since < S - 1) wait_vmcnt<(S - 2) * kL + Cfg::TM * kStores>();
-      else wait_vmcnt<(S - 2) * kL>();
+      // A step's loads go to the slot that was read before it (every wave has
+      // passed the barrier of that step's end). Its end waits for the next
+      // step's loads: at most the operations after them are outstanding then,
+      // the loads of S - 2 steps, and a tile's stores if they came in between
+      // (the loads were issued S - 2 steps ago).
+      const bool stores = since < S - 2;
+      auto wait = [&] {
+        if (stores) wait_vmcnt<(S - 2) * kL + Cfg::TM * kStores>();
+        else wait_vmcnt<(S - 2) * kL>();
+      };
       ++since;
-      // Every wave's part of the step is in LDS, and every wave is done with
-      // the slot that the next loads overwrite.
-      __builtin_amdgcn_s_barrier();
       const uint8_t* from = ring + slot * Cfg::kStageBytes;
-      ML::compute(from, from + Cfg::kABytes, 0, acc, next_loads((slot + S - 1) % S));
+      const uint8_t* next = ring + (slot + 1) % S * Cfg::kStageBytes;
+      ML::template compute_xs<true>(from, from + Cfg::kABytes, 0, acc, next_loads((slot + S - 1) % S), fr, fa, fb, next,
+                                    next + Cfg::kABytes, 0, wait);
       slot = (slot + 1) % S;
     }
     static_for<0, Cfg::TM>([&](auto pc) { write_part<decltype(pc)::value>(stage, t, acc); });

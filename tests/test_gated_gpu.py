@@ -271,6 +271,41 @@ def test_two_streams_at_once() -> None:
         assert all(torch.equal(a, b) for r in runs for a, b in zip(r, w))
 
 
+@pytest.mark.parametrize("shape", [(30, 2, 2, 256, 1152), (18, 3, 3, 384, 6400), (2, 2, 4, 256, 512)])
+def test_two_graphs_of_one_pool(shape) -> None:
+    """Split reductions and two tokens, forward and backward in one graph and
+    serving in another of the same pool, replayed in turn with other inputs."""
+    from sparsebench_amd import moe
+
+    static = [v.cuda() for v in make(*shape, seed=1)]
+
+    def train():
+        out, saved = moe.moe_gated_train(*static[:5])
+        return (out, *moe.moe_gated_backward(saved, static[5]))
+
+    def serve():
+        return (moe.moe_forward_gated(*static[:5]),)
+
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        train(), serve()
+    torch.cuda.synchronize()
+    graphs, captured = [], []
+    for step in (train, serve):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], pool=graphs[0].pool() if len(graphs) > 1 else None):
+            captured.append(step())
+    for seed in (2, 3, 4):
+        for a, b in zip(static, make(*shape, seed=seed)):
+            a.copy_(b)
+        for graph, step, got in zip(graphs, (train, serve), captured):
+            graph.replay()
+            torch.cuda.synchronize()
+            want = step()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(got, want)), (seed, step)
+
+
 # ---- one or two tokens -------------------------------------------------
 
 # (T, k, E, D, F, ids): copies of one expert or spread, up to the 64 that run
