@@ -9,9 +9,9 @@
 // while the one before it is computed and written. The finished tile leaves
 // through LDS of its own (the ring stays in use). D = 1024, F = 4096, E = 64, 128
 // rows an expert, both products: 567 us as workgroups of their own, whatever the
-// tile (each took 11 us, most of it its start and its first loads), 470 this way;
+// tile (each took 11 us, most of it its start and its first loads), 451 this way;
 // 240 is the write alone (1.6 GB at 6.9 TB/s), 284 all but the output. D = 4096,
-// F = 14336, E = 8, 512 rows an expert 1730 us, 835 TFLOP/s: there a K step takes 1.0
+// F = 14336, E = 8, 512 rows an expert 1662 us, 868 TFLOP/s: there a K step takes 1.0
 // us, twice its MFMAs. Both operands are read transposed (ds_read_b64_tr), 98
 // KB of LDS a step, and these reads run at half the rate of the others.
 //
@@ -24,7 +24,7 @@
 // experts with most rows come first, runs of a tile a CU in alternate
 // directions, so that whatever the routing every CU gets its share of the K
 // steps (E = 128, D = 2048, F = 768, one expert with 3000 of 16380 rows: in the
-// experts' order 443 us, 381 this way).
+// experts' order 443 us, 377 this way).
 
 #include "gated.hpp"
 
