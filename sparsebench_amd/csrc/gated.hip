@@ -26,8 +26,8 @@ struct UpArgs {
   int32_t num_tokens, d_model, ffn_dim;
 };
 
-// Rows ch of H and (kKeep) G | U, their columns n0 .. n0 + BN / 2 of F.
-template <class Cfg, bool kWideX, bool kKeep, int ACT>
+// Rows ch of H and (kKeep) G | U, their columns n0 .. n0 + BN / 2 of F. LDS: bytes of lds.
+template <class Cfg, bool kWideX, bool kKeep, int ACT, int LDS>
 __device__ __forceinline__ void gated_up_tile(uint8_t* __restrict__ lds, const UpArgs& a, const Chunk& ch, int n0) {
   using ML = DmaMainloop<Cfg>;
   constexpr int kHalf = Cfg::BN / 2;
@@ -54,8 +54,8 @@ __device__ __forceinline__ void gated_up_tile(uint8_t* __restrict__ lds, const U
   typename ML::Acc acc;
   ML::run(lds, src, a.d_model / Cfg::BK, acc);
 
-  // Staged as bf16 rows of kHalf columns: G, then U below it, then (over
-  // both) H; each written row by row in 16-byte chunks.
+  // Staged as bf16 rows of kHalf columns, G, U below it, H below both if they
+  // fit in LDS bytes; each written row by row in 16-byte chunks.
   const int lane = threadIdx.x & 63, wn = (threadIdx.x >> 6) % Cfg::WN;
   constexpr int kRowBytes = kHalf * 2;
   auto stage = [&](int base, auto value) {
@@ -84,21 +84,26 @@ __device__ __forceinline__ void gated_up_tile(uint8_t* __restrict__ lds, const U
           *reinterpret_cast<const u32x4_t*>(lds + base + staged_at<kRowBytes>(r, c));
     }
   };
+  constexpr int kUp = Cfg::BM * kRowBytes;
+  constexpr int kH = 3 * kUp <= LDS ? 2 * kUp : 0;  // H over G where the three do not fit
+  auto product = [](float g, float u) { return gated_act<ACT>(g) * u; };
   __syncthreads();  // every wave is done reading the ring
   if constexpr (kKeep) {
-    constexpr int kUp = Cfg::BM * kRowBytes;
     stage(0, [](float g, float) { return g; });
     stage(kUp, [](float, float u) { return u; });
+    if constexpr (kH != 0) stage(kH, product);
     __syncthreads();
     uint16_t* rows = a.gu + static_cast<int64_t>(ch.row0) * 2 * a.ffn_dim + n0;
     write(0, [&](int r, int col) { return rows + static_cast<int64_t>(r) * 2 * a.ffn_dim + col; });
     write(kUp, [&](int r, int col) { return rows + static_cast<int64_t>(r) * 2 * a.ffn_dim + a.ffn_dim + col; });
+    if constexpr (kH == 0) __syncthreads();
+  }
+  if constexpr (!kKeep || kH == 0) {
+    stage(kH, product);
     __syncthreads();
   }
-  stage(0, [](float g, float u) { return gated_act<ACT>(g) * u; });
-  __syncthreads();
   uint16_t* blocks = a.h + static_cast<int64_t>(ch.row0) * a.ffn_dim;  // the first row block's first BSR block
-  write(0, [&](int r, int col) {
+  write(kH, [&](int r, int col) {
     const int f = n0 + col;
     return blocks + static_cast<int64_t>(r / kBS) * kBS * a.ffn_dim + static_cast<int64_t>(f / kBS) * kBS * kBS +
            (r % kBS) * kBS + f % kBS;
@@ -111,7 +116,7 @@ __global__ void __launch_bounds__(Cfg::kThreads) gated_up_kernel(UpArgs a) {
   Chunk ch;
   int slice;
   if (!row_block_tile(static_cast<int>(blockIdx.x), a.ffn_dim / (Cfg::BN / 2), a.layout, &ch, &slice)) return;
-  gated_up_tile<Cfg, kWideX, kKeep, ACT>(lds, a, ch, slice * (Cfg::BN / 2));
+  gated_up_tile<Cfg, kWideX, kKeep, ACT, sizeof(lds)>(lds, a, ch, slice * (Cfg::BN / 2));
 }
 
 template <bool kKeep, int ACT>
@@ -123,7 +128,7 @@ __global__ void __launch_bounds__(512) gated_up_chunk_kernel(UpArgs a) {
   with_chunk_groups(ch.groups, [&](auto rc) {
     using Cfg = GatedUpCfg<decltype(rc)::value>;
     static_assert(Cfg::kLdsAlloc <= sizeof(lds) && Cfg::kThreads == 512, "one workgroup for all heights");
-    gated_up_tile<Cfg, false, kKeep, ACT>(lds, a, ch, slice * (kGatedBN / 2));
+    gated_up_tile<Cfg, false, kKeep, ACT, sizeof(lds)>(lds, a, ch, slice * (kGatedBN / 2));
   });
 }
 
