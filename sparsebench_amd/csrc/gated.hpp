@@ -87,7 +87,7 @@ __device__ __forceinline__ int32_t scalar_load(const int32_t* p) {
 // a padded row that is a multiple of 128.
 //
 // Two forms, with the same results: row blocks (up to 128 rows, narrow tiles,
-// for grids that leave CUs idle) and chunks of up to 256 rows, 256 columns wide.
+// for grids that leave CUs idle) and chunks of up to 320 rows, 256 columns wide.
 
 // Tile `bid` of max_row_blocks * slices -> (row block, column slice); false
 // past the live row blocks. Live tiles are spread over the XCDs in contiguous
@@ -106,9 +106,9 @@ __device__ __forceinline__ bool row_block_tile(int bid, int slices, const GatedL
   return true;
 }
 
-// The chunk form's tiles: chunks of 256 rows, the last of up to 320, x slices of 256 columns, 8
-// waves in two rows of 4 (128 x 64 a wave at 256 rows). Each tile is cut to its
-// chunk's rows in steps of R = 2 row groups of 32 (one row of 8 waves would
+// The chunk form's tiles: chunks of 256 rows, the last of up to 320, x slices of
+// 256 columns, 8 waves in two rows of 4 (128 x 64 a wave at 256 rows). Each tile
+// is cut to its chunk's rows in steps of R = 2 row groups of 32 (one row of 8 waves would
 // take odd R too, but reads more LDS fragments per MFMA than R + 1 groups in
 // two rows). An expert's weights are streamed once per 256 rows, and padding
 // rows past a chunk's last 64 are neither computed nor read.
