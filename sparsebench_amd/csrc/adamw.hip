@@ -222,13 +222,22 @@ struct Coefficients {
 // The moments' update and the weights' of 8 values.
 __device__ __forceinline__ void update(const Coefficients& k, float (&w)[8], const float (&g)[8], float (&m)[8],
                                        float (&v)[8], float (&root)[8]) {
+  uint32_t least = 0xffffffffu;  // the smallest v that is not 0, by its bits less 1
 #pragma unroll
   for (int q = 0; q < 8; ++q) {
     const float gq = g[q] * k.scale;
     m[q] = fmaf(k.a1, gq, k.b1 * m[q]);
     v[q] = fmaf(k.a2 * gq, gq, k.b2 * v[q]);
-    // Square root and reciprocal to 1 ulp each (v under 1.2e-38 counts as 0).
-    root[q] = __builtin_amdgcn_sqrtf(v[q]);
+    least = min(least, __float_as_uint(v[q]) - 1u);
+    root[q] = __builtin_amdgcn_sqrtf(v[q]);  // to 1 ulp, but 0 for subnormals
+  }
+  // Gradients under 1e-17: a root of 0 would leave eps alone, however small.
+  if (__builtin_expect(least < 0x0d800000u - 1u, 0)) {  // 2^-100
+#pragma unroll
+    for (int q = 0; q < 8; ++q) root[q] = sqrtf(v[q]);
+  }
+#pragma unroll
+  for (int q = 0; q < 8; ++q) {
     const float ratio = m[q] * __builtin_amdgcn_rcpf(fmaf(root[q], k.root_scale, k.eps));
     w[q] = fmaf(-k.size, ratio, w[q] * k.keep);
   }
