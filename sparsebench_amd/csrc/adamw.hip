@@ -7,8 +7,12 @@
 // it), else the parameter. All arithmetic in fp32, the powers in fp64.
 //
 // 8-bit states: blocks of 256 consecutive values with an fp32 scale each.
-//   m       = c |c| scale,  c in -127 .. 127 (int8),  scale = max |m| / 127^2
-//   sqrt(v) = c^2 scale,    c in 0 .. 255 (uint8),    scale = max sqrt(v) / 255^2
+//   m       = c |c| scale,  c in -127 .. 127 (int8),  scale = max |m| fp32(1 / 127^2)
+//   sqrt(v) = c^2 scale,    c in 0 .. 255 (uint8),    scale = max sqrt(v) fp32(1 / 255^2)
+//   |c|     = floor(sqrt(value / scale) + 16 random bits / 2^16)
+// These operations, and the moments' before them, are each rounded to nearest:
+// a floor passes on the last bit as a whole code, so that over steps another
+// order of roundings would give other states (and weights 6e-6 apart after 4).
 // The squares put the codes closer together towards zero (a value of 1% of
 // its block's largest still has 25 steps below it). A value between two codes
 // takes the upper one with a chance equal to its place between them in the
@@ -208,26 +212,49 @@ __device__ __forceinline__ float root_value(uint8_t code, float scale) {
   return c * c * scale;
 }
 
-// The code of a value >= 0: floor(root + bits / 2^16) of root = sqrt(value /
-// scale), inv = 2^32 / scale. In 16 fractional bits: the random ones have no more.
-__device__ __forceinline__ uint32_t code_of(float value, float inv, uint32_t bits) {
-  return (static_cast<uint32_t>(__builtin_amdgcn_sqrtf(value * inv)) + bits) >> 16;
+// The code of a value >= 0 by the rule, each operation rounded to nearest:
+// floor(sqrt(value / scale) + bits / 2^16), at most `most`.
+__device__ __forceinline__ uint32_t code_of(float value, float scale, uint32_t bits, float most) {
+#pragma clang fp contract(off)
+  const float root = sqrtf(value / (scale > 0.0f ? scale : 1.0f));
+  return static_cast<uint32_t>(fminf(root + static_cast<float>(bits) * (1.0f / 65536.0f), most));
 }
+
+// 2^16 times the same before its floor, near enough: inv is about 2^32 / scale.
+__device__ __forceinline__ uint32_t near_code(float value, float inv, uint32_t bits) {
+  return static_cast<uint32_t>(__builtin_amdgcn_sqrtf(value * inv)) + bits;
+}
+// How far near_code and the rule's sum may lie apart, in units of 2^-16 of a code:
+// 2^-23 of a root is 1 of them for 127 and 2 for 255. In 2^-23 of the root: 1 for
+// near_code's square root (1 ulp), 0.75 for inv and its product (1.5 under the
+// root), as much again for a second moment, which is a square root itself, and
+// 1.25 for the rule's own roundings; then less than 1 unit from the conversion.
+// That is less than 4 and 9 units: further than so from a border the floors agree.
+constexpr uint32_t kFirstOff = 5, kSecondOff = 10;
+__device__ __forceinline__ bool near_border(uint32_t code, uint32_t off) { return ((code + off) & 0xffffu) <= 2 * off; }
 
 struct Coefficients {
   float scale, b1, a1, b2, a2, size, root_scale, eps, keep;
   uint32_t step_key;
 };
 
-// The moments' update and the weights' of 8 values.
+// The moments' update and the weights' of 8 values. 8-bit states depend on a
+// floor, where the last bit counts: there each operation is rounded on its own.
+template <int BITS>
 __device__ __forceinline__ void update(const Coefficients& k, float (&w)[8], const float (&g)[8], float (&m)[8],
                                        float (&v)[8], float (&root)[8]) {
   uint32_t least = 0xffffffffu;  // the smallest v that is not 0, by its bits less 1
 #pragma unroll
   for (int q = 0; q < 8; ++q) {
     const float gq = g[q] * k.scale;
-    m[q] = fmaf(k.a1, gq, k.b1 * m[q]);
-    v[q] = fmaf(k.a2 * gq, gq, k.b2 * v[q]);
+    if constexpr (BITS == 32) {
+      m[q] = fmaf(k.a1, gq, k.b1 * m[q]);
+      v[q] = fmaf(k.a2 * gq, gq, k.b2 * v[q]);
+    } else {
+#pragma clang fp contract(off)
+      m[q] = k.b1 * m[q] + k.a1 * gq;
+      v[q] = k.b2 * v[q] + k.a2 * gq * gq;
+    }
     least = min(least, __float_as_uint(v[q]) - 1u);
     root[q] = __builtin_amdgcn_sqrtf(v[q]);  // to 1 ulp, but 0 for subnormals
   }
@@ -243,30 +270,41 @@ __device__ __forceinline__ void update(const Coefficients& k, float (&w)[8], con
   }
 }
 
-// The 8-bit states of a lane's 8 values from i on: codes, and the half wave's scales.
+// The 8-bit states of a lane's 8 values from i on: codes, and the half wave's
+// scales. The rule's divisions and square roots would take longer than the rest of
+// the step (636 us for 200M values with no masters, 430 this way), so a code comes
+// from an approximation, and by the rule where that lies too near a border to
+// tell (one value in 4000, so one wave in 50 at each). All 16 of a lane by the
+// rule where one of them is near a border: 463 us, and 112 registers against 94.
 __device__ __forceinline__ void encode(const Coefficients& k, const Entry& e, int64_t i, const float (&m)[8],
-                                       const float (&root)[8], uint32_t (&mc)[8], uint32_t (&vc)[8], float* m_scale,
-                                       float* v_scale) {
+                                       const float (&v)[8], const float (&root)[8], uint32_t (&mc)[8],
+                                       uint32_t (&vc)[8], float* m_scale, float* v_scale) {
   uint32_t m_max = 0, v_max = 0;
 #pragma unroll
   for (int q = 0; q < 8; ++q) {
     m_max = max(m_max, __float_as_uint(m[q]) & 0x7fffffffu);
-    v_max = max(v_max, __float_as_uint(root[q]) & 0x7fffffffu);
+    v_max = max(v_max, __float_as_uint(v[q]) & 0x7fffffffu);
   }
-  float ms = half_wave_max(m_max) * (1.0f / 16129.0f);
-  if (ms < 1e-28f) ms = 0.0f;  // 2^32 / ms would overflow: first moments under 2e-24 count as none
-  const float vs = half_wave_max(v_max) * (1.0f / 65025.0f);  // a root that is not 0 is 1e-23 or more
-  const float m_inv = ms > 0.0f ? 4294967296.0f / ms : 0.0f, v_inv = vs > 0.0f ? 4294967296.0f / vs : 0.0f;
+  const float ms = half_wave_max(m_max) * (1.0f / 16129.0f), vs = sqrtf(half_wave_max(v_max)) * (1.0f / 65025.0f);
+  const float m_inv = ms > 0.0f ? __builtin_amdgcn_rcpf(ms) * 0x1p32f : 0.0f;
+  const float v_inv = vs > 0.0f ? __builtin_amdgcn_rcpf(vs) * 0x1p32f : 0.0f;
+  // Small scales' reciprocals overflow. (Without a scale both ways give code 0.)
+  const bool by_rule = !(ms == 0.0f || ms > 0x1p-90f) || !(vs == 0.0f || vs > 0x1p-90f);
   const uint32_t key = mix(k.step_key ^ static_cast<uint32_t>(e.index)) + static_cast<uint32_t>(i >> 32);
   const uint32_t base = static_cast<uint32_t>(i) * 0x9E3779B9u + key;
 #pragma unroll
   for (int q = 0; q < 8; ++q) {
     const uint32_t bits = mix(base + q * 0x9E3779B9u);
-    const uint32_t cm = min(code_of(fabsf(m[q]), m_inv, bits & 0xffffu), 127u);
+    const uint32_t cm = near_code(fabsf(m[q]), m_inv, bits & 0xffffu), cv = near_code(root[q], v_inv, bits >> 16);
+    mc[q] = min(cm >> 16, 127u);
+    vc[q] = min(cv >> 16, 255u);
+    if (__builtin_expect(near_border(cm, kFirstOff) || by_rule, 0))
+      mc[q] = code_of(fabsf(m[q]), ms, bits & 0xffffu, 127.0f);
+    if (__builtin_expect(near_border(cv, kSecondOff) || by_rule, 0))
+      vc[q] = code_of(sqrtf(v[q]), vs, bits >> 16, 255.0f);
     const uint32_t sign = static_cast<uint32_t>(__float_as_int(m[q]) >> 31);
-    mc[q] = (cm ^ sign) - sign;
-    const uint32_t least = root[q] > 0.0f ? 1u : 0u;
-    vc[q] = min(max(code_of(root[q], v_inv, bits >> 16), least), 255u);
+    mc[q] = (mc[q] ^ sign) - sign;
+    vc[q] = max(vc[q], v[q] > 0.0f ? 1u : 0u);
   }
   *m_scale = ms;
   *v_scale = vs;
@@ -297,7 +335,7 @@ __device__ __forceinline__ void step_edge(const Coefficients& k, const Entry& e,
       v[q] = r * r;
     }
   }
-  update(k, w, g, m, v, root);
+  update<BITS>(k, w, g, m, v, root);
   if (e.master) store8(e.master, SB_DTYPE_F32, i, n, whole, w);
   store8(e.param, e.param_dtype, i, n, whole, w);
   if constexpr (BITS == 32) {
@@ -307,7 +345,7 @@ __device__ __forceinline__ void step_edge(const Coefficients& k, const Entry& e,
     // Values past the tensor's end were loaded as zeros and so add nothing.
     uint32_t mc[8], vc[8];
     float ms, vs;
-    encode(k, e, i, m, root, mc, vc, &ms, &vs);
+    encode(k, e, i, m, v, root, mc, vc, &ms, &vs);
     store_codes(e.m, i, n, whole, mc);
     store_codes(e.v, i, n, whole, vc);
     if ((threadIdx.x & 31) == 0 && i < n) {
@@ -399,7 +437,7 @@ __device__ __forceinline__ void step_whole32(const Coefficients& k, const Entry&
   g0.get(g), g1.get(g + 4);
   m0.get(m), m1.get(m + 4);
   v0.get(v), v1.get(v + 4);
-  update(k, w, g, m, v, root);
+  update<32>(k, w, g, m, v, root);
   put<SB_DTYPE_F32, 4>(e.m, i, m), put<SB_DTYPE_F32, 4>(e.m, j, m + 4);
   put<SB_DTYPE_F32, 4>(e.v, i, v), put<SB_DTYPE_F32, 4>(e.v, j, v + 4);
   if constexpr (MASTER) put<SB_DTYPE_F32, 4>(e.master, i, w), put<SB_DTYPE_F32, 4>(e.master, j, w + 4);
@@ -424,9 +462,9 @@ __device__ __forceinline__ void step_whole8(const Coefficients& k, const Entry& 
   }
   rw.get(w);
   rg.get(g);
-  update(k, w, g, m, v, root);
+  update<8>(k, w, g, m, v, root);
   uint32_t mc[8], vc[8];
-  encode(k, e, i, m, root, mc, vc, &ms, &vs);
+  encode(k, e, i, m, v, root, mc, vc, &ms, &vs);
   u32x2_t om, ov;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
