@@ -307,8 +307,11 @@ __global__ void __launch_bounds__(kThreads) few_down_kernel(FewArgs a) {
   if constexpr (TICKET) {
     // The last of the slice's workgroups (all copies and parts) adds them up:
     // the others' sums are written back before their ticket is drawn, and read
-    // from memory after the last one.
+    // from memory after the last one. Each wave waits for its own stores to be
+    // in this XCD's L2, which the barrier does not do, so that the one write-back
+    // behind it takes all of the workgroup's along.
     __shared__ int32_t last;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     if (threadIdx.x == 0) {
       __threadfence();
