@@ -10,10 +10,14 @@ namespace {
 
 constexpr int64_t kBlock = kBS;
 
+// The routing's own buffers hold routing_blocks row blocks (the padding of every
+// expert). At most a row block a copy holds rows, the first ones, so that the
+// products' rows and grids go by max_row_blocks (max_rows): with 3 tokens and 256
+// experts 3 instead of 254.
 struct Problem {
   int64_t num_tokens, num_experts, d_model, ffn_dim;
   int32_t k;
-  int64_t num_copies, max_row_blocks, max_rows, counts;
+  int64_t num_copies, routing_blocks, max_row_blocks, max_rows, counts;
 };
 
 int check_problem(int64_t num_tokens, int32_t k, int32_t num_experts, int64_t d_model, int64_t ffn_dim, Problem* p) {
@@ -30,10 +34,12 @@ int check_problem(int64_t num_tokens, int32_t k, int32_t num_experts, int64_t d_
     return fail(SB_ERR_INVALID, "gated experts: D or F too large for 32-bit buffer offsets");
   if (d_model * ffn_dim * 4 >= kI32Limit)
     return fail(SB_ERR_INVALID, "gated experts: one expert's weights too large for 32-bit buffer offsets");
-  *p = Problem{num_tokens, num_experts, d_model, ffn_dim, k, num_tokens * k, 0, 0, 0};
+  *p = Problem{num_tokens, num_experts, d_model, ffn_dim, k, num_tokens * k, 0, 0, 0, 0};
   if (int rc = sb_routing_sizes(p->num_copies, num_experts, static_cast<int32_t>(ffn_dim),
-                                static_cast<int32_t>(kBlock), &p->max_row_blocks, &p->max_rows, &p->counts))
+                                static_cast<int32_t>(kBlock), &p->routing_blocks, nullptr, &p->counts))
     return rc;
+  p->max_row_blocks = std::min(p->routing_blocks, p->num_copies);
+  p->max_rows = p->max_row_blocks * kBlock;
   if (p->max_row_blocks * (std::max(d_model, 2 * ffn_dim) / 128) >= kI32Limit || p->max_rows * (d_model / 8) >= kI32Limit)
     return fail(SB_ERR_INVALID, "problem too large");
   return SB_OK;
@@ -48,11 +54,11 @@ RoutingBuffers carve_routing(Carver& ws, const Problem& p) {
   RoutingBuffers b;
   b.tokens_per_expert = ws.take<int32_t>(p.num_experts);
   b.padded_offsets = ws.take<int32_t>(p.num_experts + 1);
-  b.row_token = ws.take<int32_t>(p.max_rows);
+  b.row_token = ws.take<int32_t>(p.routing_blocks * kBlock);
   b.copy_row = ws.take<int32_t>(p.num_copies);
-  b.row_block_expert = ws.take<int32_t>(p.max_row_blocks);
-  b.row_offsets = ws.take<int32_t>(p.max_row_blocks + 1);
-  b.col_indices = ws.take<int32_t>(p.max_row_blocks * (p.ffn_dim / kBlock));
+  b.row_block_expert = ws.take<int32_t>(p.routing_blocks);
+  b.row_offsets = ws.take<int32_t>(p.routing_blocks + 1);
+  b.col_indices = ws.take<int32_t>(p.routing_blocks * (p.ffn_dim / kBlock));
   b.error = ws.take<int32_t>(1);
   return b;
 }
