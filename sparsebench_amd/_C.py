@@ -876,6 +876,8 @@ def adamw_cuda(params, grads, masters, exp_avgs, exp_avg_sqs, step: torch.Tensor
         check(lib().sb_adamw(words.buffer_info()[0], n, 8 if eight else 32, step.data_ptr(),
                              0.0 if lr_ptr else float(lr), lr_ptr, beta1, beta2, eps, weight_decay, scale_ptr,
                              seed & 0xFFFFFFFF, stream_of(dev)))
+    # Written through their addresses: a graph that saved one of them has to be told (0.05 us a tensor).
+    torch.autograd.graph.increment_version([*params, *(masters or ())])
 
 
 def dequantize_cuda(pairs, dtype: torch.dtype) -> list[torch.Tensor]:

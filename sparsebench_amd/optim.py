@@ -77,7 +77,9 @@ def adamw_step(
     parameters' place and rounded into them; without them a bf16 parameter
     loses what its own rounding loses. step: new_step's tensor; the call reads
     s - 1 from it and advances it. lr and grad_scale may be one-element fp32
-    tensors on the GPU. All on one GPU; tensors must not overlap.
+    tensors on the GPU. All on one GPU; tensors must not overlap. Parameters
+    and masters count as modified in place: a backward pass through a graph that
+    saved one of them raises. (A captured step's replays tell no graph.)
     """
     from sparsebench_amd import _C
 
