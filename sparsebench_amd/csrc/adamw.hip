@@ -24,11 +24,11 @@
 // so the whole block, NaN or infinite.
 //
 // Bound by memory: per value 16 bytes of states (4 with 8 bits) and the
-// parameter, gradient and master: 200M bf16 values with masters 1096 us, 5.1
-// TB/s, what a copy reaches; with 8-bit states and no masters 423 us, 4.7 TB/s
-// (there the arithmetic, some 65 operations a value, takes about 340 us alone).
-// A grid of 8 workgroups per CU that walk the chunks: one workgroup per chunk
-// makes the atomic that counts them the bound (1140 us in both cases).
+// parameter, gradient and master: 200M bf16 values with masters 1190 us, 4.7
+// TB/s, where a copy reaches 5.1; with 8-bit states and no masters 435 us, 4.6
+// TB/s (there the arithmetic takes 345 us alone).
+// A grid of 8 workgroups per CU that walk the chunks: with one workgroup per
+// chunk the atomic that counts them is the bound (1212 and 1142 us).
 // One workgroup takes 2048 values at a time,
 // 8 a lane, so a block of 256 is half a wave. The tensors' addresses come
 // with the launch (kTensorsPerLaunch of them), so nothing is kept between
@@ -358,7 +358,7 @@ __device__ __forceinline__ void step_edge(const Coefficients& k, const Entry& e,
 // N aligned values of dtype D (8, or 4 of 16 or 32 bits), as loaded and as floats.
 // Runs of up to 16 bytes a lane, which whole instructions join to whole cache
 // lines, go past the caches: nothing is read again (200M values with masters:
-// 1135 us with plain accesses, 1096 this way; halves of lines so: 1700).
+// 1262 us with plain accesses, 1190 this way; halves of lines so: 1700).
 template <int D, int N>
 struct Raw {
   static constexpr int kBytes = N * (D == SB_DTYPE_F32 ? 4 : 2);

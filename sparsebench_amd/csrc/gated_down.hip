@@ -96,7 +96,8 @@ __global__ void __launch_bounds__(512) gated_down_chunk_kernel(DownArgs p) {
 }
 
 // out[r] = the sum of row r's parts, in order; rows without a token are left.
-// Bound by memory; 8 columns a lane.
+// Rounded to bf16 as an unsplit product's rows are: the sum over a token's copies
+// that follows reads the same rows either way. Bound by memory; 8 columns a lane.
 __global__ void __launch_bounds__(256)
     join_parts_kernel(const float* __restrict__ partial, const int32_t* __restrict__ row_token,
                       uint16_t* __restrict__ out, int64_t rows, int32_t chunks_per_row, int32_t parts) {
