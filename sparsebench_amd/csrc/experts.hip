@@ -567,14 +567,16 @@ __global__ void __launch_bounds__(64 * WAVES)
 // ceil(n_e / 256) chunks are at most 1 + (n_e - 1) / 256, so there are at
 // most min(E, N) + N / 256 of them for N routed rows, and N is at most
 // 128 max_row_blocks - 127 E + 127 (max_row_blocks = floor((N + 127 E) /
-// 128)). Expert tiles the grid cannot hold leave the stage to the row
-// blocks (on the device). A function of the layout's sizes only, so the
-// SDD's launch computes the same number for its own choice.
-int dsd_layer_grid(int64_t max_row_blocks, int64_t num_experts, int64_t d_model, int32_t force, int64_t* grid) {
+// 128)), or at most num_copies, which is more where the caller's row blocks
+// leave out what the N copies cannot fill. Expert tiles the grid cannot hold
+// leave the stage to the row blocks (on the device). A function of the layout's
+// sizes only, so the SDD's launch computes the same number for its own choice.
+int dsd_layer_grid(int64_t max_row_blocks, int64_t num_experts, int64_t num_copies, int64_t d_model, int32_t force,
+                   int64_t* grid) {
   int cus = 0;
   if (const int rc = device_cus(&cus)) return rc;
-  const int64_t rows = std::min(max_row_blocks * kBS, std::max<int64_t>(0, max_row_blocks * kBS - (kBS - 1) * num_experts) +
-                                                          (kBS - 1));
+  const int64_t by_layout = std::max<int64_t>(0, max_row_blocks * kBS - (kBS - 1) * num_experts) + (kBS - 1);
+  const int64_t rows = std::min(max_row_blocks * kBS, std::max(by_layout, num_copies));
   const int64_t chunk_bound =
       std::min(max_row_blocks, std::min(num_experts, rows) + rows / Chunking<dsd_rmax<4>()>::kRows);
   static_assert(Chunking<dsd_rmax<4>()>::kRows == Chunking<dsd_rmax<8>()>::kRows, "one bound for both");
@@ -601,7 +603,7 @@ int launch_sdd_layer(const void* x, const void* w1, const int32_t* row_token, co
   const int64_t tiles = max_row_blocks * (ffn_dim / kSddBN);
   int64_t dsd_grid = 0;  // no DSD expert tiles for D % 256 != 0
   if (d_model % kDsdBN == 0)
-    if (const int rc = dsd_layer_grid(max_row_blocks, num_experts, d_model, force, &dsd_grid)) return rc;
+    if (const int rc = dsd_layer_grid(max_row_blocks, num_experts, 0, d_model, force, &dsd_grid)) return rc;
   int cus = 0;
   if (const int rc = device_cus(&cus)) return rc;
   const int64_t slack = split_tail_slack(cus) + kNumXcd * (ffn_dim / kSddBN);
@@ -664,13 +666,14 @@ int launch_sdd_pairs(const void* x, const void* w1, const int32_t* row_token, co
 template <class CfgB, int WAVES>
 int launch_dsd_layer(const void* h, const void* w2, const int32_t* tokens_per_expert, const int32_t* padded_offsets,
                      const int32_t* row_block_expert, void* out, int64_t max_row_blocks, int64_t num_experts,
-                     int64_t min_rows, int64_t ffn_dim, int64_t d_model, int32_t force, hipStream_t stream) {
+                     int64_t num_copies, int64_t min_rows, int64_t ffn_dim, int64_t d_model, int32_t force,
+                     hipStream_t stream) {
   static_assert(CfgB::BN == 512 || CfgB::BN == 256, "row-block tile widths of dsd_layer_grid");
   if (!reduction_fits<CfgB>(ffn_dim) || !reduction_fits<DsdCfg<4, kDsdBN, WAVES, kDsdStages>>(ffn_dim))
     return fail(SB_ERR_INVALID, "dsd_experts: F (%lld) is not a whole number of the tiles' K steps",
                 static_cast<long long>(ffn_dim));
   int64_t tiles = 0;
-  if (const int rc = dsd_layer_grid(max_row_blocks, num_experts, d_model, force, &tiles)) return rc;
+  if (const int rc = dsd_layer_grid(max_row_blocks, num_experts, num_copies, d_model, force, &tiles)) return rc;
   const int64_t h_bytes = max_row_blocks * (ffn_dim / kBS) * kBS * kBS * 2;
   int cus = 0;
   if (const int rc = device_cus(&cus)) return rc;
@@ -763,8 +766,8 @@ int dsd_experts(const void* h, const void* w2, const int32_t* tokens_per_expert,
   // 128 x 256 when D % 512 != 0. The expert tiles take the same wave count.
   auto launch = [&](auto cfg, auto waves) {  // cfg: Tag<row-block config>
     return launch_dsd_layer<typename decltype(cfg)::type, decltype(waves)::value>(
-        h, w2, tokens_per_expert, padded_offsets, row_block_expert, out, max_row_blocks, num_experts, min_rows,
-        ffn_dim, d_model, force, s);
+        h, w2, tokens_per_expert, padded_offsets, row_block_expert, out, max_row_blocks, num_experts, num_copies,
+        min_rows, ffn_dim, d_model, force, s);
   };
   using W4 = std::integral_constant<int, 4>;
   using W8 = std::integral_constant<int, 8>;

@@ -67,3 +67,28 @@ def test_rows_of_neighbours_stay_as_they_were() -> None:
     want, saved = moe.moe_gated_train(x, idx, gates, w1, w2)
     assert torch.equal(out, want)
     assert all(torch.equal(a, b) for a, b in zip(grads, moe.moe_gated_backward(saved, grad)))
+
+
+@pytest.mark.gpu
+def test_every_copy_on_an_expert_of_its_own(hooks) -> None:
+    """240 copies over 250 experts: the second product's tiles by expert, by row block and
+    as it chooses, in a workspace of NaN, which a tile that no workgroup takes would leave."""
+    import torch
+
+    from sparsebench_amd._lib import check, lib, stream_of
+    from tests.test_gated_gpu import make
+
+    t, e, d, f = 240, 250, 2048, 128
+    x, idx, gates, w1, w2, _ = (v.cuda() for v in make(t, 1, e, d, f, seed=6))
+    idx.copy_(torch.randperm(e, generator=torch.Generator().manual_seed(1))[:t, None])
+    workspace = torch.empty(_C.gated_bytes(t, 1, e, d, f)[0] // 2, dtype=torch.bfloat16, device="cuda")
+    outs = []
+    for gate in (0, 1, 2):
+        hooks.expert_gate(gate)
+        workspace.fill_(float("nan"))
+        outs.append(torch.zeros_like(x))
+        check(lib().sb_gated_layer(x.data_ptr(), idx.data_ptr(), 1, gates.data_ptr(), 0, w1.data_ptr(), w2.data_ptr(),
+                                   outs[-1].data_ptr(), 0, workspace.data_ptr(), 2 * workspace.numel(), t, 1, e, d, f,
+                                   None, stream_of(x.device)))
+    assert torch.isfinite(outs[0].float()).all()
+    assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
