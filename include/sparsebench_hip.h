@@ -363,6 +363,49 @@ typedef struct {
 } SbQuantized;
 int sb_dequantize(const SbQuantized* tensors, int64_t count, int32_t out_dtype, void* stream);
 
+/* ---- Norms before and after a block ------------------------------------- */
+
+/* What a gate of sb_norm_out is broadcast over: [D], [T, 1] or [T, D]. */
+#define SB_GATE_NONE 0
+#define SB_GATE_CHANNEL 1
+#define SB_GATE_TOKEN 2
+#define SB_GATE_FULL 3
+
+/* No counterpart in the reference. With n(v) = v / sqrt(mean(v^2) + eps) over
+ * a row of d_model values (at most 32768):
+ *   sb_norm_in   out[t] = weight n(x[t])
+ *   sb_norm_out  out[t] = x[t] + scale gate weight n(y[t]),
+ *                next[t] = next_weight n(out[t]), of out as rounded (next may be NULL)
+ * Rows are of `dtype` (SB_DTYPE_*); inputs' rows start a stride of elements
+ * apart (gate_stride: of a gate with rows), outputs' rows are contiguous. A NULL
+ * weight counts as 1. Rows t >= *valid_tokens (may be NULL) are left unwritten. */
+int sb_norm_in(const void* x, int64_t x_stride, const void* weight, int32_t weight_dtype, void* out, int32_t dtype,
+               int64_t num_tokens, int64_t d_model, float eps, const int32_t* valid_tokens, void* stream);
+int sb_norm_out(const void* y, int64_t y_stride, const void* x, int64_t x_stride, const void* weight,
+                int32_t weight_dtype, const void* gate, int32_t gate_dtype, int32_t gate_kind, int64_t gate_stride,
+                float scale, const void* next_weight, int32_t next_dtype, void* out, void* next, int32_t dtype,
+                int64_t num_tokens, int64_t d_model, float eps, const int32_t* valid_tokens, void* stream);
+
+/* Their gradients. Of sb_norm_in: dx = grad_x (may be NULL: 0) + the norm's at
+ * x, dweight. Of sb_norm_out, from the gradients of out and of next (may be
+ * NULL; then out, dx and dnext_weight are not used, and grad_out is x's
+ * gradient): dy, dx, and each of dweight, dgate (contiguous, of the gate's
+ * shape) and dnext_weight; of weights, where not NULL. Each has its operand's
+ * type. Sums over tokens are fp32 and in a fixed order. workspace: *workspace_bytes
+ * of sb_norm_sizes on the same device, 256-byte aligned. */
+int sb_norm_sizes(int64_t num_tokens, int64_t d_model, int64_t* workspace_bytes);
+int sb_norm_in_backward(const void* grad, int64_t grad_stride, const void* x, int64_t x_stride, const void* weight,
+                        int32_t weight_dtype, const void* grad_x, int64_t grad_x_stride, void* dx, void* dweight,
+                        int32_t dtype, int64_t num_tokens, int64_t d_model, float eps, const int32_t* valid_tokens,
+                        void* workspace, int64_t workspace_bytes, void* stream);
+int sb_norm_out_backward(const void* grad_out, int64_t grad_out_stride, const void* grad_next,
+                         int64_t grad_next_stride, const void* y, int64_t y_stride, const void* out,
+                         int64_t out_stride, const void* weight, int32_t weight_dtype, const void* gate,
+                         int32_t gate_dtype, int32_t gate_kind, int64_t gate_stride, float scale,
+                         const void* next_weight, int32_t next_dtype, void* dy, void* dx, void* dweight, void* dgate,
+                         void* dnext_weight, int32_t dtype, int64_t num_tokens, int64_t d_model, float eps,
+                         const int32_t* valid_tokens, void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

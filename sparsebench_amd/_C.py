@@ -910,3 +910,160 @@ def dequantize_cuda(pairs, dtype: torch.dtype) -> list[torch.Tensor]:
     with _device_of(flat):
         check(lib().sb_dequantize(words.buffer_info()[0], len(pairs), _GATE_DTYPES[dtype], stream_of(dev)))
     return out
+
+
+# ---- norms before and after a block (this build's C ABI) ----
+
+_NORM_MAX_D = 32768
+
+
+def _check_rows(t: torch.Tensor, name: str, like: torch.Tensor | None = None) -> None:
+    """[T, D] with contiguous rows on a GPU; with `like`, of its shape, type and device."""
+    if not t.is_cuda or t.dim() != 2 or t.dtype not in _GATE_DTYPES:
+        _fail(f"{name} must be a [T, D] bfloat16, float16 or float32 CUDA tensor, got {_shape(t)} {t.dtype}")
+    if like is not None and (t.shape != like.shape or t.dtype != like.dtype or t.device != like.device):
+        _fail(f"{name} must be a {_shape(like)} {like.dtype} tensor on {like.device}, got {_shape(t)} {t.dtype} on "
+              f"{t.device}")
+    if t.shape[1] != 1 and t.stride(1) != 1:
+        _fail(f"{name} must have contiguous rows")
+    if not 0 < t.shape[1] <= _NORM_MAX_D:
+        _fail(f"rows must have 1 to {_NORM_MAX_D} values, got {t.shape[1]}")
+
+
+def _check_vector(t: torch.Tensor | None, name: str, like: torch.Tensor) -> None:
+    if t is not None and not (t.device == like.device and t.dtype in _GATE_DTYPES and t.shape == like.shape[1:]
+                              and t.is_contiguous()):
+        _fail(f"{name} must be a contiguous [{like.shape[1]}] bfloat16, float16 or float32 tensor on {like.device}")
+
+
+def _check_norm_gate(gate: torch.Tensor | None, like: torch.Tensor) -> tuple[int, int]:
+    """(kind, row stride) of a gate."""
+    if gate is None:
+        return 0, 0
+    t, d = like.shape
+    if gate.device != like.device or gate.dtype not in _GATE_DTYPES:
+        _fail(f"gate must be a bfloat16, float16 or float32 tensor on {like.device}, got {gate.dtype} on {gate.device}")
+    if gate.shape == (d,) and gate.is_contiguous():
+        return 1, 0
+    if gate.shape == (t, d) and (d == 1 or gate.stride(1) == 1):
+        return 3, gate.stride(0)
+    if gate.shape == (t, 1):
+        return 2, gate.stride(0)
+    _fail(f"gate must be [D], [T, 1] or [T, D] with contiguous rows, got {_shape(gate)}")
+
+
+def _check_norm(eps: float, valid_tokens: torch.Tensor | None, like: torch.Tensor) -> None:
+    if not eps >= 0:
+        _fail(f"eps must not be negative, got {eps}")
+    if valid_tokens is not None and not (valid_tokens.device == like.device and _valid_tokens_ok(valid_tokens)):
+        _fail("valid_tokens must be a one-element int32 CUDA tensor")
+
+
+def _dtype_code(t: torch.Tensor | None) -> int:
+    return 0 if t is None else _GATE_DTYPES[t.dtype]
+
+
+def norm_in_cuda(x: torch.Tensor, weight: torch.Tensor | None, eps: float,
+                 valid_tokens: torch.Tensor | None = None) -> torch.Tensor:
+    """weight x / sqrt(mean(x^2) + eps) of each row (include/sparsebench_hip.h: sb_norm_in)."""
+    _check_rows(x, "x")
+    _check_vector(weight, "weight", x)
+    _check_norm(eps, valid_tokens, x)
+    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    with _device_of(x):
+        check(lib().sb_norm_in(x.data_ptr(), x.stride(0), _ptr(weight), _dtype_code(weight), out.data_ptr(),
+                               _GATE_DTYPES[x.dtype], *x.shape, eps, _ptr(valid_tokens), stream_of(x.device)))
+    return out
+
+
+def norm_out_cuda(y: torch.Tensor, x: torch.Tensor, weight: torch.Tensor | None, gate: torch.Tensor | None,
+                  scale: float, eps: float, next_weight: torch.Tensor | None,
+                  valid_tokens: torch.Tensor | None = None):
+    """x + scale gate weight n(y), or that and its own norm (sb_norm_out)."""
+    _check_rows(x, "x")
+    _check_rows(y, "y", x)
+    _check_vector(weight, "weight", x)
+    _check_vector(next_weight, "next_weight", x)
+    kind, gate_stride = _check_norm_gate(gate, x)
+    _check_norm(eps, valid_tokens, x)
+    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    following = None if next_weight is None else torch.empty_like(out)
+    with _device_of(x):
+        check(lib().sb_norm_out(
+            y.data_ptr(), y.stride(0), x.data_ptr(), x.stride(0), _ptr(weight), _dtype_code(weight), _ptr(gate),
+            _dtype_code(gate), kind, gate_stride, scale, _ptr(next_weight), _dtype_code(next_weight), out.data_ptr(),
+            _ptr(following), _GATE_DTYPES[x.dtype], *x.shape, eps, _ptr(valid_tokens), stream_of(x.device)))
+    return out if following is None else (out, following)
+
+
+@functools.lru_cache(maxsize=256)
+def _norm_bytes(num_tokens: int, d_model: int, device: int) -> int:
+    size = ctypes.c_int64()
+    check(lib().sb_norm_sizes(num_tokens, d_model, ctypes.byref(size)))
+    return size.value
+
+
+def _norm_workspace(like: torch.Tensor) -> torch.Tensor:
+    """For the device that is current, like's."""
+    return torch.empty(_norm_bytes(*like.shape, like.get_device()), dtype=torch.uint8, device=like.device)
+
+
+def norm_in_backward_cuda(grad: torch.Tensor, x: torch.Tensor, weight: torch.Tensor | None, eps: float,
+                          grad_x: torch.Tensor | None, valid_tokens: torch.Tensor | None = None
+                          ) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """The gradients (x, weight) of norm_in_cuda, x's with grad_x added (sb_norm_in_backward)."""
+    _check_rows(x, "x")
+    _check_rows(grad, "grad", x)
+    if grad_x is not None:
+        _check_rows(grad_x, "grad_x", x)
+    _check_vector(weight, "weight", x)
+    _check_norm(eps, valid_tokens, x)
+    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    if x.shape[0] == 0:  # sums of nothing
+        return dx, None if weight is None else torch.zeros_like(weight)
+    dweight = None if weight is None else torch.empty_like(weight)
+    with _device_of(x):
+        workspace = _norm_workspace(x)
+        check(lib().sb_norm_in_backward(
+            grad.data_ptr(), grad.stride(0), x.data_ptr(), x.stride(0), _ptr(weight), _dtype_code(weight),
+            _ptr(grad_x), 0 if grad_x is None else grad_x.stride(0), dx.data_ptr(), _ptr(dweight),
+            _GATE_DTYPES[x.dtype], *x.shape, eps, _ptr(valid_tokens), workspace.data_ptr(), workspace.numel(),
+            stream_of(x.device)))
+    return dx, dweight
+
+
+def norm_out_backward_cuda(grad_out: torch.Tensor, y: torch.Tensor, weight: torch.Tensor | None,
+                           gate: torch.Tensor | None, scale: float, eps: float, out: torch.Tensor | None,
+                           grad_next: torch.Tensor | None, next_weight: torch.Tensor | None,
+                           valid_tokens: torch.Tensor | None = None):
+    """The gradients (y, x, weight, gate, next_weight) of norm_out_cuda (sb_norm_out_backward)."""
+    _check_rows(y, "y")
+    _check_rows(grad_out, "grad_out", y)
+    if (grad_next is None) != (next_weight is None) or (grad_next is not None and out is None):
+        _fail("the next norm's gradient needs grad_next, next_weight and out")
+    if grad_next is not None:
+        _check_rows(grad_next, "grad_next", y)
+        _check_rows(out, "out", y)
+    _check_vector(weight, "weight", y)
+    _check_vector(next_weight, "next_weight", y)
+    kind, gate_stride = _check_norm_gate(gate, y)
+    _check_norm(eps, valid_tokens, y)
+    opts = {"dtype": y.dtype, "device": y.device}
+    if y.shape[0] == 0:  # sums of nothing
+        return (torch.empty_like(y), grad_out, *(None if w is None else torch.zeros_like(w)
+                                                 for w in (weight, gate, next_weight)))
+    dy = torch.empty(y.shape, **opts)
+    dx = None if grad_next is None else torch.empty(y.shape, **opts)
+    dweight, dnext = (None if w is None else torch.empty_like(w) for w in (weight, next_weight))
+    dgate = None if gate is None else torch.empty(gate.shape, dtype=gate.dtype, device=gate.device)
+    following = out if grad_next is not None else None
+    with _device_of(y):
+        workspace = _norm_workspace(y)
+        check(lib().sb_norm_out_backward(
+            grad_out.data_ptr(), grad_out.stride(0), _ptr(grad_next), 0 if grad_next is None else grad_next.stride(0),
+            y.data_ptr(), y.stride(0), _ptr(following), 0 if following is None else following.stride(0),
+            _ptr(weight), _dtype_code(weight), _ptr(gate), _dtype_code(gate), kind, gate_stride, scale,
+            _ptr(next_weight), _dtype_code(next_weight), dy.data_ptr(), _ptr(dx), _ptr(dweight), _ptr(dgate),
+            _ptr(dnext), _GATE_DTYPES[y.dtype], *y.shape, eps, _ptr(valid_tokens), workspace.data_ptr(),
+            workspace.numel(), stream_of(y.device)))
+    return dy, grad_out if dx is None else dx, dweight, dgate, dnext
