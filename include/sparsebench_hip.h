@@ -406,6 +406,35 @@ int sb_norm_out_backward(const void* grad_out, int64_t grad_out_stride, const vo
                          void* dnext_weight, int32_t dtype, int64_t num_tokens, int64_t d_model, float eps,
                          const int32_t* valid_tokens, void* workspace, int64_t workspace_bytes, void* stream);
 
+/* ---- Gated experts with 4-bit weights ------------------------------------ */
+
+/* No counterpart in the reference: sb_gated_layer for few tokens (at most 2048
+ * copies, T k) with weights of 4 bits. A weight is a code of one sign, two
+ * exponent and one mantissa bits (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their
+ * negatives) times 2^(s - 127), one byte s for 32 along the reduction (255:
+ * NaN). Of w [E, K, N] the codes are [E, N/32, K/32, 32, 16] bytes: 32
+ * consecutive k of a column, the even ones in the low halves; the scales
+ * [E, N/32, K/32, 32]. w1 is [E, D, 2F] (gate, then up columns), w2 [E, F, D];
+ * D and F are multiples of 128. The other operands, *valid_tokens and ids out
+ * of range are as in sb_gated_layer; h is rounded to bf16 between the products.
+ * workspace: *workspace_bytes of sb_experts4_sizes on the same device,
+ * 256-byte aligned. */
+int sb_experts4_sizes(int64_t num_tokens, int32_t k, int32_t num_experts, int64_t d_model, int64_t ffn_dim,
+                      int64_t* workspace_bytes);
+int sb_experts4_layer(const void* x, const void* expert_idx, int32_t idx_is_i64, const void* gates, int32_t gate_dtype,
+                      const void* w1_codes, const void* w1_scales, const void* w2_codes, const void* w2_scales,
+                      void* out, int32_t act, void* workspace, int64_t workspace_bytes, int64_t num_tokens, int32_t k,
+                      int32_t num_experts, int64_t d_model, int64_t ffn_dim, const int32_t* valid_tokens, void* stream);
+
+/* w [E, K, N] (K, N multiples of 32) -> codes and scales, and back (bf16). The
+ * scale is the largest power of two that leaves the group's largest value at 4
+ * or more of it; values are rounded to the nearest code, halves to the even one,
+ * and from 6 up to 6. A group with an infinity or NaN becomes NaN. */
+int sb_quantize4(const void* w, int32_t dtype, void* codes, void* scales, int64_t num_experts, int64_t k, int64_t n,
+                 void* stream);
+int sb_dequantize4(const void* codes, const void* scales, void* w, int64_t num_experts, int64_t k, int64_t n,
+                   void* stream);
+
 #ifdef __cplusplus
 }
 #endif

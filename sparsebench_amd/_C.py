@@ -1067,3 +1067,97 @@ def norm_out_backward_cuda(grad_out: torch.Tensor, y: torch.Tensor, weight: torc
             _ptr(dnext), _GATE_DTYPES[y.dtype], *y.shape, eps, _ptr(valid_tokens), workspace.data_ptr(),
             workspace.numel(), stream_of(y.device)))
     return dy, grad_out if dx is None else dx, dweight, dgate, dnext
+
+
+# ---- gated experts with 4-bit weights (this build's C ABI) ----
+
+_MAX_COPIES4 = 2048
+
+
+@functools.lru_cache(maxsize=256)
+def _experts4_bytes(num_tokens: int, k: int, num_experts: int, d_model: int, ffn_dim: int, device: int) -> int:
+    size = ctypes.c_int64()
+    check(lib().sb_experts4_sizes(num_tokens, k, num_experts, d_model, ffn_dim, ctypes.byref(size)))
+    return size.value
+
+
+def _check_codes(codes: torch.Tensor, scales: torch.Tensor, name: str) -> tuple[int, int, int]:
+    """(E, K, N) of 4-bit weights."""
+    if (codes.dim() != 5 or codes.shape[3:] != (32, 16) or scales.shape != codes.shape[:4] or not codes.is_cuda
+            or codes.device != scales.device or codes.dtype != torch.uint8 or scales.dtype != torch.uint8):
+        _fail(f"{name} must be uint8 codes [E, N/32, K/32, 32, 16] and scales [E, N/32, K/32, 32] on one GPU, got "
+              f"{_shape(codes)} {codes.dtype} and {_shape(scales)} {scales.dtype}")
+    if not (codes.is_contiguous() and scales.is_contiguous()) or codes.data_ptr() % 16:
+        _fail(f"{name} must be contiguous, its codes 16-byte aligned")
+    e, nt, kg = codes.shape[:3]
+    return e, 32 * kg, 32 * nt
+
+
+def experts4_layer_cuda(x: torch.Tensor, expert_idx: torch.Tensor, expert_weight: torch.Tensor, w1, w2,
+                        activation: str, valid_tokens: torch.Tensor | None = None) -> torch.Tensor:
+    """gated_layer_cuda with (codes, scales) pairs as weights (include/sparsebench_hip.h: sb_experts4_layer)."""
+    if x.dim() != 2 or expert_idx.dim() != 2 or expert_idx.shape != expert_weight.shape or x.shape[0] != expert_idx.shape[0]:
+        _fail(f"x must be [T, D], expert_idx and expert_weight [T, k], got {_shape(x)}, {_shape(expert_idx)} and "
+              f"{_shape(expert_weight)}")
+    (e, d, columns), (experts, f, out_columns) = _check_codes(*w1, "w1"), _check_codes(*w2, "w2")
+    if e != experts or x.shape[1] != d or out_columns != d or columns != 2 * f:
+        _fail(f"x must be [T, D], w1 of [E, D, 2F] and w2 of [E, F, D], got {_shape(x)}, {[e, d, columns]} and "
+              f"{[experts, f, out_columns]}")
+    if any(t.device != x.device for t in (expert_idx, expert_weight, w1[0], w2[0])):
+        _fail("all inputs must be on the same GPU")
+    if x.dtype != torch.bfloat16 or not x.is_contiguous() or x.data_ptr() % 16:
+        _fail("x must be contiguous 16-byte aligned bfloat16")
+    if expert_weight.dtype not in _GATE_DTYPES:
+        _fail(f"expert_weight must be bfloat16, float16 or float32, got {expert_weight.dtype}")
+    if expert_idx.dtype not in _INDEX_DTYPES:
+        _fail(f"expert_idx must be int32 or int64, got {expert_idx.dtype}")
+    if activation not in _ACTIVATIONS:
+        _fail(f"activation must be one of {sorted(_ACTIVATIONS)}, got {activation!r}")
+    if valid_tokens is not None and not (valid_tokens.device == x.device and _valid_tokens_ok(valid_tokens)):
+        _fail("valid_tokens must be a one-element int32 CUDA tensor")
+    t, k = expert_idx.shape
+    if k == 0:
+        _fail(f"expert_weight must be [T, k] with k > 0, got {_shape(expert_weight)}")
+    if t * k > _MAX_COPIES4:
+        _fail(f"at most {_MAX_COPIES4} copies (T k), got {t * k}: more are faster through dequantize_experts and "
+              "moe_forward_gated")
+    out = torch.empty_like(x)
+    if t == 0:
+        return out
+    expert_idx, gates = expert_idx.contiguous(), expert_weight.contiguous()
+    with _device_of(x):
+        size = _experts4_bytes(t, k, e, d, f, x.get_device())
+        workspace = torch.empty(size, dtype=torch.uint8, device=x.device)
+        check(lib().sb_experts4_layer(
+            x.data_ptr(), expert_idx.data_ptr(), _INDEX_DTYPES[expert_idx.dtype], gates.data_ptr(),
+            _GATE_DTYPES[gates.dtype], w1[0].data_ptr(), w1[1].data_ptr(), w2[0].data_ptr(), w2[1].data_ptr(),
+            out.data_ptr(), _ACTIVATIONS[activation], workspace.data_ptr(), size, t, k, e, d, f, _ptr(valid_tokens),
+            stream_of(x.device)))
+    return out
+
+
+def quantize4_cuda(w: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """(codes, scales) of w [E, K, N] (include/sparsebench_hip.h: sb_quantize4)."""
+    if not w.is_cuda or w.dim() != 3 or w.dtype not in _GATE_DTYPES:
+        _fail(f"w must be an [E, K, N] bfloat16, float16 or float32 CUDA tensor, got {_shape(w)} {w.dtype}")
+    e, k, n = w.shape
+    if e == 0 or k == 0 or n == 0 or k % 32 or n % 32:
+        _fail(f"K and N must be positive multiples of 32, got {_shape(w)}")
+    w = w.contiguous()
+    scales = torch.empty(e, n // 32, k // 32, 32, dtype=torch.uint8, device=w.device)
+    codes = torch.empty(*scales.shape, 16, dtype=torch.uint8, device=w.device)
+    with _device_of(w):
+        check(lib().sb_quantize4(w.data_ptr(), _GATE_DTYPES[w.dtype], codes.data_ptr(), scales.data_ptr(), e, k, n,
+                                 stream_of(w.device)))
+    return codes, scales
+
+
+def dequantize4_cuda(codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
+    """w [E, K, N] bf16 of codes and scales (include/sparsebench_hip.h: sb_dequantize4)."""
+    e, k, n = _check_codes(codes, scales, "w")
+    w = torch.empty(e, k, n, dtype=torch.bfloat16, device=codes.device)
+    if w.numel():
+        with _device_of(codes):
+            check(lib().sb_dequantize4(codes.data_ptr(), scales.data_ptr(), w.data_ptr(), e, k, n,
+                                       stream_of(codes.device)))
+    return w

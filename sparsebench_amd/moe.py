@@ -292,3 +292,52 @@ def moe_gated_backward(saved: GatedSaved, grad_out: torch.Tensor) -> GatedGrads:
 
     return GatedGrads(*_C.gated_backward_cuda(grad_out, saved.x, saved.expert_weight, saved.w1, saved.w2, saved.kept,
                                               saved.activation, saved.valid_tokens))
+
+
+# ---- gated experts with 4-bit weights, for decode steps ----
+
+
+class Experts4(NamedTuple):
+    """Expert weights [E, K, N] in 4 bits: codes [E, N/32, K/32, 32, 16] (32 consecutive k
+    of a column in 16 bytes, the even ones in the low halves) and scales [E, N/32, K/32,
+    32], both uint8. A code's sign, two exponent and one mantissa bits stand for 0, 0.5, 1,
+    1.5, 2, 3, 4 or 6 and their negatives, a scale byte s for 2^(s - 127) (255: NaN)."""
+
+    codes: torch.Tensor
+    scales: torch.Tensor
+
+
+def quantize_experts(w: torch.Tensor) -> Experts4:
+    """w [E, K, N] (K the reduction's side; bf16 / fp16 / fp32, K and N multiples of 32) in 4
+    bits: each 32 along K share the largest power of two that leaves the largest of them at 4
+    or more of it, and are rounded to the nearest code, halves to the even one, 6 and more to
+    6. A group with an infinity or NaN becomes NaN. For w1 [E, D, 2F] and w2 [E, F, D] of
+    moe_forward_gated_4bit."""
+    from sparsebench_amd import _C
+
+    return Experts4(*_C.quantize4_cuda(w))
+
+
+def dequantize_experts(w: Experts4) -> torch.Tensor:
+    """The weights [E, K, N] that 4-bit ones stand for, in bf16 (exact but for values under its
+    smallest normal): what moe_forward_gated takes for prompts."""
+    from sparsebench_amd import _C
+
+    return _C.dequantize4_cuda(*w)
+
+
+def moe_forward_gated_4bit(
+    x: torch.Tensor,
+    expert_idx: torch.Tensor,
+    expert_weight: torch.Tensor,
+    w1: Experts4,
+    w2: Experts4,
+    activation: str = "silu",
+    valid_tokens: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """moe_forward_gated with 4-bit experts, for decode steps: at most 2048 copies (T k).
+    w1 of [E, D, 2F], w2 of [E, F, D]; the other operands as there. The products take the
+    weights at their exact values and sum in fp32; H is rounded to bf16 between them."""
+    from sparsebench_amd import _C
+
+    return _C.experts4_layer_cuda(x, expert_idx, expert_weight, w1, w2, activation, valid_tokens)
