@@ -435,6 +435,42 @@ int sb_quantize4(const void* w, int32_t dtype, void* codes, void* scales, int64_
 int sb_dequantize4(const void* codes, const void* scales, void* w, int64_t num_experts, int64_t k, int64_t n,
                    void* stream);
 
+/* ---- Orthogonalised updates (Muon) ---------------------------------------- */
+
+/* One tensor of sb_muon: `matrices` matrices of rows x columns, each array's
+ * matrices and rows some strides of elements apart, a row's values contiguous.
+ * param and grad are of their SB_DTYPE_* codes; momentum is fp32; master is
+ * NULL, or fp32 weights that are updated in the parameter's place and rounded
+ * into it. */
+typedef struct {
+  void* param;
+  const void* grad;
+  float* momentum;
+  float* master;
+  int64_t matrices, rows, columns;
+  int64_t param_matrix, param_row, grad_matrix, grad_row, momentum_matrix, momentum_row, master_matrix, master_row;
+  int32_t param_dtype;
+  int32_t grad_dtype;
+} SbMuonTensor;
+
+/* No counterpart in the reference: one step of `count` tensors, in place. For
+ * each matrix, with g = grad * *grad_scale (NULL: 1),
+ *   m = momentum m + (1 - momentum) g,  u = (1 - momentum) g + momentum m (nesterov) or m
+ *   X = u / (|u| + 1e-7) (Frobenius); steps times X = a X + (b A + c A^2) X, A = X X^T
+ *       on the smaller side, (a, b, c) = (3.4445, -4.7750, 2.0315)
+ *   w = w (1 - lr weight_decay) - lr update_rms sqrt(max(rows, columns)) X
+ * The products take fp16 operands and sum in fp32; X is kept to twice fp16's
+ * bits. lr_ptr (NULL: lr) and grad_scale: one fp32 on the device. `tensors` is
+ * read before the call returns. workspace: *workspace_bytes of sb_muon_sizes for
+ * the list on the same device, 256-byte aligned. sb_orthogonalize: param = X of
+ * grad (momentum and master NULL); param may be grad. */
+int sb_muon_sizes(const SbMuonTensor* tensors, int64_t count, int64_t* workspace_bytes);
+int sb_muon(const SbMuonTensor* tensors, int64_t count, float lr, const float* lr_ptr, float momentum,
+            int32_t nesterov, float weight_decay, float update_rms, int32_t steps, const float* grad_scale,
+            void* workspace, int64_t workspace_bytes, void* stream);
+int sb_orthogonalize(const SbMuonTensor* tensors, int64_t count, int32_t steps, void* workspace,
+                     int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

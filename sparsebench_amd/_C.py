@@ -1161,3 +1161,117 @@ def dequantize4_cuda(codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
             check(lib().sb_dequantize4(codes.data_ptr(), scales.data_ptr(), w.data_ptr(), e, k, n,
                                        stream_of(codes.device)))
     return w
+
+
+# ---- orthogonalised updates (this build's C ABI) ----
+
+_MAX_STEPS = 32
+
+
+def _stack_of(t: torch.Tensor, what: str, written: bool) -> tuple[int, int, int, int, int]:
+    """(matrices, rows, columns, stride of matrices, of rows) of a tensor [..., rows, columns]
+    whose rows are contiguous and whose leading dimensions are one; of tensors that are
+    written, no two elements in one place."""
+    if t.dim() < 2:
+        _fail(f"{what} must be matrices [..., rows, columns], got {_shape(t)}")
+    rows, columns = t.shape[-2:]
+    if columns > 1 and t.stride(-1) != 1:
+        _fail(f"{what} must have contiguous rows")
+    matrices, stride = 1, 0
+    for size, step in zip(reversed(t.shape[:-2]), reversed(t.stride()[:-2])):
+        if size == 1:
+            continue
+        if matrices > 1 and step != matrices * stride:
+            _fail(f"{what} must have leading dimensions that are one stride apart")
+        stride = step if matrices == 1 else stride
+        matrices *= size
+    if written and t.numel() > 0:
+        span = 1
+        for size, step in sorted(((s, d) for s, d in ((matrices, stride), (rows, t.stride(-2)), (columns, 1)) if s > 1),
+                                 key=lambda d: d[1]):
+            if step < span:
+                _fail(f"{what} must not overlap themselves")
+            span += (size - 1) * step
+    return matrices, rows, columns, stride, t.stride(-2)
+
+
+def _check_stacks(tensors, device: int, what: str, dtypes, shapes=None) -> None:
+    if not all(t.get_device() == device for t in tensors):
+        _fail(f"{what} must be on one GPU")
+    if not all(t.dtype in dtypes for t in tensors):
+        _fail(f"{what} must be of {', '.join(str(d).removeprefix('torch.') for d in dtypes)}")
+    if shapes is not None and list(map(_shape_of, tensors)) != shapes:
+        _fail(f"{what} must have the parameters' shapes")
+
+
+def _muon_words(params, grads, momenta, masters) -> array.array:
+    """The list as sb_muon takes it (SbMuonTensor, 16 words each)."""
+    words = array.array("q")
+    none = itertools.repeat(None)
+    for p, g, m, w in zip(params, grads, momenta or none, masters or none):
+        stack = _stack_of(p, "parameters", True)
+        _, _, _, *g_strides = _stack_of(g, "gradients", False)
+        _, _, _, *m_strides = (0,) * 5 if m is None else _stack_of(m, "momenta", True)
+        _, _, _, *w_strides = (0,) * 5 if w is None else _stack_of(w, "masters", True)
+        words.extend((p.data_ptr(), g.data_ptr(), 0 if m is None else m.data_ptr(), 0 if w is None else w.data_ptr(),
+                      *stack, *g_strides, *m_strides, *w_strides,
+                      _GATE_DTYPES[p.dtype] | _GATE_DTYPES[g.dtype] << 32))
+    return words
+
+
+def _muon_workspace(words: array.array, count: int, device: torch.device) -> torch.Tensor:
+    size = ctypes.c_int64()
+    check(lib().sb_muon_sizes(words.buffer_info()[0], count, ctypes.byref(size)))
+    return torch.empty(size.value, dtype=torch.uint8, device=device)
+
+
+def _check_steps(steps: int) -> None:
+    if not 1 <= steps <= _MAX_STEPS:
+        _fail(f"steps must be 1 to {_MAX_STEPS}, got {steps}")
+
+
+def muon_cuda(params, grads, momenta, masters, lr, momentum: float, nesterov: bool, weight_decay: float,
+              update_rms: float, steps: int, grad_scale) -> None:
+    """One orthogonalised step of a list of stacks of matrices, in place (include/sparsebench_hip.h: sb_muon)."""
+    n = len(params)
+    if not (len(grads) == len(momenta) == n) or (masters is not None and len(masters) != n):
+        _fail("params, grads, momenta and masters must be lists of one length")
+    _check_steps(steps)
+    if not 0 <= momentum < 1:
+        _fail(f"momentum must be in [0, 1), got {momentum}")
+    if n == 0:
+        return
+    dev, index = params[0].device, params[0].get_device()
+    if index < 0:
+        _fail("parameters must be on one GPU")
+    shapes = list(map(_shape_of, params))
+    _check_stacks(params, index, "parameters", _GATE_DTYPES)
+    _check_stacks(grads, index, "gradients", _GATE_DTYPES, shapes)
+    _check_stacks(momenta, index, "momenta", (torch.float32,), shapes)
+    if masters is not None:
+        _check_stacks(masters, index, "masters", (torch.float32,), shapes)
+    words = _muon_words(params, grads, momenta, masters)
+    lr_ptr, scale_ptr = _device_scalar(lr, "lr", dev), _device_scalar(grad_scale, "grad_scale", dev)
+    with _device_of(params[0]):
+        if scale_ptr is None and grad_scale is not None:  # a number: as a device scalar
+            scale = torch.full((1,), float(grad_scale), dtype=torch.float32, device=dev)
+            scale_ptr = scale.data_ptr()
+        workspace = _muon_workspace(words, n, dev)
+        check(lib().sb_muon(words.buffer_info()[0], n, 0.0 if lr_ptr else float(lr), lr_ptr, momentum, int(nesterov),
+                            weight_decay, update_rms, steps, scale_ptr, workspace.data_ptr(), workspace.numel(),
+                            stream_of(dev)))
+    torch.autograd.graph.increment_version([*params, *(masters or ())])
+
+
+def orthogonalize_cuda(matrices: torch.Tensor, steps: int) -> torch.Tensor:
+    """Newton-Schulz products of each matrix (include/sparsebench_hip.h: sb_orthogonalize)."""
+    _check_steps(steps)
+    if not matrices.is_cuda or matrices.dtype not in _GATE_DTYPES:
+        _fail(f"matrices must be a bfloat16, float16 or float32 CUDA tensor, got {matrices.dtype} on {matrices.device}")
+    out = torch.empty(matrices.shape, dtype=matrices.dtype, device=matrices.device)
+    words = _muon_words([out], [matrices], None, None)
+    with _device_of(matrices):
+        workspace = _muon_workspace(words, 1, matrices.device)
+        check(lib().sb_orthogonalize(words.buffer_info()[0], 1, steps, workspace.data_ptr(), workspace.numel(),
+                                     stream_of(matrices.device)))
+    return out

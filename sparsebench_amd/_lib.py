@@ -113,6 +113,9 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     ),
     "sb_quantize4": (_c_int, [_ptr, _i32, _ptr, _ptr, _i64, _i64, _i64, _ptr]),
     "sb_dequantize4": (_c_int, [_ptr, _ptr, _ptr, _i64, _i64, _i64, _ptr]),
+    "sb_muon_sizes": (_c_int, [_ptr, _i64, ctypes.POINTER(_i64)]),
+    "sb_muon": (_c_int, [_ptr, _i64, _f32, _ptr, _f32, _i32, _f32, _f32, _i32, _ptr, _ptr, _i64, _ptr]),
+    "sb_orthogonalize": (_c_int, [_ptr, _i64, _i32, _ptr, _i64, _ptr]),
     "sb_norm_in": (_c_int, [_ptr, _i64, _ptr, _i32, _ptr, _i32, _i64, _i64, _f32, _ptr, _ptr]),
     "sb_norm_out": (
         _c_int,

@@ -35,6 +35,7 @@
 namespace sb {
 
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 typedef short i16x4_t __attribute__((ext_vector_type(4)));
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
@@ -103,10 +104,11 @@ __device__ __forceinline__ void wait_vmcnt() {
 // does, one 16-byte read a fragment. GATED: the tile's columns are BN / 2 of
 // one matrix, then as many of another; a wave's 32-column blocks alternate
 // between the two, so that acc[2j] and acc[2j + 1] hold the same columns of
-// the first and the second.
+// the first and the second. F16: the operands are fp16, not bf16 (the loads
+// and LDS layouts are those of any 16-bit type).
 template <int BM_, int BN_, int BK_, int STAGES_, int WM_ = 2, int WN_ = 2, int CPA_ = 0, int CPB_ = 0, int PIPE_ = 0,
           int EPI_PARTS_ = 1, int APAIR_ = 0, int BSTAGES_ = 0, int XW_ = 0, int AT_ = 0, int BT_ = 0,
-          int GATED_ = 0>
+          int GATED_ = 0, int F16_ = 0>
 struct DmaCfg {
   static constexpr int BM = BM_, BN = BN_, BK = BK_, STAGES = STAGES_;
   static constexpr int BSTAGES = BSTAGES_ > 0 ? BSTAGES_ : STAGES_;
@@ -115,7 +117,7 @@ struct DmaCfg {
   static constexpr int PIPE = PIPE_;
   static constexpr int EPI_PARTS = EPI_PARTS_;
   static constexpr bool APAIR = APAIR_ != 0;
-  static constexpr bool AT = AT_ != 0, BT = BT_ != 0, GATED = GATED_ != 0;
+  static constexpr bool AT = AT_ != 0, BT = BT_ != 0, GATED = GATED_ != 0, F16 = F16_ != 0;
   static constexpr int WM = WM_, WN = WN_;
   static constexpr int kComputeWaves = WM * WN;
   static constexpr int kWaves = kComputeWaves + XW_;
@@ -521,12 +523,19 @@ struct DmaMainloop {
       }
     }
   };
+  __device__ __forceinline__ static f32x16_t mfma(const bf16x8_t& b, const bf16x8_t& a, const f32x16_t& c) {
+    if constexpr (Cfg::F16)
+      return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, b), __builtin_bit_cast(f16x8_t, a), c,
+                                                    0, 0, 0);
+    else
+      return __builtin_amdgcn_mfma_f32_32x32x16_bf16(b, a, c, 0, 0, 0);
+  }
   __device__ __forceinline__ static void mfmas(Acc& acc, const bf16x8_t (&a)[Cfg::TM], const bf16x8_t (&b)[Cfg::TN]) {
 #pragma unroll
     for (int jn = 0; jn < Cfg::TN; ++jn)
 #pragma unroll
       for (int i = 0; i < Cfg::TM; ++i)
-        acc[jn][i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(b[jn], a[i], acc[jn][i], 0, 0, 0);
+        acc[jn][i] = mfma(b[jn], a[i], acc[jn][i]);
   }
 
   // One K step's fragments and MFMAs, from A slot `as` (K half `khalf` of
@@ -554,7 +563,7 @@ struct DmaMainloop {
           constexpr int i = decltype(ic)::value;
 #pragma unroll
           for (int jn = 0; jn < Cfg::TN; ++jn)
-            acc[jn][i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(b[s & 1][jn], a[i], acc[jn][i], 0, 0, 0);
+            acc[jn][i] = mfma(b[s & 1][jn], a[i], acc[jn][i]);
           if constexpr (s + 1 < kSub) a[i] = read_a1(s + 1, i);
           // This sub-step's share of the DMA, spread over its row groups.
           constexpr int q0 = s * kDma / kSub + i * (kDma / kSub) / Cfg::TM;

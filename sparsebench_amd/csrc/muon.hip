@@ -1,0 +1,799 @@
+// Orthogonalised updates: momentum, Newton-Schulz products, step.
+//
+//   m = b m + (1 - b) g,  u = (1 - b) g + b m  (nesterov; else m),  g = grad * grad_scale
+//   X = u / (|u|_F + eps), the smaller side as rows
+//   steps times:  A = X X^T,  B = b5 A + c5 A A,  X = a5 X + B X
+//   w = w (1 - lr wd) - lr update_rms sqrt(max(rows, columns)) X
+//
+// (a5, b5, c5) = (3.4445, -4.7750, 2.0315): singular values in (0, 1] go to
+// about [0.68, 1.2] in five steps, and none ever passes 1.21, whatever the
+// input. So |X| < 1.21, |A| < 1.47 and |B| < 2.81, entry by entry, and all are
+// held in fp16 times 2^14: no entry overflows, and those down to 2^-28 are normal.
+// bf16 would lose what matters: a small singular value grows 3.44-fold each
+// step while the rounding errors of the large ones grow along with it (a
+// gradient with a few strong directions, 768 x 1024: 3.2% off in bf16, 0.4% in fp16).
+// Most of that comes from rounding X itself, so what the rounding leaves goes
+// into a second fp16 matrix, added in a5 X, which costs no product; most of the
+// rest from the diagonals of A and B, which are kept in fp32 beside matrices with
+// zeros there: (D + O)^2 = D^2 + D O + O D + O O, and B's diagonal joins a5 X.
+//
+// A and B are symmetric: only tiles on and above the diagonal are computed, and
+// written twice. The products run on the LDS-DMA main loop (gemm_dma.hpp), X X^T
+// with B's columns as rows. Matrices are padded with zeros to whole tiles, which
+// the products leave zero. All matrices of one size go together, whatever tensors
+// they come from and whichever side is the smaller.
+
+#include <cmath>
+#include <vector>
+
+#include "gemm_dma.hpp"
+#include "workspace.hpp"
+
+namespace sb {
+namespace {
+
+constexpr float kA5 = 3.4445f, kB5 = -4.7750f, kC5 = 2.0315f;
+constexpr float kScale = 16384.0f, kUnscale = 1.0f / 16384.0f;
+constexpr float kNormEps = 1e-7f;
+constexpr int kThreads = 256;
+constexpr int kMaxSteps = 32;
+constexpr int64_t kBatchBytes = int64_t{6} << 30;  // of a batch's workspace, where that holds a matrix
+
+// ------------------------------------------------------------ the list ---
+
+struct Entry {
+  void* param;
+  const void* grad;
+  float *momentum, *master;
+  int64_t param_matrix, param_row, grad_matrix, grad_row, momentum_matrix, momentum_row, master_matrix, master_row;
+  int32_t first;  // its first matrix in the batch
+  int32_t rows, columns;
+  uint8_t param_dtype, grad_dtype, wide, tall;  // wide: vectors of 8 may be used; tall: rows > columns
+};
+constexpr int kEntries = 16;
+
+struct Table {
+  Entry e[kEntries];
+  int32_t count;
+};
+
+struct Hyper {
+  const float *lr_ptr, *grad_scale;
+  float lr, momentum, weight_decay, update_rms;
+  int32_t nesterov;
+};
+
+// The batch's entry of a matrix, and the matrix's place in it.
+__device__ __forceinline__ const Entry& entry_of(const Table& t, int matrix, int64_t* at) {
+  int i = 0;
+  while (i + 1 < t.count && t.e[i + 1].first <= matrix) ++i;
+  i = uniform(i);
+  *at = matrix - t.e[i].first;
+  return t.e[i];
+}
+
+__device__ __forceinline__ float value_of(uint16_t bits, int dtype) {
+  return dtype == SB_DTYPE_BF16 ? bf16_to_f32(bits) : static_cast<float>(__builtin_bit_cast(_Float16, bits));
+}
+
+// Values i .. i + 7 of p (n of them there).
+__device__ __forceinline__ void load8(const void* p, int dtype, int64_t i, int n, bool wide, float (&v)[8]) {
+  if (dtype == SB_DTYPE_F32) {
+    const float* f = static_cast<const float*>(p) + i;
+    if (wide && n >= 8) {
+      const f32x4_t a = *reinterpret_cast<const f32x4_t*>(f), b = *reinterpret_cast<const f32x4_t*>(f + 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = a[e], v[4 + e] = b[e];
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = e < n ? f[e] : 0.0f;
+    }
+    return;
+  }
+  const uint16_t* h = static_cast<const uint16_t*>(p) + i;
+  if (wide && n >= 8) {
+    const u32x4_t a = *reinterpret_cast<const u32x4_t*>(h);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = value_of(static_cast<uint16_t>(a[e / 2] >> (16 * (e & 1))), dtype);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = e < n ? value_of(h[e], dtype) : 0.0f;
+  }
+}
+
+__device__ __forceinline__ uint16_t half_bits(float v) { return __builtin_bit_cast(uint16_t, static_cast<_Float16>(v)); }
+
+__device__ __forceinline__ u32x4_t pack8(const uint16_t (&bits)[8]) {
+  u32x4_t a;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) a[q] = bits[2 * q] | static_cast<uint32_t>(bits[2 * q + 1]) << 16;
+  return a;
+}
+
+__device__ __forceinline__ void store8(void* p, int dtype, int64_t i, int n, bool wide, const float (&v)[8]) {
+  if (dtype == SB_DTYPE_F32) {
+    float* f = static_cast<float*>(p) + i;
+    if (wide && n >= 8) {
+      *reinterpret_cast<f32x4_t*>(f) = f32x4_t{v[0], v[1], v[2], v[3]};
+      *reinterpret_cast<f32x4_t*>(f + 4) = f32x4_t{v[4], v[5], v[6], v[7]};
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (e < n) f[e] = v[e];
+    }
+    return;
+  }
+  uint16_t bits[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) bits[e] = dtype == SB_DTYPE_BF16 ? f32_to_bf16(v[e]) : half_bits(v[e]);
+  uint16_t* h = static_cast<uint16_t*>(p) + i;
+  if (wide && n >= 8) {
+    *reinterpret_cast<u32x4_t*>(h) = pack8(bits);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < n) h[e] = bits[e];
+  }
+}
+
+// What is orthogonalised, at eight values: of the momentum as it is after this
+// step, or the gradient alone where there is none.
+__device__ __forceinline__ void update_values(const Entry& e, const Hyper& h, float (&g)[8], const float (&m)[8]) {
+  if (!e.momentum || !h.nesterov) {
+    if (e.momentum)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) g[i] = m[i];
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) g[i] = (1.0f - h.momentum) * g[i] + h.momentum * m[i];
+}
+
+__device__ __forceinline__ void load_grad(const Entry& e, const Hyper& h, int64_t matrix, int row, int col, int n,
+                                          float (&g)[8]) {
+  load8(e.grad, e.grad_dtype, matrix * e.grad_matrix + row * e.grad_row + col, n, e.wide, g);
+  if (h.grad_scale) {
+    const float s = *h.grad_scale;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) g[i] *= s;
+  }
+}
+
+// ------------------------------------------------- momentum and its size ---
+
+constexpr int kVectors = 8;  // of 8 values, a lane's of a chunk
+
+int64_t chunks_of(int64_t rows, int64_t columns) {
+  return (rows * ((columns + 7) / 8) + kThreads * kVectors - 1) / (kThreads * kVectors);
+}
+
+// m after this step, and the sum of u^2 over the chunk: in fp64, so that no
+// gradient is too small or too large for its square.
+__global__ void __launch_bounds__(kThreads) momentum_kernel(Table t, Hyper h, double* __restrict__ partial) {
+  __shared__ double sums[kThreads / 64];
+  int64_t matrix;
+  const Entry& e = entry_of(t, static_cast<int>(blockIdx.y), &matrix);
+  const uint32_t per_row = static_cast<uint32_t>((e.columns + 7) / 8), all = per_row * static_cast<uint32_t>(e.rows);
+  double ss = 0.0;
+#pragma unroll 2
+  for (int i = 0; i < kVectors; ++i) {
+    const uint32_t at = (blockIdx.x * kVectors + i) * kThreads + threadIdx.x;
+    if (at >= all) break;
+    const int row = static_cast<int>(at / per_row), col = static_cast<int>(at % per_row) * 8, n = e.columns - col;
+    float g[8], m[8] = {};
+    load_grad(e, h, matrix, row, col, n, g);
+    if (e.momentum) {
+      const int64_t place = matrix * e.momentum_matrix + row * e.momentum_row + col;
+      load8(e.momentum, SB_DTYPE_F32, place, n, e.wide, m);
+#pragma unroll
+      for (int q = 0; q < 8; ++q) m[q] = h.momentum * m[q] + (1.0f - h.momentum) * g[q];
+      store8(e.momentum, SB_DTYPE_F32, place, n, e.wide, m);
+    }
+    update_values(e, h, g, m);
+#pragma unroll
+    for (int q = 0; q < 8; ++q) ss = fma(static_cast<double>(g[q]), static_cast<double>(g[q]), ss);
+  }
+  for (int s = 32; s > 0; s >>= 1) ss += __shfl_xor(ss, s);
+  if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = ss;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < kThreads / 64; ++w) ss += sums[w];
+    partial[static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x] = ss;
+  }
+}
+
+// factor[matrix] = 2^14 / (|u| + eps), the chunks' sums in a fixed order.
+__global__ void __launch_bounds__(kThreads)
+    norm_kernel(const double* __restrict__ partial, int32_t chunks, float* __restrict__ factor) {
+  __shared__ double sums[kThreads / 64];
+  double ss = 0.0;
+  for (int i = threadIdx.x; i < chunks; i += kThreads) ss += partial[static_cast<int64_t>(blockIdx.x) * chunks + i];
+  for (int s = 32; s > 0; s >>= 1) ss += __shfl_xor(ss, s);
+  if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = ss;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < kThreads / 64; ++w) ss += sums[w];
+    factor[blockIdx.x] = static_cast<float>(static_cast<double>(kScale) / (sqrt(ss) + static_cast<double>(kNormEps)));
+  }
+}
+
+// ------------------------------------------------------- X and its way back ---
+
+// X [mp, np] of each matrix: hi, and lo = what hi's rounding left.
+struct Padded {
+  uint16_t *hi, *lo;
+  int32_t mp, np;
+};
+
+constexpr int kTile = 64;
+
+// A tile of 64 x 64 of the tensor, and its place in X: for a tall tensor the
+// transposed one, through LDS (a row of 65 values: no two of a column in one bank).
+struct TilePlace {
+  int row, col;  // in the tensor
+};
+
+__device__ __forceinline__ TilePlace tile_place(const Entry& e, const Padded& x) {
+  const int across = (e.tall ? x.mp : x.np) / kTile;
+  return {static_cast<int>(blockIdx.x) / across * kTile, static_cast<int>(blockIdx.x) % across * kTile};
+}
+
+__global__ void __launch_bounds__(kThreads)
+    fill_kernel(Table t, Hyper h, const float* __restrict__ factor, Padded x) {
+  __shared__ float lds[kTile][kTile + 1];
+  int64_t matrix;
+  const Entry& e = entry_of(t, static_cast<int>(blockIdx.y), &matrix);
+  const TilePlace tp = tile_place(e, x);
+  const float f = factor[blockIdx.y];
+  const int64_t base = static_cast<int64_t>(blockIdx.y) * x.mp * x.np;
+  auto put = [&](int row, int col, const float (&v)[8]) {  // in X
+    uint16_t hi[8], lo[8];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      hi[q] = half_bits(v[q]);
+      lo[q] = half_bits(v[q] - value_of(hi[q], SB_DTYPE_F16));
+    }
+    const int64_t at = base + static_cast<int64_t>(row) * x.np + col;
+    *reinterpret_cast<u32x4_t*>(x.hi + at) = pack8(hi);
+    *reinterpret_cast<u32x4_t*>(x.lo + at) = pack8(lo);
+  };
+#pragma unroll
+  for (int i = 0; i < kTile * kTile / 8 / kThreads; ++i) {
+    const int item = i * kThreads + static_cast<int>(threadIdx.x), r = item / 8, c = item % 8 * 8;
+    const int row = tp.row + r, col = tp.col + c, n = e.columns - col;
+    float g[8] = {}, m[8] = {};
+    if (row < e.rows && n > 0) {
+      load_grad(e, h, matrix, row, col, n, g);
+      if (e.momentum)
+        load8(e.momentum, SB_DTYPE_F32, matrix * e.momentum_matrix + row * e.momentum_row + col, n, e.wide, m);
+      update_values(e, h, g, m);
+    }
+#pragma unroll
+    for (int q = 0; q < 8; ++q) g[q] *= f;
+    if (!e.tall) {
+      put(row, col, g);
+    } else {
+#pragma unroll
+      for (int q = 0; q < 8; ++q) lds[r][c + q] = g[q];
+    }
+  }
+  if (!e.tall) return;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kTile * kTile / 8 / kThreads; ++i) {
+    const int item = i * kThreads + static_cast<int>(threadIdx.x), r = item / 8, c = item % 8 * 8;
+    float v[8];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) v[q] = lds[c + q][r];
+    put(tp.col + r, tp.row + c, v);
+  }
+}
+
+// The weights' step from the last X; without a momentum X itself.
+__global__ void __launch_bounds__(kThreads) apply_kernel(Table t, Hyper h, Padded x) {
+  __shared__ float lds[kTile][kTile + 1];
+  int64_t matrix;
+  const Entry& e = entry_of(t, static_cast<int>(blockIdx.y), &matrix);
+  const TilePlace tp = tile_place(e, x);
+  const int64_t base = static_cast<int64_t>(blockIdx.y) * x.mp * x.np;
+  auto get = [&](int row, int col, float (&v)[8]) {
+    const int64_t at = base + static_cast<int64_t>(row) * x.np + col;
+    const u32x4_t hi = *reinterpret_cast<const u32x4_t*>(x.hi + at), lo = *reinterpret_cast<const u32x4_t*>(x.lo + at);
+#pragma unroll
+    for (int q = 0; q < 8; ++q)
+      v[q] = (value_of(static_cast<uint16_t>(hi[q / 2] >> (16 * (q & 1))), SB_DTYPE_F16) +
+              value_of(static_cast<uint16_t>(lo[q / 2] >> (16 * (q & 1))), SB_DTYPE_F16)) * kUnscale;
+  };
+  if (e.tall) {
+#pragma unroll
+    for (int i = 0; i < kTile * kTile / 8 / kThreads; ++i) {
+      const int item = i * kThreads + static_cast<int>(threadIdx.x), r = item / 8, c = item % 8 * 8;
+      float v[8];
+      get(tp.col + r, tp.row + c, v);
+#pragma unroll
+      for (int q = 0; q < 8; ++q) lds[c + q][r] = v[q];
+    }
+    __syncthreads();
+  }
+  const float lr = h.lr_ptr ? *h.lr_ptr : h.lr;
+  const float keep = 1.0f - lr * h.weight_decay;
+  const float size = lr * h.update_rms * sqrtf(static_cast<float>(max(e.rows, e.columns)));
+#pragma unroll
+  for (int i = 0; i < kTile * kTile / 8 / kThreads; ++i) {
+    const int item = i * kThreads + static_cast<int>(threadIdx.x), r = item / 8, c = item % 8 * 8;
+    const int row = tp.row + r, col = tp.col + c, n = e.columns - col;
+    if (row >= e.rows || n <= 0) continue;
+    float v[8];
+    if (e.tall) {
+#pragma unroll
+      for (int q = 0; q < 8; ++q) v[q] = lds[r][c + q];
+    } else {
+      get(row, col, v);
+    }
+    const int64_t place = matrix * e.param_matrix + row * e.param_row + col;
+    if (e.momentum) {
+      float w[8];
+      const int64_t at = e.master ? matrix * e.master_matrix + row * e.master_row + col : place;
+      load8(e.master ? e.master : e.param, e.master ? SB_DTYPE_F32 : e.param_dtype, at, n, e.wide, w);
+#pragma unroll
+      for (int q = 0; q < 8; ++q) v[q] = w[q] * keep - size * v[q];
+      if (e.master) store8(e.master, SB_DTYPE_F32, at, n, e.wide, v);
+    }
+    store8(e.param, e.param_dtype, place, n, e.wide, v);
+  }
+}
+
+// ------------------------------------------------------------- products ---
+
+struct ProductArgs {
+  const uint16_t* x;     // [M][mp][np], hi
+  uint16_t *gram, *poly; // A and B but for their diagonals, [M][mp][mp]
+  float *gram_diag, *poly_diag;  // [M][mp], not scaled
+  uint16_t* lo;          // of x, updated in place
+  uint16_t* next;        // hi of the next X
+  int32_t mp, np, matrices;
+};
+
+template <class Cfg>
+struct Operands {
+  __amdgpu_buffer_rsrc_t ra, rb;
+  uint32_t a_off[Cfg::kAInstr], b_off[Cfg::kBInstr];
+  uint32_t a_step, b_step;
+  __device__ __forceinline__ uint32_t a_voff(int q) const { return a_off[q]; }
+  __device__ __forceinline__ uint32_t b_voff(int q) const { return b_off[q]; }
+  __device__ __forceinline__ void a_src(int t, __amdgpu_buffer_rsrc_t* r, uint32_t* s) const {
+    *r = ra;
+    *s = static_cast<uint32_t>(t) * a_step;
+  }
+  __device__ __forceinline__ void b_src(int t, __amdgpu_buffer_rsrc_t* r, uint32_t* s) const {
+    *r = rb;
+    *s = static_cast<uint32_t>(t) * b_step;
+  }
+};
+
+// C rows i0 .., columns j0 .. of a [mp, k] times b: [k, columns], or with BT
+// the rows of b [columns, k].
+template <class Cfg>
+__device__ __forceinline__ void product(uint8_t* __restrict__ lds, const uint16_t* a, const uint16_t* b, int mp, int k,
+                                        int columns, int i0, int j0, typename DmaMainloop<Cfg>::Acc& acc) {
+  Operands<Cfg> src;
+  src.ra = make_rsrc(a, static_cast<uint32_t>(mp) * static_cast<uint32_t>(k) * 2u);
+  src.rb = make_rsrc(b, static_cast<uint32_t>(columns) * static_cast<uint32_t>(k) * 2u);
+  const ADmaPos<Cfg> ap;
+#pragma unroll
+  for (int q = 0; q < Cfg::kAInstr; ++q)
+    src.a_off[q] = (static_cast<uint32_t>(i0 + ap.row[q]) * static_cast<uint32_t>(k) + ap.chunk[q] * 8u) * 2u;
+  src.a_step = Cfg::BK * 2;
+  if constexpr (Cfg::BT) {
+    const BtDmaPos<Cfg> bp;
+#pragma unroll
+    for (int q = 0; q < Cfg::kBInstr; ++q)
+      src.b_off[q] = (static_cast<uint32_t>(j0 + bp.row[q]) * static_cast<uint32_t>(k) + bp.chunk[q] * 8u) * 2u;
+    src.b_step = Cfg::BK * 2;
+  } else {
+    const BDmaPos<Cfg> bp;
+#pragma unroll
+    for (int q = 0; q < Cfg::kBInstr; ++q)
+      src.b_off[q] = (static_cast<uint32_t>(bp.row[q]) * static_cast<uint32_t>(columns) + j0 + bp.col[q]) * 2u;
+    src.b_step = Cfg::BK * static_cast<uint32_t>(columns) * 2u;
+  }
+  DmaMainloop<Cfg>::run(lds, src, k / Cfg::BK, acc);
+}
+
+// The accumulators in fp32 through LDS, a group of 32 rows of each row of waves
+// at a time (part): rows(part, fn) calls fn(row, col, 8 values) with rows and
+// columns in the tile, neighbouring lanes on neighbouring columns; with mirror,
+// fn(col, row, 8 values of a column) as well, eight rows each.
+template <class Cfg>
+struct Epilogue {
+  using ML = DmaMainloop<Cfg>;
+  static constexpr int kRows = 32 * Cfg::WM, kChunks = Cfg::BN / 4;
+  static_assert(kRows * Cfg::BN * 4 <= Cfg::kLdsAlloc, "a part fits the ring");
+  __device__ __forceinline__ static int place(int r, int col) {  // of the 16 bytes that hold (r, col)
+    return r * (Cfg::BN * 4) + (((col >> 2) ^ (r & 15)) << 4);
+  }
+  __device__ __forceinline__ static int tile_row(int part, int r) { return r / 32 * Cfg::WTM + 32 * part + r % 32; }
+
+  template <int PART>
+  __device__ __forceinline__ static void put(uint8_t* __restrict__ lds, const typename ML::Acc& acc) {
+    const int lane = threadIdx.x & 63, wm = (threadIdx.x >> 6) / Cfg::WN;
+    const int r = 32 * wm + (lane & 31);
+    __syncthreads();
+#pragma unroll
+    for (int jn = 0; jn < Cfg::TN; ++jn)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<f32x4_t*>(lds + place(r, ML::out_col(jn, g))) =
+            f32x4_t{acc[jn][PART][4 * g], acc[jn][PART][4 * g + 1], acc[jn][PART][4 * g + 2], acc[jn][PART][4 * g + 3]};
+    __syncthreads();
+  }
+
+  template <class Fn>
+  __device__ __forceinline__ static void rows(const uint8_t* __restrict__ lds, int part, Fn fn) {
+    constexpr int kItems = kRows * Cfg::BN / 8;
+#pragma unroll
+    for (int i = 0; i < kItems / Cfg::kThreads; ++i) {
+      const int item = i * Cfg::kThreads + static_cast<int>(threadIdx.x);
+      const int r = item / (Cfg::BN / 8), c = item % (Cfg::BN / 8) * 8;
+      const f32x4_t a = *reinterpret_cast<const f32x4_t*>(lds + place(r, c));
+      const f32x4_t b = *reinterpret_cast<const f32x4_t*>(lds + place(r, c + 4));
+      float v[8];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) v[q] = a[q], v[4 + q] = b[q];
+      fn(tile_row(part, r), c, v);
+    }
+  }
+
+  template <class Fn>
+  __device__ __forceinline__ static void columns(const uint8_t* __restrict__ lds, int part, Fn fn) {
+    constexpr int kGroups = kRows / 8, kItems = kGroups * Cfg::BN;
+#pragma unroll
+    for (int i = 0; i < kItems / Cfg::kThreads; ++i) {
+      const int item = i * Cfg::kThreads + static_cast<int>(threadIdx.x);
+      const int c = item / kGroups, r = item % kGroups * 8;
+      float v[8];
+#pragma unroll
+      for (int q = 0; q < 8; ++q) v[q] = *reinterpret_cast<const float*>(lds + place(r + q, c) + (c & 3) * 4);
+      fn(c, tile_row(part, r), v);
+    }
+  }
+};
+
+// Tile `at` of the tiles on and above the diagonal of n x n.
+__host__ __device__ __forceinline__ void upper_tile(int at, int n, int* i, int* j) {
+  int row = 0;
+  while (at >= n - row) at -= n - row, ++row;
+  *i = row;
+  *j = row + at;
+}
+
+// SQUARE 0: A = X X^T. SQUARE 1: B = b5 A + c5 A A. Diagonals apart, in fp32.
+template <class Cfg, int SQUARE>
+__global__ void __launch_bounds__(Cfg::kThreads, 1) symmetric_kernel(ProductArgs p) {
+  using ML = DmaMainloop<Cfg>;
+  using Ep = Epilogue<Cfg>;
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[Cfg::kLdsAlloc];
+  const int n = p.mp / Cfg::BM, per = n * (n + 1) / 2;
+  const int at = xcd_remap(static_cast<int>(blockIdx.x), per * p.matrices);
+  int i, j;
+  upper_tile(uniform(at % per), n, &i, &j);
+  const int64_t matrix = uniform(at / per);
+  const int i0 = i * Cfg::BM, j0 = j * Cfg::BN;
+  const int64_t square = matrix * p.mp * p.mp;
+  const uint16_t* gram = p.gram + square;
+  float* diag = p.gram_diag + matrix * p.mp;
+  typename ML::Acc acc;
+  if constexpr (SQUARE) {
+    product<Cfg>(lds, gram, gram, p.mp, p.mp, p.mp, i0, j0, acc);
+  } else {
+    const uint16_t* x = p.x + matrix * p.mp * p.np;
+    product<Cfg>(lds, x, x, p.mp, p.np, p.mp, i0, j0, acc);
+  }
+  uint16_t* out = (SQUARE ? p.poly : p.gram) + square;
+  static_for<0, Cfg::TM>([&](auto part) {
+    constexpr int P = decltype(part)::value;
+    Ep::template put<P>(lds, acc);
+    auto write = [&](int64_t row, int64_t col, const float (&v)[8]) {
+      uint16_t bits[8];
+      if constexpr (SQUARE) {
+        const u32x4_t a = *reinterpret_cast<const u32x4_t*>(gram + row * p.mp + col);
+        const float here = diag[row];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          const float o = value_of(static_cast<uint16_t>(a[q / 2] >> (16 * (q & 1))), SB_DTYPE_F16);
+          bits[q] = half_bits(kB5 * o + kC5 * (kUnscale * v[q] + (here + diag[col + q]) * o));
+          if (row == col + q) {
+            bits[q] = 0;
+            p.poly_diag[matrix * p.mp + row] = kB5 * here + kC5 * (kUnscale * kUnscale * v[q] + here * here);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          bits[q] = half_bits(v[q] * kUnscale);
+          if (row == col + q) {
+            bits[q] = 0;
+            diag[row] = kUnscale * kUnscale * v[q];
+          }
+        }
+      }
+      *reinterpret_cast<u32x4_t*>(out + row * p.mp + col) = pack8(bits);
+    };
+    Ep::rows(lds, P, [&](int r, int c, const float (&v)[8]) { write(i0 + r, j0 + c, v); });
+    if (i != j) Ep::columns(lds, P, [&](int c, int r, const float (&v)[8]) { write(j0 + c, i0 + r, v); });
+  });
+}
+
+// next, lo = (a5 + B's diagonal) X + B X.
+template <class Cfg>
+__global__ void __launch_bounds__(Cfg::kThreads, 1) update_kernel(ProductArgs p) {
+  using ML = DmaMainloop<Cfg>;
+  using Ep = Epilogue<Cfg>;
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[Cfg::kLdsAlloc];
+  const int mt = p.mp / Cfg::BM, per = mt * (p.np / Cfg::BN);
+  const int at = xcd_remap(static_cast<int>(blockIdx.x), per * p.matrices);
+  const int64_t matrix = uniform(at / per);
+  const int i0 = uniform(at % per % mt) * Cfg::BM, j0 = uniform(at % per / mt) * Cfg::BN;
+  const int64_t whole = matrix * p.mp * p.np;
+  typename ML::Acc acc;
+  product<Cfg>(lds, p.poly + matrix * p.mp * p.mp, p.x + whole, p.mp, p.mp, p.np, i0, j0, acc);
+  static_for<0, Cfg::TM>([&](auto part) {
+    constexpr int P = decltype(part)::value;
+    Ep::template put<P>(lds, acc);
+    Ep::rows(lds, P, [&](int r, int c, const float (&v)[8]) {
+      const int64_t place = whole + static_cast<int64_t>(i0 + r) * p.np + j0 + c;
+      const u32x4_t h = *reinterpret_cast<const u32x4_t*>(p.x + place), l = *reinterpret_cast<const u32x4_t*>(p.lo + place);
+      const float self = kA5 + p.poly_diag[matrix * p.mp + i0 + r];
+      uint16_t hi[8], lo[8];
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        const float x = value_of(static_cast<uint16_t>(h[q / 2] >> (16 * (q & 1))), SB_DTYPE_F16) +
+                        value_of(static_cast<uint16_t>(l[q / 2] >> (16 * (q & 1))), SB_DTYPE_F16);
+        const float y = fmaf(kUnscale, v[q], self * x);
+        hi[q] = half_bits(y);
+        lo[q] = half_bits(y - value_of(hi[q], SB_DTYPE_F16));
+      }
+      *reinterpret_cast<u32x4_t*>(p.next + place) = pack8(hi);
+      *reinterpret_cast<u32x4_t*>(p.lo + place) = pack8(lo);
+    });
+  });
+}
+
+// 256 x 256 tiles of 8 waves (X X^T in K steps of 64, two stages of A and three
+// of B; the others in steps of 32, A two at a time), or 128 x 128 of 4.
+using WideGram = DmaCfg<256, 256, 64, 2, 2, 4, 0, 0, 5, 1, 0, 3, 0, 0, 1, 0, 1>;
+using WideRows = DmaCfg<256, 256, 32, 4, 2, 4, 0, 0, 5, 1, 1, 0, 0, 0, 0, 0, 1>;
+using NarrowGram = DmaCfg<128, 128, 64, 3, 2, 2, 0, 0, 5, 1, 0, 0, 0, 0, 1, 0, 1>;
+using NarrowRows = DmaCfg<128, 128, 64, 3, 2, 2, 0, 0, 5, 1, 0, 0, 0, 0, 0, 0, 1>;
+
+int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
+
+// A batch: matrices of one size.
+struct Shape {
+  int64_t m, n;
+  int64_t mp, np;
+  bool wide;
+  int64_t most;  // matrices of a batch
+};
+
+int64_t batch_bytes(const Shape& s, int64_t matrices);
+
+Shape shape_of(int64_t rows, int64_t columns, int64_t matrices, int cus) {
+  Shape s;
+  s.m = std::min(rows, columns);
+  s.n = std::max(rows, columns);
+  // Wide tiles where padding to them costs little and there is one for each CU.
+  const int64_t m256 = round_up(s.m, 256), n256 = round_up(s.n, 256);
+  const int64_t m128 = round_up(s.m, 128), n128 = round_up(s.n, 128);
+  s.wide = m256 * n256 * 5 <= m128 * n128 * 6 && matrices * (m256 / 256) * (m256 / 256 + 1) / 2 >= cus;
+  s.mp = s.wide ? m256 : m128;
+  s.np = s.wide ? n256 : n128;
+  s.most = 1;
+  while (s.most < 65535 && batch_bytes(s, s.most * 2) <= kBatchBytes) s.most *= 2;
+  s.most = std::min<int64_t>(s.most, 65535);
+  return s;
+}
+
+struct Buffers {
+  uint16_t *hi[2], *lo, *gram, *poly;
+  float *gram_diag, *poly_diag;
+  double* partial;
+  float* factor;
+  int64_t used;
+};
+
+Buffers carve(void* workspace, const Shape& s, int64_t matrices) {
+  Carver ws{static_cast<uint8_t*>(workspace)};
+  Buffers b;
+  b.hi[0] = ws.take<uint16_t>(matrices * s.mp * s.np);
+  b.hi[1] = ws.take<uint16_t>(matrices * s.mp * s.np);
+  b.lo = ws.take<uint16_t>(matrices * s.mp * s.np);
+  b.gram = ws.take<uint16_t>(matrices * s.mp * s.mp);
+  b.poly = ws.take<uint16_t>(matrices * s.mp * s.mp);
+  b.gram_diag = ws.take<float>(matrices * s.mp);
+  b.poly_diag = ws.take<float>(matrices * s.mp);
+  b.partial = ws.take<double>(matrices * std::max(chunks_of(s.m, s.n), chunks_of(s.n, s.m)));
+  b.factor = ws.take<float>(matrices);
+  b.used = ws.used;
+  return b;
+}
+
+int64_t batch_bytes(const Shape& s, int64_t matrices) { return carve(nullptr, s, matrices).used; }
+
+template <class Gram, class Rows>
+int run_steps(const Shape& s, const Buffers& b, int64_t matrices, int32_t steps, hipStream_t stream) {
+  if (!reduction_fits<Gram>(s.np) || !reduction_fits<Rows>(s.mp))
+    return fail(SB_ERR_INVALID, "orthogonalise: problem too large");
+  const int64_t t = s.mp / Gram::BM, upper = matrices * t * (t + 1) / 2, all = matrices * t * (s.np / Rows::BN);
+  if (all > 2147483647LL) return fail(SB_ERR_INVALID, "orthogonalise: problem too large");
+  for (int32_t i = 0; i < steps; ++i) {
+    const ProductArgs p{b.hi[i & 1], b.gram, b.poly, b.gram_diag, b.poly_diag, b.lo, b.hi[(i + 1) & 1], static_cast<int32_t>(s.mp),
+                        static_cast<int32_t>(s.np), static_cast<int32_t>(matrices)};
+    symmetric_kernel<Gram, 0><<<static_cast<uint32_t>(upper), Gram::kThreads, 0, stream>>>(p);
+    if (const int rc = check_launch("orthogonalise: X X^T")) return rc;
+    symmetric_kernel<Rows, 1><<<static_cast<uint32_t>(upper), Rows::kThreads, 0, stream>>>(p);
+    if (const int rc = check_launch("orthogonalise: A A")) return rc;
+    update_kernel<Rows><<<static_cast<uint32_t>(all), Rows::kThreads, 0, stream>>>(p);
+    if (const int rc = check_launch("orthogonalise: B X")) return rc;
+  }
+  return SB_OK;
+}
+
+int run_batch(const Table& t, const Hyper& h, const Shape& s, int64_t matrices, int32_t steps, void* workspace,
+              hipStream_t stream) {
+  const Buffers b = carve(workspace, s, matrices);
+  const uint32_t y = static_cast<uint32_t>(matrices);
+  const int64_t chunks = std::max(chunks_of(s.m, s.n), chunks_of(s.n, s.m));
+  const int64_t tiles = (s.mp / kTile) * (s.np / kTile);
+  if (chunks > 2147483647LL || tiles > 2147483647LL) return fail(SB_ERR_INVALID, "orthogonalise: problem too large");
+  momentum_kernel<<<dim3(static_cast<uint32_t>(chunks), y), kThreads, 0, stream>>>(t, h, b.partial);
+  if (const int rc = check_launch("orthogonalise: momentum")) return rc;
+  norm_kernel<<<y, kThreads, 0, stream>>>(b.partial, static_cast<int32_t>(chunks), b.factor);
+  if (const int rc = check_launch("orthogonalise: norm")) return rc;
+  const Padded first{b.hi[0], b.lo, static_cast<int32_t>(s.mp), static_cast<int32_t>(s.np)};
+  fill_kernel<<<dim3(static_cast<uint32_t>(tiles), y), kThreads, 0, stream>>>(t, h, b.factor, first);
+  if (const int rc = check_launch("orthogonalise: fill")) return rc;
+  if (const int rc = s.wide ? run_steps<WideGram, WideRows>(s, b, matrices, steps, stream)
+                            : run_steps<NarrowGram, NarrowRows>(s, b, matrices, steps, stream))
+    return rc;
+  const Padded last{b.hi[steps & 1], b.lo, static_cast<int32_t>(s.mp), static_cast<int32_t>(s.np)};
+  apply_kernel<<<dim3(static_cast<uint32_t>(tiles), y), kThreads, 0, stream>>>(t, h, last);
+  return check_launch("orthogonalise: step");
+}
+
+bool known_dtype(int64_t d) { return d == SB_DTYPE_BF16 || d == SB_DTYPE_F16 || d == SB_DTYPE_F32; }
+
+int check_list(const SbMuonTensor* tensors, int64_t count) {
+  if (count < 0 || (count > 0 && !tensors)) return fail(SB_ERR_INVALID, "muon: null buffer");
+  for (int64_t i = 0; i < count; ++i) {
+    const SbMuonTensor& a = tensors[i];
+    if (a.matrices < 0 || a.rows < 0 || a.columns < 0) return fail(SB_ERR_INVALID, "muon: negative size");
+    if (a.matrices == 0 || a.rows == 0 || a.columns == 0) continue;
+    if (a.rows >= kI32Limit || a.columns >= kI32Limit || a.matrices >= kI32Limit ||
+        round_up(a.rows, 256) * round_up(a.columns, 256) >= kI32Limit / 2 ||
+        round_up(std::min(a.rows, a.columns), 256) > 32768)
+      return fail(SB_ERR_INVALID, "muon: matrices of under 2^30 values with a side up to 32768, got %lld x %lld",
+                  static_cast<long long>(a.rows), static_cast<long long>(a.columns));
+    if (!a.param || !a.grad) return fail(SB_ERR_INVALID, "muon: null buffer");
+    if (!known_dtype(a.param_dtype) || !known_dtype(a.grad_dtype))
+      return fail(SB_ERR_INVALID, "muon: unsupported dtype code");
+    for (const int64_t stride : {a.param_matrix, a.param_row, a.grad_matrix, a.grad_row, a.momentum_matrix,
+                                 a.momentum_row, a.master_matrix, a.master_row})
+      if (stride < 0) return fail(SB_ERR_INVALID, "muon: negative stride");
+  }
+  return SB_OK;
+}
+
+bool empty(const SbMuonTensor& a) { return a.matrices == 0 || a.rows == 0 || a.columns == 0; }
+
+bool wide_values(const SbMuonTensor& a) {
+  auto ok = [](const void* p, int64_t dtype, int64_t matrix, int64_t row) {
+    const int64_t bytes = dtype == SB_DTYPE_F32 ? 4 : 2;
+    return !p || (aligned16(p) && matrix * bytes % 16 == 0 && row * bytes % 16 == 0);
+  };
+  return ok(a.param, a.param_dtype, a.param_matrix, a.param_row) && ok(a.grad, a.grad_dtype, a.grad_matrix, a.grad_row) &&
+         ok(a.momentum, SB_DTYPE_F32, a.momentum_matrix, a.momentum_row) &&
+         ok(a.master, SB_DTYPE_F32, a.master_matrix, a.master_row);
+}
+
+// f(shape, total matrices of that size) for each size in the list, by its first tensor.
+template <class F>
+int for_each_size(const SbMuonTensor* tensors, int64_t count, int cus, F&& f) {
+  std::vector<std::pair<int64_t, int64_t>> seen;
+  for (int64_t i = 0; i < count; ++i) {
+    if (empty(tensors[i])) continue;
+    const auto size = std::minmax(tensors[i].rows, tensors[i].columns);
+    const std::pair<int64_t, int64_t> key{size.first, size.second};
+    if (std::find(seen.begin(), seen.end(), key) != seen.end()) continue;
+    seen.push_back(key);
+    int64_t total = 0;
+    for (int64_t q = i; q < count; ++q) {
+      const auto other = std::minmax(tensors[q].rows, tensors[q].columns);
+      if (!empty(tensors[q]) && other.first == key.first && other.second == key.second) total += tensors[q].matrices;
+    }
+    if (const int rc = f(shape_of(key.first, key.second, total, cus), total, i)) return rc;
+  }
+  return SB_OK;
+}
+
+int run_list(const SbMuonTensor* tensors, int64_t count, const Hyper& h, int32_t steps, void* workspace,
+             int64_t workspace_bytes, hipStream_t stream) {
+  if (steps < 1 || steps > kMaxSteps) return fail(SB_ERR_INVALID, "muon: 1 to %d steps, got %d", kMaxSteps, steps);
+  int cus = 0;
+  if (const int rc = device_cus(&cus)) return rc;
+  return for_each_size(tensors, count, cus, [&](const Shape& s, int64_t total, int64_t first) {
+    if (const int rc = check_workspace(workspace, workspace_bytes, batch_bytes(s, std::min(total, s.most)))) return rc;
+    Table t{};
+    int64_t matrices = 0;
+    auto flush = [&]() -> int {
+      const int rc = matrices ? run_batch(t, h, s, matrices, steps, workspace, stream) : SB_OK;
+      t = Table{};
+      matrices = 0;
+      return rc;
+    };
+    for (int64_t i = first; i < count; ++i) {
+      const SbMuonTensor& a = tensors[i];
+      if (empty(a) || std::min(a.rows, a.columns) != s.m || std::max(a.rows, a.columns) != s.n) continue;
+      for (int64_t at = 0; at < a.matrices;) {
+        if (t.count == kEntries || matrices == s.most)
+          if (const int rc = flush()) return rc;
+        const int64_t take = std::min(a.matrices - at, s.most - matrices);
+        const int64_t pe = a.param_dtype == SB_DTYPE_F32 ? 4 : 2, ge = a.grad_dtype == SB_DTYPE_F32 ? 4 : 2;
+        t.e[t.count++] = Entry{static_cast<uint8_t*>(a.param) + at * a.param_matrix * pe,
+                               static_cast<const uint8_t*>(a.grad) + at * a.grad_matrix * ge,
+                               a.momentum ? a.momentum + at * a.momentum_matrix : nullptr,
+                               a.master ? a.master + at * a.master_matrix : nullptr,
+                               a.param_matrix, a.param_row, a.grad_matrix, a.grad_row, a.momentum_matrix,
+                               a.momentum_row, a.master_matrix, a.master_row, static_cast<int32_t>(matrices),
+                               static_cast<int32_t>(a.rows), static_cast<int32_t>(a.columns),
+                               static_cast<uint8_t>(a.param_dtype), static_cast<uint8_t>(a.grad_dtype),
+                               static_cast<uint8_t>(wide_values(a)), static_cast<uint8_t>(a.rows > a.columns)};
+        matrices += take;
+        at += take;
+      }
+    }
+    return flush();
+  });
+}
+
+}  // namespace
+}  // namespace sb
+
+using namespace sb;
+
+extern "C" int sb_muon_sizes(const SbMuonTensor* tensors, int64_t count, int64_t* workspace_bytes) {
+  if (const int rc = check_list(tensors, count)) return rc;
+  int cus = 0;
+  if (const int rc = device_cus(&cus)) return rc;
+  int64_t most = 256;
+  if (const int rc = for_each_size(tensors, count, cus, [&](const Shape& s, int64_t total, int64_t) {
+        most = std::max(most, batch_bytes(s, std::min(total, s.most)));
+        return SB_OK;
+      }))
+    return rc;
+  if (workspace_bytes) *workspace_bytes = most;
+  return clear_ok();
+}
+
+extern "C" int sb_muon(const SbMuonTensor* tensors, int64_t count, float lr, const float* lr_ptr, float momentum,
+                       int32_t nesterov, float weight_decay, float update_rms, int32_t steps, const float* grad_scale,
+                       void* workspace, int64_t workspace_bytes, void* stream) {
+  if (const int rc = check_list(tensors, count)) return rc;
+  for (int64_t i = 0; i < count; ++i)
+    if (!empty(tensors[i]) && !tensors[i].momentum) return fail(SB_ERR_INVALID, "muon: null buffer");
+  if (!(momentum >= 0.0f && momentum < 1.0f)) return fail(SB_ERR_INVALID, "muon: momentum must be in [0, 1)");
+  const Hyper h{lr_ptr, grad_scale, lr, momentum, weight_decay, update_rms, nesterov != 0};
+  if (const int rc = run_list(tensors, count, h, steps, workspace, workspace_bytes, as_stream(stream))) return rc;
+  return clear_ok();
+}
+
+extern "C" int sb_orthogonalize(const SbMuonTensor* tensors, int64_t count, int32_t steps, void* workspace,
+                                int64_t workspace_bytes, void* stream) {
+  if (const int rc = check_list(tensors, count)) return rc;
+  for (int64_t i = 0; i < count; ++i)
+    if (tensors[i].momentum || tensors[i].master)
+      return fail(SB_ERR_INVALID, "orthogonalise: neither momentum nor master");
+  const Hyper h{};
+  if (const int rc = run_list(tensors, count, h, steps, workspace, workspace_bytes, as_stream(stream))) return rc;
+  return clear_ok();
+}

@@ -1,4 +1,5 @@
-"""The AdamW step of a list of tensors in one kernel, with fp32 or 8-bit states.
+"""Updates: the AdamW step of a list of tensors in one kernel, with fp32 or 8-bit
+states, and the orthogonalised step of matrices (Muon).
 
     adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, lr, ...)   one step, in place
     new_step(device)                    the step counter that it advances
@@ -6,10 +7,15 @@
     dequantize(states, dtype)           the values that 8-bit states stand for
     AdamW(params, ...)                  states and counter kept together
 
-It updates what moe.moe_gated_backward gives gradients of, and any other
+    muon_step(params, grads, momenta, lr, ...)   one step of stacks of matrices, in place
+    orthogonalize(matrices)                      its Newton-Schulz products alone
+    Muon(params, ...)                            with its momenta
+
+They update what moe.moe_gated_backward gives gradients of, and any other
 tensors beside them. Nothing syncs: the step count lives on the GPU, and
 learning rate and gradient scale may too, so that a captured step can be
-replayed with other values.
+replayed with other values. Expert weights are stacks of matrices, which Muon
+takes as they are; the vectors beside them (norms, gates) and the router are AdamW's.
 """
 
 from __future__ import annotations
@@ -123,3 +129,87 @@ class AdamW:
         """One step; grads[i] is the gradient of the i-th parameter."""
         adamw_step(self.params, grads, self.exp_avgs, self.exp_avg_sqs, self.step_count, self.lr, self.betas, self.eps,
                    self.weight_decay, self.masters, grad_scale, self.seed)
+
+
+# ---- orthogonalised updates ----
+
+
+def orthogonalize(matrices: torch.Tensor, steps: int = 5) -> torch.Tensor:
+    """Newton-Schulz products of each matrix of a stack [..., rows, columns]: with the
+    smaller side as rows,
+
+        X = M / (|M| + 1e-7),  steps times X = a X + (b A + c A^2) X,  A = X X^T
+
+    (a, b, c) = (3.4445, -4.7750, 2.0315), which takes singular values from (0, 1] towards 1
+    (to about [0.7, 1.2] in five steps). bf16 / fp16 / fp32, of any size and of any strides
+    whose rows are contiguous. The products take fp16 operands, sum in fp32, and keep X to
+    twice fp16's bits: the result is within about 0.2% of exact arithmetic's, in the
+    matrix's norm, before it is rounded to the input's type. Results do not depend on
+    the other matrices of the stack."""
+    from sparsebench_amd import _C
+
+    return _C.orthogonalize_cuda(matrices, steps)
+
+
+def muon_step(
+    params: Sequence[torch.Tensor],
+    grads: Sequence[torch.Tensor],
+    momenta: Sequence[torch.Tensor],
+    lr: float | torch.Tensor,
+    momentum: float = 0.95,
+    nesterov: bool = True,
+    weight_decay: float = 0.0,
+    update_rms: float = 0.2,
+    steps: int = 5,
+    masters: Sequence[torch.Tensor] | None = None,
+    grad_scale: float | torch.Tensor | None = None,
+) -> None:
+    """One orthogonalised step of every matrix of every tensor, in place:
+
+        m = momentum m + (1 - momentum) g,  g = grad * grad_scale
+        u = (1 - momentum) g + momentum m  (nesterov), or m
+        w = w (1 - lr weight_decay) - lr update_rms sqrt(max(rows, columns)) orthogonalize(u)
+
+    so that an update's values have about the size update_rms (0.2: AdamW's, whose lr
+    then fits). params, grads: bf16 / fp16 / fp32 tensors [..., rows, columns], each
+    gradient of its parameter's shape; momenta: fp32, likewise, zeros at first. Their
+    rows must be contiguous, and may lie any strides apart: w1[..., :F] and w1[..., F:] of
+    the gated layer are two stacks, each expert's gate and up matrix orthogonalised by
+    itself. masters: fp32 weights updated in the parameters' place and rounded into them.
+    lr and grad_scale may be one-element fp32 tensors on the GPU. All on one GPU; tensors
+    must not overlap. Matrices of one size are taken together. Parameters and masters
+    count as modified in place, as in adamw_step; nothing syncs, and a step can be captured."""
+    from sparsebench_amd import _C
+
+    _C.muon_cuda(params, grads, momenta, masters, lr, momentum, nesterov, weight_decay, update_rms, steps, grad_scale)
+
+
+class Muon:
+    """muon_step with its momenta: step(grads) updates the matrices given here.
+
+    master_weights: fp32 masters of all parameters, copied from them here (self.masters)."""
+
+    def __init__(
+        self,
+        params: Iterable[torch.Tensor],
+        lr: float | torch.Tensor = 1e-3,
+        momentum: float = 0.95,
+        nesterov: bool = True,
+        weight_decay: float = 0.0,
+        update_rms: float = 0.2,
+        steps: int = 5,
+        master_weights: bool = False,
+    ) -> None:
+        self.params = list(params)
+        if not self.params:
+            raise ValueError("no parameters")
+        self.lr, self.momentum, self.nesterov, self.weight_decay = lr, momentum, nesterov, weight_decay
+        self.update_rms, self.steps = update_rms, steps
+        self.momenta = [torch.zeros(p.shape, dtype=torch.float32, device=p.device) for p in self.params]
+        # A view's copy keeps its strides; rows are all that the step needs contiguous.
+        self.masters = [p.detach().to(torch.float32, copy=True) for p in self.params] if master_weights else None
+
+    def step(self, grads: Sequence[torch.Tensor], grad_scale: float | torch.Tensor | None = None) -> None:
+        """One step; grads[i] is the gradient of the i-th parameter."""
+        muon_step(self.params, grads, self.momenta, self.lr, self.momentum, self.nesterov, self.weight_decay,
+                  self.update_rms, self.steps, self.masters, grad_scale)

@@ -1,0 +1,257 @@
+"""Orthogonalised updates against their formulas in 64 bits.
+
+Tolerances. In each step the entries of A and B beside the diagonal are rounded to fp16, at most
+2^-11 relative and independent: a noise matrix E whose product E X has, for m rows from 32 on,
+about the Frobenius norm 2^-11 / sqrt(3) |B| |X| / |X| of X's own, |b s + c s^2| <= 2.81 being B's
+size. Five steps' errors add up to at most 5 * 2.81 * 2^-11 / sqrt(3) = 0.4% of X, if later steps
+leave them as they are: those that fall on directions with singular values of 0.3 and more, where
+the polynomial's slope is at most 1.5 in size and turns negative, do; what falls on smaller ones
+grows up to 3.44-fold a step, but so does X there. Below 32 rows too few roundings average:
+there the test takes the first-order bound for roundings that all conspire, from the matrix's own
+singular values (rounding_bound). Rounding to the result's type adds half a step of it.
+"""
+
+import math
+
+import pytest
+import torch
+
+from sparsebench_amd import optim
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda"
+PRODUCTS = 5 * 2.8 * 2.0**-11 / math.sqrt(3)
+
+
+def newton_schulz(u, steps=5):
+    u = u.double()
+    x = u if u.shape[-2] <= u.shape[-1] else u.transpose(-1, -2)
+    x = x / (torch.linalg.matrix_norm(x, keepdim=True) + 1e-7)
+    for _ in range(steps):
+        a = x @ x.transpose(-1, -2)
+        x = 3.4445 * x + (-4.7750 * a + 2.0315 * (a @ a)) @ x
+    return x if u.shape[-2] <= u.shape[-1] else x.transpose(-1, -2)
+
+
+def gradient(*shape, seed=0, strong=2.0, dtype=torch.float32, scale=1e-3):
+    """A few strong directions over noise."""
+    g = torch.Generator().manual_seed(seed)
+    *lead, r, c = shape
+    low = torch.randn(*lead, r, 3, generator=g) @ torch.randn(*lead, 3, c, generator=g)
+    return ((torch.randn(*shape, generator=g) + strong * low) * scale).to(dtype).to(DEV)
+
+
+def slope_bound(s):
+    """The largest gain of a step at singular values s: of its divided differences over
+    pairs of values, with either sign, which a matrix function's derivative consists of."""
+    f = 3.4445 * s - 4.7750 * s**3 + 2.0315 * s**5
+    v, fv = torch.cat([s, -s]), torch.cat([f, -f])
+    d = v[:, None] - v[None, :]
+    slopes = torch.where(d.abs() > 1e-6, (fv[:, None] - fv[None, :]) / torch.where(d.abs() > 1e-6, d, 1.0),
+                         (3.4445 - 3 * 4.7750 * v**2 + 5 * 2.0315 * v**4)[:, None])
+    return slopes.abs().max(), f
+
+
+def rounding_bound(u, steps=5):
+    """Of |error| / |result|, where fewer than 32 rows do not average: a step's error is at most
+    2^-11 (|A|_F |b + 2 c A| + |B|_F) |X| for the entries' roundings and 2^-10 |A|_F |b + 2 c A|
+    |X| for A being hi hi^T, and grows by each later step's gain."""
+    s = torch.linalg.svdvals(u.double())
+    s = s / s.norm()
+    total, size = 0.0, 0.0
+    for _ in range(steps):
+        a = s * s
+        slope = (-4.7750 + 2 * 2.0315 * a).abs().max()
+        made = 2.0**-11 * (3 * a.norm() * slope + (-4.7750 * a + 2.0315 * a * a).norm()) * s.max()
+        gain, s = slope_bound(s)
+        total = total * gain + made * math.sqrt(len(s))
+    return (total / s.norm()).item()
+
+
+def check(got, want, u):
+    assert got.shape == want.shape
+    for g, w, x in zip(*(t.double().reshape(-1, *got.shape[-2:]) for t in (got, want, u))):
+        tol = PRODUCTS if min(x.shape) >= 32 else rounding_bound(x)
+        tol += torch.finfo(got.dtype).eps / 2
+        assert (g - w).norm() <= tol * w.norm(), ((g - w).norm() / w.norm()).item()
+
+
+SIZES = [(1, 1), (1, 40), (40, 1), (2, 3), (7, 128), (128, 128), (129, 127), (64, 1000), (1000, 64), (255, 257), (300, 200),
+         (256, 512), (512, 256), (77, 1001), (384, 640), (520, 1100)]
+
+
+@pytest.mark.parametrize("size", SIZES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_orthogonalize(size, dtype) -> None:
+    u = gradient(2, *size, seed=size[0], dtype=dtype)
+    got = optim.orthogonalize(u)
+    assert got.dtype == dtype
+    check(got, newton_schulz(u), u)
+
+
+@pytest.mark.parametrize("size", [(3, 1024, 1280), (300, 256, 256), (70, 512, 256), (130, 200, 250)])
+def test_many_matrices(size) -> None:
+    """Enough of them for the wide tiles, or a ragged number of narrow ones."""
+    u = gradient(*size, seed=3, dtype=torch.bfloat16)
+    got = optim.orthogonalize(u)
+    check(got, newton_schulz(u), u)
+    # Alone it takes narrow tiles, whose sums have the same order.
+    assert torch.equal(optim.orthogonalize(u[-1]), got[-1])
+
+
+def test_largest_side() -> None:
+    u = gradient(2304, 9000, seed=5, dtype=torch.bfloat16)
+    check(optim.orthogonalize(u), newton_schulz(u), u)
+
+
+@pytest.mark.parametrize("steps", [1, 2, 3, 8])
+def test_steps(steps) -> None:
+    u = gradient(2, 100, 150, seed=7)
+    got, want = optim.orthogonalize(u, steps), newton_schulz(u, steps)
+    assert (got.double() - want).norm() <= (PRODUCTS * max(1, steps / 5)) * want.norm()
+
+
+def test_leading_dimensions_and_strides() -> None:
+    u = gradient(2, 3, 60, 50, seed=8)
+    got = optim.orthogonalize(u)
+    assert got.shape == u.shape
+    assert torch.equal(got[1, 2], optim.orthogonalize(u[1, 2]))
+    wide = gradient(4, 60, 133, seed=9, dtype=torch.bfloat16)
+    for view in (wide[:, :, :64], wide[:, :, 64:133], wide[:, 1:, 3:70], wide[::2], wide.transpose(0, 1)[5:9]):
+        assert torch.equal(optim.orthogonalize(view), optim.orthogonalize(view.contiguous()))
+    one = u[0, :1].expand(3, 60, 50)
+    assert torch.equal(optim.orthogonalize(one)[2], optim.orthogonalize(u[0, 0]))
+
+
+def test_zeros_tiny_huge_and_not_finite() -> None:
+    """Zeros give zeros, sizes do not matter, and a matrix that is not finite stays alone."""
+    u = gradient(6, 48, 80, seed=10)
+    want = optim.orthogonalize(u)
+    v = u.clone()
+    v[0], v[1], v[2] = 0, u[1] * 2.0**60, u[2] * 2.0**20
+    v[3, 5, 7], v[4, 0, 0] = float("nan"), float("inf")
+    got = optim.orthogonalize(v)
+    assert not got[0].any() and torch.equal(got[5], want[5])
+    check(got[1:3], newton_schulz(u[1:3]), u[1:3])
+    assert got[3].isnan().all() and not got[4].isfinite().any()
+    small = optim.orthogonalize(torch.full((1, 2), 2.0**-100, device=DEV))
+    assert (small.abs() < 1e-20).all()  # far under the 1e-7 beside the norm
+
+
+def test_empty() -> None:
+    for shape in ((0, 4, 4), (2, 0, 4), (2, 4, 0)):
+        assert optim.orthogonalize(torch.zeros(*shape, device=DEV)).shape == shape
+    optim.muon_step([], [], [], lr=1.0)
+
+
+def step_reference(w, g, m, lr, momentum, nesterov, decay, rms, scale):
+    g = g.double() * scale
+    m = momentum * m.double() + (1 - momentum) * g
+    u = (1 - momentum) * g + momentum * m if nesterov else m
+    size = lr * rms * math.sqrt(max(w.shape[-2:]))
+    return w.double() * (1 - lr * decay), size * newton_schulz(u), m
+
+
+def check_weights(got, kept, update):
+    """Weights: the step's own error, and roundings of the weight's type and of fp32."""
+    tol = PRODUCTS * update.norm() + (torch.finfo(got.dtype).eps / 2 + 2.0**-22) * (kept - update).norm()
+    assert (got.double() - (kept - update)).norm() <= tol
+
+
+@pytest.mark.parametrize("param", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("masters", [False, True])
+@pytest.mark.parametrize("nesterov", [False, True])
+def test_step(param, masters, nesterov) -> None:
+    """Tensors of several sizes and strides; sizes that go together whichever side is the smaller."""
+    flat = gradient(3, 64, 2 * 96, seed=20, scale=0.05).to(param)
+    params = [flat[:, :, :96], flat[:, :, 96:], gradient(2, 96, 64, seed=21, scale=0.05).to(param),
+              gradient(33, 37, seed=22, scale=0.05).to(param)]
+    grad_type = torch.float32 if param == torch.float16 else param
+    grads = [gradient(*p.shape, seed=30 + i, dtype=grad_type) for i, p in enumerate(params)]
+    momenta = [gradient(*p.shape, seed=40 + i) for i, p in enumerate(params)]
+    ms = [p.float() for p in params] if masters else None
+    start = [(p.clone(), m.clone()) for p, m in zip(params, momenta)]
+    lr, mu, decay, rms, scale = 0.02, 0.9, 0.1, 0.3, 0.5
+    optim.muon_step(params, grads, momenta, lr, mu, nesterov, decay, rms, masters=ms, grad_scale=scale)
+    for i, (w, m) in enumerate(start):
+        kept, update, want_m = step_reference(w, grads[i], m, lr, mu, nesterov, decay, rms, scale)
+        # 3 roundings of fp32 in m, of terms no larger than its own size and g's
+        assert ((momenta[i].double() - want_m).abs() <= 2.0**-22 * (m.abs() + grads[i].abs()).double()).all()
+        check_weights(params[i], kept, update)
+        if masters:
+            check_weights(ms[i], kept, update)
+            assert torch.equal(params[i], ms[i].to(param))
+
+
+def test_many_tensors_of_one_size_and_of_many() -> None:
+    """More tensors than one launch takes; each as if alone."""
+    shapes = [(24, 40)] * 20 + [(40, 24)] * 19 + [(8, 200), (3, 5, 9), (1, 1)]
+
+    def make():
+        params = [gradient(*s, seed=50 + i, scale=0.1) for i, s in enumerate(shapes)]
+        grads = [gradient(*s, seed=150 + i) for i, s in enumerate(shapes)]
+        return params, grads, [torch.zeros_like(p) for p in params]
+
+    params, grads, momenta = make()
+    optim.muon_step(params, grads, momenta, 0.1)
+    alone, grads, others = make()
+    for p, g, m in zip(alone, grads, others):
+        optim.muon_step([p], [g], [m], 0.1)
+    assert all(torch.equal(a, b) for a, b in zip(params, alone))
+    assert all(torch.equal(a, b) for a, b in zip(momenta, others))
+
+
+def test_class_keeps_momenta_and_masters() -> None:
+    w1 = gradient(2, 64, 2 * 48, seed=60, scale=0.1, dtype=torch.bfloat16)
+    w2 = gradient(2, 48, 64, seed=61, scale=0.1, dtype=torch.bfloat16)
+    views = [w1[..., :48], w1[..., 48:], w2]
+    opt = optim.Muon(views, lr=0.01, weight_decay=0.1, master_weights=True)
+    wants = [v.double() for v in views]
+    ms = [torch.zeros(v.shape, dtype=torch.float64, device=DEV) for v in views]
+    moved = [0.0] * 3
+    for step in range(3):
+        grads = [gradient(*v.shape, seed=70 + 10 * step + i, dtype=torch.bfloat16) for i, v in enumerate(views)]
+        opt.step(grads)
+        for i, g in enumerate(grads):
+            kept, update, ms[i] = step_reference(wants[i], g, ms[i], 0.01, 0.95, True, 0.1, 0.2, 1.0)
+            wants[i] = kept - update
+            moved[i] += update.norm()
+    for i, v in enumerate(views):
+        assert (opt.masters[i].double() - wants[i]).norm() <= PRODUCTS * moved[i] + 3 * 2.0**-22 * wants[i].norm()
+        assert torch.equal(v, opt.masters[i].to(torch.bfloat16))
+    with pytest.raises(ValueError, match="no parameters"):
+        optim.Muon([])
+
+
+def test_modified_in_place_for_autograd() -> None:
+    w = gradient(32, 32, seed=80).requires_grad_()
+    loss = (w * w).sum()
+    optim.muon_step([w.detach()], [torch.ones_like(w)], [torch.zeros(32, 32, device=DEV)], 0.1)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        loss.backward()
+
+
+def test_graph_replays_with_other_rates_and_gradients() -> None:
+    shapes = [(4, 96, 160), (2, 160, 96), (50, 30)]
+    params = [gradient(*s, seed=90 + i, scale=0.1, dtype=torch.bfloat16) for i, s in enumerate(shapes)]
+    grads = [gradient(*s, seed=95 + i, dtype=torch.bfloat16) for i, s in enumerate(shapes)]
+    momenta = [torch.zeros(s, device=DEV) for s in shapes]
+    lr, scale = torch.tensor([0.01], device=DEV), torch.tensor([1.0], device=DEV)
+    mine = [[t.clone() for t in ts] for ts in (params, momenta)]
+    optim.muon_step([p.clone() for p in params], grads, [m.clone() for m in momenta], lr, grad_scale=scale)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        optim.muon_step(params, grads, momenta, lr, weight_decay=0.1, grad_scale=scale)
+    side = torch.cuda.Stream()
+    for i in range(4):
+        lr.fill_(0.01 * (i + 1)), scale.fill_(0.5 + i)
+        for j, g in enumerate(grads):
+            g.copy_(gradient(*g.shape, seed=200 + 10 * i + j, dtype=torch.bfloat16))
+        side.wait_stream(torch.cuda.current_stream())
+        graph.replay()
+        with torch.cuda.stream(side):
+            optim.muon_step(mine[0], grads, mine[1], lr, weight_decay=0.1, grad_scale=scale)
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(params + momenta, mine[0] + mine[1]))
