@@ -39,17 +39,17 @@ __global__ void __launch_bounds__(norm_threads(G)) norm_kernel(NormArgs a) {
   const int64_t limit = a.valid_tokens ? min(a.num_tokens, static_cast<int64_t>(max(0, *a.valid_tokens))) : a.num_tokens;
   float w[OUT ? S::kValues : 1], v[NEXT ? S::kValues : 1];
   if constexpr (OUT) {
-    load_vector<S>(a.weight, a.weight_dtype, a.d, t, 1.0f, w);
+    load_vector<S, VEC>(a.weight, a.weight_dtype, 0, a.d, t, 1.0f, w);
     if (a.gate_kind == SB_GATE_CHANNEL) {
       float g[S::kValues];
-      load_vector<S>(a.gate, a.gate_dtype, a.d, t, 0.0f, g);
+      load_vector<S, VEC>(a.gate, a.gate_dtype, 0, a.d, t, 0.0f, g);
 #pragma unroll
       for (int i = 0; i < S::kValues; ++i) w[i] *= g[i];
     }
 #pragma unroll
     for (int i = 0; i < S::kValues; ++i) w[i] *= a.scale;
   }
-  if constexpr (NEXT) load_vector<S>(a.next_weight, a.next_dtype, a.d, t, 1.0f, v);
+  if constexpr (NEXT) load_vector<S, VEC>(a.next_weight, a.next_dtype, 0, a.d, t, 1.0f, v);
 
   for (int64_t row = static_cast<int64_t>(blockIdx.x) * kGroups + threadIdx.x / G; row < limit;
        row += static_cast<int64_t>(gridDim.x) * kGroups) {
@@ -66,11 +66,10 @@ __global__ void __launch_bounds__(norm_threads(G)) norm_kernel(NormArgs a) {
       float r = 1.0f / sqrtf(ss[0] * a.inv_d + a.eps);
       if (a.gate_kind == SB_GATE_TOKEN) r *= load_as_f32(a.gate, a.gate_dtype, row * a.gate_stride);
       if (a.gate_kind == SB_GATE_FULL) {
+        float g[S::kValues];
+        load_vector<S, VEC>(a.gate, a.gate_dtype, row * a.gate_stride, a.d, t, 0.0f, g);
 #pragma unroll
-        for (int i = 0; i < S::kValues; ++i) {
-          const int at = S::column(i, t);
-          y[i] *= at < a.d ? load_as_f32(a.gate, a.gate_dtype, row * a.gate_stride + at) : 0.0f;
-        }
+        for (int i = 0; i < S::kValues; ++i) y[i] *= g[i];
       }
 #pragma unroll
       for (int i = 0; i < S::kValues; ++i) x[i] = rounded<DTYPE>(fmaf(y[i] * r, w[i], x[i]));
@@ -95,7 +94,7 @@ int launch_norm(const NormArgs& a, int32_t dtype, bool vec, hipStream_t stream) 
   int cus = 0;
   if (const int rc = device_cus(&cus)) return rc;
   return with_dtype(dtype, [&](auto type) {
-    with_norm_form(a.d, vec, [&](auto g, auto chunks, auto vectors) {
+    with_norm_form<false>(a.d, vec, [&](auto g, auto chunks, auto vectors) {
       constexpr int G = decltype(g)::value, kThreads = norm_threads(G), kGroups = kThreads / G;
       const int64_t groups = (a.num_tokens + kGroups - 1) / kGroups;
       const uint32_t grid = static_cast<uint32_t>(std::min<int64_t>(groups, int64_t{2048 / kThreads} * cus));
@@ -127,7 +126,7 @@ extern "C" int sb_norm_in(const void* x, int64_t x_stride, const void* weight, i
   a.eps = eps;
   a.inv_d = 1.0f / static_cast<float>(d_model);
   a.valid_tokens = valid_tokens;
-  const bool vec = norm_vectors(d_model, dtype, {x, out}, {x_stride});
+  const bool vec = norm_vectors(d_model, {{x, x_stride, dtype}, {out, 0, dtype}, {weight, 0, weight_dtype}});
   if (const int rc = launch_norm<false, true>(a, dtype, vec, as_stream(stream))) return rc;
   return clear_ok();
 }
@@ -164,7 +163,10 @@ extern "C" int sb_norm_out(const void* y, int64_t y_stride, const void* x, int64
   a.eps = eps;
   a.inv_d = 1.0f / static_cast<float>(d_model);
   a.valid_tokens = valid_tokens;
-  const bool vec = norm_vectors(d_model, dtype, {y, x, out, next ? next : out}, {y_stride, x_stride});
+  const bool vec = norm_vectors(
+      d_model, {{y, y_stride, dtype}, {x, x_stride, dtype}, {out, 0, dtype}, {next, 0, dtype}, {weight, 0, weight_dtype},
+                {gate_kind == SB_GATE_TOKEN ? nullptr : gate, gate_kind == SB_GATE_FULL ? gate_stride : 0, gate_dtype},
+                {next_weight, 0, next_dtype}});
   if (const int rc = next ? launch_norm<true, true>(a, dtype, vec, as_stream(stream))
                           : launch_norm<true, false>(a, dtype, vec, as_stream(stream)))
     return rc;

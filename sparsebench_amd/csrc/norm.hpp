@@ -64,39 +64,56 @@ struct Share {
   }
 };
 
-// The row's values that belong to thread t; 0 past its end.
+// The row's values that belong to thread t, 0 past its end: loaded, and then taken,
+// so that the next row's loads may be under way while one is worked on.
 template <class S, int DTYPE, bool VEC>
-__device__ __forceinline__ void load_row(const void* row, int d, int t, float (&v)[S::kValues]) {
-  if constexpr (VEC) {
+struct RowRegs {
+  static constexpr int kPerVector = DTYPE == SB_DTYPE_F32 ? 4 : 8;
+  std::conditional_t<VEC, u32x4_t, float> raw[VEC ? S::kValues / kPerVector : S::kValues];
+
+  __device__ __forceinline__ void load(const void* row, int d, int t) {
+    if constexpr (VEC) {
 #pragma unroll
-    for (int c = 0; c < S::kValues / 8; ++c) {
-      const int at = S::column(8 * c, t);
-      const bool there = at < d;
-      if constexpr (DTYPE == SB_DTYPE_F32) {
-        const f32x4_t* p = reinterpret_cast<const f32x4_t*>(static_cast<const float*>(row) + (there ? at : 0));
-        const f32x4_t a = p[0], b = p[1];
+      for (int c = 0; c < S::kValues / 8; ++c) {
+        const int at = S::column(8 * c, t);
+        const bool there = at < d;
+        const auto* p = reinterpret_cast<const u32x4_t*>(static_cast<const uint8_t*>(row) +
+                                                         (there ? at : 0) * (DTYPE == SB_DTYPE_F32 ? 4 : 2));
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[8 * c + e] = there ? a[e] : 0.0f, v[8 * c + 4 + e] = there ? b[e] : 0.0f;
-      } else {
-        u32x4_t a = *reinterpret_cast<const u32x4_t*>(static_cast<const uint16_t*>(row) + (there ? at : 0));
-        if (!there) a = u32x4_t{0u, 0u, 0u, 0u};
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const uint32_t pair = a[e / 2];
-          if constexpr (DTYPE == SB_DTYPE_BF16)
-            v[8 * c + e] = __uint_as_float(e & 1 ? pair & 0xffff0000u : pair << 16);
-          else
-            v[8 * c + e] = static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(pair >> (16 * (e & 1)))));
+        for (int q = 0; q < 8 / kPerVector; ++q) {
+          const u32x4_t a = p[q];
+          raw[c * (8 / kPerVector) + q] = there ? a : u32x4_t{0u, 0u, 0u, 0u};
         }
       }
-    }
-  } else {
+    } else {
 #pragma unroll
-    for (int i = 0; i < S::kValues; ++i) {
-      const int at = S::column(i, t);
-      v[i] = at < d ? load_as_f32(row, DTYPE, at) : 0.0f;
+      for (int i = 0; i < S::kValues; ++i) {
+        const int at = S::column(i, t);
+        raw[i] = at < d ? load_as_f32(row, DTYPE, at) : 0.0f;
+      }
     }
   }
+  __device__ __forceinline__ void take(float (&v)[S::kValues]) const {
+#pragma unroll
+    for (int i = 0; i < S::kValues; ++i) {
+      if constexpr (!VEC) {
+        v[i] = raw[i];
+      } else if constexpr (DTYPE == SB_DTYPE_F32) {
+        v[i] = __uint_as_float(raw[i / 4][i % 4]);
+      } else {
+        const uint32_t pair = raw[i / 8][i % 8 / 2];
+        if constexpr (DTYPE == SB_DTYPE_BF16) v[i] = __uint_as_float(i & 1 ? pair & 0xffff0000u : pair << 16);
+        else v[i] = static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(pair >> (16 * (i & 1)))));
+      }
+    }
+  }
+};
+
+template <class S, int DTYPE, bool VEC>
+__device__ __forceinline__ void load_row(const void* row, int d, int t, float (&v)[S::kValues]) {
+  RowRegs<S, DTYPE, VEC> r;
+  r.load(row, d, t);
+  r.take(v);
 }
 
 template <class S, int DTYPE, bool VEC>
@@ -134,15 +151,28 @@ __device__ __forceinline__ void store_row(void* row, int d, int t, const float (
   }
 }
 
-// A [D] vector's share (weights, gates), `otherwise` where there is none.
-template <class S>
-__device__ __forceinline__ void load_vector(const void* p, int32_t dtype, int d, int t, float otherwise,
+// f(integral_constant of a dtype known at run time, uniform).
+template <class F>
+__device__ __forceinline__ void by_dtype(int32_t dtype, F&& f) {
+  if (dtype == SB_DTYPE_BF16) f(std::integral_constant<int, SB_DTYPE_BF16>{});
+  else if (dtype == SB_DTYPE_F32) f(std::integral_constant<int, SB_DTYPE_F32>{});
+  else f(std::integral_constant<int, SB_DTYPE_F16>{});
+}
+
+// A row's or a [D] vector's share in a dtype known at run time (weights, gates);
+// `otherwise` where there is none, 0 past the end.
+template <class S, bool VEC>
+__device__ __forceinline__ void load_vector(const void* p, int32_t dtype, int64_t first, int d, int t, float otherwise,
                                             float (&v)[S::kValues]) {
+  if (!p) {
 #pragma unroll
-  for (int i = 0; i < S::kValues; ++i) {
-    const int at = S::column(i, t);
-    v[i] = p && at < d ? load_as_f32(p, dtype, at) : otherwise;
+    for (int i = 0; i < S::kValues; ++i) v[i] = otherwise;
+    return;
   }
+  by_dtype(dtype, [&](auto type) {
+    constexpr int kType = decltype(type)::value;
+    load_row<S, kType, VEC>(static_cast<const uint8_t*>(p) + first * (kType == SB_DTYPE_F32 ? 4 : 2), d, t, v);
+  });
 }
 
 // The sum over the wave's lanes, in every lane.
@@ -189,7 +219,8 @@ struct GroupSum {
 };
 
 // f(G, NCH, VEC as integral constants) for rows of d values; false if d is too long.
-template <class F>
+// Backward rows take more registers a value, so that fewer are a thread's.
+template <bool GRAD, class F>
 bool with_norm_form(int64_t d, bool vec, F&& f) {
   auto form = [&](auto g, auto chunks) {
     if (d > int64_t{8} * decltype(g)::value * decltype(chunks)::value) return false;
@@ -198,12 +229,15 @@ bool with_norm_form(int64_t d, bool vec, F&& f) {
     return true;
   };
   using std::integral_constant;
-  return form(integral_constant<int, 64>{}, integral_constant<int, 1>{}) ||
-         form(integral_constant<int, 64>{}, integral_constant<int, 2>{}) ||
-         form(integral_constant<int, 64>{}, integral_constant<int, 4>{}) ||
-         form(integral_constant<int, 256>{}, integral_constant<int, 2>{}) ||
-         form(integral_constant<int, 256>{}, integral_constant<int, 4>{}) ||
-         form(integral_constant<int, 1024>{}, integral_constant<int, 4>{});
+  constexpr integral_constant<int, 64> wave{};
+  constexpr integral_constant<int, 256> four{};
+  constexpr integral_constant<int, 1024> sixteen{};
+  constexpr integral_constant<int, 1> one{};
+  constexpr integral_constant<int, 2> two{};
+  constexpr integral_constant<int, 4> quad{};
+  if (form(wave, one) || form(wave, two)) return true;
+  if constexpr (GRAD) return form(four, one) || form(four, two) || form(sixteen, one) || form(sixteen, two) || form(sixteen, quad);
+  else return form(wave, quad) || form(four, two) || form(four, quad) || form(sixteen, quad);
 }
 
 constexpr int64_t kNormMaxD = 32768;
@@ -220,13 +254,16 @@ int with_dtype(int32_t dtype, F&& f) {
   }
 }
 
-// Where vectors of 8 may be used: all of these bytes multiples of 16.
-inline bool norm_vectors(int64_t d, int32_t dtype, std::initializer_list<const void*> rows,
-                         std::initializer_list<int64_t> strides) {
-  const int64_t bytes = dtype == SB_DTYPE_F32 ? 4 : 2;
+// Where vectors of 8 may be used: every row of every operand starts at a multiple of 16 bytes.
+struct NormOperand {
+  const void* p;  // null: not there
+  int64_t stride;
+  int32_t dtype;
+};
+inline bool norm_vectors(int64_t d, std::initializer_list<NormOperand> operands) {
   bool ok = d % 8 == 0;
-  for (const void* p : rows) ok = ok && aligned16(p);
-  for (int64_t s : strides) ok = ok && s * bytes % 16 == 0;
+  for (const NormOperand& o : operands)
+    ok = ok && (!o.p || (aligned16(o.p) && o.stride * (o.dtype == SB_DTYPE_F32 ? 4 : 2) % 16 == 0));
   return ok;
 }
 

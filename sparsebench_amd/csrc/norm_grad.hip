@@ -31,13 +31,31 @@ __global__ void __launch_bounds__(norm_threads(G)) norm_grad_kernel(NormArgs a) 
   GroupSum<G, 1> sum1(sums1);
   const int t = threadIdx.x % G;
   const int64_t limit = a.valid_tokens ? min(a.num_tokens, static_cast<int64_t>(max(0, *a.valid_tokens))) : a.num_tokens;
+  struct Rows {
+    RowRegs<S, DTYPE, VEC> d, o, dn, y;
+  };
+  auto load = [&](int64_t row, Rows& r) {
+    auto one = [&](RowRegs<S, DTYPE, VEC>& regs, const void* p, int64_t stride) {
+      regs.load(static_cast<const uint8_t*>(p) + row * stride * kElem, a.d, t);
+    };
+    if (OUT || a.grad_out) one(r.d, a.grad_out, a.grad_out_stride);
+    if constexpr (NEXT) {
+      one(r.o, a.x, a.x_stride);
+      one(r.dn, a.grad_next, a.grad_next_stride);
+    }
+    if constexpr (OUT) one(r.y, a.y, a.y_stride);
+  };
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kGroups;
+  int64_t row = static_cast<int64_t>(blockIdx.x) * kGroups + threadIdx.x / G;
+  Rows ahead;
+  if (VEC && row < limit) load(row, ahead);  // before the weights: they are waited for first
   // w: the weight, times the gate where that is one of the channels.
   float w[OUT ? N : 1], v[NEXT ? N : 1], q[OUT ? N : 1], dv[NEXT ? N : 1];
   if constexpr (OUT) {
-    load_vector<S>(a.weight, a.weight_dtype, a.d, t, 1.0f, w);
+    load_vector<S, VEC>(a.weight, a.weight_dtype, 0, a.d, t, 1.0f, w);
     if (a.gate_kind == SB_GATE_CHANNEL) {
       float g[N];
-      load_vector<S>(a.gate, a.gate_dtype, a.d, t, 0.0f, g);
+      load_vector<S, VEC>(a.gate, a.gate_dtype, 0, a.d, t, 0.0f, g);
 #pragma unroll
       for (int i = 0; i < N; ++i) w[i] *= g[i];
     }
@@ -45,28 +63,29 @@ __global__ void __launch_bounds__(norm_threads(G)) norm_grad_kernel(NormArgs a) 
     for (int i = 0; i < N; ++i) q[i] = 0.0f;
   }
   if constexpr (NEXT) {
-    load_vector<S>(a.next_weight, a.next_dtype, a.d, t, 1.0f, v);
+    load_vector<S, VEC>(a.next_weight, a.next_dtype, 0, a.d, t, 1.0f, v);
 #pragma unroll
     for (int i = 0; i < N; ++i) dv[i] = 0.0f;
   }
 
-  for (int64_t row = static_cast<int64_t>(blockIdx.x) * kGroups + threadIdx.x / G; row < limit;
-       row += static_cast<int64_t>(gridDim.x) * kGroups) {
+  for (; row < limit; row += step) {
     const int64_t to = row * a.d * kElem;
     float d[N], o[NEXT ? N : 1], dn[NEXT ? N : 1], y[OUT ? N : 1];
+    if constexpr (!VEC) load(row, ahead);
     if (OUT || a.grad_out) {
-      load_row<S, DTYPE, VEC>(static_cast<const uint8_t*>(a.grad_out) + row * a.grad_out_stride * kElem, a.d, t, d);
+      ahead.d.take(d);
     } else {
 #pragma unroll
       for (int i = 0; i < N; ++i) d[i] = 0.0f;
     }
-    float s[3] = {0.0f, 0.0f, 0.0f};  // sums of o^2, y^2 and v dn o
     if constexpr (NEXT) {
-      load_row<S, DTYPE, VEC>(static_cast<const uint8_t*>(a.x) + row * a.x_stride * kElem, a.d, t, o);
-      load_row<S, DTYPE, VEC>(static_cast<const uint8_t*>(a.grad_next) + row * a.grad_next_stride * kElem, a.d, t, dn);
+      ahead.o.take(o);
+      ahead.dn.take(dn);
     }
+    if constexpr (OUT) ahead.y.take(y);
+    if (VEC && row + step < limit) load(row + step, ahead);  // under way while this row is worked on
+    float s[3] = {0.0f, 0.0f, 0.0f};  // sums of o^2, y^2 and v dn o
     if constexpr (OUT) {
-      load_row<S, DTYPE, VEC>(static_cast<const uint8_t*>(a.y) + row * a.y_stride * kElem, a.d, t, y);
 #pragma unroll
       for (int i = 0; i < N; ++i) s[1] = fmaf(y[i], y[i], s[1]);
     }
@@ -98,15 +117,17 @@ __global__ void __launch_bounds__(norm_threads(G)) norm_grad_kernel(NormArgs a) 
         d[i] *= a.scale;
       }
       if (a.gate_kind == SB_GATE_FULL) {
+        float g[N], dg[N];
+        load_vector<S, VEC>(a.gate, a.gate_dtype, row * a.gate_stride, a.d, t, 0.0f, g);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-          const int at = S::column(i, t);
-          if (at < a.d) {
-            const float g = load_as_f32(a.gate, a.gate_dtype, row * a.gate_stride + at);
-            store_as(a.dgate, a.gate_dtype, row * a.d + at, w[i] * y[i] * d[i]);
-            d[i] *= g;
-          }
+          dg[i] = w[i] * y[i] * d[i];
+          d[i] *= g[i];
         }
+        by_dtype(a.gate_dtype, [&](auto type) {
+          constexpr int kType = decltype(type)::value;
+          store_row<S, kType, VEC>(static_cast<uint8_t*>(a.dgate) + row * a.d * (kType == SB_DTYPE_F32 ? 4 : 2), a.d, t, dg);
+        });
       }
       float p[1] = {0.0f};
 #pragma unroll
@@ -134,59 +155,56 @@ __global__ void __launch_bounds__(norm_threads(G)) norm_grad_kernel(NormArgs a) 
       if constexpr (NEXT) mine[a.d + at] = dv[i];
     }
   } else {
-    __shared__ float part[2][8 * G * NCH];
-    for (int g = 0; g < kGroups; ++g) {
-      if (static_cast<int>(threadIdx.x) / G == g) {
+    __shared__ float part[kGroups][8 * G * NCH];
+    auto join = [&](const float (&mine_of)[N], float* to) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-          const int at = S::column(i, t);
-          if constexpr (OUT) part[0][at] = g ? part[0][at] + q[i] : q[i];
-          if constexpr (NEXT) part[1][at] = g ? part[1][at] + dv[i] : dv[i];
-        }
+      for (int i = 0; i < N; ++i) part[threadIdx.x / G][S::column(i, t)] = mine_of[i];
+      __syncthreads();
+      for (int at = threadIdx.x; at < a.d; at += kThreads) {
+        float s = part[0][at];
+#pragma unroll
+        for (int g = 1; g < kGroups; ++g) s += part[g][at];
+        to[at] = s;
       }
       __syncthreads();
-    }
-    for (int at = threadIdx.x; at < a.d; at += kThreads) {
-      if constexpr (OUT) mine[at] = part[0][at];
-      if constexpr (NEXT) mine[a.d + at] = part[1][at];
-    }
+    };
+    if constexpr (OUT) join(q, mine);
+    if constexpr (NEXT) join(dv, mine + a.d);
   }
 }
 
-// The sums over the workgroups: 16 waves take every 16th of them for 64
-// columns, then are added in order. `half` 0: the weight (and a gate of the
-// channels), 1: the next weight.
+// The sums over the workgroups: 64 rows of 16 lanes take every 64th of them for
+// 16 columns, then are added in order. blockIdx.y 0: the weight (and a gate of
+// the channels), 1: the next weight.
 struct SumArgs {
   const float* partial;
   const void *weight, *gate;
   void *dweight, *dgate, *dnext;
   int32_t parts, d, weight_dtype, gate_dtype, next_dtype;
 };
-constexpr int kSumWaves = 16;
+constexpr int kSumRows = 64, kSumCols = 16;
 
-__global__ void __launch_bounds__(64 * kSumWaves) norm_sum_kernel(SumArgs a) {
-  __shared__ float sums[kSumWaves][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int half = blockIdx.y, at = static_cast<int>(blockIdx.x) * 64 + lane;
+__global__ void __launch_bounds__(kSumRows * kSumCols) norm_sum_kernel(SumArgs a) {
+  __shared__ float sums[kSumRows][kSumCols];
+  const int c = threadIdx.x % kSumCols, r = threadIdx.x / kSumCols;
+  const int half = blockIdx.y, at = static_cast<int>(blockIdx.x) * kSumCols + c;
   if (half == 0 ? !a.dweight && !a.dgate : !a.dnext) return;
   float s = 0.0f;
   if (at < a.d) {
     const float* from = a.partial + static_cast<int64_t>(half) * a.d + at;
-    int i = wave;
-    for (; i + 3 * kSumWaves < a.parts; i += 4 * kSumWaves) {
-      float v[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] = from[static_cast<int64_t>(i + j * kSumWaves) * 2 * a.d];
-      s += (v[0] + v[1]) + (v[2] + v[3]);
-    }
-    for (; i < a.parts; i += kSumWaves) s += from[static_cast<int64_t>(i) * 2 * a.d];
+#pragma unroll 8
+    for (int i = r; i < a.parts; i += kSumRows) s += from[static_cast<int64_t>(i) * 2 * a.d];
   }
-  sums[wave][lane] = s;
+  sums[r][c] = s;
   __syncthreads();
-  if (wave != 0 || at >= a.d) return;
+  if (r >= 4) return;
   s = 0.0f;
 #pragma unroll
-  for (int i = 0; i < kSumWaves; ++i) s += sums[i][lane];
+  for (int i = 0; i < kSumRows / 4; ++i) s += sums[i * 4 + r][c];
+  // The four rows of lanes of the first wave.
+  s += __shfl_xor(s, 16);
+  s += __shfl_xor(s, 32);
+  if (r != 0 || at >= a.d) return;
   if (half == 1) {
     store_as(a.dnext, a.next_dtype, at, s);
     return;
@@ -199,7 +217,7 @@ __global__ void __launch_bounds__(64 * kSumWaves) norm_sum_kernel(SumArgs a) {
 // the device holds at once.
 int64_t grad_workgroups(int64_t num_tokens, int64_t d, int cus) {
   int64_t grid = 1;
-  with_norm_form(d, true, [&](auto g, auto, auto) {
+  with_norm_form<true>(d, true, [&](auto g, auto, auto) {
     constexpr int kThreads = norm_threads(decltype(g)::value), kGroups = kThreads / decltype(g)::value;
     grid = std::min<int64_t>((num_tokens + kGroups - 1) / kGroups, int64_t{std::max(1, 512 / kThreads)} * cus);
   });
@@ -209,7 +227,7 @@ int64_t grad_workgroups(int64_t num_tokens, int64_t d, int cus) {
 template <bool OUT, bool NEXT>
 int launch_grad(const NormArgs& a, int32_t dtype, bool vec, uint32_t grid, hipStream_t stream) {
   return with_dtype(dtype, [&](auto type) {
-    with_norm_form(a.d, vec, [&](auto g, auto chunks, auto vectors) {
+    with_norm_form<true>(a.d, vec, [&](auto g, auto chunks, auto vectors) {
       constexpr int G = decltype(g)::value;
       norm_grad_kernel<decltype(type)::value, G, decltype(chunks)::value, decltype(vectors)::value, OUT, NEXT>
           <<<grid, norm_threads(G), 0, stream>>>(a);
@@ -236,7 +254,7 @@ int run_grad(NormArgs& a, int32_t dtype, bool out, bool next, bool vec, void* dw
                   dweight,        channel ? a.dgate : nullptr,  dnext,
                   static_cast<int32_t>(grid), a.d, a.weight_dtype, a.gate_dtype, a.next_dtype};
   if (!s.dweight && !s.dgate && !s.dnext) return SB_OK;
-  norm_sum_kernel<<<dim3(static_cast<uint32_t>((a.d + 63) / 64), 2), 64 * kSumWaves, 0, stream>>>(s);
+  norm_sum_kernel<<<dim3(static_cast<uint32_t>((a.d + kSumCols - 1) / kSumCols), 2), kSumRows * kSumCols, 0, stream>>>(s);
   return check_launch("norm gradients: sums");
 }
 
@@ -276,8 +294,8 @@ extern "C" int sb_norm_in_backward(const void* grad, int64_t grad_stride, const 
   a.d = static_cast<int32_t>(d_model);
   a.eps = eps;
   a.valid_tokens = valid_tokens;
-  const bool vec = norm_vectors(d_model, dtype, {grad, x, dx, grad_x ? grad_x : dx},
-                                {grad_stride, x_stride, grad_x ? grad_x_stride : 0});
+  const bool vec = norm_vectors(d_model, {{grad, grad_stride, dtype}, {x, x_stride, dtype}, {dx, 0, dtype},
+                                          {grad_x, grad_x_stride, dtype}, {weight, 0, weight_dtype}});
   if (const int rc = run_grad(a, dtype, false, true, vec, nullptr, dweight, workspace, workspace_bytes, as_stream(stream)))
     return rc;
   return clear_ok();
@@ -326,8 +344,11 @@ extern "C" int sb_norm_out_backward(const void* grad_out, int64_t grad_out_strid
   a.d = static_cast<int32_t>(d_model);
   a.eps = eps;
   a.valid_tokens = valid_tokens;
-  const bool vec = norm_vectors(d_model, dtype, {grad_out, y, dy, next ? grad_next : y, next ? out : y, next ? dx : dy},
-                                {grad_out_stride, y_stride, next ? grad_next_stride : 0, next ? out_stride : 0});
+  const bool vec = norm_vectors(
+      d_model, {{grad_out, grad_out_stride, dtype}, {y, y_stride, dtype}, {dy, 0, dtype}, {grad_next, grad_next_stride, dtype},
+                {next ? out : nullptr, out_stride, dtype}, {next ? dx : nullptr, 0, dtype}, {weight, 0, weight_dtype},
+                {gate_kind == SB_GATE_TOKEN ? nullptr : gate, gate_kind == SB_GATE_FULL ? gate_stride : 0, gate_dtype},
+                {gate_kind == SB_GATE_FULL ? dgate : nullptr, 0, gate_dtype}, {next_weight, 0, next_dtype}});
   if (const int rc = run_grad(a, dtype, true, next, vec, dweight, next ? dnext_weight : nullptr, workspace,
                               workspace_bytes, as_stream(stream)))
     return rc;
