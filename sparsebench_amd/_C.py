@@ -919,59 +919,61 @@ _NORM_MAX_D = 32768
 
 def _check_rows(t: torch.Tensor, name: str, like: torch.Tensor | None = None) -> None:
     """[T, D] with contiguous rows on a GPU; with `like`, of its shape, type and device."""
-    if not t.is_cuda or t.dim() != 2 or t.dtype not in _GATE_DTYPES:
+    shape = t.shape
+    if t.get_device() < 0 or len(shape) != 2 or t.dtype not in _GATE_DTYPES:
         _fail(f"{name} must be a [T, D] bfloat16, float16 or float32 CUDA tensor, got {_shape(t)} {t.dtype}")
-    if like is not None and (t.shape != like.shape or t.dtype != like.dtype or t.device != like.device):
+    if like is not None and (shape != like.shape or t.dtype is not like.dtype or t.get_device() != like.get_device()):
         _fail(f"{name} must be a {_shape(like)} {like.dtype} tensor on {like.device}, got {_shape(t)} {t.dtype} on "
               f"{t.device}")
-    if t.shape[1] != 1 and t.stride(1) != 1:
+    if not t.is_contiguous() and shape[1] != 1 and t.stride(1) != 1:
         _fail(f"{name} must have contiguous rows")
-    if not 0 < t.shape[1] <= _NORM_MAX_D:
-        _fail(f"rows must have 1 to {_NORM_MAX_D} values, got {t.shape[1]}")
+    if not 0 < shape[1] <= _NORM_MAX_D:
+        _fail(f"rows must have 1 to {_NORM_MAX_D} values, got {shape[1]}")
 
 
-def _check_vector(t: torch.Tensor | None, name: str, like: torch.Tensor) -> None:
-    if t is not None and not (t.device == like.device and t.dtype in _GATE_DTYPES and t.shape == like.shape[1:]
-                              and t.is_contiguous()):
+def _check_vector(t: torch.Tensor | None, name: str, like: torch.Tensor) -> int:
+    """Its dtype's code."""
+    if t is None:
+        return 0
+    code = _GATE_DTYPES.get(t.dtype)
+    if code is None or t.get_device() != like.get_device() or t.shape != like.shape[1:] or not t.is_contiguous():
         _fail(f"{name} must be a contiguous [{like.shape[1]}] bfloat16, float16 or float32 tensor on {like.device}")
+    return code
 
 
-def _check_norm_gate(gate: torch.Tensor | None, like: torch.Tensor) -> tuple[int, int]:
-    """(kind, row stride) of a gate."""
+def _check_norm_gate(gate: torch.Tensor | None, like: torch.Tensor) -> tuple[int, int, int]:
+    """(dtype's code, kind, row stride) of a gate."""
     if gate is None:
-        return 0, 0
+        return 0, 0, 0
     t, d = like.shape
-    if gate.device != like.device or gate.dtype not in _GATE_DTYPES:
+    code = _GATE_DTYPES.get(gate.dtype)
+    if code is None or gate.get_device() != like.get_device():
         _fail(f"gate must be a bfloat16, float16 or float32 tensor on {like.device}, got {gate.dtype} on {gate.device}")
     if gate.shape == (d,) and gate.is_contiguous():
-        return 1, 0
+        return code, 1, 0
     if gate.shape == (t, d) and (d == 1 or gate.stride(1) == 1):
-        return 3, gate.stride(0)
+        return code, 3, gate.stride(0)
     if gate.shape == (t, 1):
-        return 2, gate.stride(0)
+        return code, 2, gate.stride(0)
     _fail(f"gate must be [D], [T, 1] or [T, D] with contiguous rows, got {_shape(gate)}")
 
 
 def _check_norm(eps: float, valid_tokens: torch.Tensor | None, like: torch.Tensor) -> None:
     if not eps >= 0:
         _fail(f"eps must not be negative, got {eps}")
-    if valid_tokens is not None and not (valid_tokens.device == like.device and _valid_tokens_ok(valid_tokens)):
+    if valid_tokens is not None and not (valid_tokens.get_device() == like.get_device() and _valid_tokens_ok(valid_tokens)):
         _fail("valid_tokens must be a one-element int32 CUDA tensor")
-
-
-def _dtype_code(t: torch.Tensor | None) -> int:
-    return 0 if t is None else _GATE_DTYPES[t.dtype]
 
 
 def norm_in_cuda(x: torch.Tensor, weight: torch.Tensor | None, eps: float,
                  valid_tokens: torch.Tensor | None = None) -> torch.Tensor:
     """weight x / sqrt(mean(x^2) + eps) of each row (include/sparsebench_hip.h: sb_norm_in)."""
     _check_rows(x, "x")
-    _check_vector(weight, "weight", x)
+    weight_code = _check_vector(weight, "weight", x)
     _check_norm(eps, valid_tokens, x)
     out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     with _device_of(x):
-        check(lib().sb_norm_in(x.data_ptr(), x.stride(0), _ptr(weight), _dtype_code(weight), out.data_ptr(),
+        check(lib().sb_norm_in(x.data_ptr(), x.stride(0), _ptr(weight), weight_code, out.data_ptr(),
                                _GATE_DTYPES[x.dtype], *x.shape, eps, _ptr(valid_tokens), stream_of(x.device)))
     return out
 
@@ -982,16 +984,15 @@ def norm_out_cuda(y: torch.Tensor, x: torch.Tensor, weight: torch.Tensor | None,
     """x + scale gate weight n(y), or that and its own norm (sb_norm_out)."""
     _check_rows(x, "x")
     _check_rows(y, "y", x)
-    _check_vector(weight, "weight", x)
-    _check_vector(next_weight, "next_weight", x)
-    kind, gate_stride = _check_norm_gate(gate, x)
+    weight_code, next_code = _check_vector(weight, "weight", x), _check_vector(next_weight, "next_weight", x)
+    gate_code, kind, gate_stride = _check_norm_gate(gate, x)
     _check_norm(eps, valid_tokens, x)
     out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     following = None if next_weight is None else torch.empty_like(out)
     with _device_of(x):
         check(lib().sb_norm_out(
-            y.data_ptr(), y.stride(0), x.data_ptr(), x.stride(0), _ptr(weight), _dtype_code(weight), _ptr(gate),
-            _dtype_code(gate), kind, gate_stride, scale, _ptr(next_weight), _dtype_code(next_weight), out.data_ptr(),
+            y.data_ptr(), y.stride(0), x.data_ptr(), x.stride(0), _ptr(weight), weight_code, _ptr(gate),
+            gate_code, kind, gate_stride, scale, _ptr(next_weight), next_code, out.data_ptr(),
             _ptr(following), _GATE_DTYPES[x.dtype], *x.shape, eps, _ptr(valid_tokens), stream_of(x.device)))
     return out if following is None else (out, following)
 
@@ -1016,7 +1017,7 @@ def norm_in_backward_cuda(grad: torch.Tensor, x: torch.Tensor, weight: torch.Ten
     _check_rows(grad, "grad", x)
     if grad_x is not None:
         _check_rows(grad_x, "grad_x", x)
-    _check_vector(weight, "weight", x)
+    weight_code = _check_vector(weight, "weight", x)
     _check_norm(eps, valid_tokens, x)
     dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     if x.shape[0] == 0:  # sums of nothing
@@ -1025,7 +1026,7 @@ def norm_in_backward_cuda(grad: torch.Tensor, x: torch.Tensor, weight: torch.Ten
     with _device_of(x):
         workspace = _norm_workspace(x)
         check(lib().sb_norm_in_backward(
-            grad.data_ptr(), grad.stride(0), x.data_ptr(), x.stride(0), _ptr(weight), _dtype_code(weight),
+            grad.data_ptr(), grad.stride(0), x.data_ptr(), x.stride(0), _ptr(weight), weight_code,
             _ptr(grad_x), 0 if grad_x is None else grad_x.stride(0), dx.data_ptr(), _ptr(dweight),
             _GATE_DTYPES[x.dtype], *x.shape, eps, _ptr(valid_tokens), workspace.data_ptr(), workspace.numel(),
             stream_of(x.device)))
@@ -1044,9 +1045,8 @@ def norm_out_backward_cuda(grad_out: torch.Tensor, y: torch.Tensor, weight: torc
     if grad_next is not None:
         _check_rows(grad_next, "grad_next", y)
         _check_rows(out, "out", y)
-    _check_vector(weight, "weight", y)
-    _check_vector(next_weight, "next_weight", y)
-    kind, gate_stride = _check_norm_gate(gate, y)
+    weight_code, next_code = _check_vector(weight, "weight", y), _check_vector(next_weight, "next_weight", y)
+    gate_code, kind, gate_stride = _check_norm_gate(gate, y)
     _check_norm(eps, valid_tokens, y)
     opts = {"dtype": y.dtype, "device": y.device}
     if y.shape[0] == 0:  # sums of nothing
@@ -1062,8 +1062,8 @@ def norm_out_backward_cuda(grad_out: torch.Tensor, y: torch.Tensor, weight: torc
         check(lib().sb_norm_out_backward(
             grad_out.data_ptr(), grad_out.stride(0), _ptr(grad_next), 0 if grad_next is None else grad_next.stride(0),
             y.data_ptr(), y.stride(0), _ptr(following), 0 if following is None else following.stride(0),
-            _ptr(weight), _dtype_code(weight), _ptr(gate), _dtype_code(gate), kind, gate_stride, scale,
-            _ptr(next_weight), _dtype_code(next_weight), dy.data_ptr(), _ptr(dx), _ptr(dweight), _ptr(dgate),
+            _ptr(weight), weight_code, _ptr(gate), gate_code, kind, gate_stride, scale, _ptr(next_weight), next_code,
+            dy.data_ptr(), _ptr(dx), _ptr(dweight), _ptr(dgate),
             _ptr(dnext), _GATE_DTYPES[y.dtype], *y.shape, eps, _ptr(valid_tokens), workspace.data_ptr(),
             workspace.numel(), stream_of(y.device)))
     return dy, grad_out if dx is None else dx, dweight, dgate, dnext
@@ -1083,39 +1083,45 @@ def _experts4_bytes(num_tokens: int, k: int, num_experts: int, d_model: int, ffn
 
 def _check_codes(codes: torch.Tensor, scales: torch.Tensor, name: str) -> tuple[int, int, int]:
     """(E, K, N) of 4-bit weights."""
-    if (codes.dim() != 5 or codes.shape[3:] != (32, 16) or scales.shape != codes.shape[:4] or not codes.is_cuda
-            or codes.device != scales.device or codes.dtype != torch.uint8 or scales.dtype != torch.uint8):
+    shape = codes.shape
+    if (len(shape) != 5 or shape[3] != 32 or shape[4] != 16 or scales.shape != shape[:4] or codes.get_device() < 0
+            or codes.get_device() != scales.get_device() or not codes.dtype is scales.dtype is torch.uint8):
         _fail(f"{name} must be uint8 codes [E, N/32, K/32, 32, 16] and scales [E, N/32, K/32, 32] on one GPU, got "
               f"{_shape(codes)} {codes.dtype} and {_shape(scales)} {scales.dtype}")
     if not (codes.is_contiguous() and scales.is_contiguous()) or codes.data_ptr() % 16:
         _fail(f"{name} must be contiguous, its codes 16-byte aligned")
-    e, nt, kg = codes.shape[:3]
-    return e, 32 * kg, 32 * nt
+    return shape[0], 32 * shape[2], 32 * shape[1]
 
 
 def experts4_layer_cuda(x: torch.Tensor, expert_idx: torch.Tensor, expert_weight: torch.Tensor, w1, w2,
                         activation: str, valid_tokens: torch.Tensor | None = None) -> torch.Tensor:
     """gated_layer_cuda with (codes, scales) pairs as weights (include/sparsebench_hip.h: sb_experts4_layer)."""
-    if x.dim() != 2 or expert_idx.dim() != 2 or expert_idx.shape != expert_weight.shape or x.shape[0] != expert_idx.shape[0]:
+    (c1, s1), (c2, s2) = w1, w2
+    try:
+        (t, width), (rows, k) = x.shape, expert_idx.shape
+    except ValueError:
+        t, width, rows, k = 0, 0, -1, 0
+    if t != rows or expert_idx.shape != expert_weight.shape:
         _fail(f"x must be [T, D], expert_idx and expert_weight [T, k], got {_shape(x)}, {_shape(expert_idx)} and "
               f"{_shape(expert_weight)}")
-    (e, d, columns), (experts, f, out_columns) = _check_codes(*w1, "w1"), _check_codes(*w2, "w2")
-    if e != experts or x.shape[1] != d or out_columns != d or columns != 2 * f:
+    (e, d, columns), (experts, f, out_columns) = _check_codes(c1, s1, "w1"), _check_codes(c2, s2, "w2")
+    if e != experts or width != d or out_columns != d or columns != 2 * f:
         _fail(f"x must be [T, D], w1 of [E, D, 2F] and w2 of [E, F, D], got {_shape(x)}, {[e, d, columns]} and "
               f"{[experts, f, out_columns]}")
-    if any(t.device != x.device for t in (expert_idx, expert_weight, w1[0], w2[0])):
+    device = x.get_device()
+    if not (device == expert_idx.get_device() == expert_weight.get_device() == c1.get_device() == c2.get_device()):
         _fail("all inputs must be on the same GPU")
-    if x.dtype != torch.bfloat16 or not x.is_contiguous() or x.data_ptr() % 16:
+    if x.dtype is not torch.bfloat16 or not x.is_contiguous() or x.data_ptr() % 16:
         _fail("x must be contiguous 16-byte aligned bfloat16")
-    if expert_weight.dtype not in _GATE_DTYPES:
+    gate_code, index_code = _GATE_DTYPES.get(expert_weight.dtype), _INDEX_DTYPES.get(expert_idx.dtype)
+    if gate_code is None:
         _fail(f"expert_weight must be bfloat16, float16 or float32, got {expert_weight.dtype}")
-    if expert_idx.dtype not in _INDEX_DTYPES:
+    if index_code is None:
         _fail(f"expert_idx must be int32 or int64, got {expert_idx.dtype}")
     if activation not in _ACTIVATIONS:
         _fail(f"activation must be one of {sorted(_ACTIVATIONS)}, got {activation!r}")
-    if valid_tokens is not None and not (valid_tokens.device == x.device and _valid_tokens_ok(valid_tokens)):
+    if valid_tokens is not None and not (valid_tokens.get_device() == device and _valid_tokens_ok(valid_tokens)):
         _fail("valid_tokens must be a one-element int32 CUDA tensor")
-    t, k = expert_idx.shape
     if k == 0:
         _fail(f"expert_weight must be [T, k] with k > 0, got {_shape(expert_weight)}")
     if t * k > _MAX_COPIES4:
@@ -1126,13 +1132,12 @@ def experts4_layer_cuda(x: torch.Tensor, expert_idx: torch.Tensor, expert_weight
         return out
     expert_idx, gates = expert_idx.contiguous(), expert_weight.contiguous()
     with _device_of(x):
-        size = _experts4_bytes(t, k, e, d, f, x.get_device())
+        size = _experts4_bytes(t, k, e, d, f, device)
         workspace = torch.empty(size, dtype=torch.uint8, device=x.device)
         check(lib().sb_experts4_layer(
-            x.data_ptr(), expert_idx.data_ptr(), _INDEX_DTYPES[expert_idx.dtype], gates.data_ptr(),
-            _GATE_DTYPES[gates.dtype], w1[0].data_ptr(), w1[1].data_ptr(), w2[0].data_ptr(), w2[1].data_ptr(),
-            out.data_ptr(), _ACTIVATIONS[activation], workspace.data_ptr(), size, t, k, e, d, f, _ptr(valid_tokens),
-            stream_of(x.device)))
+            x.data_ptr(), expert_idx.data_ptr(), index_code, gates.data_ptr(), gate_code, c1.data_ptr(), s1.data_ptr(),
+            c2.data_ptr(), s2.data_ptr(), out.data_ptr(), _ACTIVATIONS[activation], workspace.data_ptr(), size, t, k, e,
+            d, f, _ptr(valid_tokens), stream_of(x.device)))
     return out
 
 

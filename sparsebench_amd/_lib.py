@@ -169,5 +169,7 @@ def check(rc: int) -> None:
 
 
 def stream_of(device: torch.device) -> int:
-    """Handle of torch's current stream on `device` (what every op launches on)."""
-    return torch.cuda.current_stream(device).cuda_stream
+    """Handle of torch's current stream on `device` (what every op launches on). Asked for
+    without a Stream object, which takes 1.8 us to make."""
+    index = device.index
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
