@@ -217,7 +217,7 @@ __global__ void __launch_bounds__(kThreads)
   }
 }
 
-// ------------------------------------------------------- X and its way back ---
+// ---------------------------------------------------------------- X ---
 
 // X [mp, np] of each matrix: hi, and lo = what hi's rounding left.
 struct Padded {
@@ -289,68 +289,22 @@ __global__ void __launch_bounds__(kThreads)
   }
 }
 
-// The weights' step from the last X; without a momentum X itself.
-__global__ void __launch_bounds__(kThreads) apply_kernel(Table t, Hyper h, Padded x) {
-  __shared__ float lds[kTile][kTile + 1];
-  int64_t matrix;
-  const Entry& e = entry_of(t, static_cast<int>(blockIdx.y), &matrix);
-  const TilePlace tp = tile_place(e, x);
-  const int64_t base = static_cast<int64_t>(blockIdx.y) * x.mp * x.np;
-  auto get = [&](int row, int col, float (&v)[8]) {
-    const int64_t at = base + static_cast<int64_t>(row) * x.np + col;
-    const u32x4_t hi = *reinterpret_cast<const u32x4_t*>(x.hi + at), lo = *reinterpret_cast<const u32x4_t*>(x.lo + at);
-#pragma unroll
-    for (int q = 0; q < 8; ++q)
-      v[q] = (value_of(static_cast<uint16_t>(hi[q / 2] >> (16 * (q & 1))), SB_DTYPE_F16) +
-              value_of(static_cast<uint16_t>(lo[q / 2] >> (16 * (q & 1))), SB_DTYPE_F16)) * kUnscale;
-  };
-  if (e.tall) {
-#pragma unroll
-    for (int i = 0; i < kTile * kTile / 8 / kThreads; ++i) {
-      const int item = i * kThreads + static_cast<int>(threadIdx.x), r = item / 8, c = item % 8 * 8;
-      float v[8];
-      get(tp.col + r, tp.row + c, v);
-#pragma unroll
-      for (int q = 0; q < 8; ++q) lds[c + q][r] = v[q];
-    }
-    __syncthreads();
-  }
-  const float lr = h.lr_ptr ? *h.lr_ptr : h.lr;
-  const float keep = 1.0f - lr * h.weight_decay;
-  const float size = lr * h.update_rms * sqrtf(static_cast<float>(max(e.rows, e.columns)));
-#pragma unroll
-  for (int i = 0; i < kTile * kTile / 8 / kThreads; ++i) {
-    const int item = i * kThreads + static_cast<int>(threadIdx.x), r = item / 8, c = item % 8 * 8;
-    const int row = tp.row + r, col = tp.col + c, n = e.columns - col;
-    if (row >= e.rows || n <= 0) continue;
-    float v[8];
-    if (e.tall) {
-#pragma unroll
-      for (int q = 0; q < 8; ++q) v[q] = lds[r][c + q];
-    } else {
-      get(row, col, v);
-    }
-    const int64_t place = matrix * e.param_matrix + row * e.param_row + col;
-    if (e.momentum) {
-      float w[8];
-      const int64_t at = e.master ? matrix * e.master_matrix + row * e.master_row + col : place;
-      load8(e.master ? e.master : e.param, e.master ? SB_DTYPE_F32 : e.param_dtype, at, n, e.wide, w);
-#pragma unroll
-      for (int q = 0; q < 8; ++q) v[q] = w[q] * keep - size * v[q];
-      if (e.master) store8(e.master, SB_DTYPE_F32, at, n, e.wide, v);
-    }
-    store8(e.param, e.param_dtype, place, n, e.wide, v);
-  }
-}
-
 // ------------------------------------------------------------- products ---
 
+// A symmetric matrix: the entries beside the diagonal in fp16 times `scale`, with
+// zeros on it, and the diagonal in fp32. Each [M][mp][mp] and [M][mp].
+struct Symmetric {
+  uint16_t* off;
+  float* diag;
+  float scale;
+};
+
 struct ProductArgs {
-  const uint16_t* x;     // [M][mp][np], hi
-  uint16_t *gram, *poly; // A and B but for their diagonals, [M][mp][mp]
-  float *gram_diag, *poly_diag;  // [M][mp], not scaled
-  uint16_t* lo;          // of x, updated in place
-  uint16_t* next;        // hi of the next X
+  const uint16_t* x;  // [M][mp][np], hi
+  uint16_t* lo;       // of x, updated in place
+  uint16_t* next;     // hi of the next X
+  Symmetric left, right, out;
+  float of_left, of_right, of_product;  // out = of_left L + of_right R + of_product L R
   int32_t mp, np, matrices;
 };
 
@@ -400,61 +354,120 @@ __device__ __forceinline__ void product(uint8_t* __restrict__ lds, const uint16_
   DmaMainloop<Cfg>::run(lds, src, k / Cfg::BK, acc);
 }
 
-// The accumulators in fp32 through LDS, a group of 32 rows of each row of waves
-// at a time (part): rows(part, fn) calls fn(row, col, 8 values) with rows and
-// columns in the tile, neighbouring lanes on neighbouring columns; with mirror,
-// fn(col, row, 8 values of a column) as well, eight rows each.
-template <class Cfg>
+// The accumulators in fp32 through LDS, kGroups groups of 32 rows of each row of
+// waves at a time (a part): rows(part, fn) calls fn(row, col, 8 values) with rows
+// and columns in the tile, neighbouring lanes on neighbouring columns. What fn
+// leaves may be kept in the values' place, as 8 halves or as the values: mirror and
+// columns then give it by columns, fn(col, row, of rows row ..), neighbouring lanes
+// on the rows of a column that lie together.
+template <class Cfg, int kGroups_ = (Cfg::TM >= 2 && 64 * Cfg::WM * Cfg::BN * 4 <= Cfg::kLdsAlloc ? 2 : 1)>
 struct Epilogue {
   using ML = DmaMainloop<Cfg>;
-  static constexpr int kRows = 32 * Cfg::WM, kChunks = Cfg::BN / 4;
-  static_assert(kRows * Cfg::BN * 4 <= Cfg::kLdsAlloc, "a part fits the ring");
+  static constexpr int kGroups = kGroups_;
+  static constexpr int kParts = Cfg::TM / kGroups;
+  static constexpr int kRun = 32 * kGroups, kRows = kRun * Cfg::WM;  // rows that lie together, rows of a part
+  static_assert(kRows * Cfg::BN * 4 <= Cfg::kLdsAlloc && Cfg::TM % kGroups == 0, "a part fits the ring");
   __device__ __forceinline__ static int place(int r, int col) {  // of the 16 bytes that hold (r, col)
     return r * (Cfg::BN * 4) + (((col >> 2) ^ (r & 15)) << 4);
   }
-  __device__ __forceinline__ static int tile_row(int part, int r) { return r / 32 * Cfg::WTM + 32 * part + r % 32; }
+  __device__ __forceinline__ static int tile_row(int part, int r) { return r / kRun * Cfg::WTM + kRun * part + r % kRun; }
 
   template <int PART>
   __device__ __forceinline__ static void put(uint8_t* __restrict__ lds, const typename ML::Acc& acc) {
     const int lane = threadIdx.x & 63, wm = (threadIdx.x >> 6) / Cfg::WN;
-    const int r = 32 * wm + (lane & 31);
     __syncthreads();
 #pragma unroll
-    for (int jn = 0; jn < Cfg::TN; ++jn)
+    for (int i = 0; i < kGroups; ++i) {
+      const int r = kRun * wm + 32 * i + (lane & 31);
 #pragma unroll
-      for (int g = 0; g < 4; ++g)
-        *reinterpret_cast<f32x4_t*>(lds + place(r, ML::out_col(jn, g))) =
-            f32x4_t{acc[jn][PART][4 * g], acc[jn][PART][4 * g + 1], acc[jn][PART][4 * g + 2], acc[jn][PART][4 * g + 3]};
+      for (int jn = 0; jn < Cfg::TN; ++jn)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const f32x16_t& v = acc[jn][PART * kGroups + i];
+          *reinterpret_cast<f32x4_t*>(lds + place(r, ML::out_col(jn, g))) =
+              f32x4_t{v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]};
+        }
+    }
     __syncthreads();
   }
 
-  template <class Fn>
-  __device__ __forceinline__ static void rows(const uint8_t* __restrict__ lds, int part, Fn fn) {
-    constexpr int kItems = kRows * Cfg::BN / 8;
+  // A thread's i-th eight values of a part: row r of the part, columns c ..
+  static constexpr int kItems = kRows * Cfg::BN / 8 / Cfg::kThreads;
+  __device__ __forceinline__ static int item_row(int i) { return (i * Cfg::kThreads + static_cast<int>(threadIdx.x)) / (Cfg::BN / 8); }
+  __device__ __forceinline__ static int item_col(int i) { return (i * Cfg::kThreads + static_cast<int>(threadIdx.x)) % (Cfg::BN / 8) * 8; }
+
+  // all[i] = the eight halves of `from` [.., stride] at item i of a part: asked for
+  // before the part's barriers, since one by one each would wait for memory.
+  __device__ __forceinline__ static void fetch(const uint16_t* from, int64_t stride, int part, u32x4_t (&all)[kItems]) {
 #pragma unroll
-    for (int i = 0; i < kItems / Cfg::kThreads; ++i) {
-      const int item = i * Cfg::kThreads + static_cast<int>(threadIdx.x);
-      const int r = item / (Cfg::BN / 8), c = item % (Cfg::BN / 8) * 8;
+    for (int i = 0; i < kItems; ++i)
+      all[i] = *reinterpret_cast<const u32x4_t*>(from + tile_row(part, item_row(i)) * stride + item_col(i));
+  }
+
+  // fn(i, row, col, values). KEEP 1: its result, 8 halves, is kept in the values'
+  // place; 2: the values, as it leaves them.
+  template <int KEEP, class Fn>
+  __device__ __forceinline__ static void rows(uint8_t* __restrict__ lds, int part, Fn fn) {
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) {
+      const int r = item_row(i), c = item_col(i);
       const f32x4_t a = *reinterpret_cast<const f32x4_t*>(lds + place(r, c));
       const f32x4_t b = *reinterpret_cast<const f32x4_t*>(lds + place(r, c + 4));
       float v[8];
 #pragma unroll
       for (int q = 0; q < 4; ++q) v[q] = a[q], v[4 + q] = b[q];
-      fn(tile_row(part, r), c, v);
+      const u32x4_t out = fn(i, tile_row(part, r), c, v);
+      if constexpr (KEEP == 1) *reinterpret_cast<u32x4_t*>(lds + place(r, c)) = out;
+      if constexpr (KEEP == 2) {
+        *reinterpret_cast<f32x4_t*>(lds + place(r, c)) = f32x4_t{v[0], v[1], v[2], v[3]};
+        *reinterpret_cast<f32x4_t*>(lds + place(r, c + 4)) = f32x4_t{v[4], v[5], v[6], v[7]};
+      }
     }
   }
 
+  // A thread turns blocks of 8 x 8 halves around in registers.
+  template <class Fn>
+  __device__ __forceinline__ static void mirror(const uint8_t* __restrict__ lds, int part, Fn fn) {
+    constexpr int kTurns = kRows * Cfg::BN / 64, kBlocks = kRun / 8;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kTurns / Cfg::kThreads; ++i) {
+      const int item = i * Cfg::kThreads + static_cast<int>(threadIdx.x);
+      const int r = (item % kBlocks + item / (kBlocks * (Cfg::BN / 8)) * kBlocks) * 8, c = item / kBlocks % (Cfg::BN / 8) * 8;
+      u32x4_t in[8];
+#pragma unroll
+      for (int q = 0; q < 8; ++q) in[q] = *reinterpret_cast<const u32x4_t*>(lds + place(r + q, c));
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {  // column c + q: half q of each row
+        u32x4_t out;
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+          out[w] = q & 1 ? __builtin_amdgcn_perm(in[2 * w + 1][q / 2], in[2 * w][q / 2], 0x07060302u)
+                         : __builtin_amdgcn_perm(in[2 * w + 1][q / 2], in[2 * w][q / 2], 0x05040100u);
+        fn(c + q, tile_row(part, r), out);
+      }
+    }
+  }
+
+  // A thread's i-th eight values of a column: rows turn_row(i) .. of the part.
+  static constexpr int kRunItems = kRun / 8;
+  __device__ __forceinline__ static int turn_col(int i) {
+    return (i * Cfg::kThreads + static_cast<int>(threadIdx.x)) / kRunItems % Cfg::BN;
+  }
+  __device__ __forceinline__ static int turn_row(int i) {
+    const int item = i * Cfg::kThreads + static_cast<int>(threadIdx.x);
+    return (item % kRunItems + item / (kRunItems * Cfg::BN) * kRunItems) * 8;
+  }
   template <class Fn>
   __device__ __forceinline__ static void columns(const uint8_t* __restrict__ lds, int part, Fn fn) {
-    constexpr int kGroups = kRows / 8, kItems = kGroups * Cfg::BN;
+    __syncthreads();
 #pragma unroll
-    for (int i = 0; i < kItems / Cfg::kThreads; ++i) {
-      const int item = i * Cfg::kThreads + static_cast<int>(threadIdx.x);
-      const int c = item / kGroups, r = item % kGroups * 8;
+    for (int i = 0; i < kItems; ++i) {
+      const int c = turn_col(i), r = turn_row(i);
       float v[8];
 #pragma unroll
       for (int q = 0; q < 8; ++q) v[q] = *reinterpret_cast<const float*>(lds + place(r + q, c) + (c & 3) * 4);
-      fn(c, tile_row(part, r), v);
+      fn(i, c, tile_row(part, r), v);
     }
   }
 };
@@ -467,8 +480,10 @@ __host__ __device__ __forceinline__ void upper_tile(int at, int n, int* i, int* 
   *j = row + at;
 }
 
-// SQUARE 0: A = X X^T. SQUARE 1: B = b5 A + c5 A A. Diagonals apart, in fp32.
-template <class Cfg, int SQUARE>
+// GRAM: out = X X^T. Otherwise out = of_left L + of_right R + of_product L R of
+// symmetric matrices that commute, so that the result is symmetric too. With
+// L = l + O, R = r + S: L R = l r + l S + O r + O S.
+template <class Cfg, bool GRAM>
 __global__ void __launch_bounds__(Cfg::kThreads, 1) symmetric_kernel(ProductArgs p) {
   using ML = DmaMainloop<Cfg>;
   using Ep = Epilogue<Cfg>;
@@ -479,52 +494,72 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1) symmetric_kernel(ProductArgs
   upper_tile(uniform(at % per), n, &i, &j);
   const int64_t matrix = uniform(at / per);
   const int i0 = i * Cfg::BM, j0 = j * Cfg::BN;
-  const int64_t square = matrix * p.mp * p.mp;
-  const uint16_t* gram = p.gram + square;
-  float* diag = p.gram_diag + matrix * p.mp;
+  const int64_t square = matrix * p.mp * p.mp, line = matrix * p.mp;
   typename ML::Acc acc;
-  if constexpr (SQUARE) {
-    product<Cfg>(lds, gram, gram, p.mp, p.mp, p.mp, i0, j0, acc);
-  } else {
+  float unit;  // of the accumulators
+  if constexpr (GRAM) {
     const uint16_t* x = p.x + matrix * p.mp * p.np;
     product<Cfg>(lds, x, x, p.mp, p.np, p.mp, i0, j0, acc);
+    unit = kUnscale * kUnscale;
+  } else {
+    product<Cfg>(lds, p.left.off + square, p.right.off + square, p.mp, p.mp, p.mp, i0, j0, acc);
+    unit = p.of_product / (p.left.scale * p.right.scale);
   }
-  uint16_t* out = (SQUARE ? p.poly : p.gram) + square;
-  static_for<0, Cfg::TM>([&](auto part) {
+  const float scale = p.out.scale;
+  uint16_t* out = p.out.off + square;
+  static_for<0, Ep::kParts>([&](auto part) {
     constexpr int P = decltype(part)::value;
+    u32x4_t ls[GRAM ? 1 : Ep::kItems], rs[GRAM ? 1 : Ep::kItems];
+    if constexpr (!GRAM) {
+      const int64_t tile = square + static_cast<int64_t>(i0) * p.mp + j0;
+      Ep::fetch(p.left.off + tile, p.mp, P, ls);
+      Ep::fetch(p.right.off + tile, p.mp, P, rs);
+    }
     Ep::template put<P>(lds, acc);
-    auto write = [&](int64_t row, int64_t col, const float (&v)[8]) {
-      uint16_t bits[8];
-      if constexpr (SQUARE) {
-        const u32x4_t a = *reinterpret_cast<const u32x4_t*>(gram + row * p.mp + col);
-        const float here = diag[row];
+    Ep::template rows<1>(lds, P, [&](int item, int r, int c, float (&v)[8]) {
+      const int row = i0 + r, col = j0 + c;
+      float w[8];
+#pragma unroll
+      for (int q = 0; q < 8; ++q) w[q] = v[q] * unit;
+      float l = 0.0f, rd = 0.0f;
+      if constexpr (!GRAM) {
+        const f32x4_t d0 = *reinterpret_cast<const f32x4_t*>(p.right.diag + line + col);
+        const f32x4_t d1 = *reinterpret_cast<const f32x4_t*>(p.right.diag + line + col + 4);
+        l = p.left.diag[line + row];
+        rd = p.right.diag[line + row];
+        const float of_s = (p.of_right + p.of_product * l) / p.right.scale, of_o = 1.0f / p.left.scale;
 #pragma unroll
         for (int q = 0; q < 8; ++q) {
-          const float o = value_of(static_cast<uint16_t>(a[q / 2] >> (16 * (q & 1))), SB_DTYPE_F16);
-          bits[q] = half_bits(kB5 * o + kC5 * (kUnscale * v[q] + (here + diag[col + q]) * o));
-          if (row == col + q) {
-            bits[q] = 0;
-            p.poly_diag[matrix * p.mp + row] = kB5 * here + kC5 * (kUnscale * kUnscale * v[q] + here * here);
-          }
-        }
-      } else {
-#pragma unroll
-        for (int q = 0; q < 8; ++q) {
-          bits[q] = half_bits(v[q] * kUnscale);
-          if (row == col + q) {
-            bits[q] = 0;
-            diag[row] = kUnscale * kUnscale * v[q];
-          }
+          const float o = value_of(static_cast<uint16_t>(ls[item][q / 2] >> (16 * (q & 1))), SB_DTYPE_F16);
+          const float s = value_of(static_cast<uint16_t>(rs[item][q / 2] >> (16 * (q & 1))), SB_DTYPE_F16);
+          w[q] += of_s * s + (p.of_left + p.of_product * (q < 4 ? d0[q] : d1[q - 4])) * (of_o * o);
         }
       }
-      *reinterpret_cast<u32x4_t*>(out + row * p.mp + col) = pack8(bits);
-    };
-    Ep::rows(lds, P, [&](int r, int c, const float (&v)[8]) { write(i0 + r, j0 + c, v); });
-    if (i != j) Ep::columns(lds, P, [&](int c, int r, const float (&v)[8]) { write(j0 + c, i0 + r, v); });
+      uint16_t bits[8];
+#pragma unroll
+      for (int q = 0; q < 8; ++q) bits[q] = half_bits(w[q] * scale);
+      if (i == j && row - col >= 0 && row - col < 8) {
+        const int q = row - col;
+        float self = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          self = q == e ? v[e] * unit : self;
+          bits[e] = q == e ? 0 : bits[e];
+        }
+        p.out.diag[line + row] = GRAM ? self : self + p.of_left * l + p.of_right * rd + p.of_product * (l * rd);
+      }
+      const u32x4_t all = pack8(bits);
+      *reinterpret_cast<u32x4_t*>(out + static_cast<int64_t>(row) * p.mp + col) = all;
+      return all;
+    });
+    if (i != j)
+      Ep::mirror(lds, P, [&](int c, int r, u32x4_t v) {
+        *reinterpret_cast<u32x4_t*>(out + static_cast<int64_t>(j0 + c) * p.mp + i0 + r) = v;
+      });
   });
 }
 
-// next, lo = (a5 + B's diagonal) X + B X.
+// next, lo = of_right X + L X: of X's own rows of_right and L's diagonal.
 template <class Cfg>
 __global__ void __launch_bounds__(Cfg::kThreads, 1) update_kernel(ProductArgs p) {
   using ML = DmaMainloop<Cfg>;
@@ -534,28 +569,99 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1) update_kernel(ProductArgs p)
   const int at = xcd_remap(static_cast<int>(blockIdx.x), per * p.matrices);
   const int64_t matrix = uniform(at / per);
   const int i0 = uniform(at % per % mt) * Cfg::BM, j0 = uniform(at % per / mt) * Cfg::BN;
-  const int64_t whole = matrix * p.mp * p.np;
+  const int64_t whole = matrix * p.mp * p.np, tile = whole + static_cast<int64_t>(i0) * p.np + j0;
   typename ML::Acc acc;
-  product<Cfg>(lds, p.poly + matrix * p.mp * p.mp, p.x + whole, p.mp, p.mp, p.np, i0, j0, acc);
-  static_for<0, Cfg::TM>([&](auto part) {
+  product<Cfg>(lds, p.left.off + matrix * p.mp * p.mp, p.x + whole, p.mp, p.mp, p.np, i0, j0, acc);
+  const float unit = 1.0f / p.left.scale;
+  static_for<0, Ep::kParts>([&](auto part) {
     constexpr int P = decltype(part)::value;
+    u32x4_t his[Ep::kItems], los[Ep::kItems];
+    Ep::fetch(p.x + tile, p.np, P, his);
+    Ep::fetch(p.lo + tile, p.np, P, los);
     Ep::template put<P>(lds, acc);
-    Ep::rows(lds, P, [&](int r, int c, const float (&v)[8]) {
-      const int64_t place = whole + static_cast<int64_t>(i0 + r) * p.np + j0 + c;
-      const u32x4_t h = *reinterpret_cast<const u32x4_t*>(p.x + place), l = *reinterpret_cast<const u32x4_t*>(p.lo + place);
-      const float self = kA5 + p.poly_diag[matrix * p.mp + i0 + r];
+    Ep::template rows<0>(lds, P, [&](int item, int r, int c, float (&v)[8]) {
+      const int64_t place = tile + static_cast<int64_t>(r) * p.np + c;
+      const float self = p.of_right + p.left.diag[matrix * p.mp + i0 + r];
       uint16_t hi[8], lo[8];
 #pragma unroll
       for (int q = 0; q < 8; ++q) {
-        const float x = value_of(static_cast<uint16_t>(h[q / 2] >> (16 * (q & 1))), SB_DTYPE_F16) +
-                        value_of(static_cast<uint16_t>(l[q / 2] >> (16 * (q & 1))), SB_DTYPE_F16);
-        const float y = fmaf(kUnscale, v[q], self * x);
+        const float x = value_of(static_cast<uint16_t>(his[item][q / 2] >> (16 * (q & 1))), SB_DTYPE_F16) +
+                        value_of(static_cast<uint16_t>(los[item][q / 2] >> (16 * (q & 1))), SB_DTYPE_F16);
+        const float y = fmaf(unit, v[q], self * x);
         hi[q] = half_bits(y);
         lo[q] = half_bits(y - value_of(hi[q], SB_DTYPE_F16));
       }
       *reinterpret_cast<u32x4_t*>(p.next + place) = pack8(hi);
       *reinterpret_cast<u32x4_t*>(p.lo + place) = pack8(lo);
+      return u32x4_t{};
     });
+  });
+}
+
+// The last step, with the weights' step in its place (apply): w = keep w - size X;
+// without a momentum X itself.
+template <class Cfg>
+__global__ void __launch_bounds__(Cfg::kThreads, 1) last_kernel(ProductArgs p, Table t, Hyper h) {
+  using ML = DmaMainloop<Cfg>;
+  using Ep = Epilogue<Cfg, 1>;  // the weights take the registers of the other rows
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[Cfg::kLdsAlloc];
+  const int mt = p.mp / Cfg::BM, per = mt * (p.np / Cfg::BN);
+  const int at = xcd_remap(static_cast<int>(blockIdx.x), per * p.matrices);
+  const int matrix = uniform(at / per);
+  const int i0 = uniform(at % per % mt) * Cfg::BM, j0 = uniform(at % per / mt) * Cfg::BN;
+  const int64_t tile = static_cast<int64_t>(matrix) * p.mp * p.np + static_cast<int64_t>(i0) * p.np + j0;
+  int64_t place;
+  const Entry e = entry_of(t, matrix, &place);
+  typename ML::Acc acc;
+  product<Cfg>(lds, p.left.off + static_cast<int64_t>(matrix) * p.mp * p.mp, p.x + static_cast<int64_t>(matrix) * p.mp * p.np,
+               p.mp, p.mp, p.np, i0, j0, acc);
+  const float unit = 1.0f / p.left.scale;
+  const float lr = h.lr_ptr ? *h.lr_ptr : h.lr;
+  const float keep = 1.0f - lr * h.weight_decay;
+  const float size = lr * h.update_rms * sqrtf(static_cast<float>(max(e.rows, e.columns)));
+  void* const weights = e.master ? e.master : e.param;
+  const int weights_dtype = e.master ? SB_DTYPE_F32 : e.param_dtype;
+  const int64_t weights_at = place * (e.master ? e.master_matrix : e.param_matrix);
+  const int64_t weights_row = e.master ? e.master_row : e.param_row;
+  // Weights at row, col .. of the tensor: `there` of them (none outside).
+  auto there = [&](int row, int col) { return row < e.rows ? e.columns - col : 0; };
+  auto fetch = [&](int row, int col, float (&w)[8]) {
+    if (e.momentum && there(row, col) > 0)
+      load8(weights, weights_dtype, weights_at + row * weights_row + col, there(row, col), e.wide, w);
+  };
+  auto step = [&](int row, int col, const float (&w)[8], const float (&x)[8]) {
+    const int n = there(row, col);
+    if (n <= 0) return;
+    float v[8];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) v[q] = e.momentum ? w[q] * keep - size * x[q] : x[q];
+    if (e.master) store8(e.master, SB_DTYPE_F32, weights_at + row * weights_row + col, n, e.wide, v);
+    store8(e.param, e.param_dtype, place * e.param_matrix + row * e.param_row + col, n, e.wide, v);
+  };
+  static_for<0, Ep::kParts>([&](auto part) {
+    constexpr int P = decltype(part)::value;
+    u32x4_t his[Ep::kItems], los[Ep::kItems];
+    float w[Ep::kItems][8];
+    Ep::fetch(p.x + tile, p.np, P, his);
+    Ep::fetch(p.lo + tile, p.np, P, los);
+#pragma unroll
+    for (int i = 0; i < Ep::kItems; ++i) {
+      if (e.tall) fetch(j0 + Ep::turn_col(i), i0 + Ep::tile_row(P, Ep::turn_row(i)), w[i]);
+      else fetch(i0 + Ep::tile_row(P, Ep::item_row(i)), j0 + Ep::item_col(i), w[i]);
+    }
+    Ep::template put<P>(lds, acc);
+    Ep::template rows<2>(lds, P, [&](int item, int r, int c, float (&v)[8]) {
+      const float self = p.of_right + p.left.diag[static_cast<int64_t>(matrix) * p.mp + i0 + r];
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        const float x = value_of(static_cast<uint16_t>(his[item][q / 2] >> (16 * (q & 1))), SB_DTYPE_F16) +
+                        value_of(static_cast<uint16_t>(los[item][q / 2] >> (16 * (q & 1))), SB_DTYPE_F16);
+        v[q] = fmaf(unit, v[q], self * x) * kUnscale;
+      }
+      if (!e.tall) step(i0 + r, j0 + c, w[item], v);
+      return u32x4_t{};
+    });
+    if (e.tall) Ep::columns(lds, P, [&](int item, int c, int r, const float (&v)[8]) { step(j0 + c, i0 + r, w[item], v); });
   });
 }
 
@@ -572,7 +678,7 @@ int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 struct Shape {
   int64_t m, n;
   int64_t mp, np;
-  bool wide;
+  bool wide, pairs;
   int64_t most;  // matrices of a batch
 };
 
@@ -586,6 +692,7 @@ Shape shape_of(int64_t rows, int64_t columns, int64_t matrices, int cus) {
   const int64_t m256 = round_up(s.m, 256), n256 = round_up(s.n, 256);
   const int64_t m128 = round_up(s.m, 128), n128 = round_up(s.n, 128);
   s.wide = m256 * n256 * 5 <= m128 * n128 * 6 && matrices * (m256 / 256) * (m256 / 256 + 1) / 2 >= cus;
+  s.pairs = s.wide && s.n >= 2 * s.m;
   s.mp = s.wide ? m256 : m128;
   s.np = s.wide ? n256 : n128;
   s.most = 1;
@@ -595,8 +702,8 @@ Shape shape_of(int64_t rows, int64_t columns, int64_t matrices, int cus) {
 }
 
 struct Buffers {
-  uint16_t *hi[2], *lo, *gram, *poly;
-  float *gram_diag, *poly_diag;
+  uint16_t *hi[2], *lo;
+  Symmetric square[4];
   double* partial;
   float* factor;
   int64_t used;
@@ -608,10 +715,10 @@ Buffers carve(void* workspace, const Shape& s, int64_t matrices) {
   b.hi[0] = ws.take<uint16_t>(matrices * s.mp * s.np);
   b.hi[1] = ws.take<uint16_t>(matrices * s.mp * s.np);
   b.lo = ws.take<uint16_t>(matrices * s.mp * s.np);
-  b.gram = ws.take<uint16_t>(matrices * s.mp * s.mp);
-  b.poly = ws.take<uint16_t>(matrices * s.mp * s.mp);
-  b.gram_diag = ws.take<float>(matrices * s.mp);
-  b.poly_diag = ws.take<float>(matrices * s.mp);
+  for (int i = 0; i < (s.pairs ? 4 : 2); ++i) {
+    b.square[i].off = ws.take<uint16_t>(matrices * s.mp * s.mp);
+    b.square[i].diag = ws.take<float>(matrices * s.mp);
+  }
   b.partial = ws.take<double>(matrices * std::max(chunks_of(s.m, s.n), chunks_of(s.n, s.m)));
   b.factor = ws.take<float>(matrices);
   b.used = ws.used;
@@ -620,20 +727,60 @@ Buffers carve(void* workspace, const Shape& s, int64_t matrices) {
 
 int64_t batch_bytes(const Shape& s, int64_t matrices) { return carve(nullptr, s, matrices).used; }
 
+// The steps, one or two at a time. Two: with P = a5 + B of A = X X^T, the next
+// step's A is P A P = a5^2 A + (2 a5 B + B^2) A, and both steps' factor of X is
+// P' P = a5^2 + (a5 B + a5 B' + B' B): six products of m^3 (half of each) in place of
+// one X X^T and one B X of m^2 n, and of X's passage through memory. Worth it where
+// n is 2 m or more; the last step is taken alone, where an error has the same weight
+// whichever way (n = 2 m: 0.07% of the result against 0.06%, by the norms; n < 2 m
+// would lose more, square ones 0.14% against 0.07%).
 template <class Gram, class Rows>
-int run_steps(const Shape& s, const Buffers& b, int64_t matrices, int32_t steps, hipStream_t stream) {
+int run_steps(const Table& table, const Hyper& h, const Shape& s, const Buffers& b, int64_t matrices, int32_t steps,
+              hipStream_t stream) {
   if (!reduction_fits<Gram>(s.np) || !reduction_fits<Rows>(s.mp))
     return fail(SB_ERR_INVALID, "orthogonalise: problem too large");
   const int64_t t = s.mp / Gram::BM, upper = matrices * t * (t + 1) / 2, all = matrices * t * (s.np / Rows::BN);
-  if (all > 2147483647LL) return fail(SB_ERR_INVALID, "orthogonalise: problem too large");
-  for (int32_t i = 0; i < steps; ++i) {
-    const ProductArgs p{b.hi[i & 1], b.gram, b.poly, b.gram_diag, b.poly_diag, b.lo, b.hi[(i + 1) & 1], static_cast<int32_t>(s.mp),
-                        static_cast<int32_t>(s.np), static_cast<int32_t>(matrices)};
-    symmetric_kernel<Gram, 0><<<static_cast<uint32_t>(upper), Gram::kThreads, 0, stream>>>(p);
+  if (all > 2147483647LL || upper > 2147483647LL) return fail(SB_ERR_INVALID, "orthogonalise: problem too large");
+  ProductArgs p{};
+  p.lo = b.lo;
+  p.mp = static_cast<int32_t>(s.mp);
+  p.np = static_cast<int32_t>(s.np);
+  p.matrices = static_cast<int32_t>(matrices);
+  auto scaled = [&](int i, float scale) { return Symmetric{b.square[i].off, b.square[i].diag, scale}; };
+  auto multiply = [&](const Symmetric& l, const Symmetric& r, const Symmetric& out, float of_l, float of_r, float of_lr) {
+    p.left = l, p.right = r, p.out = out;
+    p.of_left = of_l, p.of_right = of_r, p.of_product = of_lr;
+    symmetric_kernel<Rows, false><<<static_cast<uint32_t>(upper), Rows::kThreads, 0, stream>>>(p);
+    return check_launch("orthogonalise: A A");
+  };
+  int at = 0;
+  for (int32_t done = 0; done < steps;) {
+    const bool two = s.pairs && steps - done >= 3;
+    p.x = b.hi[at];
+    p.next = b.hi[at ^ 1];
+    const Symmetric a = scaled(0, kScale), poly = scaled(1, kScale);
+    p.out = a;
+    symmetric_kernel<Gram, true><<<static_cast<uint32_t>(upper), Gram::kThreads, 0, stream>>>(p);
     if (const int rc = check_launch("orthogonalise: X X^T")) return rc;
-    symmetric_kernel<Rows, 1><<<static_cast<uint32_t>(upper), Rows::kThreads, 0, stream>>>(p);
-    if (const int rc = check_launch("orthogonalise: A A")) return rc;
-    update_kernel<Rows><<<static_cast<uint32_t>(all), Rows::kThreads, 0, stream>>>(p);
+    if (const int rc = multiply(a, a, poly, kB5, 0.0f, kC5)) return rc;
+    Symmetric factor = poly;
+    float own = kA5;
+    if (two) {
+      // |2 a5 B + B^2| and |P' P - a5^2| stay under 11.9.
+      const Symmetric wide = scaled(2, kScale / 4), next_a = scaled(3, kScale), next_poly = scaled(0, kScale);
+      if (const int rc = multiply(poly, poly, wide, 2.0f * kA5, 0.0f, 1.0f)) return rc;
+      if (const int rc = multiply(wide, a, next_a, 0.0f, kA5 * kA5, 1.0f)) return rc;
+      if (const int rc = multiply(next_a, next_a, next_poly, kB5, 0.0f, kC5)) return rc;
+      if (const int rc = multiply(next_poly, poly, wide, kA5, kA5, 1.0f)) return rc;
+      factor = wide;
+      own = kA5 * kA5;
+    }
+    p.left = factor;
+    p.of_right = own;
+    at ^= 1;
+    done += two ? 2 : 1;
+    if (done < steps) update_kernel<Rows><<<static_cast<uint32_t>(all), Rows::kThreads, 0, stream>>>(p);
+    else last_kernel<Rows><<<static_cast<uint32_t>(all), Rows::kThreads, 0, stream>>>(p, table, h);
     if (const int rc = check_launch("orthogonalise: B X")) return rc;
   }
   return SB_OK;
@@ -653,12 +800,8 @@ int run_batch(const Table& t, const Hyper& h, const Shape& s, int64_t matrices, 
   const Padded first{b.hi[0], b.lo, static_cast<int32_t>(s.mp), static_cast<int32_t>(s.np)};
   fill_kernel<<<dim3(static_cast<uint32_t>(tiles), y), kThreads, 0, stream>>>(t, h, b.factor, first);
   if (const int rc = check_launch("orthogonalise: fill")) return rc;
-  if (const int rc = s.wide ? run_steps<WideGram, WideRows>(s, b, matrices, steps, stream)
-                            : run_steps<NarrowGram, NarrowRows>(s, b, matrices, steps, stream))
-    return rc;
-  const Padded last{b.hi[steps & 1], b.lo, static_cast<int32_t>(s.mp), static_cast<int32_t>(s.np)};
-  apply_kernel<<<dim3(static_cast<uint32_t>(tiles), y), kThreads, 0, stream>>>(t, h, last);
-  return check_launch("orthogonalise: step");
+  return s.wide ? run_steps<WideGram, WideRows>(t, h, s, b, matrices, steps, stream)
+                : run_steps<NarrowGram, NarrowRows>(t, h, s, b, matrices, steps, stream);
 }
 
 bool known_dtype(int64_t d) { return d == SB_DTYPE_BF16 || d == SB_DTYPE_F16 || d == SB_DTYPE_F32; }

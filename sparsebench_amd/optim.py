@@ -144,8 +144,8 @@ def orthogonalize(matrices: torch.Tensor, steps: int = 5) -> torch.Tensor:
     (to about [0.7, 1.2] in five steps). bf16 / fp16 / fp32, of any size and of any strides
     whose rows are contiguous. The products take fp16 operands, sum in fp32, and keep X to
     twice fp16's bits: the result is within about 0.2% of exact arithmetic's, in the
-    matrix's norm, before it is rounded to the input's type. Results do not depend on
-    the other matrices of the stack."""
+    matrix's norm, before it is rounded to the input's type. Matrices do not mix, but how
+    many there are of a size chooses the kernels' tiles, and with them the last bits."""
     from sparsebench_amd import _C
 
     return _C.orthogonalize_cuda(matrices, steps)

@@ -90,14 +90,14 @@ def test_orthogonalize(size, dtype) -> None:
     check(got, newton_schulz(u), u)
 
 
-@pytest.mark.parametrize("size", [(3, 1024, 1280), (300, 256, 256), (70, 512, 256), (130, 200, 250)])
+@pytest.mark.parametrize("size", [(3, 1024, 1280), (26, 1024, 2100), (300, 256, 256), (270, 520, 250), (70, 512, 256), (130, 200, 250)])
 def test_many_matrices(size) -> None:
     """Enough of them for the wide tiles, or a ragged number of narrow ones."""
     u = gradient(*size, seed=3, dtype=torch.bfloat16)
     got = optim.orthogonalize(u)
     check(got, newton_schulz(u), u)
-    # Alone it takes narrow tiles, whose sums have the same order.
-    assert torch.equal(optim.orthogonalize(u[-1]), got[-1])
+    alone = optim.orthogonalize(u[-1])  # one matrix takes other tiles: other roundings
+    assert (alone.double() - got[-1].double()).norm() <= 2 * (PRODUCTS + 2.0**-8) * got[-1].double().norm()
 
 
 def test_largest_side() -> None:
