@@ -16,6 +16,7 @@ from typing import NamedTuple
 
 import torch
 
+from sparsebench_amd.norm import norm_in, norm_out
 from sparsebench_amd.routing import AssignedRouting, route_assigned, route_device, route_rounded
 from sparsebench_amd.spmm import dsd, sdd
 
@@ -341,3 +342,42 @@ def moe_forward_gated_4bit(
     from sparsebench_amd import _C
 
     return _C.experts4_layer_cuda(x, expert_idx, expert_weight, w1, w2, activation, valid_tokens)
+
+
+# ---- the gated layer with the norms around it ----
+
+
+def moe_block_gated(
+    x: torch.Tensor,
+    route: Callable[[torch.Tensor], tuple[torch.Tensor, torch.Tensor]],
+    w1: torch.Tensor | Experts4,
+    w2: torch.Tensor | Experts4,
+    in_weight: torch.Tensor | None = None,
+    out_weight: torch.Tensor | None = None,
+    gate: torch.Tensor | None = None,
+    scale: float = 1.0,
+    next_weight: torch.Tensor | None = None,
+    normed: torch.Tensor | None = None,
+    eps: float = 1e-6,
+    activation: str = "silu",
+    valid_tokens: torch.Tensor | None = None,
+) -> torch.Tensor | tuple[torch.Tensor, torch.Tensor]:
+    """The residual stream after a gated layer between its two norms:
+
+        n = norm_in(x, in_weight),  ids, weights = route(n)
+        out = norm_out(gated layer(n, ids, weights), x, out_weight, gate, scale)
+
+    x [T, D] bf16. Experts in bf16 go through moe_forward_gated, Experts4 through
+    moe_forward_gated_4bit (both w1 and w2 then). With next_weight it returns (out,
+    norm_in(out, next_weight)); the second is the next block's `normed`, which takes
+    in_weight's place there. Operands are those of the calls it makes (norm.norm_in,
+    norm.norm_out); it syncs and allocates no more than these and route do."""
+    if isinstance(w1, Experts4) != isinstance(w2, Experts4):
+        raise ValueError("w1 and w2: both of them Experts4, or neither")
+    if normed is None:
+        normed = norm_in(x, in_weight, eps, valid_tokens)
+    elif in_weight is not None:
+        raise ValueError("normed is the layer's input already: in_weight must be None")
+    layer = moe_forward_gated_4bit if isinstance(w1, Experts4) else moe_forward_gated
+    y = layer(normed, *route(normed), w1, w2, activation, valid_tokens)
+    return norm_out(y, x, out_weight, gate, scale, eps, next_weight, valid_tokens)

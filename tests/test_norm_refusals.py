@@ -119,3 +119,9 @@ def test_python_calls_refuse_cpu_tensors() -> None:
 def test_python_calls_refuse(make, match) -> None:
     with pytest.raises(RuntimeError, match=match):
         make(torch.zeros(4, 64, device="cuda"), torch.ones(64, device="cuda"))
+
+
+def test_both_import_paths() -> None:
+    import sparsebench.norm
+
+    assert sparsebench.norm is norm
