@@ -431,8 +431,9 @@ struct Epilogue {
     constexpr int kTurns = kRows * Cfg::BN / 64, kBlocks = kRun / 8;
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < kTurns / Cfg::kThreads; ++i) {
+    for (int i = 0; i * Cfg::kThreads < kTurns; ++i) {
       const int item = i * Cfg::kThreads + static_cast<int>(threadIdx.x);
+      if (item >= kTurns) break;
       const int r = (item % kBlocks + item / (kBlocks * (Cfg::BN / 8)) * kBlocks) * 8, c = item / kBlocks % (Cfg::BN / 8) * 8;
       u32x4_t in[8];
 #pragma unroll
@@ -666,11 +667,13 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1) last_kernel(ProductArgs p, T
 }
 
 // 256 x 256 tiles of 8 waves (X X^T in K steps of 64, two stages of A and three
-// of B; the others in steps of 32, A two at a time), or 128 x 128 of 4.
+// of B; the others in steps of 32, A two at a time), 128 x 128 of 4, or 64 x 64 of 4.
 using WideGram = DmaCfg<256, 256, 64, 2, 2, 4, 0, 0, 5, 1, 0, 3, 0, 0, 1, 0, 1>;
 using WideRows = DmaCfg<256, 256, 32, 4, 2, 4, 0, 0, 5, 1, 1, 0, 0, 0, 0, 0, 1>;
 using NarrowGram = DmaCfg<128, 128, 64, 3, 2, 2, 0, 0, 5, 1, 0, 0, 0, 0, 1, 0, 1>;
 using NarrowRows = DmaCfg<128, 128, 64, 3, 2, 2, 0, 0, 5, 1, 0, 0, 0, 0, 0, 0, 1>;
+using SmallGram = DmaCfg<64, 64, 64, 6, 2, 2, 0, 0, 5, 1, 0, 0, 0, 0, 1, 0, 1>;
+using SmallRows = DmaCfg<64, 64, 64, 6, 2, 2, 0, 0, 5, 1, 0, 0, 0, 0, 0, 0, 1>;
 
 int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
@@ -678,7 +681,8 @@ int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 struct Shape {
   int64_t m, n;
   int64_t mp, np;
-  bool wide, pairs;
+  int tile;  // 256, 128 or 64
+  bool pairs;
   int64_t most;  // matrices of a batch
 };
 
@@ -688,13 +692,21 @@ Shape shape_of(int64_t rows, int64_t columns, int64_t matrices, int cus) {
   Shape s;
   s.m = std::min(rows, columns);
   s.n = std::max(rows, columns);
-  // Wide tiles where padding to them costs little and there is one for each CU.
   const int64_t m256 = round_up(s.m, 256), n256 = round_up(s.n, 256);
   const int64_t m128 = round_up(s.m, 128), n128 = round_up(s.n, 128);
-  s.wide = m256 * n256 * 5 <= m128 * n128 * 6 && matrices * (m256 / 256) * (m256 / 256 + 1) / 2 >= cus;
-  s.pairs = s.wide && s.n >= 2 * s.m;
-  s.mp = s.wide ? m256 : m128;
-  s.np = s.wide ? n256 : n128;
+  const int64_t m64 = round_up(s.m, 64), n64 = round_up(s.n, 64);
+  auto upper = [&](int64_t side, int64_t tile) { return matrices * (side / tile) * (side / tile + 1) / 2; };
+  // Wide tiles where padding to them costs little and there is one for each CU. Small
+  // ones where A's all run at once, whose time is then a launch's and a tile's own, or
+  // where padding to 128 would double the work. Small against narrow, five steps in bf16:
+  // 24 of 256 x 512 (240 small tiles of A) 139 us against 165, one of 1024 x 1024 (136)
+  // 163 : 239, 24 of 128 x 4096 (72) 339 : 359; but 8 of 512 x 512 (288) 180 : 174, 25 of
+  // them (900) 398 : 255; 1000 of 64 x 256 386 : 652, of 192 x 192 1655 : 1647.
+  if (m256 * n256 * 5 <= m128 * n128 * 6 && upper(m256, 256) >= cus) s.tile = 256;
+  else s.tile = upper(m64, 64) <= cus || 2 * m64 * n64 <= m128 * n128 ? 64 : 128;
+  s.pairs = s.tile == 256 && s.n >= 2 * s.m;
+  s.mp = round_up(s.m, s.tile);
+  s.np = round_up(s.n, s.tile);
   s.most = 1;
   while (s.most < 65535 && batch_bytes(s, s.most * 2) <= kBatchBytes) s.most *= 2;
   s.most = std::min<int64_t>(s.most, 65535);
@@ -800,8 +812,9 @@ int run_batch(const Table& t, const Hyper& h, const Shape& s, int64_t matrices, 
   const Padded first{b.hi[0], b.lo, static_cast<int32_t>(s.mp), static_cast<int32_t>(s.np)};
   fill_kernel<<<dim3(static_cast<uint32_t>(tiles), y), kThreads, 0, stream>>>(t, h, b.factor, first);
   if (const int rc = check_launch("orthogonalise: fill")) return rc;
-  return s.wide ? run_steps<WideGram, WideRows>(t, h, s, b, matrices, steps, stream)
-                : run_steps<NarrowGram, NarrowRows>(t, h, s, b, matrices, steps, stream);
+  return s.tile == 256   ? run_steps<WideGram, WideRows>(t, h, s, b, matrices, steps, stream)
+         : s.tile == 128 ? run_steps<NarrowGram, NarrowRows>(t, h, s, b, matrices, steps, stream)
+                         : run_steps<SmallGram, SmallRows>(t, h, s, b, matrices, steps, stream);
 }
 
 bool known_dtype(int64_t d) { return d == SB_DTYPE_BF16 || d == SB_DTYPE_F16 || d == SB_DTYPE_F32; }

@@ -90,7 +90,8 @@ def test_orthogonalize(size, dtype) -> None:
     check(got, newton_schulz(u), u)
 
 
-@pytest.mark.parametrize("size", [(3, 1024, 1280), (26, 1024, 2100), (300, 256, 256), (270, 520, 250), (70, 512, 256), (130, 200, 250)])
+@pytest.mark.parametrize("size", [(3, 1024, 1280), (26, 1024, 2100), (300, 256, 256), (270, 520, 250), (70, 512, 256), (130, 200, 250),
+                                  (8, 512, 512), (7, 512, 520), (257, 64, 64), (256, 64, 129), (300, 130, 70)])
 def test_many_matrices(size) -> None:
     """Enough of them for the wide tiles, or a ragged number of narrow ones."""
     u = gradient(*size, seed=3, dtype=torch.bfloat16)
@@ -182,6 +183,25 @@ def test_step(param, masters, nesterov) -> None:
         if masters:
             check_weights(ms[i], kept, update)
             assert torch.equal(params[i], ms[i].to(param))
+
+
+@pytest.mark.parametrize(("count", "rows", "columns"), [(90, 256, 200), (64, 512, 512), (300, 40, 60), (2, 300, 700)])
+def test_step_of_many(count, rows, columns) -> None:
+    """Narrow, wide and small tiles; gate and up halves and a tall second matrix in one batch."""
+    flat = gradient(count, rows, 2 * columns, seed=25, scale=0.05, dtype=torch.bfloat16)
+    params = [flat[:, :, :columns], flat[:, :, columns:], gradient(count, columns, rows, seed=26, dtype=torch.bfloat16)]
+    grads = [gradient(*p.shape, seed=35 + i, dtype=torch.bfloat16) for i, p in enumerate(params)]
+    momenta = [gradient(*p.shape, seed=45 + i) for i, p in enumerate(params)]
+    ms = [p.float() for p in params]
+    start = [m.clone() for m in momenta]
+    optim.muon_step(params, grads, momenta, 0.02, weight_decay=0.1, masters=ms)
+    for i, m in enumerate(start):
+        first = (gradient(count, rows, 2 * columns, seed=25, scale=0.05, dtype=torch.bfloat16).float()
+                 [:, :, i * columns:(i + 1) * columns] if i < 2 else
+                 gradient(count, columns, rows, seed=26, dtype=torch.bfloat16).float())
+        kept, update, _ = step_reference(first, grads[i], m, 0.02, 0.95, True, 0.1, 0.2, 1.0)
+        check_weights(ms[i], kept, update)
+        assert torch.equal(params[i], ms[i].bfloat16())
 
 
 def test_many_tensors_of_one_size_and_of_many() -> None:
