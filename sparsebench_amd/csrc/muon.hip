@@ -24,7 +24,6 @@
 // they come from and whichever side is the smaller.
 
 #include <cmath>
-#include <vector>
 
 #include "gemm_dma.hpp"
 #include "workspace.hpp"
@@ -667,13 +666,16 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1) last_kernel(ProductArgs p, T
 }
 
 // 256 x 256 tiles of 8 waves (X X^T in K steps of 64, two stages of A and three
-// of B; the others in steps of 32, A two at a time), 128 x 128 of 4, or 64 x 64 of 4.
+// of B; the others in steps of 32, A two at a time), 128 x 128 of 4 (64 KB of LDS, so
+// that two workgroups share a CU: against three stages of 64, one a CU, 100 of 256 x 256
+// take 228 us for 287, 20 of 1024 x 1024 737 for 893), or 64 x 64 of 4 (X X^T, whose
+// reductions are long, with a stage more; six stages each: 141 us for 111 at 24 of 256 x 512).
 using WideGram = DmaCfg<256, 256, 64, 2, 2, 4, 0, 0, 5, 1, 0, 3, 0, 0, 1, 0, 1>;
 using WideRows = DmaCfg<256, 256, 32, 4, 2, 4, 0, 0, 5, 1, 1, 0, 0, 0, 0, 0, 1>;
-using NarrowGram = DmaCfg<128, 128, 64, 3, 2, 2, 0, 0, 5, 1, 0, 0, 0, 0, 1, 0, 1>;
-using NarrowRows = DmaCfg<128, 128, 64, 3, 2, 2, 0, 0, 5, 1, 0, 0, 0, 0, 0, 0, 1>;
-using SmallGram = DmaCfg<64, 64, 64, 6, 2, 2, 0, 0, 5, 1, 0, 0, 0, 0, 1, 0, 1>;
-using SmallRows = DmaCfg<64, 64, 64, 6, 2, 2, 0, 0, 5, 1, 0, 0, 0, 0, 0, 0, 1>;
+using NarrowGram = DmaCfg<128, 128, 32, 4, 2, 2, 0, 0, 5, 1, 0, 0, 0, 0, 1, 0, 1>;
+using NarrowRows = DmaCfg<128, 128, 32, 4, 2, 2, 0, 0, 5, 1, 0, 0, 0, 0, 0, 0, 1>;
+using SmallGram = DmaCfg<64, 64, 64, 4, 2, 2, 0, 0, 5, 1, 0, 0, 0, 0, 1, 0, 1>;
+using SmallRows = DmaCfg<64, 64, 64, 3, 2, 2, 0, 0, 5, 1, 0, 0, 0, 0, 0, 0, 1>;
 
 int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
@@ -692,19 +694,32 @@ Shape shape_of(int64_t rows, int64_t columns, int64_t matrices, int cus) {
   Shape s;
   s.m = std::min(rows, columns);
   s.n = std::max(rows, columns);
-  const int64_t m256 = round_up(s.m, 256), n256 = round_up(s.n, 256);
-  const int64_t m128 = round_up(s.m, 128), n128 = round_up(s.n, 128);
-  const int64_t m64 = round_up(s.m, 64), n64 = round_up(s.n, 64);
-  auto upper = [&](int64_t side, int64_t tile) { return matrices * (side / tile) * (side / tile + 1) / 2; };
-  // Wide tiles where padding to them costs little and there is one for each CU. Small
-  // ones where A's all run at once, whose time is then a launch's and a tile's own, or
-  // where padding to 128 would double the work. Small against narrow, five steps in bf16:
-  // 24 of 256 x 512 (240 small tiles of A) 139 us against 165, one of 1024 x 1024 (136)
-  // 163 : 239, 24 of 128 x 4096 (72) 339 : 359; but 8 of 512 x 512 (288) 180 : 174, 25 of
-  // them (900) 398 : 255; 1000 of 64 x 256 386 : 652, of 192 x 192 1655 : 1647.
-  if (m256 * n256 * 5 <= m128 * n128 * 6 && upper(m256, 256) >= cus) s.tile = 256;
-  else s.tile = upper(m64, 64) <= cus || 2 * m64 * n64 <= m128 * n128 ? 64 : 128;
-  s.pairs = s.tile == 256 && s.n >= 2 * s.m;
+  auto steps_of_a = [&](int64_t tile) {  // A's tiles on and above the diagonal, times their K steps in A A
+    const int64_t t = round_up(s.m, tile) / tile;
+    return matrices * t * (t + 1) / 2 * t;
+  };
+  auto padded = [&](int64_t tile) {  // m^2 n
+    const double m = static_cast<double>(round_up(s.m, tile));
+    return m * m * static_cast<double>(round_up(s.n, tile));
+  };
+  // Wide tiles (one workgroup a CU) where matrices are large and padding to them costs
+  // little, small ones where the work is little or padding to 128 would add a third.
+  // us for five steps of bf16 stacks, wide, narrow, small:
+  //   128 of 768 x 2048  3850  4323  5172     24 of 256 x 512       158  112
+  //   20 of 2048 x 2048  4123  5011  7252     200 of 256 x 256      360  325
+  //   64 of 768 x 2048   2172  2214  2631     3 of 1024 x 1024      238  203
+  //   26 of 1024 x 4096  2586  2357  2911     7 of 1024 x 1024      326  371
+  //   400 of 512 x 512   2958  2877  3411     90 of 512 x 1024      988  1106
+  //   100 of 512 x 2048  1982  1670  1931     100 of 320 x 1024     698  556
+  //   300 of 256 x 256    691   481   471     1000 of 192 x 192    1500  900
+  if (s.m > 512 && 2 * padded(256) <= 3 * padded(64) && 2 * steps_of_a(256) >= int64_t{9} * cus) s.tile = 256;
+  else if (steps_of_a(64) <= int64_t{32} * cus || 4 * padded(64) <= 3 * padded(128)) s.tile = 64;
+  else s.tile = 128;
+  // Two steps at a time (run_steps) where X is long, and not so little that launches
+  // count: 24 of 256 x 512 would take 117 us for 112, 16 of 512 x 2048 take 335 for 404,
+  // 1 of 128 x 4096 121 for 140.
+  s.pairs = s.n >= 2 * s.m &&
+            (s.n >= 2048 || matrices * (round_up(s.m, 64) / 64) * (round_up(s.n, 64) / 64) >= int64_t{4} * cus);
   s.mp = round_up(s.m, s.tile);
   s.np = round_up(s.n, s.tile);
   s.most = 1;
@@ -855,19 +870,18 @@ bool wide_values(const SbMuonTensor& a) {
 // f(shape, total matrices of that size) for each size in the list, by its first tensor.
 template <class F>
 int for_each_size(const SbMuonTensor* tensors, int64_t count, int cus, F&& f) {
-  std::vector<std::pair<int64_t, int64_t>> seen;
+  auto same = [&](int64_t i, int64_t q) {
+    return !empty(tensors[q]) && std::minmax(tensors[i].rows, tensors[i].columns) == std::minmax(tensors[q].rows, tensors[q].columns);
+  };
   for (int64_t i = 0; i < count; ++i) {
     if (empty(tensors[i])) continue;
-    const auto size = std::minmax(tensors[i].rows, tensors[i].columns);
-    const std::pair<int64_t, int64_t> key{size.first, size.second};
-    if (std::find(seen.begin(), seen.end(), key) != seen.end()) continue;
-    seen.push_back(key);
+    bool first = true;
+    for (int64_t q = 0; q < i && first; ++q) first = !same(i, q);
+    if (!first) continue;
     int64_t total = 0;
-    for (int64_t q = i; q < count; ++q) {
-      const auto other = std::minmax(tensors[q].rows, tensors[q].columns);
-      if (!empty(tensors[q]) && other.first == key.first && other.second == key.second) total += tensors[q].matrices;
-    }
-    if (const int rc = f(shape_of(key.first, key.second, total, cus), total, i)) return rc;
+    for (int64_t q = i; q < count; ++q)
+      if (same(i, q)) total += tensors[q].matrices;
+    if (const int rc = f(shape_of(tensors[i].rows, tensors[i].columns, total, cus), total, i)) return rc;
   }
   return SB_OK;
 }

@@ -371,7 +371,9 @@ def moe_block_gated(
     moe_forward_gated_4bit (both w1 and w2 then). With next_weight it returns (out,
     norm_in(out, next_weight)); the second is the next block's `normed`, which takes
     in_weight's place there. Operands are those of the calls it makes (norm.norm_in,
-    norm.norm_out); it syncs and allocates no more than these and route do."""
+    norm.norm_out); it syncs and allocates no more than these and route do. Rows t >=
+    valid_tokens of what route is given hold no values, and what it returns for them does
+    not matter."""
     if isinstance(w1, Experts4) != isinstance(w2, Experts4):
         raise ValueError("w1 and w2: both of them Experts4, or neither")
     if normed is None:

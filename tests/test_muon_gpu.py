@@ -91,7 +91,8 @@ def test_orthogonalize(size, dtype) -> None:
 
 
 @pytest.mark.parametrize("size", [(3, 1024, 1280), (26, 1024, 2100), (300, 256, 256), (270, 520, 250), (70, 512, 256), (130, 200, 250),
-                                  (8, 512, 512), (7, 512, 520), (257, 64, 64), (256, 64, 129), (300, 130, 70)])
+                                  (8, 512, 512), (7, 512, 520), (257, 64, 64), (256, 64, 129), (300, 130, 70),
+                                  (80, 768, 768), (64, 700, 1500), (3, 2560, 2600), (30, 200, 2100), (1000, 100, 130)])
 def test_many_matrices(size) -> None:
     """Enough of them for the wide tiles, or a ragged number of narrow ones."""
     u = gradient(*size, seed=3, dtype=torch.bfloat16)
@@ -185,7 +186,8 @@ def test_step(param, masters, nesterov) -> None:
             assert torch.equal(params[i], ms[i].to(param))
 
 
-@pytest.mark.parametrize(("count", "rows", "columns"), [(90, 256, 200), (64, 512, 512), (300, 40, 60), (2, 300, 700)])
+@pytest.mark.parametrize(("count", "rows", "columns"), [(90, 256, 200), (64, 512, 512), (300, 40, 60), (2, 300, 700),
+                                                      (27, 768, 770)])
 def test_step_of_many(count, rows, columns) -> None:
     """Narrow, wide and small tiles; gate and up halves and a tall second matrix in one batch."""
     flat = gradient(count, rows, 2 * columns, seed=25, scale=0.05, dtype=torch.bfloat16)
