@@ -40,17 +40,25 @@ __device__ __forceinline__ float load_as_f32(const void* p, int32_t dtype, int64
   return dtype == SB_DTYPE_BF16 ? bf16_to_f32(bits) : static_cast<float>(__builtin_bit_cast(_Float16, bits));
 }
 
+// An fp32 result rounded to fp16: in two steps, as a result that was stored in fp32 in
+// between. Without the barrier the compiler fuses the last operation and the conversion
+// into one rounding, which takes other values at about one in 2^13.
+__device__ __forceinline__ uint16_t f32_to_f16(float v) {
+  asm("" : "+v"(v));
+  return __builtin_bit_cast(uint16_t, static_cast<_Float16>(v));
+}
+
 __device__ __forceinline__ void store_as(void* p, int32_t dtype, int64_t i, float v) {
   if (dtype == SB_DTYPE_F32) static_cast<float*>(p)[i] = v;
   else if (dtype == SB_DTYPE_BF16) static_cast<uint16_t*>(p)[i] = f32_to_bf16(v);
-  else static_cast<_Float16*>(p)[i] = static_cast<_Float16>(v);
+  else static_cast<uint16_t*>(p)[i] = f32_to_f16(v);
 }
 
 template <int DTYPE>
 __device__ __forceinline__ float rounded(float v) {
   if constexpr (DTYPE == SB_DTYPE_F32) return v;
   else if constexpr (DTYPE == SB_DTYPE_BF16) return bf16_to_f32(f32_to_bf16(v));
-  else return static_cast<float>(static_cast<_Float16>(v));
+  else return static_cast<float>(__builtin_bit_cast(_Float16, f32_to_f16(v)));
 }
 
 // A row's share of a thread, 8 NCH values. VEC: chunks of 8 consecutive values
@@ -135,8 +143,7 @@ __device__ __forceinline__ void store_row(void* row, int d, int t, const float (
           if constexpr (DTYPE == SB_DTYPE_BF16) {
             a[q] = pack_bf16x2(lo, hi);
           } else {
-            a[q] = __builtin_bit_cast(uint16_t, static_cast<_Float16>(lo)) |
-                   static_cast<uint32_t>(__builtin_bit_cast(uint16_t, static_cast<_Float16>(hi))) << 16;
+            a[q] = f32_to_f16(lo) | static_cast<uint32_t>(f32_to_f16(hi)) << 16;
           }
         }
         *reinterpret_cast<u32x4_t*>(static_cast<uint16_t*>(row) + at) = a;
