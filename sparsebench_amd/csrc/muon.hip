@@ -690,12 +690,16 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1) last_kernel(ProductArgs p, T
 }
 
 // 256 x 256 tiles of 8 waves (X X^T in K steps of 64, two stages of A and three
-// of B; the others in steps of 32, A two at a time), 128 x 128 of 4 (64 KB of LDS, so
-// that two workgroups share a CU: against three stages of 64, one a CU, 100 of 256 x 256
-// take 228 us for 287, 20 of 1024 x 1024 737 for 893), or 64 x 64 of 4 (X X^T, whose
-// reductions are long, with a stage more; six stages each: 141 us for 111 at 24 of 256 x 512).
+// of B; B X in steps of 32, A two at a time; the squares' short reductions in 128 x 128
+// tiles, two workgroups a CU, whose epilogues then run beside products: 100 of 768 x 2048
+// 3160 us for 3325, 64 of 1024 x 4096 5219 : 5337, 20 of 2048 x 2048 4212 : 4161), 128 x
+// 128 of 4 (64 KB of LDS, so that two workgroups share a CU: against three stages of 64,
+// one a CU, 100 of 256 x 256 take 228 us for 287, 20 of 1024 x 1024 737 for 893), or
+// 64 x 64 of 4 (X X^T, whose reductions are long, with a stage more; six stages each:
+// 141 us for 111 at 24 of 256 x 512).
 using WideGram = DmaCfg<256, 256, 64, 2, 2, 4, 0, 0, 5, 1, 0, 3, 0, 0, 1, 0, 1>;
 using WideRows = DmaCfg<256, 256, 32, 4, 2, 4, 0, 0, 5, 1, 1, 0, 0, 0, 0, 0, 1>;
+using WideSquare = DmaCfg<128, 128, 32, 4, 2, 2, 0, 0, 5, 1, 1, 0, 0, 0, 0, 0, 1>;
 using NarrowGram = DmaCfg<128, 128, 32, 4, 2, 2, 0, 0, 5, 1, 0, 0, 0, 0, 1, 0, 1>;
 using NarrowRows = DmaCfg<128, 128, 32, 4, 2, 2, 0, 0, 5, 1, 0, 0, 0, 0, 0, 0, 1>;
 using SmallGram = DmaCfg<64, 64, 64, 4, 2, 2, 0, 0, 5, 1, 0, 0, 0, 0, 1, 0, 1>;
@@ -789,13 +793,14 @@ int64_t batch_bytes(const Shape& s, int64_t matrices) { return carve(nullptr, s,
 // n is 2 m or more; the last step is taken alone, where an error has the same weight
 // whichever way (n = 2 m: 0.07% of the result against 0.06%, by the norms; n < 2 m
 // would lose more, square ones 0.14% against 0.07%).
-template <class Gram, class Rows>
+template <class Gram, class Square, class Rows>
 int run_steps(const Table& table, const Hyper& h, const Shape& s, const Buffers& b, int64_t matrices, int32_t steps,
               hipStream_t stream) {
-  if (!reduction_fits<Gram>(s.np) || !reduction_fits<Rows>(s.mp))
+  if (!reduction_fits<Gram>(s.np) || !reduction_fits<Square>(s.mp) || !reduction_fits<Rows>(s.mp))
     return fail(SB_ERR_INVALID, "orthogonalise: problem too large");
-  const int64_t t = s.mp / Gram::BM, upper = matrices * t * (t + 1) / 2, all = matrices * t * (s.np / Rows::BN);
-  if (all > 2147483647LL || upper > 2147483647LL) return fail(SB_ERR_INVALID, "orthogonalise: problem too large");
+  auto upper = [&](int64_t tile) { return matrices * (s.mp / tile) * (s.mp / tile + 1) / 2; };
+  const int64_t all = matrices * (s.mp / Rows::BM) * (s.np / Rows::BN);
+  if (all > 2147483647LL || upper(Square::BM) > 2147483647LL) return fail(SB_ERR_INVALID, "orthogonalise: problem too large");
   ProductArgs p{};
   p.lo = b.lo;
   p.mp = static_cast<int32_t>(s.mp);
@@ -805,7 +810,7 @@ int run_steps(const Table& table, const Hyper& h, const Shape& s, const Buffers&
   auto multiply = [&](const Symmetric& l, const Symmetric& r, const Symmetric& out, float of_l, float of_r, float of_lr) {
     p.left = l, p.right = r, p.out = out;
     p.of_left = of_l, p.of_right = of_r, p.of_product = of_lr;
-    symmetric_kernel<Rows, false><<<static_cast<uint32_t>(upper), Rows::kThreads, 0, stream>>>(p);
+    symmetric_kernel<Square, false><<<static_cast<uint32_t>(upper(Square::BM)), Square::kThreads, 0, stream>>>(p);
     return check_launch("orthogonalise: A A");
   };
   int at = 0;
@@ -815,7 +820,7 @@ int run_steps(const Table& table, const Hyper& h, const Shape& s, const Buffers&
     p.next = b.hi[at ^ 1];
     const Symmetric a = scaled(0, kScale), poly = scaled(1, kScale);
     p.out = a;
-    symmetric_kernel<Gram, true><<<static_cast<uint32_t>(upper), Gram::kThreads, 0, stream>>>(p);
+    symmetric_kernel<Gram, true><<<static_cast<uint32_t>(upper(Gram::BM)), Gram::kThreads, 0, stream>>>(p);
     if (const int rc = check_launch("orthogonalise: X X^T")) return rc;
     if (const int rc = multiply(a, a, poly, kB5, 0.0f, kC5)) return rc;
     Symmetric factor = poly;
@@ -858,9 +863,9 @@ int run_batch(const Table& t, const Hyper& h, const Shape& s, int64_t matrices, 
   fill_kernel<<<dim3(static_cast<uint32_t>(tiles), y), kThreads, 0, stream>>>(t, h, b.partial, static_cast<int32_t>(chunks),
                                                                             b.factor, first);
   if (const int rc = check_launch("orthogonalise: fill")) return rc;
-  return s.tile == 256   ? run_steps<WideGram, WideRows>(t, h, s, b, matrices, steps, stream)
-         : s.tile == 128 ? run_steps<NarrowGram, NarrowRows>(t, h, s, b, matrices, steps, stream)
-                         : run_steps<SmallGram, SmallRows>(t, h, s, b, matrices, steps, stream);
+  return s.tile == 256   ? run_steps<WideGram, WideSquare, WideRows>(t, h, s, b, matrices, steps, stream)
+         : s.tile == 128 ? run_steps<NarrowGram, NarrowRows, NarrowRows>(t, h, s, b, matrices, steps, stream)
+                         : run_steps<SmallGram, SmallRows, SmallRows>(t, h, s, b, matrices, steps, stream);
 }
 
 bool known_dtype(int64_t d) { return d == SB_DTYPE_BF16 || d == SB_DTYPE_F16 || d == SB_DTYPE_F32; }
