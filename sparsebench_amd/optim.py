@@ -177,7 +177,8 @@ def muon_step(
     the gated layer are two stacks, each expert's gate and up matrix orthogonalised by
     itself. masters: fp32 weights updated in the parameters' place and rounded into them.
     lr and grad_scale may be one-element fp32 tensors on the GPU. All on one GPU; tensors
-    must not overlap. Matrices of one size are taken together. Parameters and masters
+    must not overlap (an fp32 parameter may be its own master). Matrices of one size are
+    taken together. Parameters and masters
     count as modified in place, as in adamw_step; nothing syncs, and a step can be captured."""
     from sparsebench_amd import _C
 

@@ -126,6 +126,25 @@ def test_leading_dimensions_and_strides() -> None:
     assert torch.equal(optim.orthogonalize(one)[2], optim.orthogonalize(u[0, 0]))
 
 
+def test_more_matrices_than_a_batch() -> None:
+    u = gradient(70000, 2, 3, seed=6)
+    got = optim.orthogonalize(u)
+    pick = torch.tensor([0, 65534, 65535, 65536, 69999], device=DEV)
+    check(got[pick], newton_schulz(u[pick]), u[pick])
+    assert torch.equal(got[65000:], optim.orthogonalize(u[65000:].flip(0)).flip(0))
+
+
+def test_one_tensor_twice_is_refused() -> None:
+    w, g = gradient(2, 32, 32, seed=11), gradient(2, 32, 32, seed=12)
+    m = [torch.zeros_like(w) for _ in range(2)]
+    with pytest.raises(RuntimeError, match="must not overlap"):
+        optim.muon_step([w, w], [g, g], m, 0.1)
+    with pytest.raises(RuntimeError, match="must not overlap"):
+        optim.muon_step([w, w.clone()], [g, g], [m[0], m[0]], 0.1)
+    with pytest.raises(RuntimeError, match="must not overlap"):
+        optim.muon_step([w], [g], [w], 0.1)
+
+
 def test_zeros_tiny_huge_and_not_finite() -> None:
     """Zeros give zeros, sizes do not matter, and a matrix that is not finite stays alone."""
     u = gradient(6, 48, 80, seed=10)
