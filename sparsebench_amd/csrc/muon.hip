@@ -690,13 +690,11 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1) last_kernel(ProductArgs p, T
 }
 
 // 256 x 256 tiles of 8 waves (X X^T in K steps of 64, two stages of A and three
-// of B; B X in steps of 32, A two at a time; the squares' short reductions in 128 x 128
-// tiles, two workgroups a CU, whose epilogues then run beside products: 100 of 768 x 2048
-// 3160 us for 3325, 64 of 1024 x 4096 5219 : 5337, 20 of 2048 x 2048 4212 : 4161), 128 x
-// 128 of 4 (64 KB of LDS, so that two workgroups share a CU: against three stages of 64,
-// one a CU, 100 of 256 x 256 take 228 us for 287, 20 of 1024 x 1024 737 for 893), or
-// 64 x 64 of 4 (X X^T, whose reductions are long, with a stage more; six stages each:
-// 141 us for 111 at 24 of 256 x 512).
+// of B; the others in steps of 32, A two at a time), 128 x 128 of 4 (64 KB of LDS, so
+// that two workgroups share a CU: against three stages of 64, one a CU, 100 of 256 x 256
+// take 228 us for 287, 20 of 1024 x 1024 737 for 893), or 64 x 64 of 4 (X X^T, whose
+// reductions are long, with a stage more; six stages each: 141 us for 111 at 24 of
+// 256 x 512).
 using WideGram = DmaCfg<256, 256, 64, 2, 2, 4, 0, 0, 5, 1, 0, 3, 0, 0, 1, 0, 1>;
 using WideRows = DmaCfg<256, 256, 32, 4, 2, 4, 0, 0, 5, 1, 1, 0, 0, 0, 0, 0, 1>;
 using WideSquare = DmaCfg<128, 128, 32, 4, 2, 2, 0, 0, 5, 1, 1, 0, 0, 0, 0, 0, 1>;
@@ -863,9 +861,20 @@ int run_batch(const Table& t, const Hyper& h, const Shape& s, int64_t matrices, 
   fill_kernel<<<dim3(static_cast<uint32_t>(tiles), y), kThreads, 0, stream>>>(t, h, b.partial, static_cast<int32_t>(chunks),
                                                                             b.factor, first);
   if (const int rc = check_launch("orthogonalise: fill")) return rc;
-  return s.tile == 256   ? run_steps<WideGram, WideSquare, WideRows>(t, h, s, b, matrices, steps, stream)
-         : s.tile == 128 ? run_steps<NarrowGram, NarrowRows, NarrowRows>(t, h, s, b, matrices, steps, stream)
-                         : run_steps<SmallGram, SmallRows, SmallRows>(t, h, s, b, matrices, steps, stream);
+  if (s.tile == 64) return run_steps<SmallGram, SmallRows, SmallRows>(t, h, s, b, matrices, steps, stream);
+  if (s.tile == 128) return run_steps<NarrowGram, NarrowRows, NarrowRows>(t, h, s, b, matrices, steps, stream);
+  // The squares of wide matrices in the tiles whose rounds are shorter: 128 x 128, two
+  // a CU, take 1.15 times as long for their area (128 of 1024 x 1024 237 us for 227 in
+  // 9 rounds of half a wide one's for 5 of those; 64 of them 117 for 129, 5 for 3).
+  int cus = 0;
+  if (const int rc = device_cus(&cus)) return rc;
+  auto rounds = [&](int64_t tile, int64_t at_once) {
+    const int64_t n = s.mp / tile;
+    return (matrices * n * (n + 1) / 2 + at_once - 1) / at_once;
+  };
+  return 23 * rounds(128, int64_t{2} * cus) < 40 * rounds(256, cus)
+             ? run_steps<WideGram, WideSquare, WideRows>(t, h, s, b, matrices, steps, stream)
+             : run_steps<WideGram, WideRows, WideRows>(t, h, s, b, matrices, steps, stream);
 }
 
 bool known_dtype(int64_t d) { return d == SB_DTYPE_BF16 || d == SB_DTYPE_F16 || d == SB_DTYPE_F32; }
