@@ -583,6 +583,113 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1) symmetric_kernel(ProductArgs
   });
 }
 
+// A and what follows from it for matrices of one tile, a workgroup each: the squares
+// stay in LDS, fp16 beside the diagonals as everywhere. out = B of one step, or the
+// factor of X in two (run_steps), in place of 2 or 6 launches: three of 40 x 1001 63 us
+// for 78, one of 64 x 4096 93 : 106, 1000 of 64 x 256 179 : 217. One LDS array: with a
+// second one the compiler lets every read in the main loop wait for all loads (one of
+// 64 x 4096: 177). Matrices of 128 lose: a workgroup's product of 128^3 takes 3 us.
+template <class Cfg>
+__device__ __forceinline__ void chain(uint8_t* __restrict__ lds, const typename DmaMainloop<Cfg>::Acc& gram,
+                                      const Symmetric& result, int64_t matrix, int32_t two) {
+  using ML = DmaMainloop<Cfg>;
+  constexpr int N = Cfg::BM, kBytes = N * N * 2;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int row0 = wave / Cfg::WN * Cfg::WTM + (lane & 31), col0 = wave % Cfg::WN * Cfg::WTN + (lane & 31);
+  auto scale_of = [](int of) { return of == 2 ? kScale / 4 : kScale; };
+  auto diag = [&](int of, int r) -> float& { return reinterpret_cast<float*>(lds + 4 * kBytes)[of * N + r]; };
+  // Where columns c .. of row r of square `of` are: chunks of 8 halves, turned by the row.
+  auto at = [&](int of, int r, int c) {
+    return lds + of * kBytes + r * (2 * N) + (((c >> 3) ^ ((r ^ (r >> 3)) & 7)) << 4) + (c & 7) * 2;
+  };
+  // Square `to`, from fn(row, first of four columns, the accumulators' values).
+  auto store = [&](int to, const typename ML::Acc& acc, auto fn) {
+    const float scale = scale_of(to);
+#pragma unroll
+    for (int i = 0; i < Cfg::TM; ++i)
+#pragma unroll
+      for (int j = 0; j < Cfg::TN; ++j)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const int row = row0 + 32 * i, col = ML::out_col(j, g);
+          float v[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = acc[j][i][4 * g + e];
+          fn(row, col, v);
+          uint16_t bits[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            bits[e] = half_bits(v[e] * scale);
+            if (row == col + e) diag(to, row) = v[e], bits[e] = 0;
+          }
+          *reinterpret_cast<u32x2_t*>(at(to, row, col)) =
+              u32x2_t{bits[0] | static_cast<uint32_t>(bits[1]) << 16, bits[2] | static_cast<uint32_t>(bits[3]) << 16};
+        }
+    __syncthreads();
+  };
+  // to = of_l L + of_r R + of_lr L R, as symmetric_kernel; `to` is another square than both.
+  auto multiply = [&](int l, int r, int to, float of_l, float of_r, float of_lr) {
+    typename ML::Acc acc = {};
+#pragma unroll
+    for (int k0 = 0; k0 < N; k0 += 16) {
+      const int k = k0 + 8 * (lane >> 5);
+      bf16x8_t a[Cfg::TM], b[Cfg::TN];
+#pragma unroll
+      for (int i = 0; i < Cfg::TM; ++i) a[i] = *reinterpret_cast<const bf16x8_t*>(at(l, row0 + 32 * i, k));
+#pragma unroll
+      for (int j = 0; j < Cfg::TN; ++j) b[j] = *reinterpret_cast<const bf16x8_t*>(at(r, col0 + 32 * j, k));
+#pragma unroll
+      for (int j = 0; j < Cfg::TN; ++j)
+#pragma unroll
+        for (int i = 0; i < Cfg::TM; ++i) acc[j][i] = ML::mfma(b[j], a[i], acc[j][i]);
+    }
+    const float ls = 1.0f / scale_of(l), rs = 1.0f / scale_of(r), unit = of_lr * ls * rs;
+    store(to, acc, [&](int row, int col, float (&v)[4]) {
+      const u32x2_t o = *reinterpret_cast<const u32x2_t*>(at(l, row, col)), s = *reinterpret_cast<const u32x2_t*>(at(r, row, col));
+      const float ld = diag(l, row), rd = diag(r, row);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float oe = value_of(static_cast<uint16_t>(o[e / 2] >> (16 * (e & 1))), SB_DTYPE_F16) * ls;
+        const float se = value_of(static_cast<uint16_t>(s[e / 2] >> (16 * (e & 1))), SB_DTYPE_F16) * rs;
+        v[e] *= unit;
+        if (row == col + e) v[e] += of_l * ld + of_r * rd + of_lr * (ld * rd);
+        else v[e] += (of_r + of_lr * ld) * se + (of_l + of_lr * diag(r, col + e)) * oe;
+      }
+    });
+  };
+  __syncthreads();
+  store(0, gram, [&](int, int, float (&v)[4]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] *= kUnscale * kUnscale;
+  });
+  // B; then 2 a5 B + B^2, the next A and its B, and the factor of both steps. One copy
+  // of the product's code, since a launch fetches every line of it anew.
+#pragma unroll 1
+  for (int i = 0; i < (two ? 5 : 1); ++i) {
+    const int l = i == 4 ? 0 : i, r = i == 2 ? 0 : i == 4 ? 1 : i, to = i == 4 ? 2 : (i + 1) & 3;
+    const bool poly = i == 0 || i == 3;
+    multiply(l, r, to, poly ? kB5 : i == 1 ? 2.0f * kA5 : i == 2 ? 0.0f : kA5, i == 2 ? kA5 * kA5 : i == 4 ? kA5 : 0.0f,
+             poly ? kC5 : 1.0f);
+  }
+  const int out = two ? 2 : 1;
+  for (int i = threadIdx.x; i < N * N / 8; i += Cfg::kThreads) {
+    const int r = i / (N / 8), c = i % (N / 8) * 8;
+    *reinterpret_cast<u32x4_t*>(result.off + matrix * N * N + r * N + c) = *reinterpret_cast<const u32x4_t*>(at(out, r, c));
+  }
+  for (int i = threadIdx.x; i < N; i += Cfg::kThreads) result.diag[matrix * N + i] = diag(out, i);
+}
+
+template <class Cfg>
+__global__ void __launch_bounds__(Cfg::kThreads, 1) chain_kernel(ProductArgs p, int32_t two) {
+  static_assert(Cfg::BN == Cfg::BM && Cfg::F16 && Cfg::kLdsAlloc >= 4 * Cfg::BM * (Cfg::BM * 2 + 4));  // squares, diagonals
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[Cfg::kLdsAlloc];
+  const int64_t matrix = blockIdx.x;
+  typename DmaMainloop<Cfg>::Acc acc;
+  const uint16_t* x = p.x + matrix * p.mp * p.np;
+  product<Cfg>(lds, x, x, p.mp, p.np, p.mp, 0, 0, acc);
+  chain<Cfg>(lds, acc, p.out, matrix, two);
+}
+
 // next, lo = of_right X + L X: of X's own rows of_right and L's diagonal.
 template <class Cfg>
 __global__ void __launch_bounds__(Cfg::kThreads, 1) update_kernel(ProductArgs p) {
@@ -710,6 +817,7 @@ struct Shape {
   int64_t m, n;
   int64_t mp, np;
   int tile;  // 256, 128 or 64
+  bool chain;  // chain_kernel
   int32_t vectors;  // a lane's of a chunk
   bool pairs;
   int64_t most;  // matrices of a batch
@@ -745,8 +853,9 @@ Shape shape_of(int64_t rows, int64_t columns, int64_t matrices, int cus) {
   // Two steps at a time (run_steps) where X is long, and not so little that launches
   // count: 24 of 256 x 512 would take 117 us for 112, 16 of 512 x 2048 take 335 for 404,
   // 1 of 128 x 4096 121 for 140.
+  s.chain = s.tile == 64 && s.m <= 64;
   s.pairs = s.n >= 2 * s.m &&
-            (s.n >= 2048 || matrices * (round_up(s.m, 64) / 64) * (round_up(s.n, 64) / 64) >= int64_t{4} * cus);
+            (s.chain || s.n >= 2048 || matrices * (round_up(s.m, 64) / 64) * (round_up(s.n, 64) / 64) >= int64_t{4} * cus);
   s.mp = round_up(s.m, s.tile);
   s.np = round_up(s.n, s.tile);
   // Shorter chunks where they are few (24 of 256 x 512, 192 chunks of 8 vectors: 13.5 us).
@@ -772,7 +881,7 @@ Buffers carve(void* workspace, const Shape& s, int64_t matrices) {
   b.hi[0] = ws.take<uint16_t>(matrices * s.mp * s.np);
   b.hi[1] = ws.take<uint16_t>(matrices * s.mp * s.np);
   b.lo = ws.take<uint16_t>(matrices * s.mp * s.np);
-  for (int i = 0; i < (s.pairs ? 4 : 2); ++i) {
+  for (int i = 0; i < (s.pairs && !s.chain ? 4 : 2); ++i) {
     b.square[i].off = ws.take<uint16_t>(matrices * s.mp * s.mp);
     b.square[i].diag = ws.take<float>(matrices * s.mp);
   }
@@ -791,7 +900,7 @@ int64_t batch_bytes(const Shape& s, int64_t matrices) { return carve(nullptr, s,
 // n is 2 m or more; the last step is taken alone, where an error has the same weight
 // whichever way (n = 2 m: 0.07% of the result against 0.06%, by the norms; n < 2 m
 // would lose more, square ones 0.14% against 0.07%).
-template <class Gram, class Square, class Rows>
+template <class Gram, class Square, class Rows, bool CHAIN = false>
 int run_steps(const Table& table, const Hyper& h, const Shape& s, const Buffers& b, int64_t matrices, int32_t steps,
               hipStream_t stream) {
   if (!reduction_fits<Gram>(s.np) || !reduction_fits<Square>(s.mp) || !reduction_fits<Rows>(s.mp))
@@ -817,24 +926,29 @@ int run_steps(const Table& table, const Hyper& h, const Shape& s, const Buffers&
     p.x = b.hi[at];
     p.next = b.hi[at ^ 1];
     const Symmetric a = scaled(0, kScale), poly = scaled(1, kScale);
-    p.out = a;
-    symmetric_kernel<Gram, true><<<static_cast<uint32_t>(upper(Gram::BM)), Gram::kThreads, 0, stream>>>(p);
-    if (const int rc = check_launch("orthogonalise: X X^T")) return rc;
-    if (const int rc = multiply(a, a, poly, kB5, 0.0f, kC5)) return rc;
     Symmetric factor = poly;
-    float own = kA5;
-    if (two) {
-      // |2 a5 B + B^2| and |P' P - a5^2| stay under 11.9.
-      const Symmetric wide = scaled(2, kScale / 4), next_a = scaled(3, kScale), next_poly = scaled(0, kScale);
-      if (const int rc = multiply(poly, poly, wide, 2.0f * kA5, 0.0f, 1.0f)) return rc;
-      if (const int rc = multiply(wide, a, next_a, 0.0f, kA5 * kA5, 1.0f)) return rc;
-      if (const int rc = multiply(next_a, next_a, next_poly, kB5, 0.0f, kC5)) return rc;
-      if (const int rc = multiply(next_poly, poly, wide, kA5, kA5, 1.0f)) return rc;
-      factor = wide;
-      own = kA5 * kA5;
+    if constexpr (CHAIN) {
+      factor = scaled(0, two ? kScale / 4 : kScale);
+      p.out = factor;
+      chain_kernel<Gram><<<static_cast<uint32_t>(matrices), Gram::kThreads, 0, stream>>>(p, two);
+      if (const int rc = check_launch("orthogonalise: A")) return rc;
+    } else {
+      p.out = a;
+      symmetric_kernel<Gram, true><<<static_cast<uint32_t>(upper(Gram::BM)), Gram::kThreads, 0, stream>>>(p);
+      if (const int rc = check_launch("orthogonalise: X X^T")) return rc;
+      if (const int rc = multiply(a, a, poly, kB5, 0.0f, kC5)) return rc;
+      if (two) {
+        // |2 a5 B + B^2| and |P' P - a5^2| stay under 11.9.
+        const Symmetric wide = scaled(2, kScale / 4), next_a = scaled(3, kScale), next_poly = scaled(0, kScale);
+        if (const int rc = multiply(poly, poly, wide, 2.0f * kA5, 0.0f, 1.0f)) return rc;
+        if (const int rc = multiply(wide, a, next_a, 0.0f, kA5 * kA5, 1.0f)) return rc;
+        if (const int rc = multiply(next_a, next_a, next_poly, kB5, 0.0f, kC5)) return rc;
+        if (const int rc = multiply(next_poly, poly, wide, kA5, kA5, 1.0f)) return rc;
+        factor = wide;
+      }
     }
     p.left = factor;
-    p.of_right = own;
+    p.of_right = two ? kA5 * kA5 : kA5;
     at ^= 1;
     done += two ? 2 : 1;
     if (done < steps) update_kernel<Rows><<<static_cast<uint32_t>(all), Rows::kThreads, 0, stream>>>(p);
@@ -861,6 +975,7 @@ int run_batch(const Table& t, const Hyper& h, const Shape& s, int64_t matrices, 
   fill_kernel<<<dim3(static_cast<uint32_t>(tiles), y), kThreads, 0, stream>>>(t, h, b.partial, static_cast<int32_t>(chunks),
                                                                             b.factor, first);
   if (const int rc = check_launch("orthogonalise: fill")) return rc;
+  if (s.chain) return run_steps<SmallGram, SmallRows, SmallRows, true>(t, h, s, b, matrices, steps, stream);
   if (s.tile == 64) return run_steps<SmallGram, SmallRows, SmallRows>(t, h, s, b, matrices, steps, stream);
   if (s.tile == 128) return run_steps<NarrowGram, NarrowRows, NarrowRows>(t, h, s, b, matrices, steps, stream);
   // The squares of wide matrices in the tiles whose rounds are shorter: 128 x 128, two
