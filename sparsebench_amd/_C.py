@@ -671,7 +671,7 @@ _HERE = contextlib.nullcontext()
 
 def _device_of(t: torch.Tensor) -> contextlib.AbstractContextManager:
     """Makes t's device current for a launch, where it is not."""
-    return _HERE if t.get_device() == torch.cuda.current_device() else torch.cuda.device(t.device)
+    return _HERE if t.get_device() == torch._C._cuda_getDevice() else torch.cuda.device(t.device)
 
 
 @functools.lru_cache(maxsize=256)
@@ -931,6 +931,11 @@ def _check_rows(t: torch.Tensor, name: str, like: torch.Tensor | None = None) ->
         _fail(f"rows must have 1 to {_NORM_MAX_D} values, got {shape[1]}")
 
 
+def _new_rows(like: torch.Tensor) -> torch.Tensor:
+    """Contiguous, of like's shape and type (empty_like takes half of empty's 1.9 us, but keeps strides)."""
+    return torch.empty_like(like) if like.is_contiguous() else torch.empty(like.shape, dtype=like.dtype, device=like.device)
+
+
 def _check_vector(t: torch.Tensor | None, name: str, like: torch.Tensor) -> int:
     """Its dtype's code."""
     if t is None:
@@ -971,7 +976,7 @@ def norm_in_cuda(x: torch.Tensor, weight: torch.Tensor | None, eps: float,
     _check_rows(x, "x")
     weight_code = _check_vector(weight, "weight", x)
     _check_norm(eps, valid_tokens, x)
-    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    out = _new_rows(x)
     with _device_of(x):
         check(lib().sb_norm_in(x.data_ptr(), x.stride(0), _ptr(weight), weight_code, out.data_ptr(),
                                _GATE_DTYPES[x.dtype], *x.shape, eps, _ptr(valid_tokens), stream_of(x.device)))
@@ -987,7 +992,7 @@ def norm_out_cuda(y: torch.Tensor, x: torch.Tensor, weight: torch.Tensor | None,
     weight_code, next_code = _check_vector(weight, "weight", x), _check_vector(next_weight, "next_weight", x)
     gate_code, kind, gate_stride = _check_norm_gate(gate, x)
     _check_norm(eps, valid_tokens, x)
-    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    out = _new_rows(x)
     following = None if next_weight is None else torch.empty_like(out)
     with _device_of(x):
         check(lib().sb_norm_out(
@@ -1019,7 +1024,7 @@ def norm_in_backward_cuda(grad: torch.Tensor, x: torch.Tensor, weight: torch.Ten
         _check_rows(grad_x, "grad_x", x)
     weight_code = _check_vector(weight, "weight", x)
     _check_norm(eps, valid_tokens, x)
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    dx = _new_rows(x)
     if x.shape[0] == 0:  # sums of nothing
         return dx, None if weight is None else torch.zeros_like(weight)
     dweight = None if weight is None else torch.empty_like(weight)
@@ -1048,12 +1053,11 @@ def norm_out_backward_cuda(grad_out: torch.Tensor, y: torch.Tensor, weight: torc
     weight_code, next_code = _check_vector(weight, "weight", y), _check_vector(next_weight, "next_weight", y)
     gate_code, kind, gate_stride = _check_norm_gate(gate, y)
     _check_norm(eps, valid_tokens, y)
-    opts = {"dtype": y.dtype, "device": y.device}
     if y.shape[0] == 0:  # sums of nothing
         return (torch.empty_like(y), grad_out, *(None if w is None else torch.zeros_like(w)
                                                  for w in (weight, gate, next_weight)))
-    dy = torch.empty(y.shape, **opts)
-    dx = None if grad_next is None else torch.empty(y.shape, **opts)
+    dy = _new_rows(y)
+    dx = None if grad_next is None else _new_rows(y)
     dweight, dnext = (None if w is None else torch.empty_like(w) for w in (weight, next_weight))
     dgate = None if gate is None else torch.empty(gate.shape, dtype=gate.dtype, device=gate.device)
     following = out if grad_next is not None else None
