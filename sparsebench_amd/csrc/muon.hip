@@ -850,9 +850,8 @@ Shape shape_of(int64_t rows, int64_t columns, int64_t matrices, int cus) {
   if (s.m > 512 && 2 * padded(256) <= 3 * padded(64) && 2 * steps_of_a(256) >= int64_t{9} * cus) s.tile = 256;
   else if (steps_of_a(64) <= int64_t{32} * cus || 4 * padded(64) <= 3 * padded(128)) s.tile = 64;
   else s.tile = 128;
-  // Two steps at a time (run_steps) where X is long, and not so little that launches
-  // count: 24 of 256 x 512 would take 117 us for 112, 16 of 512 x 2048 take 335 for 404,
-  // 1 of 128 x 4096 121 for 140.
+  // The first two steps at a time (run_steps) where X is long, and not so little that
+  // launches count: 16 of 512 x 2048 take 395 us for 404, 1 of 128 x 4096 135 for 140.
   s.chain = s.tile == 64 && s.m <= 64;
   s.pairs = s.n >= 2 * s.m &&
             (s.chain || s.n >= 2048 || matrices * (round_up(s.m, 64) / 64) * (round_up(s.n, 64) / 64) >= int64_t{4} * cus);
@@ -895,11 +894,14 @@ int64_t batch_bytes(const Shape& s, int64_t matrices) { return carve(nullptr, s,
 
 // The steps, one or two at a time. Two: with P = a5 + B of A = X X^T, the next
 // step's A is P A P = a5^2 A + (2 a5 B + B^2) A, and both steps' factor of X is
-// P' P = a5^2 + (a5 B + a5 B' + B' B): six products of m^3 (half of each) in place of
-// one X X^T and one B X of m^2 n, and of X's passage through memory. Worth it where
-// n is 2 m or more; the last step is taken alone, where an error has the same weight
-// whichever way (n = 2 m: 0.07% of the result against 0.06%, by the norms; n < 2 m
-// would lose more, square ones 0.14% against 0.07%).
+// P' P = a5^2 + (a5 B + a5 B' + B' B): five products of m^3 (half of each) for two, in
+// place of one X X^T and one B X of m^2 n and of X's passage through memory. Worth it
+// where n is 2 m or more, and only for the first two steps: the factor's entries beside
+// the diagonal are those of P' P, up to 11.9 in size where B's are 2.8, and so is their
+// rounding. While the singular values' squares add up to 1, few are large enough for
+// that to count (256 x 512, over spectra of decades and steps: 0.27% of the result, as
+// with single steps). In the next two it does (0.74%; 0.69% measured for 300 x 700, a
+// quarter of the singular values ten times the others). chain_kernel still takes every pair.
 template <class Gram, class Square, class Rows, bool CHAIN = false>
 int run_steps(const Table& table, const Hyper& h, const Shape& s, const Buffers& b, int64_t matrices, int32_t steps,
               hipStream_t stream) {
@@ -922,7 +924,7 @@ int run_steps(const Table& table, const Hyper& h, const Shape& s, const Buffers&
   };
   int at = 0;
   for (int32_t done = 0; done < steps;) {
-    const bool two = s.pairs && steps - done >= 3;
+    const bool two = s.pairs && (CHAIN || done == 0) && steps - done >= 3;
     p.x = b.hi[at];
     p.next = b.hi[at ^ 1];
     const Symmetric a = scaled(0, kScale), poly = scaled(1, kScale);

@@ -1,0 +1,86 @@
+"""Orthogonalised updates of matrices with prescribed singular values: a few strong directions
+over weak ones, values spread over decades, nearly low rank.
+
+Tolerance for up to five steps: 0.4%, as for other gradients (test_muon_gpu.PRODUCTS). In a step
+the entries of A and B beside the diagonal are rounded to fp16, 2^-11 of each at most and
+independent; |b s + c s^2| <= 2.81 is B's size, and a noise of that size in B times X is
+2.81 * 2^-11 / sqrt(3) of |X|: five of them 0.4%. It must not depend on where the singular values
+lie:
+
+- Two steps taken as one have a factor of up to 11.9 in 2.81's place. For the first two the singular
+  values' squares add up to 1, so that the factor's entries do not: |W|_F^2 <= sum_k min(11.9, 211
+  s_k^2)^2 <= 11.9 * 211, and its noise 50 / sqrt(m) * 2^-11 / sqrt(3): less than two single steps'
+  from 80 rows on, and within 5% of the whole from 65.
+- X's roundings must reach both terms of a X + B X alike, or what B X lacks grows with X's weak
+  directions; the test's spectra go down to 1e-4 of the largest value.
+- Up to 64 rows do not average, and there the roundings' remainders are kept; what is left is X X^T
+  of X rounded to fp16, whose n products a value average: 4.8 * 2 * 2^-11 / sqrt(3 n) a step, 0.17%
+  in five steps for n > 64. Up to n = 64 nothing is left but fp32's and 2^-22's roundings: five steps
+  of 2.81 * 2^-22 that grow up to 3.44^4-fold, and X's own of 2^-22: 0.1% is ample.
+
+Beyond five steps the polynomial's slope is taken by the singular values that it wanders through:
+between 0.68 and 1.21 it lies in [-1.6, 4.1], 1.9 in quadratic mean over that range, for errors along
+X itself, and 1 for all others (the divided differences of two values with opposite signs): 1.5 a step
+covers it.
+"""
+
+import pytest
+import torch
+
+from sparsebench_amd import optim
+from tests.test_muon_gpu import PRODUCTS, newton_schulz, step_reference
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda"
+
+
+def share(m, part, small):
+    return torch.where(torch.arange(m) < max(1, int(part * m)), 1.0, small).double()
+
+
+SPECTRA = {
+    "spread over 1e-2": lambda m: 10 ** (-2 * torch.arange(m) / max(1, m - 1)).double(),
+    "spread over 1e-4": lambda m: 10 ** (-4 * torch.arange(m) / max(1, m - 1)).double(),
+    "half 0.01": lambda m: share(m, 0.5, 0.01),
+    "half 1e-3": lambda m: share(m, 0.5, 1e-3),
+    "half 1e-4": lambda m: share(m, 0.5, 1e-4),
+    "quarter 0.1": lambda m: share(m, 0.25, 0.1),
+    "quarter 1e-3": lambda m: share(m, 0.25, 1e-3),
+    "twentieth 0.1": lambda m: share(m, 0.05, 0.1),
+    "one 1e-3": lambda m: share(m, 0.0, 1e-3),
+}
+
+
+def matrices(count, rows, columns, spectrum, seed=0, scale=1e-3):
+    """[count, rows, columns] fp32 with the spectrum's singular values; up to three differ."""
+    g = torch.Generator().manual_seed(seed)
+    m, n = min(rows, columns), max(rows, columns)
+
+    def orthogonal(size):
+        return torch.linalg.qr(torch.randn(min(count, 3), size, m, generator=g, dtype=torch.float64))[0]
+
+    x = (orthogonal(m) * (scale * SPECTRA[spectrum](m))) @ orthogonal(n).mT
+    x = x if rows <= columns else x.mT
+    return x[torch.arange(count) % len(x)].float().contiguous().to(DEV)
+
+
+def tolerance(u, steps=5):
+    few = max(u.shape[-2:]) <= 64
+    return (1e-3 if few else PRODUCTS) * 1.5 ** max(0, steps - 5)
+
+
+def check(got, want, tol):
+    for g, w in zip(got.double(), want):
+        assert (g - w).norm() <= tol * w.norm(), ((g - w).norm() / w.norm()).item()
+
+
+# Wide, narrow and small tiles; n >= 2 m (two steps at a time) and less.
+LARGE = [(64, 520, 1100), (64, 640, 640), (60, 300, 700), (3, 400, 1024), (2, 1024, 300)]
+
+
+@pytest.mark.parametrize("spectrum", SPECTRA)
+@pytest.mark.parametrize("size", LARGE)
+def test_two_steps_at_a_time(size, spectrum) -> None:
+    u = matrices(*size, spectrum, seed=1)
+    check(optim.orthogonalize(u), newton_schulz(u), tolerance(u))
