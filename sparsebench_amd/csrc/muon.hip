@@ -323,39 +323,46 @@ struct Symmetric {
 };
 
 struct ProductArgs {
-  const uint16_t* x;  // [M][mp][np], hi
-  uint16_t* lo;       // of x, updated in place
-  uint16_t* next;     // hi of the next X
+  const uint16_t *x, *lo;     // [M][mp][np]
+  uint16_t *next, *next_lo;   // of the next X; next_lo may be lo where products do not read that
   Symmetric left, right, out;
   float of_left, of_right, of_product;  // out = of_left L + of_right R + of_product L R
   int32_t mp, np, matrices;
 };
 
-template <class Cfg>
+// PARTS products one after another into one sum: a b, then a times what b's rounding left.
+template <class Cfg, int PARTS>
 struct Operands {
-  __amdgpu_buffer_rsrc_t ra, rb;
+  __amdgpu_buffer_rsrc_t ra, rb, rb_rest;
   uint32_t a_off[Cfg::kAInstr], b_off[Cfg::kBInstr];
   uint32_t a_step, b_step;
+  int steps;  // of a part
   __device__ __forceinline__ uint32_t a_voff(int q) const { return a_off[q]; }
   __device__ __forceinline__ uint32_t b_voff(int q) const { return b_off[q]; }
+  __device__ __forceinline__ uint32_t step_of(int t) const {
+    return static_cast<uint32_t>(PARTS > 1 && t >= steps ? t - steps : t);
+  }
   __device__ __forceinline__ void a_src(int t, __amdgpu_buffer_rsrc_t* r, uint32_t* s) const {
     *r = ra;
-    *s = static_cast<uint32_t>(t) * a_step;
+    *s = step_of(t) * a_step;
   }
   __device__ __forceinline__ void b_src(int t, __amdgpu_buffer_rsrc_t* r, uint32_t* s) const {
-    *r = rb;
-    *s = static_cast<uint32_t>(t) * b_step;
+    *r = PARTS > 1 && t >= steps ? rb_rest : rb;
+    *s = step_of(t) * b_step;
   }
 };
 
-// C rows i0 .., columns j0 .. of a [mp, k] times b: [k, columns], or with BT
-// the rows of b [columns, k].
-template <class Cfg>
-__device__ __forceinline__ void product(uint8_t* __restrict__ lds, const uint16_t* a, const uint16_t* b, int mp, int k,
-                                        int columns, int i0, int j0, typename DmaMainloop<Cfg>::Acc& acc) {
-  Operands<Cfg> src;
+// C rows i0 .., columns j0 .. of a [mp, k] times b (and b_rest): [k, columns], or with
+// BT the rows of b [columns, k].
+template <class Cfg, int PARTS = 1>
+__device__ __forceinline__ void product(uint8_t* __restrict__ lds, const uint16_t* a, const uint16_t* b,
+                                        const uint16_t* b_rest, int mp, int k, int columns, int i0, int j0,
+                                        typename DmaMainloop<Cfg>::Acc& acc) {
+  Operands<Cfg, PARTS> src;
   src.ra = make_rsrc(a, static_cast<uint32_t>(mp) * static_cast<uint32_t>(k) * 2u);
   src.rb = make_rsrc(b, static_cast<uint32_t>(columns) * static_cast<uint32_t>(k) * 2u);
+  if constexpr (PARTS > 1) src.rb_rest = make_rsrc(b_rest, static_cast<uint32_t>(columns) * static_cast<uint32_t>(k) * 2u);
+  src.steps = k / Cfg::BK;
   const ADmaPos<Cfg> ap;
 #pragma unroll
   for (int q = 0; q < Cfg::kAInstr; ++q)
@@ -374,7 +381,7 @@ __device__ __forceinline__ void product(uint8_t* __restrict__ lds, const uint16_
       src.b_off[q] = (static_cast<uint32_t>(bp.row[q]) * static_cast<uint32_t>(columns) + j0 + bp.col[q]) * 2u;
     src.b_step = Cfg::BK * static_cast<uint32_t>(columns) * 2u;
   }
-  DmaMainloop<Cfg>::run(lds, src, k / Cfg::BK, acc);
+  DmaMainloop<Cfg>::run(lds, src, PARTS * src.steps, acc);
 }
 
 // The accumulators in fp32 through LDS, kGroups groups of 32 rows of each row of
@@ -523,10 +530,10 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1) symmetric_kernel(ProductArgs
   float unit;  // of the accumulators
   if constexpr (GRAM) {
     const uint16_t* x = p.x + matrix * p.mp * p.np;
-    product<Cfg>(lds, x, x, p.mp, p.np, p.mp, i0, j0, acc);
+    product<Cfg>(lds, x, x, nullptr, p.mp, p.np, p.mp, i0, j0, acc);
     unit = kUnscale * kUnscale;
   } else {
-    product<Cfg>(lds, p.left.off + square, p.right.off + square, p.mp, p.mp, p.mp, i0, j0, acc);
+    product<Cfg>(lds, p.left.off + square, p.right.off + square, nullptr, p.mp, p.mp, p.mp, i0, j0, acc);
     unit = p.of_product / (p.left.scale * p.right.scale);
   }
   const float scale = p.out.scale;
@@ -686,12 +693,13 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1) chain_kernel(ProductArgs p, 
   const int64_t matrix = blockIdx.x;
   typename DmaMainloop<Cfg>::Acc acc;
   const uint16_t* x = p.x + matrix * p.mp * p.np;
-  product<Cfg>(lds, x, x, p.mp, p.np, p.mp, 0, 0, acc);
+  product<Cfg>(lds, x, x, nullptr, p.mp, p.np, p.mp, 0, 0, acc);
   chain<Cfg>(lds, acc, p.out, matrix, two);
 }
 
-// next, lo = of_right X + L X: of X's own rows of_right and L's diagonal.
-template <class Cfg>
+// next, next_lo = of_right X + L X: of X's own rows of_right and L's diagonal. PARTS 2:
+// L times X's remainder too (run_batch says where).
+template <class Cfg, int PARTS>
 __global__ void __launch_bounds__(Cfg::kThreads, 1) update_kernel(ProductArgs p) {
   using ML = DmaMainloop<Cfg>;
   using Ep = Epilogue<Cfg>;
@@ -702,7 +710,7 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1) update_kernel(ProductArgs p)
   const int i0 = uniform(at % per % mt) * Cfg::BM, j0 = uniform(at % per / mt) * Cfg::BN;
   const int64_t whole = matrix * p.mp * p.np, tile = whole + static_cast<int64_t>(i0) * p.np + j0;
   typename ML::Acc acc;
-  product<Cfg>(lds, p.left.off + matrix * p.mp * p.mp, p.x + whole, p.mp, p.mp, p.np, i0, j0, acc);
+  product<Cfg, PARTS>(lds, p.left.off + matrix * p.mp * p.mp, p.x + whole, p.lo + whole, p.mp, p.mp, p.np, i0, j0, acc);
   const float unit = 1.0f / p.left.scale;
   static_for<0, Ep::kParts>([&](auto part) {
     constexpr int P = decltype(part)::value;
@@ -723,7 +731,7 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1) update_kernel(ProductArgs p)
         lo[q] = half_bits(y - value_of(hi[q], SB_DTYPE_F16));
       }
       *reinterpret_cast<u32x4_t*>(p.next + place) = pack8(hi);
-      *reinterpret_cast<u32x4_t*>(p.lo + place) = pack8(lo);
+      *reinterpret_cast<u32x4_t*>(p.next_lo + place) = pack8(lo);
       return u32x4_t{};
     });
   });
@@ -731,7 +739,7 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1) update_kernel(ProductArgs p)
 
 // The last step, with the weights' step in its place (apply): w = keep w - size X;
 // without a momentum X itself.
-template <class Cfg>
+template <class Cfg, int PARTS>
 __global__ void __launch_bounds__(Cfg::kThreads, 1) last_kernel(ProductArgs p, Table t, Hyper h) {
   using ML = DmaMainloop<Cfg>;
   using Ep = Epilogue<Cfg, 1>;  // the weights take the registers of the other rows
@@ -740,12 +748,12 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1) last_kernel(ProductArgs p, T
   const int at = xcd_remap(static_cast<int>(blockIdx.x), per * p.matrices);
   const int matrix = uniform(at / per);
   const int i0 = uniform(at % per % mt) * Cfg::BM, j0 = uniform(at % per / mt) * Cfg::BN;
-  const int64_t tile = static_cast<int64_t>(matrix) * p.mp * p.np + static_cast<int64_t>(i0) * p.np + j0;
+  const int64_t whole = static_cast<int64_t>(matrix) * p.mp * p.np, tile = whole + static_cast<int64_t>(i0) * p.np + j0;
   int64_t place;
   const Entry e = entry_of(t, matrix, &place);
   typename ML::Acc acc;
-  product<Cfg>(lds, p.left.off + static_cast<int64_t>(matrix) * p.mp * p.mp, p.x + static_cast<int64_t>(matrix) * p.mp * p.np,
-               p.mp, p.mp, p.np, i0, j0, acc);
+  product<Cfg, PARTS>(lds, p.left.off + static_cast<int64_t>(matrix) * p.mp * p.mp, p.x + whole, p.lo + whole, p.mp, p.mp,
+                      p.np, i0, j0, acc);
   const float unit = 1.0f / p.left.scale;
   const float lr = h.lr_ptr ? *h.lr_ptr : h.lr;
   const float keep = 1.0f - lr * h.weight_decay;
@@ -867,7 +875,7 @@ Shape shape_of(int64_t rows, int64_t columns, int64_t matrices, int cus) {
 }
 
 struct Buffers {
-  uint16_t *hi[2], *lo;
+  uint16_t *hi[2], *lo[2];
   Symmetric square[4];
   double* partial;
   float* factor;
@@ -879,7 +887,8 @@ Buffers carve(void* workspace, const Shape& s, int64_t matrices) {
   Buffers b;
   b.hi[0] = ws.take<uint16_t>(matrices * s.mp * s.np);
   b.hi[1] = ws.take<uint16_t>(matrices * s.mp * s.np);
-  b.lo = ws.take<uint16_t>(matrices * s.mp * s.np);
+  b.lo[0] = ws.take<uint16_t>(matrices * s.mp * s.np);
+  b.lo[1] = ws.take<uint16_t>(matrices * s.mp * s.np);  // read by more steps than sizes are asked for
   for (int i = 0; i < (s.pairs && !s.chain ? 4 : 2); ++i) {
     b.square[i].off = ws.take<uint16_t>(matrices * s.mp * s.mp);
     b.square[i].diag = ws.take<float>(matrices * s.mp);
@@ -902,7 +911,7 @@ int64_t batch_bytes(const Shape& s, int64_t matrices) { return carve(nullptr, s,
 // that to count (256 x 512, over spectra of decades and steps: 0.27% of the result, as
 // with single steps). In the next two it does (0.74%; 0.69% measured for 300 x 700, a
 // quarter of the singular values ten times the others). chain_kernel still takes every pair.
-template <class Gram, class Square, class Rows, bool CHAIN = false>
+template <class Gram, class Square, class Rows, int PARTS, bool CHAIN = false>
 int run_steps(const Table& table, const Hyper& h, const Shape& s, const Buffers& b, int64_t matrices, int32_t steps,
               hipStream_t stream) {
   if (!reduction_fits<Gram>(s.np) || !reduction_fits<Square>(s.mp) || !reduction_fits<Rows>(s.mp))
@@ -911,7 +920,6 @@ int run_steps(const Table& table, const Hyper& h, const Shape& s, const Buffers&
   const int64_t all = matrices * (s.mp / Rows::BM) * (s.np / Rows::BN);
   if (all > 2147483647LL || upper(Square::BM) > 2147483647LL) return fail(SB_ERR_INVALID, "orthogonalise: problem too large");
   ProductArgs p{};
-  p.lo = b.lo;
   p.mp = static_cast<int32_t>(s.mp);
   p.np = static_cast<int32_t>(s.np);
   p.matrices = static_cast<int32_t>(matrices);
@@ -927,6 +935,8 @@ int run_steps(const Table& table, const Hyper& h, const Shape& s, const Buffers&
     const bool two = s.pairs && (CHAIN || done == 0) && steps - done >= 3;
     p.x = b.hi[at];
     p.next = b.hi[at ^ 1];
+    p.lo = b.lo[PARTS > 1 ? at : 0];
+    p.next_lo = b.lo[PARTS > 1 ? at ^ 1 : 0];
     const Symmetric a = scaled(0, kScale), poly = scaled(1, kScale);
     Symmetric factor = poly;
     if constexpr (CHAIN) {
@@ -953,12 +963,20 @@ int run_steps(const Table& table, const Hyper& h, const Shape& s, const Buffers&
     p.of_right = two ? kA5 * kA5 : kA5;
     at ^= 1;
     done += two ? 2 : 1;
-    if (done < steps) update_kernel<Rows><<<static_cast<uint32_t>(all), Rows::kThreads, 0, stream>>>(p);
-    else last_kernel<Rows><<<static_cast<uint32_t>(all), Rows::kThreads, 0, stream>>>(p, table, h);
+    if (done < steps) update_kernel<Rows, PARTS><<<static_cast<uint32_t>(all), Rows::kThreads, 0, stream>>>(p);
+    else last_kernel<Rows, PARTS><<<static_cast<uint32_t>(all), Rows::kThreads, 0, stream>>>(p, table, h);
     if (const int rc = check_launch("orthogonalise: B X")) return rc;
   }
   return SB_OK;
 }
+
+constexpr int64_t kRemainderRows = 192;
+constexpr int32_t kFewSteps = 5;
+
+template <class T>
+struct Tag {
+  using type = T;
+};
 
 int run_batch(const Table& t, const Hyper& h, const Shape& s, int64_t matrices, int32_t steps, void* workspace,
               hipStream_t stream) {
@@ -973,13 +991,29 @@ int run_batch(const Table& t, const Hyper& h, const Shape& s, int64_t matrices, 
     norm_kernel<<<y, kThreads, 0, stream>>>(b.partial, static_cast<int32_t>(chunks), b.factor);
     if (const int rc = check_launch("orthogonalise: norm")) return rc;
   }
-  const Padded first{b.hi[0], b.lo, static_cast<int32_t>(s.mp), static_cast<int32_t>(s.np)};
+  const Padded first{b.hi[0], b.lo[0], static_cast<int32_t>(s.mp), static_cast<int32_t>(s.np)};
   fill_kernel<<<dim3(static_cast<uint32_t>(tiles), y), kThreads, 0, stream>>>(t, h, b.partial, static_cast<int32_t>(chunks),
                                                                             b.factor, first);
   if (const int rc = check_launch("orthogonalise: fill")) return rc;
-  if (s.chain) return run_steps<SmallGram, SmallRows, SmallRows, true>(t, h, s, b, matrices, steps, stream);
-  if (s.tile == 64) return run_steps<SmallGram, SmallRows, SmallRows>(t, h, s, b, matrices, steps, stream);
-  if (s.tile == 128) return run_steps<NarrowGram, NarrowRows, NarrowRows>(t, h, s, b, matrices, steps, stream);
+  if (s.chain) return run_steps<SmallGram, SmallRows, SmallRows, 1, true>(t, h, s, b, matrices, steps, stream);
+  // B X takes X rounded to fp16, a5 X all of it. What B X lacks is noise in the rows of the
+  // large singular values, whose product with the noise in A falls on the small ones'.
+  // Beyond 192 rows and in up to five steps the result stays within 0.35% whatever the
+  // singular values; with 65 rows it is up to 0.8% off, and in eight steps up to 17% (half
+  // of the singular values 1e-4 of the others). There B is multiplied with X's remainder
+  // too: 0.2% in five steps, 0.6% in eight. That takes 3 to 13% longer for few rows (3 of
+  // 77 x 1001 93 us for 90, 100 of 128 x 4096 751 for 668), more for many (eight steps of
+  // 128 of 768 x 2048: 8300 for 6700).
+  const bool remainder = s.m <= kRemainderRows || steps > kFewSteps;
+  auto run = [&](auto gram, auto square, auto rows) {
+    using G = typename decltype(gram)::type;
+    using S = typename decltype(square)::type;
+    using R = typename decltype(rows)::type;
+    return remainder ? run_steps<G, S, R, 2>(t, h, s, b, matrices, steps, stream)
+                     : run_steps<G, S, R, 1>(t, h, s, b, matrices, steps, stream);
+  };
+  if (s.tile == 64) return run(Tag<SmallGram>{}, Tag<SmallRows>{}, Tag<SmallRows>{});
+  if (s.tile == 128) return run(Tag<NarrowGram>{}, Tag<NarrowRows>{}, Tag<NarrowRows>{});
   // The squares of wide matrices in the tiles whose rounds are shorter: 128 x 128, two
   // a CU, take 1.15 times as long for their area (128 of 1024 x 1024 237 us for 227 in
   // 9 rounds of half a wide one's for 5 of those; 64 of them 117 for 129, 5 for 3).
@@ -989,9 +1023,8 @@ int run_batch(const Table& t, const Hyper& h, const Shape& s, int64_t matrices, 
     const int64_t n = s.mp / tile;
     return (matrices * n * (n + 1) / 2 + at_once - 1) / at_once;
   };
-  return 23 * rounds(128, int64_t{2} * cus) < 40 * rounds(256, cus)
-             ? run_steps<WideGram, WideSquare, WideRows>(t, h, s, b, matrices, steps, stream)
-             : run_steps<WideGram, WideRows, WideRows>(t, h, s, b, matrices, steps, stream);
+  if (23 * rounds(128, int64_t{2} * cus) < 40 * rounds(256, cus)) return run(Tag<WideGram>{}, Tag<WideSquare>{}, Tag<WideRows>{});
+  return run(Tag<WideGram>{}, Tag<WideRows>{}, Tag<WideRows>{});
 }
 
 bool known_dtype(int64_t d) { return d == SB_DTYPE_BF16 || d == SB_DTYPE_F16 || d == SB_DTYPE_F32; }

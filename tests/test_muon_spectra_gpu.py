@@ -84,3 +84,23 @@ LARGE = [(64, 520, 1100), (64, 640, 640), (60, 300, 700), (3, 400, 1024), (2, 10
 def test_two_steps_at_a_time(size, spectrum) -> None:
     u = matrices(*size, spectrum, seed=1)
     check(optim.orthogonalize(u), newton_schulz(u), tolerance(u))
+
+
+# Small and narrow tiles, few matrices and many.
+MEDIUM = [(2, 65, 65), (3, 77, 1001), (3, 130, 66), (5, 128, 128), (2, 512, 128), (2, 200, 200), (2, 193, 1544), (1, 256, 256), (400, 70, 150),
+          (300, 100, 130), (200, 256, 200)]
+
+
+@pytest.mark.parametrize("spectrum", SPECTRA)
+@pytest.mark.parametrize("size", MEDIUM)
+def test_some_hundred_rows(size, spectrum) -> None:
+    u = matrices(*size, spectrum, seed=2)
+    check(optim.orthogonalize(u), newton_schulz(u), tolerance(u))
+
+
+@pytest.mark.parametrize("spectrum", SPECTRA)
+@pytest.mark.parametrize("size", [(2, 77, 1001), (1, 128, 128), (2, 300, 300), (3, 1024, 300), (64, 520, 1100), (300, 100, 130)])
+@pytest.mark.parametrize("steps", [2, 3, 6, 8])
+def test_fewer_and_more_steps(steps, size, spectrum) -> None:
+    u = matrices(*size, spectrum, seed=3)
+    check(optim.orthogonalize(u, steps), newton_schulz(u, steps), tolerance(u, steps))
