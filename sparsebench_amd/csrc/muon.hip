@@ -315,11 +315,13 @@ __global__ void __launch_bounds__(kThreads)
 // ------------------------------------------------------------- products ---
 
 // A symmetric matrix: the entries beside the diagonal in fp16 times `scale`, with
-// zeros on it, and the diagonal in fp32. Each [M][mp][mp] and [M][mp].
+// zeros on it, and the diagonal in fp32. Each [M][mp][mp] and [M][mp]. rest: what off's
+// rounding left, times `scale` (chain_kernel's factors alone).
 struct Symmetric {
   uint16_t* off;
   float* diag;
   float scale;
+  uint16_t* rest;
 };
 
 struct ProductArgs {
@@ -330,38 +332,40 @@ struct ProductArgs {
   int32_t mp, np, matrices;
 };
 
-// PARTS products one after another into one sum: a b, then a times what b's rounding left.
+// Up to PARTS products one after another into one sum: a b, then a times what b's rounding
+// left, then what a's left times b.
 template <class Cfg, int PARTS>
 struct Operands {
-  __amdgpu_buffer_rsrc_t ra, rb, rb_rest;
+  __amdgpu_buffer_rsrc_t ra, rb, ra_rest, rb_rest;
   uint32_t a_off[Cfg::kAInstr], b_off[Cfg::kBInstr];
   uint32_t a_step, b_step;
   int steps;  // of a part
   __device__ __forceinline__ uint32_t a_voff(int q) const { return a_off[q]; }
   __device__ __forceinline__ uint32_t b_voff(int q) const { return b_off[q]; }
   __device__ __forceinline__ uint32_t step_of(int t) const {
-    return static_cast<uint32_t>(PARTS > 1 && t >= steps ? t - steps : t);
+    return static_cast<uint32_t>(PARTS > 2 && t >= 2 * steps ? t - 2 * steps : PARTS > 1 && t >= steps ? t - steps : t);
   }
   __device__ __forceinline__ void a_src(int t, __amdgpu_buffer_rsrc_t* r, uint32_t* s) const {
-    *r = ra;
+    *r = PARTS > 2 && t >= 2 * steps ? ra_rest : ra;
     *s = step_of(t) * a_step;
   }
   __device__ __forceinline__ void b_src(int t, __amdgpu_buffer_rsrc_t* r, uint32_t* s) const {
-    *r = PARTS > 1 && t >= steps ? rb_rest : rb;
+    *r = PARTS > 1 && t >= steps && !(PARTS > 2 && t >= 2 * steps) ? rb_rest : rb;
     *s = step_of(t) * b_step;
   }
 };
 
-// C rows i0 .., columns j0 .. of a [mp, k] times b (and b_rest): [k, columns], or with
-// BT the rows of b [columns, k].
+// C rows i0 .., columns j0 .. of a [mp, k] times b: [k, columns], or with BT the rows of b
+// [columns, k]. The remainders are not looked at where `parts` does not reach them.
 template <class Cfg, int PARTS = 1>
-__device__ __forceinline__ void product(uint8_t* __restrict__ lds, const uint16_t* a, const uint16_t* b,
-                                        const uint16_t* b_rest, int mp, int k, int columns, int i0, int j0,
-                                        typename DmaMainloop<Cfg>::Acc& acc) {
+__device__ __forceinline__ void product(uint8_t* __restrict__ lds, const uint16_t* a, const uint16_t* a_rest,
+                                        const uint16_t* b, const uint16_t* b_rest, int mp, int k, int columns, int i0,
+                                        int j0, typename DmaMainloop<Cfg>::Acc& acc, int parts = PARTS) {
   Operands<Cfg, PARTS> src;
   src.ra = make_rsrc(a, static_cast<uint32_t>(mp) * static_cast<uint32_t>(k) * 2u);
   src.rb = make_rsrc(b, static_cast<uint32_t>(columns) * static_cast<uint32_t>(k) * 2u);
   if constexpr (PARTS > 1) src.rb_rest = make_rsrc(b_rest, static_cast<uint32_t>(columns) * static_cast<uint32_t>(k) * 2u);
+  if constexpr (PARTS > 2) src.ra_rest = make_rsrc(a_rest, static_cast<uint32_t>(mp) * static_cast<uint32_t>(k) * 2u);
   src.steps = k / Cfg::BK;
   const ADmaPos<Cfg> ap;
 #pragma unroll
@@ -381,7 +385,7 @@ __device__ __forceinline__ void product(uint8_t* __restrict__ lds, const uint16_
       src.b_off[q] = (static_cast<uint32_t>(bp.row[q]) * static_cast<uint32_t>(columns) + j0 + bp.col[q]) * 2u;
     src.b_step = Cfg::BK * static_cast<uint32_t>(columns) * 2u;
   }
-  DmaMainloop<Cfg>::run(lds, src, PARTS * src.steps, acc);
+  DmaMainloop<Cfg>::run(lds, src, parts * src.steps, acc);
 }
 
 // The accumulators in fp32 through LDS, kGroups groups of 32 rows of each row of
@@ -530,10 +534,10 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1) symmetric_kernel(ProductArgs
   float unit;  // of the accumulators
   if constexpr (GRAM) {
     const uint16_t* x = p.x + matrix * p.mp * p.np;
-    product<Cfg>(lds, x, x, nullptr, p.mp, p.np, p.mp, i0, j0, acc);
+    product<Cfg>(lds, x, nullptr, x, nullptr, p.mp, p.np, p.mp, i0, j0, acc);
     unit = kUnscale * kUnscale;
   } else {
-    product<Cfg>(lds, p.left.off + square, p.right.off + square, nullptr, p.mp, p.mp, p.mp, i0, j0, acc);
+    product<Cfg>(lds, p.left.off + square, nullptr, p.right.off + square, nullptr, p.mp, p.mp, p.mp, i0, j0, acc);
     unit = p.of_product / (p.left.scale * p.right.scale);
   }
   const float scale = p.out.scale;
@@ -591,11 +595,17 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1) symmetric_kernel(ProductArgs
 }
 
 // A and what follows from it for matrices of one tile, a workgroup each: the squares
-// stay in LDS, fp16 beside the diagonals as everywhere. out = B of one step, or the
-// factor of X in two (run_steps), in place of 2 or 6 launches: three of 40 x 1001 63 us
-// for 78, one of 64 x 4096 93 : 106, 1000 of 64 x 256 179 : 217. One LDS array: with a
-// second one the compiler lets every read in the main loop wait for all loads (one of
-// 64 x 4096: 177). Matrices of 128 lose: a workgroup's product of 128^3 takes 3 us.
+// stay in LDS. out = B of one step, or the factor of X in two (run_steps), in place of 2 or
+// 6 launches. So few rows do not average their roundings (nearly low rank, 2 x 3 7% off, 7 x 128
+// 2%, 64 x 128 0.8%), and products are short here: each square keeps what its rounding to
+// fp16 left beside it, products are L R with both remainders' cross terms, and the factor's
+// remainder goes into X as well. X X^T takes X rounded to fp16 where n > 64, whose roundings
+// average over n (0.26% for 2 rows of 65, 0.03% of 1000), and for n <= 64, one K step, its
+// remainder too (5e-5). Three of 40 x 1001 76 us, one of 64 x 4096 108, 1000 of 64 x 256 222;
+// without remainders 66, 96 and 182, and as launches of symmetric_kernel 78, 106 and 217.
+// One LDS array: with a second one the compiler lets every read in the main loop wait for
+// all loads (one of 64 x 4096: 177 without remainders). Matrices of 128 lose: a workgroup's
+// product of 128^3 takes 3 us.
 template <class Cfg>
 __device__ __forceinline__ void chain(uint8_t* __restrict__ lds, const typename DmaMainloop<Cfg>::Acc& gram,
                                       const Symmetric& result, int64_t matrix, int32_t two) {
@@ -604,10 +614,11 @@ __device__ __forceinline__ void chain(uint8_t* __restrict__ lds, const typename 
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int row0 = wave / Cfg::WN * Cfg::WTM + (lane & 31), col0 = wave % Cfg::WN * Cfg::WTN + (lane & 31);
   auto scale_of = [](int of) { return of == 2 ? kScale / 4 : kScale; };
-  auto diag = [&](int of, int r) -> float& { return reinterpret_cast<float*>(lds + 4 * kBytes)[of * N + r]; };
-  // Where columns c .. of row r of square `of` are: chunks of 8 halves, turned by the row.
-  auto at = [&](int of, int r, int c) {
-    return lds + of * kBytes + r * (2 * N) + (((c >> 3) ^ ((r ^ (r >> 3)) & 7)) << 4) + (c & 7) * 2;
+  auto diag = [&](int of, int r) -> float& { return reinterpret_cast<float*>(lds + 8 * kBytes)[of * N + r]; };
+  // Where columns c .. of row r of square `of` are, or of its remainder: chunks of 8
+  // halves, turned by the row.
+  auto at = [&](int of, int rest, int r, int c) {
+    return lds + (2 * of + rest) * kBytes + r * (2 * N) + (((c >> 3) ^ ((r ^ (r >> 3)) & 7)) << 4) + (c & 7) * 2;
   };
   // Square `to`, from fn(row, first of four columns, the accumulators' values).
   auto store = [&](int to, const typename ML::Acc& acc, auto fn) {
@@ -623,14 +634,19 @@ __device__ __forceinline__ void chain(uint8_t* __restrict__ lds, const typename 
 #pragma unroll
           for (int e = 0; e < 4; ++e) v[e] = acc[j][i][4 * g + e];
           fn(row, col, v);
-          uint16_t bits[4];
+          uint16_t bits[2][4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            bits[e] = half_bits(v[e] * scale);
-            if (row == col + e) diag(to, row) = v[e], bits[e] = 0;
+            const float x = v[e] * scale;
+            bits[0][e] = half_bits(x);
+            bits[1][e] = half_bits(x - value_of(bits[0][e], SB_DTYPE_F16));
+            if (row == col + e) diag(to, row) = v[e], bits[0][e] = bits[1][e] = 0;
           }
-          *reinterpret_cast<u32x2_t*>(at(to, row, col)) =
-              u32x2_t{bits[0] | static_cast<uint32_t>(bits[1]) << 16, bits[2] | static_cast<uint32_t>(bits[3]) << 16};
+#pragma unroll
+          for (int rest = 0; rest < 2; ++rest)
+            *reinterpret_cast<u32x2_t*>(at(to, rest, row, col)) =
+                u32x2_t{bits[rest][0] | static_cast<uint32_t>(bits[rest][1]) << 16,
+                        bits[rest][2] | static_cast<uint32_t>(bits[rest][3]) << 16};
         }
     __syncthreads();
   };
@@ -640,24 +656,33 @@ __device__ __forceinline__ void chain(uint8_t* __restrict__ lds, const typename 
 #pragma unroll
     for (int k0 = 0; k0 < N; k0 += 16) {
       const int k = k0 + 8 * (lane >> 5);
-      bf16x8_t a[Cfg::TM], b[Cfg::TN];
+      bf16x8_t a[2][Cfg::TM], b[2][Cfg::TN];
 #pragma unroll
-      for (int i = 0; i < Cfg::TM; ++i) a[i] = *reinterpret_cast<const bf16x8_t*>(at(l, row0 + 32 * i, k));
+      for (int rest = 0; rest < 2; ++rest) {
 #pragma unroll
-      for (int j = 0; j < Cfg::TN; ++j) b[j] = *reinterpret_cast<const bf16x8_t*>(at(r, col0 + 32 * j, k));
+        for (int i = 0; i < Cfg::TM; ++i) a[rest][i] = *reinterpret_cast<const bf16x8_t*>(at(l, rest, row0 + 32 * i, k));
 #pragma unroll
-      for (int j = 0; j < Cfg::TN; ++j)
+        for (int j = 0; j < Cfg::TN; ++j) b[rest][j] = *reinterpret_cast<const bf16x8_t*>(at(r, rest, col0 + 32 * j, k));
+      }
 #pragma unroll
-        for (int i = 0; i < Cfg::TM; ++i) acc[j][i] = ML::mfma(b[j], a[i], acc[j][i]);
+      for (int part = 0; part < 3; ++part)  // hi hi, hi lo, lo hi
+#pragma unroll
+        for (int j = 0; j < Cfg::TN; ++j)
+#pragma unroll
+          for (int i = 0; i < Cfg::TM; ++i) acc[j][i] = ML::mfma(b[part == 1][j], a[part == 2][i], acc[j][i]);
     }
     const float ls = 1.0f / scale_of(l), rs = 1.0f / scale_of(r), unit = of_lr * ls * rs;
     store(to, acc, [&](int row, int col, float (&v)[4]) {
-      const u32x2_t o = *reinterpret_cast<const u32x2_t*>(at(l, row, col)), s = *reinterpret_cast<const u32x2_t*>(at(r, row, col));
+      auto entry = [&](int of, int rest) { return *reinterpret_cast<const u32x2_t*>(at(of, rest, row, col)); };
+      const u32x2_t o[2] = {entry(l, 0), entry(l, 1)}, s[2] = {entry(r, 0), entry(r, 1)};
+      auto value = [](const u32x2_t(&parts)[2], int e) {
+        return value_of(static_cast<uint16_t>(parts[0][e / 2] >> (16 * (e & 1))), SB_DTYPE_F16) +
+               value_of(static_cast<uint16_t>(parts[1][e / 2] >> (16 * (e & 1))), SB_DTYPE_F16);
+      };
       const float ld = diag(l, row), rd = diag(r, row);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float oe = value_of(static_cast<uint16_t>(o[e / 2] >> (16 * (e & 1))), SB_DTYPE_F16) * ls;
-        const float se = value_of(static_cast<uint16_t>(s[e / 2] >> (16 * (e & 1))), SB_DTYPE_F16) * rs;
+        const float oe = value(o, e) * ls, se = value(s, e) * rs;
         v[e] *= unit;
         if (row == col + e) v[e] += of_l * ld + of_r * rd + of_lr * (ld * rd);
         else v[e] += (of_r + of_lr * ld) * se + (of_l + of_lr * diag(r, col + e)) * oe;
@@ -681,24 +706,26 @@ __device__ __forceinline__ void chain(uint8_t* __restrict__ lds, const typename 
   const int out = two ? 2 : 1;
   for (int i = threadIdx.x; i < N * N / 8; i += Cfg::kThreads) {
     const int r = i / (N / 8), c = i % (N / 8) * 8;
-    *reinterpret_cast<u32x4_t*>(result.off + matrix * N * N + r * N + c) = *reinterpret_cast<const u32x4_t*>(at(out, r, c));
+    *reinterpret_cast<u32x4_t*>(result.off + matrix * N * N + r * N + c) = *reinterpret_cast<const u32x4_t*>(at(out, 0, r, c));
+    *reinterpret_cast<u32x4_t*>(result.rest + matrix * N * N + r * N + c) = *reinterpret_cast<const u32x4_t*>(at(out, 1, r, c));
   }
   for (int i = threadIdx.x; i < N; i += Cfg::kThreads) result.diag[matrix * N + i] = diag(out, i);
 }
 
 template <class Cfg>
 __global__ void __launch_bounds__(Cfg::kThreads, 1) chain_kernel(ProductArgs p, int32_t two) {
-  static_assert(Cfg::BN == Cfg::BM && Cfg::F16 && Cfg::kLdsAlloc >= 4 * Cfg::BM * (Cfg::BM * 2 + 4));  // squares, diagonals
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[Cfg::kLdsAlloc];
+  static_assert(Cfg::BN == Cfg::BM && Cfg::F16);
+  constexpr int kSquares = 4 * Cfg::BM * (Cfg::BM * 4 + 4);  // with remainders, and diagonals
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[Cfg::kLdsAlloc > kSquares ? Cfg::kLdsAlloc : kSquares];
   const int64_t matrix = blockIdx.x;
   typename DmaMainloop<Cfg>::Acc acc;
-  const uint16_t* x = p.x + matrix * p.mp * p.np;
-  product<Cfg>(lds, x, x, nullptr, p.mp, p.np, p.mp, 0, 0, acc);
+  const uint16_t *x = p.x + matrix * p.mp * p.np, *lo = p.lo + matrix * p.mp * p.np;
+  product<Cfg, 3>(lds, x, lo, x, lo, p.mp, p.np, p.mp, 0, 0, acc, p.np <= Cfg::BK ? 3 : 1);
   chain<Cfg>(lds, acc, p.out, matrix, two);
 }
 
 // next, next_lo = of_right X + L X: of X's own rows of_right and L's diagonal. PARTS 2:
-// L times X's remainder too (run_batch says where).
+// L times X's remainder too (run_batch says where). 3: and L's remainder times X.
 template <class Cfg, int PARTS>
 __global__ void __launch_bounds__(Cfg::kThreads, 1) update_kernel(ProductArgs p) {
   using ML = DmaMainloop<Cfg>;
@@ -710,7 +737,9 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1) update_kernel(ProductArgs p)
   const int i0 = uniform(at % per % mt) * Cfg::BM, j0 = uniform(at % per / mt) * Cfg::BN;
   const int64_t whole = matrix * p.mp * p.np, tile = whole + static_cast<int64_t>(i0) * p.np + j0;
   typename ML::Acc acc;
-  product<Cfg, PARTS>(lds, p.left.off + matrix * p.mp * p.mp, p.x + whole, p.lo + whole, p.mp, p.mp, p.np, i0, j0, acc);
+  const int64_t square = matrix * p.mp * p.mp;
+  product<Cfg, PARTS>(lds, p.left.off + square, PARTS > 2 ? p.left.rest + square : nullptr, p.x + whole, p.lo + whole, p.mp,
+                      p.mp, p.np, i0, j0, acc);
   const float unit = 1.0f / p.left.scale;
   static_for<0, Ep::kParts>([&](auto part) {
     constexpr int P = decltype(part)::value;
@@ -752,8 +781,9 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1) last_kernel(ProductArgs p, T
   int64_t place;
   const Entry e = entry_of(t, matrix, &place);
   typename ML::Acc acc;
-  product<Cfg, PARTS>(lds, p.left.off + static_cast<int64_t>(matrix) * p.mp * p.mp, p.x + whole, p.lo + whole, p.mp, p.mp,
-                      p.np, i0, j0, acc);
+  const int64_t square = static_cast<int64_t>(matrix) * p.mp * p.mp;
+  product<Cfg, PARTS>(lds, p.left.off + square, PARTS > 2 ? p.left.rest + square : nullptr, p.x + whole, p.lo + whole, p.mp,
+                      p.mp, p.np, i0, j0, acc);
   const float unit = 1.0f / p.left.scale;
   const float lr = h.lr_ptr ? *h.lr_ptr : h.lr;
   const float keep = 1.0f - lr * h.weight_decay;
@@ -892,6 +922,7 @@ Buffers carve(void* workspace, const Shape& s, int64_t matrices) {
   for (int i = 0; i < (s.pairs && !s.chain ? 4 : 2); ++i) {
     b.square[i].off = ws.take<uint16_t>(matrices * s.mp * s.mp);
     b.square[i].diag = ws.take<float>(matrices * s.mp);
+    b.square[i].rest = ws.take<uint16_t>(s.chain && i == 0 ? matrices * s.mp * s.mp : 0);
   }
   b.partial = ws.take<double>(matrices * std::max(chunks_of(s.m, s.n, s.vectors), chunks_of(s.n, s.m, s.vectors)));
   b.factor = ws.take<float>(matrices);
@@ -910,7 +941,8 @@ int64_t batch_bytes(const Shape& s, int64_t matrices) { return carve(nullptr, s,
 // rounding. While the singular values' squares add up to 1, few are large enough for
 // that to count (256 x 512, over spectra of decades and steps: 0.27% of the result, as
 // with single steps). In the next two it does (0.74%; 0.69% measured for 300 x 700, a
-// quarter of the singular values ten times the others). chain_kernel still takes every pair.
+// quarter of the singular values ten times the others). chain_kernel's factors keep what their
+// rounding leaves, and take every pair.
 template <class Gram, class Square, class Rows, int PARTS, bool CHAIN = false>
 int run_steps(const Table& table, const Hyper& h, const Shape& s, const Buffers& b, int64_t matrices, int32_t steps,
               hipStream_t stream) {
@@ -923,7 +955,7 @@ int run_steps(const Table& table, const Hyper& h, const Shape& s, const Buffers&
   p.mp = static_cast<int32_t>(s.mp);
   p.np = static_cast<int32_t>(s.np);
   p.matrices = static_cast<int32_t>(matrices);
-  auto scaled = [&](int i, float scale) { return Symmetric{b.square[i].off, b.square[i].diag, scale}; };
+  auto scaled = [&](int i, float scale) { return Symmetric{b.square[i].off, b.square[i].diag, scale, b.square[i].rest}; };
   auto multiply = [&](const Symmetric& l, const Symmetric& r, const Symmetric& out, float of_l, float of_r, float of_lr) {
     p.left = l, p.right = r, p.out = out;
     p.of_left = of_l, p.of_right = of_r, p.of_product = of_lr;
@@ -995,7 +1027,7 @@ int run_batch(const Table& t, const Hyper& h, const Shape& s, int64_t matrices, 
   fill_kernel<<<dim3(static_cast<uint32_t>(tiles), y), kThreads, 0, stream>>>(t, h, b.partial, static_cast<int32_t>(chunks),
                                                                             b.factor, first);
   if (const int rc = check_launch("orthogonalise: fill")) return rc;
-  if (s.chain) return run_steps<SmallGram, SmallRows, SmallRows, 1, true>(t, h, s, b, matrices, steps, stream);
+  if (s.chain) return run_steps<SmallGram, SmallRows, SmallRows, 3, true>(t, h, s, b, matrices, steps, stream);
   // B X takes X rounded to fp16, a5 X all of it. What B X lacks is noise in the rows of the
   // large singular values, whose product with the noise in A falls on the small ones'.
   // Beyond 192 rows and in up to five steps the result stays within 0.35% whatever the

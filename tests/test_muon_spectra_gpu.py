@@ -104,3 +104,29 @@ def test_some_hundred_rows(size, spectrum) -> None:
 def test_fewer_and_more_steps(steps, size, spectrum) -> None:
     u = matrices(*size, spectrum, seed=3)
     check(optim.orthogonalize(u, steps), newton_schulz(u, steps), tolerance(u, steps))
+
+
+# All squares of a step, or of two, in one workgroup.
+FEW = [(5, 2, 3), (5, 2, 40), (3, 2, 1000), (4, 3, 3), (3, 9, 4), (3, 64, 5), (2, 7, 128), (2, 16, 64), (2, 33, 66), (1000, 16, 33), (2, 64, 64),
+       (2, 64, 128), (2, 64, 4100), (3, 40, 1001)]
+
+
+@pytest.mark.parametrize("spectrum", SPECTRA)
+@pytest.mark.parametrize("size", FEW)
+@pytest.mark.parametrize("steps", [1, 3, 5, 8])
+def test_few_rows(steps, size, spectrum) -> None:
+    u = matrices(*size, spectrum, seed=4)
+    check(optim.orthogonalize(u, steps), newton_schulz(u, steps), tolerance(u, steps))
+
+
+def test_step_of_few_rows() -> None:
+    """Tall and wide, with momenta and masters: the update itself within the same tolerance."""
+    params = [matrices(2, r, c, "one 1e-3", seed=5, scale=0.05) for r, c in ((12, 60), (60, 12), (48, 300))]
+    grads = [matrices(2, *p.shape[1:], "half 1e-3", seed=6) for p in params]
+    momenta = [torch.zeros_like(p) for p in params]
+    start = [p.clone() for p in params]
+    optim.muon_step(params, grads, momenta, 1.0, update_rms=1.0)
+    for p, g, w in zip(params, grads, start):
+        kept, update, _ = step_reference(w, g, torch.zeros_like(w), 1.0, 0.95, True, 0.0, 1.0, 1.0)
+        # the update is of size 5 to 70 beside weights of 0.05: their rounding is 2^-24 of it
+        check((p.double() - kept), -update, tolerance(g) + 2.0**-23)
