@@ -858,10 +858,7 @@ struct Shape {
   bool chain;  // chain_kernel
   int32_t vectors;  // a lane's of a chunk
   bool pairs;
-  int64_t most;  // matrices of a batch
 };
-
-int64_t batch_bytes(const Shape& s, int64_t matrices);
 
 Shape shape_of(int64_t rows, int64_t columns, int64_t matrices, int cus) {
   Shape s;
@@ -898,9 +895,6 @@ Shape shape_of(int64_t rows, int64_t columns, int64_t matrices, int cus) {
   // Shorter chunks where they are few (24 of 256 x 512, 192 chunks of 8 vectors: 13.5 us).
   s.vectors = kVectors;
   while (s.vectors > 1 && matrices * chunks_of(s.m, s.n, s.vectors) < int64_t{4} * cus) s.vectors /= 2;
-  s.most = 1;
-  while (s.most < 65535 && batch_bytes(s, s.most * 2) <= kBatchBytes) s.most *= 2;
-  s.most = std::min<int64_t>(s.most, 65535);
   return s;
 }
 
@@ -918,7 +912,7 @@ Buffers carve(void* workspace, const Shape& s, int64_t matrices) {
   b.hi[0] = ws.take<uint16_t>(matrices * s.mp * s.np);
   b.hi[1] = ws.take<uint16_t>(matrices * s.mp * s.np);
   b.lo[0] = ws.take<uint16_t>(matrices * s.mp * s.np);
-  b.lo[1] = ws.take<uint16_t>(matrices * s.mp * s.np);  // read by more steps than sizes are asked for
+  b.lo[1] = ws.take<uint16_t>(matrices * s.mp * s.np);  // sizes do not know whether steps will need it
   for (int i = 0; i < (s.pairs && !s.chain ? 4 : 2); ++i) {
     b.square[i].off = ws.take<uint16_t>(matrices * s.mp * s.mp);
     b.square[i].diag = ws.take<float>(matrices * s.mp);
@@ -931,6 +925,13 @@ Buffers carve(void* workspace, const Shape& s, int64_t matrices) {
 }
 
 int64_t batch_bytes(const Shape& s, int64_t matrices) { return carve(nullptr, s, matrices).used; }
+
+// Matrices of a batch.
+int64_t most_of(const Shape& s) {
+  int64_t most = 1;
+  while (most < 65535 && batch_bytes(s, most * 2) <= kBatchBytes) most *= 2;
+  return std::min<int64_t>(most, 65535);
+}
 
 // The steps, one or two at a time. Two: with P = a5 + B of A = X X^T, the next
 // step's A is P A P = a5^2 A + (2 a5 B + B^2) A, and both steps' factor of X is
@@ -1094,9 +1095,10 @@ bool wide_values(const SbMuonTensor& a) {
          ok(a.master, SB_DTYPE_F32, a.master_matrix, a.master_row);
 }
 
-// f(shape, total matrices of that size) for each size in the list, by its first tensor.
+// f(table, shape, matrices) for each batch: matrices of one size, of up to kEntries tensors,
+// as many as their workspace's bound lets in. Their own number chooses their shape.
 template <class F>
-int for_each_size(const SbMuonTensor* tensors, int64_t count, int cus, F&& f) {
+int for_each_batch(const SbMuonTensor* tensors, int64_t count, int cus, F&& f) {
   auto same = [&](int64_t i, int64_t q) {
     return !empty(tensors[q]) && std::minmax(tensors[i].rows, tensors[i].columns) == std::minmax(tensors[q].rows, tensors[q].columns);
   };
@@ -1108,33 +1110,22 @@ int for_each_size(const SbMuonTensor* tensors, int64_t count, int cus, F&& f) {
     int64_t total = 0;
     for (int64_t q = i; q < count; ++q)
       if (same(i, q)) total += tensors[q].matrices;
-    if (const int rc = f(shape_of(tensors[i].rows, tensors[i].columns, total, cus), total, i)) return rc;
-  }
-  return SB_OK;
-}
-
-int run_list(const SbMuonTensor* tensors, int64_t count, const Hyper& h, int32_t steps, void* workspace,
-             int64_t workspace_bytes, hipStream_t stream) {
-  if (steps < 1 || steps > kMaxSteps) return fail(SB_ERR_INVALID, "muon: 1 to %d steps, got %d", kMaxSteps, steps);
-  int cus = 0;
-  if (const int rc = device_cus(&cus)) return rc;
-  return for_each_size(tensors, count, cus, [&](const Shape& s, int64_t total, int64_t first) {
-    if (const int rc = check_workspace(workspace, workspace_bytes, batch_bytes(s, std::min(total, s.most)))) return rc;
+    const int64_t most = most_of(shape_of(tensors[i].rows, tensors[i].columns, total, cus));
     Table t{};
     int64_t matrices = 0;
     auto flush = [&]() -> int {
-      const int rc = matrices ? run_batch(t, h, s, matrices, steps, workspace, stream) : SB_OK;
+      const int rc = matrices ? f(t, shape_of(tensors[i].rows, tensors[i].columns, matrices, cus), matrices) : SB_OK;
       t = Table{};
       matrices = 0;
       return rc;
     };
-    for (int64_t i = first; i < count; ++i) {
-      const SbMuonTensor& a = tensors[i];
-      if (empty(a) || std::min(a.rows, a.columns) != s.m || std::max(a.rows, a.columns) != s.n) continue;
+    for (int64_t q = i; q < count; ++q) {
+      if (!same(i, q)) continue;
+      const SbMuonTensor& a = tensors[q];
       for (int64_t at = 0; at < a.matrices;) {
-        if (t.count == kEntries || matrices == s.most)
+        if (t.count == kEntries || matrices == most)
           if (const int rc = flush()) return rc;
-        const int64_t take = std::min(a.matrices - at, s.most - matrices);
+        const int64_t take = std::min(a.matrices - at, most - matrices);
         const int64_t pe = a.param_dtype == SB_DTYPE_F32 ? 4 : 2, ge = a.grad_dtype == SB_DTYPE_F32 ? 4 : 2;
         t.e[t.count++] = Entry{static_cast<uint8_t*>(a.param) + at * a.param_matrix * pe,
                                static_cast<const uint8_t*>(a.grad) + at * a.grad_matrix * ge,
@@ -1149,7 +1140,19 @@ int run_list(const SbMuonTensor* tensors, int64_t count, const Hyper& h, int32_t
         at += take;
       }
     }
-    return flush();
+    if (const int rc = flush()) return rc;
+  }
+  return SB_OK;
+}
+
+int run_list(const SbMuonTensor* tensors, int64_t count, const Hyper& h, int32_t steps, void* workspace,
+             int64_t workspace_bytes, hipStream_t stream) {
+  if (steps < 1 || steps > kMaxSteps) return fail(SB_ERR_INVALID, "muon: 1 to %d steps, got %d", kMaxSteps, steps);
+  int cus = 0;
+  if (const int rc = device_cus(&cus)) return rc;
+  return for_each_batch(tensors, count, cus, [&](const Table& t, const Shape& s, int64_t matrices) {
+    if (const int rc = check_workspace(workspace, workspace_bytes, batch_bytes(s, matrices))) return rc;
+    return run_batch(t, h, s, matrices, steps, workspace, stream);
   });
 }
 
@@ -1163,8 +1166,8 @@ extern "C" int sb_muon_sizes(const SbMuonTensor* tensors, int64_t count, int64_t
   int cus = 0;
   if (const int rc = device_cus(&cus)) return rc;
   int64_t most = 256;
-  if (const int rc = for_each_size(tensors, count, cus, [&](const Shape& s, int64_t total, int64_t) {
-        most = std::max(most, batch_bytes(s, std::min(total, s.most)));
+  if (const int rc = for_each_batch(tensors, count, cus, [&](const Table&, const Shape& s, int64_t matrices) {
+        most = std::max(most, batch_bytes(s, matrices));
         return SB_OK;
       }))
     return rc;

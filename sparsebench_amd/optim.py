@@ -178,7 +178,9 @@ def muon_step(
     itself. masters: fp32 weights updated in the parameters' place and rounded into them.
     lr and grad_scale may be one-element fp32 tensors on the GPU. All on one GPU; tensors
     must not overlap (an fp32 parameter may be its own master). Matrices of one size are
-    taken together. Parameters and masters
+    taken together, those of 16 tensors at a time. A step takes a workspace for the most that
+    are taken together: 8 to 14 bytes a value of theirs (the squarer, the more; sides are
+    padded to 64, 128 or 256), up to 6 GiB where that holds a matrix. Parameters and masters
     count as modified in place, as in adamw_step; nothing syncs, and a step can be captured."""
     from sparsebench_amd import _C
 
