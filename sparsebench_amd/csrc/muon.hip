@@ -1150,8 +1150,12 @@ int run_list(const SbMuonTensor* tensors, int64_t count, const Hyper& h, int32_t
   if (steps < 1 || steps > kMaxSteps) return fail(SB_ERR_INVALID, "muon: 1 to %d steps, got %d", kMaxSteps, steps);
   int cus = 0;
   if (const int rc = device_cus(&cus)) return rc;
+  // All of them before the first is launched: a list that is refused is left as it was.
+  const int rc = for_each_batch(tensors, count, cus, [&](const Table&, const Shape& s, int64_t matrices) {
+    return check_workspace(workspace, workspace_bytes, batch_bytes(s, matrices));
+  });
+  if (rc) return rc;
   return for_each_batch(tensors, count, cus, [&](const Table& t, const Shape& s, int64_t matrices) {
-    if (const int rc = check_workspace(workspace, workspace_bytes, batch_bytes(s, matrices))) return rc;
     return run_batch(t, h, s, matrices, steps, workspace, stream);
   });
 }
