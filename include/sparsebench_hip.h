@@ -441,7 +441,7 @@ int sb_dequantize4(const void* codes, const void* scales, void* w, int64_t num_e
  * matrices and rows some strides of elements apart, a row's values contiguous.
  * param and grad are of their SB_DTYPE_* codes; momentum is fp32; master is
  * NULL, or fp32 weights that are updated in the parameter's place and rounded
- * into it. */
+ * into it. Sides padded to 64, a matrix has under 2^30 values. */
 typedef struct {
   void* param;
   const void* grad;

@@ -43,6 +43,7 @@ constexpr float kScale = 16384.0f, kUnscale = 1.0f / 16384.0f;
 constexpr float kNormEps = 1e-7f;
 constexpr int kThreads = 256;
 constexpr int kMaxSteps = 32;
+constexpr int64_t kMostPadded = kI32Limit / 2;  // values of a padded matrix: their offsets in bytes take 31 bits
 constexpr int64_t kBatchBytes = int64_t{6} << 30;  // of a batch's workspace, where that holds a matrix
 
 // ------------------------------------------------------------ the list ---
@@ -882,8 +883,9 @@ Shape shape_of(int64_t rows, int64_t columns, int64_t matrices, int cus) {
   //   400 of 512 x 512   2958  2877  3411     90 of 512 x 1024      988  1106
   //   100 of 512 x 2048  1982  1670  1931     100 of 320 x 1024     698  556
   //   300 of 256 x 256    691   481   471     1000 of 192 x 192    1500  900
-  if (s.m > 512 && 2 * padded(256) <= 3 * padded(64) && 2 * steps_of_a(256) >= int64_t{9} * cus) s.tile = 256;
-  else if (steps_of_a(64) <= int64_t{32} * cus || 4 * padded(64) <= 3 * padded(128)) s.tile = 64;
+  auto fits = [&](int64_t tile) { return round_up(s.m, tile) * round_up(s.n, tile) < kMostPadded; };
+  if (fits(256) && s.m > 512 && 2 * padded(256) <= 3 * padded(64) && 2 * steps_of_a(256) >= int64_t{9} * cus) s.tile = 256;
+  else if (!fits(128) || steps_of_a(64) <= int64_t{32} * cus || 4 * padded(64) <= 3 * padded(128)) s.tile = 64;
   else s.tile = 128;
   // The first two steps at a time (run_steps) where X is long, and not so little that
   // launches count: 16 of 512 x 2048 take 395 us for 404, 1 of 128 x 4096 135 for 140.
@@ -1069,10 +1071,9 @@ int check_list(const SbMuonTensor* tensors, int64_t count) {
     if (a.matrices < 0 || a.rows < 0 || a.columns < 0) return fail(SB_ERR_INVALID, "muon: negative size");
     if (a.matrices == 0 || a.rows == 0 || a.columns == 0) continue;
     if (a.rows >= kI32Limit || a.columns >= kI32Limit || a.matrices >= kI32Limit ||
-        round_up(a.rows, 256) * round_up(a.columns, 256) >= kI32Limit / 2 ||
-        round_up(std::min(a.rows, a.columns), 256) > 32768)
-      return fail(SB_ERR_INVALID, "muon: matrices of under 2^30 values with a side up to 32768, got %lld x %lld",
-                  static_cast<long long>(a.rows), static_cast<long long>(a.columns));
+        round_up(a.rows, 64) * round_up(a.columns, 64) >= kMostPadded)
+      return fail(SB_ERR_INVALID, "muon: under 2^31 matrices of under 2^30 values, sides padded to 64, got %lld of %lld x %lld",
+                  static_cast<long long>(a.matrices), static_cast<long long>(a.rows), static_cast<long long>(a.columns));
     if (!a.param || !a.grad) return fail(SB_ERR_INVALID, "muon: null buffer");
     if (!known_dtype(a.param_dtype) || !known_dtype(a.grad_dtype))
       return fail(SB_ERR_INVALID, "muon: unsupported dtype code");
