@@ -461,7 +461,10 @@ typedef struct {
  *   w = w (1 - lr weight_decay) - lr update_rms sqrt(max(rows, columns)) X
  * The products take fp16 operands and sum in fp32; X is kept to twice fp16's
  * bits. lr_ptr (NULL: lr) and grad_scale: one fp32 on the device. `tensors` is
- * read before the call returns. workspace: *workspace_bytes of sb_muon_sizes for
+ * read before the call returns. What is written must not lie where anything else
+ * does (refused where strides are the same; with others it is not looked for), but a
+ * parameter may be its own fp32 master, and both their own gradient.
+ * workspace: *workspace_bytes of sb_muon_sizes for
  * the list on the same device, 256-byte aligned. sb_orthogonalize: param = X of
  * grad (momentum and master NULL); param may be grad. */
 int sb_muon_sizes(const SbMuonTensor* tensors, int64_t count, int64_t* workspace_bytes);

@@ -1260,11 +1260,6 @@ def muon_cuda(params, grads, momenta, masters, lr, momentum: float, nesterov: bo
     if masters is not None:
         _check_stacks(masters, index, "masters", (torch.float32,), shapes)
     words = _muon_words(params, grads, momenta, masters)
-    # An fp32 parameter may be its own master (both are written alike).
-    own = [w for w, p in zip(masters or (), params) if not (w.data_ptr() == p.data_ptr() and w.dtype is p.dtype)]
-    written = [t.data_ptr() for t in (*params, *momenta, *own) if t.numel()]
-    if len(set(written)) != len(written):
-        _fail("parameters, momenta and masters must not overlap: one starts where another does")
     lr_ptr, scale_ptr = _device_scalar(lr, "lr", dev), _device_scalar(grad_scale, "grad_scale", dev)
     with _device_of(params[0]):
         if scale_ptr is None and grad_scale is not None:  # a number: as a device scalar

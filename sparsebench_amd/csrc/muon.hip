@@ -30,7 +30,10 @@
 // step, momentum 1112 and X 1087 (both at 4.8 TB/s). Small lists are bound by their 17
 // launches of 4 to 10 us: 24 of 256 x 512 take 108.
 
+#include <algorithm>
 #include <cmath>
+#include <new>
+#include <vector>
 
 #include "gemm_dma.hpp"
 #include "workspace.hpp"
@@ -1086,6 +1089,90 @@ int check_list(const SbMuonTensor* tensors, int64_t count) {
 
 bool empty(const SbMuonTensor& a) { return a.matrices == 0 || a.rows == 0 || a.columns == 0; }
 
+// Where a stack's values lie: rows of `width` bytes, and two counts with their strides, the
+// larger stride first.
+struct Place {
+  int64_t first, last;  // its bytes are in [first, last)
+  int64_t width, n[2], stride[2];
+  int64_t tensor;
+  int kind;  // 0 parameter, 1 master, 2 momentum, 3 gradient
+};
+
+Place place_of(const SbMuonTensor& a, int64_t tensor, int kind, const void* p, int64_t bytes, int64_t matrix, int64_t row) {
+  Place q{};
+  q.width = a.columns * bytes;
+  q.n[0] = matrix > 0 ? a.matrices : 1, q.stride[0] = matrix * bytes;
+  q.n[1] = row > 0 ? a.rows : 1, q.stride[1] = row * bytes;
+  if (q.n[1] == 1 || (q.n[0] > 1 && q.stride[1] > q.stride[0])) std::swap(q.n[0], q.n[1]), std::swap(q.stride[0], q.stride[1]);
+  q.first = static_cast<int64_t>(reinterpret_cast<uintptr_t>(p));
+  q.last = q.first + (q.n[0] - 1) * q.stride[0] + (q.n[1] - 1) * q.stride[1] + q.width;
+  q.tensor = tensor;
+  q.kind = kind;
+  return q;
+}
+
+bool same_place(const Place& a, const Place& b) {
+  return a.first == b.first && a.last == b.last && a.width == b.width && a.n[0] == b.n[0] && a.n[1] == b.n[1] &&
+         a.stride[0] == b.stride[0];
+}
+
+// f(i) for the i of low .. high with after < at + i step < before, until it is true.
+template <class F>
+bool any_between(int64_t at, int64_t step, int64_t low, int64_t high, int64_t after, int64_t before, F&& f) {
+  if (step == 0) return after < at && at < before && f(int64_t{0});
+  auto floor_of = [&](int64_t v) { return v / step - (v % step < 0); };
+  for (int64_t i = std::max(low, floor_of(after - at) + 1), last = std::min(high, -floor_of(at - before) - 1); i <= last; ++i)
+    if (f(i)) return true;
+  return false;
+}
+
+// Whether two stacks have a byte in common. Where their strides differ that is left open: false.
+bool share_bytes(const Place& a, const Place& b) {
+  int64_t stride[2];
+  for (int d = 0; d < 2; ++d) {
+    if (a.n[d] > 1 && b.n[d] > 1 && a.stride[d] != b.stride[d]) return false;
+    stride[d] = a.n[d] > 1 ? a.stride[d] : b.n[d] > 1 ? b.stride[d] : 0;
+  }
+  // Row j of matrix i of b lies at + i stride[0] + j stride[1] from a's first one: of both
+  // rows' and matrices' numbers the differences count.
+  const int64_t at = b.first - a.first;
+  return any_between(at, stride[0], 1 - a.n[0], b.n[0] - 1, -b.width - (b.n[1] - 1) * stride[1],
+                     a.width + (a.n[1] - 1) * stride[1], [&](int64_t i) {
+                       return any_between(at + i * stride[0], stride[1], 1 - a.n[1], b.n[1] - 1, -b.width, a.width,
+                                          [](int64_t) { return true; });
+                     });
+}
+
+// No values that are written lie where others do: workgroups would race for them. A
+// parameter may be its own fp32 master, and its own gradient (or the master may): gradients
+// are read for the last time before weights are written.
+int check_apart(const SbMuonTensor* tensors, int64_t count) try {
+  std::vector<Place> places;
+  for (int64_t i = 0; i < count; ++i) {
+    const SbMuonTensor& a = tensors[i];
+    if (empty(a)) continue;
+    auto bytes = [](int32_t dtype) -> int64_t { return dtype == SB_DTYPE_F32 ? 4 : 2; };
+    places.push_back(place_of(a, i, 0, a.param, bytes(a.param_dtype), a.param_matrix, a.param_row));
+    if (a.master) places.push_back(place_of(a, i, 1, a.master, 4, a.master_matrix, a.master_row));
+    if (a.momentum) places.push_back(place_of(a, i, 2, a.momentum, 4, a.momentum_matrix, a.momentum_row));
+    places.push_back(place_of(a, i, 3, a.grad, bytes(a.grad_dtype), a.grad_matrix, a.grad_row));
+  }
+  std::sort(places.begin(), places.end(), [](const Place& a, const Place& b) { return a.first < b.first; });
+  std::vector<Place> reach;  // those before that end behind this one's start
+  for (const Place& p : places) {
+    reach.erase(std::remove_if(reach.begin(), reach.end(), [&](const Place& q) { return q.last <= p.first; }), reach.end());
+    for (const Place& q : reach) {
+      if (p.kind == 3 && q.kind == 3) continue;
+      if (p.tensor == q.tensor && p.kind != 2 && q.kind != 2 && same_place(p, q)) continue;
+      if (share_bytes(q, p)) return fail(SB_ERR_INVALID, "muon: parameters, momenta, masters and gradients must not overlap");
+    }
+    reach.push_back(p);
+  }
+  return SB_OK;
+} catch (const std::bad_alloc&) {
+  return fail(SB_ERR_INVALID, "muon: no memory for a list of %lld tensors", static_cast<long long>(count));
+}
+
 bool wide_values(const SbMuonTensor& a) {
   auto ok = [](const void* p, int64_t dtype, int64_t matrix, int64_t row) {
     const int64_t bytes = dtype == SB_DTYPE_F32 ? 4 : 2;
@@ -1149,6 +1236,7 @@ int for_each_batch(const SbMuonTensor* tensors, int64_t count, int cus, F&& f) {
 int run_list(const SbMuonTensor* tensors, int64_t count, const Hyper& h, int32_t steps, void* workspace,
              int64_t workspace_bytes, hipStream_t stream) {
   if (steps < 1 || steps > kMaxSteps) return fail(SB_ERR_INVALID, "muon: 1 to %d steps, got %d", kMaxSteps, steps);
+  if (const int rc = check_apart(tensors, count)) return rc;
   int cus = 0;
   if (const int rc = device_cus(&cus)) return rc;
   // All of them before the first is launched: a list that is refused is left as it was.
