@@ -130,3 +130,32 @@ def test_step_of_few_rows() -> None:
         kept, update, _ = step_reference(w, g, torch.zeros_like(w), 1.0, 0.95, True, 0.0, 1.0, 1.0)
         # the update is of size 5 to 70 beside weights of 0.05: their rounding is 2^-24 of it
         check((p.double() - kept), -update, tolerance(g) + 2.0**-23)
+
+
+ALIKE = {
+    "ones": lambda m, n: torch.ones(m, n),
+    "blocks": lambda m, n: torch.block_diag(torch.ones(m // 2, n // 2), torch.ones(m - m // 2, n - n // 2)),
+    "diagonal": lambda m, n: torch.eye(m, n) + 0.01,
+    "equal rows": lambda m, n: torch.randn(1, n, generator=torch.Generator().manual_seed(0)).expand(m, n),
+    "rank 2": lambda m, n: torch.randn(m, 2, generator=torch.Generator().manual_seed(1)) @ torch.randn(
+        2, n, generator=torch.Generator().manual_seed(2)),
+    "few rows": lambda m, n: torch.cat([torch.randn(1, n, generator=torch.Generator().manual_seed(3)), torch.zeros(m - 1, n)]),
+    "signs": lambda m, n: torch.randn(m, 1, generator=torch.Generator().manual_seed(4)).sign() * torch.randn(
+        1, n, generator=torch.Generator().manual_seed(5)).sign(),
+}
+
+
+@pytest.mark.parametrize("kind", ALIKE)
+@pytest.mark.parametrize("size", [(1, 100), (2, 3), (8, 100), (33, 66), (64, 64), (64, 512), (130, 65), (128, 128), (192, 400), (193, 400),
+                                  (300, 300), (700, 300), (768, 2048)])
+def test_roundings_that_are_alike(size, kind) -> None:
+    """Matrices of few different values, whose roundings do not average: those of rank r have r values
+    that count, and each step's product is off by at most 2^-11 for A's rounding, slope 4.78, by 2^-11
+    for B's, 2.75 for values of 1 (whose factor is 0.70), and by 2^-11 for X's in both. Where all push
+    one way that is 2^-11 (4.78 + 2.75 + 2 * 2.75) / 0.70 of X in a step, 0.9%. The slope of the next
+    steps, -0.7, -1.1 and -1.5 at 1, 0.70 and 0.9, turns every step's error around: two of five count."""
+    m, n = size
+    u = ALIKE[kind](m, n).float().to(DEV)
+    got, want = optim.orthogonalize(u).double(), newton_schulz(u)
+    step = 2.0**-11 * (4.78 + 2.75 + 2 * 2.75) / 0.70
+    assert (got - want).norm() <= 2 * step * want.norm()
