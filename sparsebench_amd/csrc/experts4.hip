@@ -20,9 +20,10 @@
 //
 // Bound by the weights' bytes, 17 / 32 of one each: one token, D = 4096, F = 14336, top 2
 // 22.6 us (5.5 TB/s), 14.1 (4.4) and 4.0; 24 tokens, D = 1024, F = 4096, 64 experts 31.9
-// (4.7), 20.9 (3.6) and 4.5; where experts have many rows also by the codes' conversion
-// and the rows' reads: 250 tokens, D = 2048, F = 768, 128 experts, top 4 49 (3.6), 27
-// (3.3), 4.8, and 5.8 for the sort. One token of a small layer is two launches, 9.6.
+// (4.7), 20.9 (3.6) and 4.5. Where experts have many rows the rates are lower: 250 tokens,
+// D = 2048, F = 768, 128 experts, top 4 49 (3.6), 27 (3.3), 4.8, and 5.8 for the sort. There
+// waves wait for loads 44% of their cycles and to issue 45%, as with few rows; vector
+// instructions, the conversions among them, take 6% (counters). One token of a small layer is two launches, 9.6.
 
 #include "gated_act.hpp"
 #include "gated.hpp"
@@ -529,8 +530,11 @@ struct Few4Form {
   int units, blocks, up_wk, down_wk, splits, fused_wk;  // fused_wk 0: down4 and out4
 };
 // Copies x F up to which one workgroup's share of the second product's weights is
-// read in less time than a launch takes (T = 1, D = 256, F = 512: 8.1 us a call
-// against 8.8, and 3.4 us of the host; T = 1, D = 4096, F = 14336: 57 against 48).
+// read in about the time that a launch takes. us a call of the GPU, fused and not, top 2
+// of 8 experts: T = 1, D = 1024 F = 512 9.1 10.4, F = 1024 10.4 10.7, F = 2048 11.0 11.3, F = 4096
+// 12.4 11.0; D = 4096, F = 14336 57 48. More copies take their experts in turn in a wave: T = 4,
+// F = 512 11.4 10.6, T = 8, F = 256 12.8 10.6. But a launch takes 3.4 us of the host, whose 12
+// us a call without it are the longer of the two unless the call is captured.
 constexpr int64_t kFusedMostRead = 4096;
 
 Few4Form few4_form(int64_t copies, int64_t num_experts, int64_t d_model, int64_t ffn_dim, int cus) {

@@ -16,19 +16,25 @@
 // into a second fp16 matrix, added in a5 X, which costs no product; most of the
 // rest from the diagonals of A and B, which are kept in fp32 beside matrices with
 // zeros there: (D + O)^2 = D^2 + D O + O D + O O, and B's diagonal joins a5 X.
+// Where few rows or many steps make it count, B is multiplied with X's remainder too
+// (run_batch), and up to 64 rows A's and B's are kept as well (chain_kernel). In up to five
+// steps the result is then within 0.5% in the matrix's norm wherever its singular values
+// lie: at worst 0.35% over spectra of decades, of two sizes and of nearly low rank, 0.49%
+// over matrices of few equal values, whose entries round alike, 0.03 to 0.06% for noise
+// with some strong directions; in eight steps within 1%.
 //
 // A and B are symmetric: only tiles on and above the diagonal are computed, and
 // written twice. The products run on the LDS-DMA main loop (gemm_dma.hpp), X X^T
 // with B's columns as rows. Matrices are padded with zeros to whole tiles, which
-// the products leave zero. All matrices of one size go together, whatever tensors
-// they come from and whichever side is the smaller.
+// the products leave zero. All matrices of one size go together, whichever side is the
+// smaller, those of up to 16 tensors (kEntries: the table is a kernel's argument).
 //
 // Bound by the matrix cores where matrices are large, and there by the clock that the chip
 // holds under them: 128 of 1024 x 4096 (bf16, fp32 masters) take X X^T 628 us (1094 TFLOP/s
 // of its tiles), a product of m^3 229 (750), an update 1580 (695: its epilogue moves 4
 // bytes in and 4 out a value while no product runs), the last one 2316 with the weights'
 // step, momentum 1112 and X 1087 (both at 4.8 TB/s). Small lists are bound by their 17
-// launches of 4 to 10 us: 24 of 256 x 512 take 108.
+// launches of 4 to 10 us: 24 of 256 x 512 take 114.
 
 #include <algorithm>
 #include <cmath>
@@ -879,19 +885,20 @@ Shape shape_of(int64_t rows, int64_t columns, int64_t matrices, int cus) {
   // Wide tiles (one workgroup a CU) where matrices are large and padding to them costs
   // little, small ones where the work is little or padding to 128 would add a third.
   // us for five steps of bf16 stacks, wide, narrow, small:
-  //   128 of 768 x 2048  3850  4323  5172     24 of 256 x 512       158  112
-  //   20 of 2048 x 2048  4123  5011  7252     200 of 256 x 256      360  325
-  //   64 of 768 x 2048   2172  2214  2631     3 of 1024 x 1024      238  203
-  //   26 of 1024 x 4096  2586  2357  2911     7 of 1024 x 1024      326  371
-  //   400 of 512 x 512   2958  2877  3411     90 of 512 x 1024      988  1106
-  //   100 of 512 x 2048  1982  1670  1931     100 of 320 x 1024     698  556
-  //   300 of 256 x 256    691   481   471     1000 of 192 x 192    1500  900
+  //   128 of 768 x 2048  4223  4804  5761     24 of 256 x 512       257  161   114
+  //   20 of 2048 x 2048  4183  5061  7275     200 of 256 x 256      421  396   337
+  //   64 of 768 x 2048   2239  2466  2963     3 of 1024 x 1024      405  249   210
+  //   26 of 1024 x 4096  2724  2774  3427     7 of 1024 x 1024      437  334   384
+  //   400 of 512 x 512   2900  2902  3444     90 of 512 x 1024     1151 1077  1203
+  //   100 of 512 x 2048  2052  1948  2250     100 of 320 x 1024    1170  749   592
+  //   300 of 256 x 256    653   520   478     1000 of 192 x 192    1783 1694  1017
   auto fits = [&](int64_t tile) { return round_up(s.m, tile) * round_up(s.n, tile) < kMostPadded; };
   if (fits(256) && s.m > 512 && 2 * padded(256) <= 3 * padded(64) && 2 * steps_of_a(256) >= int64_t{9} * cus) s.tile = 256;
   else if (!fits(128) || steps_of_a(64) <= int64_t{32} * cus || 4 * padded(64) <= 3 * padded(128)) s.tile = 64;
   else s.tile = 128;
   // The first two steps at a time (run_steps) where X is long, and not so little that
-  // launches count: 16 of 512 x 2048 take 395 us for 404, 1 of 128 x 4096 135 for 140.
+  // launches count: 16 of 512 x 2048 take 410 us for 455, 1 of 128 x 4096 136 for 146, 100 of
+  // 512 x 1024 1152 for 1231; 24 of 256 x 512 would take 115.5 for 113.7.
   s.chain = s.tile == 64 && s.m <= 64;
   s.pairs = s.n >= 2 * s.m &&
             (s.chain || s.n >= 2048 || matrices * (round_up(s.m, 64) / 64) * (round_up(s.n, 64) / 64) >= int64_t{4} * cus);

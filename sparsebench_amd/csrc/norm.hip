@@ -2,7 +2,7 @@
 // its scale and the residual sum (norm.hpp has the formulas).
 //
 // Bound by memory: norm_out with the next norm reads two rows and writes two.
-// One pass: the row stays in registers between its sum of squares and its use,
+// One pass: the row stays in registers (norm.hpp) between its sum of squares and its use,
 // and so does `out` for the next norm's sum, which is taken of the rounded
 // values: the next block starts from those, so norm_in of `out` gives the same
 // bits. Sums in fp32.
@@ -11,7 +11,9 @@
 // a workgroup's of 4 or 16 waves; workgroups stay and take every so many rows, so that
 // the weights are read once. Both norms, bf16: 4001 rows of 4096 in 22.7 us (5.8 TB/s of
 // reads and writes; a large copy reaches 4.9), 8192 of 1024 in 15.3 (4.4), fp32 rows of
-// 1001, loaded value by value, 2047 in 9.0 (3.6), one row of 2048 or less in 3.3.
+// 1001, loaded value by value, 2047 in 9.0 (3.6), one row of 2048 or less in 3.3. Beyond
+// D = 8192 rows go through scratch: bf16, 4096 rows of 8192 in 46 us (5.8 TB/s), 4092 of
+// 8200 in 260 (1.0), 2048 of 16384 in 189, 1024 of 32768 in 164.
 
 #include "norm.hpp"
 

@@ -7,13 +7,15 @@
 //   dw  = sum_t g p,  dg = w p summed over what g is broadcast to,  dv = sum_t dn on
 //
 // One pass: the sums of a row that need no other sum (o^2, y^2, v dn o) are
-// taken together, then sum(g w p). Rows are read once and kept in registers.
+// taken together, then sum(g w p). Rows are read once and kept in registers up to D = 4096.
 // dw and dv are summed over a workgroup's rows in registers, over its groups in
 // LDS, and over the workgroups by a second kernel, in a fixed order: the same
 // bits every time. A gate of the channels has dg = w q and dw = g q with one
 // sum q = sum_t p. Bound by memory: 4 rows read, 2 written; the next row is loaded while
 // one is worked on. 8192 rows of 1024, bf16: 21.9 us (4.6 TB/s), and the sums of 512
-// workgroups 4.0.
+// workgroups 4.0; 8192 of 4096 91 (4.4 TB/s). Beyond D = 4096 part of them goes through
+// scratch (norm.hpp): 6553 rows of 5120 181 us (2.2 TB/s), 4096 of 8192 147 (2.7), 4092 of 8200 654
+// (0.6), 2048 of 16384 381 (1.1), 1024 of 32768 792 (0.5).
 
 #include "norm.hpp"
 #include "workspace.hpp"
