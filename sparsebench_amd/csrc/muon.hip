@@ -610,7 +610,7 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1) symmetric_kernel(ProductArgs
 // 2%, 64 x 128 0.8%), and products are short here: each square keeps what its rounding to
 // fp16 left beside it, products are L R with both remainders' cross terms, and the factor's
 // remainder goes into X as well. X X^T takes X rounded to fp16 where n > 64, whose roundings
-// average over n (0.26% for 2 rows of 65, 0.03% of 1000), and for n <= 64, one K step, its
+// average over n (0.14% for 2 rows of 65, 0.03% of 1000), and for n <= 64, one K step, its
 // remainder too (5e-5). Three of 40 x 1001 76 us, one of 64 x 4096 108, 1000 of 64 x 256 222;
 // without remainders 66, 96 and 182, and as launches of symmetric_kernel 78, 106 and 217.
 // One LDS array: with a second one the compiler lets every read in the main loop wait for
